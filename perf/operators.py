@@ -236,17 +236,18 @@ def _plain_append(x, slots, cache, scale, code):
     largest = torch.zeros(touched.numel(), x.shape[1], device=x.device)
     largest.scatter_reduce_(0, group[:, None].expand(-1, x.shape[1]), x.abs().amax(-1), "amax")
     old = torch.where(kept[:, None] > 0, scales[touched], 0.0)
-    now = torch.maximum(old, largest / torch.tensor(_LARGEST[code], device=x.device))
-    divisor = torch.where(now > 0, now, 1.0)
+    need = largest / torch.tensor(_LARGEST[code], device=x.device)
+    now = torch.maximum(old, torch.where(need < torch.finfo(torch.float32).tiny, 0.0, need))
+    inverse = torch.where(now > 0, 1 / now, 0.0)
     again = (kept > 0) & (now > old).any(-1)             # a scale is raised over codes that stay
     at = touched[again]
     held = codes[at]
-    moved = _coded(held.float() * (old / divisor)[again][:, None, :, None], code)
+    moved = _coded(held.float() * (old * inverse)[again][:, None, :, None], code)
     stays = torch.arange(rows, device=x.device) < kept[again][:, None]
     raised = (now > old)[again]
     bits = torch.where((stays[:, :, None] & raised[:, None, :])[..., None], moved.view(torch.int8), held.view(torch.int8))
     codes.view(torch.int8)[at] = bits
-    codes.view(torch.int8)[block, row] = _coded(x / divisor[group][..., None], code).view(torch.int8)
+    codes.view(torch.int8)[block, row] = _coded(x * inverse[group][..., None], code).view(torch.int8)
     scales[touched] = now
 
 
