@@ -38,62 +38,13 @@
 #include <mutex>
 #include <type_traits>
 
+#include "cache_dev.cuh"
 #include "cache_geo.cuh"
 #include "check_slots.h"
+#include "check_words.h"
 #include "common.cuh"
 
 namespace fa {
-
-constexpr int kTile = 64;             // keys per work tile
-constexpr int kMaxBalanced = 512;     // sequences up to which every warp sums the lengths itself
-constexpr int kOneWave = 64;          // largest piece, in tiles, that is still run in one wave of CTAs
-constexpr int kWaves = 4;             // waves of CTAs beyond that
-
-struct DecodeGeom {
-  int shares;      // pieces the grid has room for
-  int splits;      // 0: pieces sized on the device; else that many pieces of every sequence
-  int resident;    // CTAs the GPU runs at a time
-  int max_tiles;   // tiles of a full cache
-  int row_groups;  // ceil(seqlen_q * group / rows of a unit)
-  int page_shift;  // log2(page_size) or -1
-};
-
-// The value checks of one call: their result goes to a word in mapped host memory (bit 31 = done, low
-// bits = fa_decode_check of the checks that failed), and to a word of the call's own workspace for the kernels
-// behind them.  The host word is handed to the next call once the host has read it; the kernels read theirs until the
-// last CTA has started, long after the call has returned, so no other call may write to it.
-constexpr uint32_t kCheckDone = 0x80000000u;
-constexpr int kInlineCheck = 1024;   // table entries up to which every attention CTA makes the checks itself
-struct DecodeCheck {
-  uint32_t* host;       // null = no checks in this kernel
-  const uint32_t* dev;  // null, or the result of decode_check_kernel
-};
-
-// All checks, by the threads of one CTA; every thread gets the mask of those that failed.
-__device__ __forceinline__ uint32_t decode_checks(const fa_decode_args& p, int tid, int nt) {
-  uint32_t bad = 0;
-  if (p.block_table) {
-    const int n = p.batch * p.block_table_stride;
-    for (int i = tid; i < n; i += nt)
-      if ((unsigned)p.block_table[i] >= (unsigned)p.num_pages) bad |= FA_CHECK_PAGES;
-  }
-  const long long cap = p.block_table ? (long long)p.block_table_stride * p.page_size : p.page_size;
-  for (int b = tid; b < p.batch; b += nt) {
-    if (p.cache_batch_idx && (unsigned)p.cache_batch_idx[b] >= (unsigned)p.num_pages) bad |= FA_CHECK_ROWS;
-    const int pad = p.cache_leftpad ? p.cache_leftpad[b] : 0;
-    if (pad < 0) bad |= FA_CHECK_LEFTPAD;
-    const int old = p.cache_seqlens[b];
-    const long long last = (long long)old + (p.k_new ? p.seqlen_new : 0) + pad;
-    if (old < 0 || last > cap) bad |= FA_CHECK_LENGTHS;
-    if (p.rotary_cos && last > p.rotary_seqlen) bad |= FA_CHECK_ROTARY;
-  }
-  if (!__syncthreads_or(bad)) return 0u;
-  return (__syncthreads_or(bad & FA_CHECK_PAGES) ? FA_CHECK_PAGES : 0u) |
-         (__syncthreads_or(bad & FA_CHECK_ROWS) ? FA_CHECK_ROWS : 0u) |
-         (__syncthreads_or(bad & FA_CHECK_LEFTPAD) ? FA_CHECK_LEFTPAD : 0u) |
-         (__syncthreads_or(bad & FA_CHECK_LENGTHS) ? FA_CHECK_LENGTHS : 0u) |
-         (__syncthreads_or(bad & FA_CHECK_ROTARY) ? FA_CHECK_ROTARY : 0u);
-}
 
 int cache_attention_sm100(const fa_decode_args& d, const void* q, const int64_t* q_stride, const CacheGeo& geo,
                           const ScoreCfg& cfg, cudaStream_t st);
@@ -107,223 +58,14 @@ __global__ void __launch_bounds__(1024) decode_check_kernel(const fa_decode_args
   }
 }
 
-template <typename T> __device__ __forceinline__ T hmul_rn(T a, T b);
-template <> __device__ __forceinline__ __half hmul_rn(__half a, __half b) { return __hmul_rn(a, b); }
-template <> __device__ __forceinline__ __nv_bfloat16 hmul_rn(__nv_bfloat16 a, __nv_bfloat16 b) { return __hmul_rn(a, b); }
-template <typename T> __device__ __forceinline__ T hadd_rn(T a, T b);
-template <> __device__ __forceinline__ __half hadd_rn(__half a, __half b) { return __hadd_rn(a, b); }
-template <> __device__ __forceinline__ __nv_bfloat16 hadd_rn(__nv_bfloat16 a, __nv_bfloat16 b) { return __hadd_rn(a, b); }
-template <typename T> __device__ __forceinline__ T hsub_rn(T a, T b);
-template <> __device__ __forceinline__ __half hsub_rn(__half a, __half b) { return __hsub_rn(a, b); }
-template <> __device__ __forceinline__ __nv_bfloat16 hsub_rn(__nv_bfloat16 a, __nv_bfloat16 b) { return __hsub_rn(a, b); }
-
-// Rotary on element d of a head vector x (read through `get`), every product and sum
-// rounded to T like the reference's eager arithmetic (flash_attn_interface.py:57-66).
-// A position outside the table [0, rotary_seqlen) leaves the element unrotated (the host checks
-// the lengths when validation is on; this keeps the read in bounds when it is off).
-template <typename T, typename F>
-__device__ __forceinline__ T rotary_elem(F get, int d, const T* cos, const T* sin, int pos,
-                                         int rotary_dim, int interleaved, int rotary_seqlen) {
-  if (d >= rotary_dim || pos < 0 || pos >= rotary_seqlen) return get(d);
-  const int half = rotary_dim >> 1;
-  int i, partner;
-  bool first;
-  if (interleaved) {
-    i = d >> 1;
-    first = (d & 1) == 0;
-    partner = d ^ 1;
-  } else {
-    first = d < half;
-    i = first ? d : d - half;
-    partner = first ? d + half : d - half;
-  }
-  const T c = cos[(int64_t)pos * half + i], s = sin[(int64_t)pos * half + i];
-  const T x = get(d), y = get(partner);
-  // first: x*c - y*s ; second: y*s + x*c  (y = first element of the pair)
-  return first ? hsub_rn(hmul_rn(x, c), hmul_rn(y, s)) : hadd_rn(hmul_rn(y, s), hmul_rn(x, c));
-}
-
-// Whether rotary_chunk() can read 16 (pairs side by side: 8) bytes of the tables at a time.
-template <typename T>
-__device__ __forceinline__ bool rotary_in_chunks(const T* cos, const T* sin, int rotary_dim, int interleaved) {
-  return (rotary_dim & (interleaved ? 7 : 15)) == 0 &&
-         ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & (interleaved ? 7 : 15)) == 0;
-}
-
-// The others: halves that are multiples of 4 by 8 bytes, the rest element by element.
-template <typename T>
-__device__ __forceinline__ uint4 rotary_chunk_any(const T* x, int d, const T* cos, const T* sin, int pos, int rotary_dim,
-                                                  int interleaved, int rotary_seqlen) {
-  union { uint4 v; uint2 h[2]; T e[8]; } out;
-  const int half = rotary_dim >> 1;
-  if (!interleaved && half % 4 == 0 && ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 7) == 0) {
-    union Four { uint2 v; T e[4]; };
-    out.v = *reinterpret_cast<const uint4*>(x + d);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = d + 4 * h;
-      if (at >= rotary_dim) break;
-      const bool first = at < half;
-      const int64_t i = (int64_t)pos * half + (first ? at : at - half);
-      Four self, other, c, s;
-      self.v = out.h[h];
-      other.v = *reinterpret_cast<const uint2*>(x + (first ? at + half : at - half));
-      c.v = *reinterpret_cast<const uint2*>(cos + i);
-      s.v = *reinterpret_cast<const uint2*>(sin + i);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        self.e[k] = first ? hsub_rn(hmul_rn(self.e[k], c.e[k]), hmul_rn(other.e[k], s.e[k]))
-                          : hadd_rn(hmul_rn(other.e[k], s.e[k]), hmul_rn(self.e[k], c.e[k]));
-      out.h[h] = self.v;
-    }
-    return out.v;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    out.e[k] = rotary_elem<T>([&](int j) { return x[j]; }, d + k, cos, sin, pos, rotary_dim, interleaved, rotary_seqlen);
-  return out.v;
-}
-template <typename T>
-__device__ __noinline__ uint4 rotary_chunk_call(const T* x, int d, const T* cos, const T* sin, int pos, int rotary_dim,
-                                                int interleaved, int rotary_seqlen) {
-  return rotary_chunk_any(x, d, cos, sin, pos, rotary_dim, interleaved, rotary_seqlen);
-}
-
-// 8 elements of a head row, rotated like rotary_elem.  kCall: the general case out of line.  In the main loop of decode_kernel
-// it cost registers and the order of the loads (head_dim 256, 32 x 8000 tokens, 16 heads over 4: 268 us, 233 as a call); a
-// kernel that only rotates and copies is better off without the call (4 x 256 tokens behind 300, 32 heads over 8 of 128, with
-// their attention: 42 us, 46).  Pairs side by side need no row beside the one at hand and half as much of the tables: 8 x 900
-// tokens, 4 new, 16 heads over 4 of 128: a thread per element 30.4 us, eight elements of a thread one by one 20.6, now 16.6.
-template <typename T, bool kCall>
-__device__ __forceinline__ uint4 rotary_chunk(const T* x, int d, const T* cos, const T* sin, int pos, int rotary_dim,
-                                              int interleaved, int rotary_seqlen) {
-  union { uint4 v; T e[8]; } out, self, other, c, s;
-  self.v = *reinterpret_cast<const uint4*>(x + d);
-  if (cos == nullptr || d >= rotary_dim || pos < 0 || pos >= rotary_seqlen) return self.v;
-  if (!rotary_in_chunks(cos, sin, rotary_dim, interleaved)) {
-    if (kCall) return rotary_chunk_call(x, d, cos, sin, pos, rotary_dim, interleaved, rotary_seqlen);
-    return rotary_chunk_any(x, d, cos, sin, pos, rotary_dim, interleaved, rotary_seqlen);
-  }
-  const int half = rotary_dim >> 1;
-  if (interleaved) {
-    *reinterpret_cast<uint2*>(c.e) = *reinterpret_cast<const uint2*>(cos + (int64_t)pos * half + (d >> 1));
-    *reinterpret_cast<uint2*>(s.e) = *reinterpret_cast<const uint2*>(sin + (int64_t)pos * half + (d >> 1));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const T x0 = self.e[2 * k], x1 = self.e[2 * k + 1];
-      out.e[2 * k] = hsub_rn(hmul_rn(x0, c.e[k]), hmul_rn(x1, s.e[k]));
-      out.e[2 * k + 1] = hadd_rn(hmul_rn(x0, s.e[k]), hmul_rn(x1, c.e[k]));
-    }
-    return out.v;
-  }
-  const bool first = d < half;
-  const int i = first ? d : d - half;
-  other.v = *reinterpret_cast<const uint4*>(x + (first ? d + half : d - half));
-  c.v = *reinterpret_cast<const uint4*>(cos + (int64_t)pos * half + i);
-  s.v = *reinterpret_cast<const uint4*>(sin + (int64_t)pos * half + i);
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    out.e[k] = first ? hsub_rn(hmul_rn(self.e[k], c.e[k]), hmul_rn(other.e[k], s.e[k]))
-                     : hadd_rn(hmul_rn(other.e[k], s.e[k]), hmul_rn(self.e[k], c.e[k]));
-  return out.v;
-}
-
-__device__ __forceinline__ int64_t cache_row_offset(const fa_decode_args& p, int b, int pos,
-                                                    int page_shift, const int64_t* stride) {
-  int page, row;
-  if (p.block_table) {
-    int pi;
-    if (page_shift >= 0) {
-      pi = pos >> page_shift;
-      row = pos & (p.page_size - 1);
-    } else {
-      pi = pos / p.page_size;
-      row = pos - pi * p.page_size;
-    }
-    page = p.block_table[(int64_t)b * p.block_table_stride + pi];
-  } else {
-    page = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
-    row = pos;
-  }
-  return (int64_t)page * stride[0] + (int64_t)row * stride[1];
+int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st) {
+  decode_check_kernel<<<1, 1024, 0, st>>>(a, host, dev);
+  return check_launch("decode_check");
 }
 
 // ---------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------
-// Tiles of a sequence: nt work tiles from tile lo on.  Keys that no query row sees (left of the window)
-// are skipped, new tokens never are: somebody has to append them.  An empty sequence has one
-// (empty) tile, which writes its zeros.
-struct SeqTiles {
-  int len_old, len, lo, nt;
-};
-// Rows a sequence can hold behind its left padding: lengths are taken up to here and new tokens stored up to here, so
-// that a call whose values are not checked stays inside its rows of the cache and of the table.
-__host__ __device__ __forceinline__ int cache_capacity(const fa_decode_args& p) {
-  const int64_t cap = p.block_table ? (int64_t)p.block_table_stride * p.page_size : p.page_size;
-  return (int)(cap < (1 << 30) ? cap : (1 << 30));
-}
-__device__ __forceinline__ int seq_capacity(const fa_decode_args& p, int b) {
-  return cache_capacity(p) - (p.cache_leftpad ? max(0, p.cache_leftpad[b]) : 0);
-}
-__device__ __forceinline__ SeqTiles seq_tiles(const fa_decode_args& p, const ScoreCfg& cfg, int max_tiles, int b) {
-  SeqTiles s;
-  s.len_old = max(0, min(p.cache_seqlens[b], seq_capacity(p, b)));
-  s.len = s.len_old + (p.k_new ? p.seqlen_new : 0);
-  const int first = cfg.wl >= 0 ? min(max(0, s.len - p.seqlen_q - cfg.wl), s.len_old) : 0;
-  s.lo = first / kTile;
-  s.nt = min(max(1, (s.len + kTile - 1) / kTile - s.lo), max_tiles);
-  return s;
-}
-
-// Elements [d, d + 4) of one output row, merged from the `parts` workspace rows r0, r0 + step, ...  Eight
-// pieces are loaded at a time, their common maximum taken first.  (Sixteen: longer code in front of few rows, -1 to
-// +7 % of a step's time at every head size -- 2 x 411 tokens, one head of 64: 9.7 -> 10.6 us.)
-constexpr int kMergeBatch = 8;
-template <typename T, int D>
-__device__ __forceinline__ void merge_pieces(const float* ws_o, const float* ws_l, int64_t r0, int64_t step, int parts, int d,
-                                             T* og) {
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float wsum = 0.f, m = -INFINITY;
-  for (int i0 = 0; i0 < parts; i0 += kMergeBatch) {
-    float l[kMergeBatch];
-    float4 x[kMergeBatch];
-#pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) {
-      const int i = i0 + j;
-      const int64_t r = r0 + i * step;
-      l[j] = i < parts ? ws_l[r] : -INFINITY;
-      x[j] = i < parts ? *reinterpret_cast<const float4*>(ws_o + r * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    float mn = m;
-#pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) mn = fmaxf(mn, l[j]);
-    // pieces without a finite score weigh 0, which a NaN in them survives
-    const float mf = mn == -INFINITY ? 0.f : mn;
-    const float sc = exp2f(m - mf);
-    acc.x *= sc; acc.y *= sc; acc.z *= sc; acc.w *= sc;
-    wsum *= sc;
-    m = mn;
-#pragma unroll
-    for (int j = 0; j < kMergeBatch; ++j) {
-      const float w = exp2f(l[j] - mf);
-      wsum += w;
-      acc.x += w * x[j].x; acc.y += w * x[j].y; acc.z += w * x[j].z; acc.w += w * x[j].w;
-    }
-  }
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
-  uint2 pk;
-  pk.x = Elem<T>::pack(acc.x * inv, acc.y * inv);
-  pk.y = Elem<T>::pack(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(og + d) = pk;
-}
-
-__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
 // kRows: query rows of a unit (8 or 16)
 template <int D, int kRows> struct DecodeSmem {
   static constexpr int P = TilePitch<D>::value, NS = 3, OP = D + 4;
@@ -366,77 +108,12 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
   const int hk = u / geo.row_groups, rg = u % geo.row_groups;
 
   // ---- this CTA's piece: tiles [tile0, tile0 + count) of sequence b ------------------------
-  int b, tile0, count, parts, base;              // base: first of the `parts` pieces of the sequence
-  SeqTiles w;
-  if (geo.splits == 0) {
-    // Every warp does this on its own, without shared memory or barriers (which cost a small step 2 to 4
-    // us); lane i looks after the sequences [i per, (i + 1) per).
-    const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
-    int sum = 0, longest = 0;
-    for (int i = b0; i < b1; ++i) {
-      const int nt = seq_tiles(p, cfg, geo.max_tiles, i).nt;
-      sum += nt;
-      longest = max(longest, nt);
-    }
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    const int64_t work = (int64_t)sum * U;
-    int size = (int)((work + geo.resident - 1) / geo.resident), mine = 0;
-    auto count_pieces = [&]() {
-      mine = 0;
-      for (int i = b0; i < b1; ++i) mine += (seq_tiles(p, cfg, geo.max_tiles, i).nt + size - 1) / size;
-    };
-    if (size > kOneWave) {
-      size = max(kOneWave / 2, (int)((work + kWaves * geo.resident - 1) / (kWaves * geo.resident)));
-      count_pieces();
-    } else {
-      size = max(size, (int)ceilf((float)longest / ceilf(sqrtf(7.f * longest))));
-      for (; size < longest; size += max(1, size >> 3)) {
-        count_pieces();
-        if (__reduce_add_sync(0xffffffffu, mine) * U <= geo.resident) break;
-      }
-    }
-    if (size >= longest) {                       // every sequence in one piece
-      if (share >= p.batch) return;
-      b = base = share;
-      parts = 1;
-    } else {
-      int inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-      }
-      const bool owner = share >= inc - mine && share < inc;
-      const unsigned who = __ballot_sync(0xffffffffu, owner);
-      if (who == 0u) return;                       // the grid is sized for a full cache
-      base = inc - mine;
-      b = b0;
-      parts = 0;
-      if (owner) {
-        for (;; ++b) {
-          parts = (seq_tiles(p, cfg, geo.max_tiles, b).nt + size - 1) / size;
-          if (share < base + parts) break;
-          base += parts;
-        }
-      }
-      const int src = __ffs(who) - 1;
-      b = __shfl_sync(0xffffffffu, b, src);
-      base = __shfl_sync(0xffffffffu, base, src);
-      parts = __shfl_sync(0xffffffffu, parts, src);
-    }
-    w = seq_tiles(p, cfg, geo.max_tiles, b);
-  } else {
-    b = share / geo.splits;
-    base = b * geo.splits;
-    w = seq_tiles(p, cfg, geo.max_tiles, b);
-    parts = min(geo.splits, w.nt);
-    if (share - base >= parts) return;
-  }
+  Piece piece;
+  if (!piece_of(geo, p.batch, share, U, lane, [&](int i) { return seq_tiles(p, cfg, geo.max_tiles, i).nt; }, piece)) return;
+  const int b = piece.b, parts = piece.parts, base = piece.base;
+  const SeqTiles w = seq_tiles(p, cfg, geo.max_tiles, b);
   const int len_old = w.len_old, len = w.len;
-  tile0 = (int)((int64_t)(share - base) * w.nt / parts);
-  count = (int)((int64_t)(share - base + 1) * w.nt / parts) - tile0;
-  tile0 += w.lo;
+  const int tile0 = w.lo + piece.tile0, count = piece.count;
 
   // ---- loading --------------------------------------------------------------------------
   const int lc = (lane % CPR) * 8, lr = lane / CPR;         // this lane's 16-byte column and first row
@@ -799,12 +476,6 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
 // ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
-static int page_shift_of(const fa_decode_args& a) {
-  if (a.page_size <= 0 || (a.page_size & (a.page_size - 1)) != 0) return -1;
-  int s = 0;
-  while ((1 << s) < a.page_size) ++s;
-  return s;
-}
 static int decode_unit_rows(const fa_decode_args& a) { return a.seqlen_q * (a.heads_q / a.heads_kv) <= 8 ? 8 : 16; }
 static int decode_row_groups(const fa_decode_args& a) {
   const int n = decode_unit_rows(a);
@@ -909,37 +580,8 @@ int decode_num_counters(const fa_decode_args& a) {
   return a.batch * a.heads_kv * decode_row_groups(a);
 }
 
-// Room for the pieces the kernel may make.  It picks their size so that
-//   * one wave of CTAs (two per SM, one at head_dim 256) takes all of them, while that needs no more
-//     than kOneWave tiles each: every CTA costs about 3.5 us beside its tiles (16 sequences of 4000 keys,
-//     8 heads: one wave of 32-tile pieces 55 us, two of 16 61 us, 68 us without pieces);
-//   * a sequence has no more than sqrt(7 nt) pieces of its nt tiles: a tile costs about 0.7 us and a piece
-//     0.1 us in the merge (one sequence of 8000 keys, two heads: 126 pieces 20 us, 32 pieces 16.4 us);
-//   * more work than that runs as kWaves waves, which the hardware balances over SMs of unequal speed
-//     (64 sequences of 16000 keys: one wave of equal shares 688 us, 3.5 waves 656 us = 0.98 of the copy
-//     bandwidth).
-// An explicit num_splits, and batches too large to sum in every warp, cut every sequence into the
-// same number of pieces.
 static DecodeGeom decode_geometry(const fa_decode_args& a) {
-  DecodeGeom g;
-  g.row_groups = decode_row_groups(a);
-  const int64_t cap = a.block_table ? (int64_t)a.block_table_stride * a.page_size : a.page_size;
-  const int64_t nt = cap > 0 ? (cap + kTile - 1) / kTile : 1;
-  const int64_t U = (int64_t)a.heads_kv * g.row_groups;
-  g.max_tiles = (int)nt;
-  g.splits = 0;
-  g.resident = sm_count(a.device) * (a.head_dim == 256 ? 1 : 2);
-  if (a.num_splits > 0 || a.batch > kMaxBalanced || a.batch * nt > (1 << 30)) {
-    g.splits = a.num_splits > 0 ? (int)(a.num_splits < nt ? a.num_splits : nt) : 1;
-    g.shares = a.batch * g.splits;
-  } else {
-    const int64_t most = a.batch * nt, whole = a.batch;
-    int64_t n = most * U <= (int64_t)kOneWave * g.resident ? g.resident / U : kWaves * g.resident / U + 1;
-    n += whole;                                // rounding up adds less than a piece per sequence
-    g.shares = (int)(n < most ? n : most);
-  }
-  g.page_shift = page_shift_of(a);
-  return g;
+  return decode_geometry(a, decode_row_groups(a), a.head_dim == 256 ? 1 : 2);
 }
 
 // pieces (their query rows in fp32, then the LSEs of those), then the counters if the caller brings none
@@ -1151,8 +793,10 @@ uint32_t* check_words(int device) {
   return static_cast<uint32_t*>(h);
 }
 
+}  // namespace
+
 // Index of a slot, its word at *dptr; -1 (error set) without one.  A call waits for another call's, a ticket does not.
-int take_slot(bool ticket, int device, uint32_t** dptr) {
+int take_check_word(bool ticket, int device, uint32_t** dptr) {
   uint32_t* words = check_words(device);
   if (words == nullptr) return -1;
   for (;;) {
@@ -1170,7 +814,7 @@ int take_slot(bool ticket, int device, uint32_t** dptr) {
 }
 
 // Waits until the kernel that was given the slot has written it.
-int await_slot(int i, uint32_t* failed, cudaStream_t st) {
+int await_check_word(int i, uint32_t* failed, cudaStream_t st) {
   volatile uint32_t* word = slot_word(i);
   for (uint32_t it = 1; *word == 0u; ++it) {
 #if defined(__x86_64__)
@@ -1189,6 +833,9 @@ int await_slot(int i, uint32_t* failed, cudaStream_t st) {
   return FA_OK;
 }
 
+void give_check_word(int i, bool queued) { g_slots.give(i, queued); }
+
+namespace {
 // Packed calls: both cu_seqlens arrays, by one CTA.
 __global__ void __launch_bounds__(1024) varlen_check_kernel(const int32_t* cu_q, const int32_t* cu_k, int batch, int64_t total_q,
                                                             int64_t total_k, bool k_at_most, int64_t max_q, int64_t max_k,
@@ -1242,11 +889,11 @@ int varlen_check(const int32_t* cu_q, const int32_t* cu_k, int batch, int64_t to
     return FA_ERR_LAUNCH;
   }
   uint32_t* host = nullptr;
-  const int slot = take_slot(true, device, &host);
+  const int slot = take_check_word(true, device, &host);
   if (slot < 0) return FA_ERR_UNSUPPORTED;
   varlen_check_kernel<<<1, batch > 128 ? 1024 : 128, 0, st>>>(cu_q, cu_k, batch, total_q, total_k, k_at_most, max_q, max_k, host);
   if (int r = check_launch("varlen_check")) {
-    g_slots.give(slot, false);
+    give_check_word(slot, false);
     return r;
   }
   *ticket = slot;
@@ -1258,7 +905,7 @@ int check_result(int32_t ticket, uint32_t* failed, cudaStream_t st) {
   int device = -1, current = -1;
   FA_REQUIRE(g_slots.hand_in(ticket, &device), "ticket %d is not out", ticket);
   int r = cudaGetDevice(&current) == cudaSuccess ? ensure_device(device) : FA_ERR_LAUNCH;
-  if (r == FA_OK) r = await_slot(ticket, failed, st);
+  if (r == FA_OK) r = await_check_word(ticket, failed, st);
   g_slots.give(ticket, true);
   if (current >= 0 && current != device) cudaSetDevice(current);
   return r;
@@ -1286,13 +933,12 @@ int decode_paged_checked(const fa_decode_args& a, uint32_t* failed, cudaStream_t
   const bool host_order = k.word && word == nullptr;   // no room for the word: launch nothing before the result is here
   if (host_order) k.inside = false;
   uint32_t* host = nullptr;
-  const int slot = take_slot(false, a.device, &host);
+  const int slot = take_check_word(false, a.device, &host);
   if (slot < 0) return FA_ERR_LAUNCH;
   int r = FA_OK;
   bool queued = false;                                 // a kernel that writes the host word is on the stream
   if (!k.inside) {
-    decode_check_kernel<<<1, 1024, 0, st>>>(a, host, word);
-    r = check_launch("decode_check");
+    r = launch_decode_check(a, host, word, st);
     queued = r == FA_OK;
   }
   if (r == FA_OK && !host_order) {
@@ -1304,10 +950,10 @@ int decode_paged_checked(const fa_decode_args& a, uint32_t* failed, cudaStream_t
     }
   }
   if (queued) {
-    const int w = await_slot(slot, failed, st);
+    const int w = await_check_word(slot, failed, st);
     if (r == FA_OK) r = w;
   }
-  g_slots.give(slot, queued);
+  give_check_word(slot, queued);
   if (r != FA_OK || *failed || !host_order) return r;
   return k.chunk ? chunk_run(a, k.c, nullptr, nullptr, nullptr, st) : decode_run(a, DecodeCheck{nullptr, nullptr}, st);
 }
