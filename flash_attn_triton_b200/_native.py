@@ -88,6 +88,32 @@ class RotaryArgs(C.Structure):
     ]
 
 
+class Cache8(C.Structure):
+    _fields_ = [
+        ("code", C.c_int32), ("block", C.c_int32), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("ks_stride", _I64x3), ("vs_stride", _I64x3),
+    ]
+
+
+class Append8Args(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("device", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32), ("tokens", C.c_int64),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("kc_stride", _I64x3), ("vc_stride", _I64x3),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32), ("slots", C.c_void_p), ("cache", Cache8),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class BlockTableArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32), ("batch", C.c_int32), ("page_size", C.c_int32),
+        ("cache_seqlens", C.c_void_p), ("new_lens", C.c_void_p), ("free_pages", C.c_void_p), ("num_free", C.c_int64),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int32),
+        ("num_slots", C.c_int64), ("slots", C.c_void_p), ("cu_seqlens", C.c_void_p), ("pages_used", C.c_void_p),
+    ]
+
+
 EXPORTS = {
     "fa_fwd": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
     "fa_bwd_preprocess": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
@@ -113,6 +139,15 @@ EXPORTS = {
     "fa_decode_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs)]),
     "fa_decode_paged_static": (C.c_int, [C.POINTER(DecodeArgs), C.c_void_p]),
     "fa_decode_static_scratch_bytes": (C.c_size_t, []),
+    "fa_decode_paged8": (C.c_int, [C.POINTER(DecodeArgs), C.POINTER(Cache8), C.c_void_p]),
+    "fa_decode_paged8_checked": (C.c_int, [C.POINTER(DecodeArgs), C.POINTER(Cache8), C.POINTER(C.c_uint32), C.c_void_p]),
+    "fa_decode8_workspace_bytes": (C.c_size_t, [C.POINTER(DecodeArgs), C.POINTER(Cache8)]),
+    "fa_decode8_counters": (C.c_int32, [C.POINTER(DecodeArgs), C.POINTER(Cache8)]),
+    "fa_append8": (C.c_int, [C.POINTER(Append8Args), C.c_void_p]),
+    "fa_append8_checked": (C.c_int, [C.POINTER(Append8Args), C.POINTER(C.c_uint32), C.c_void_p]),
+    "fa_append8_workspace_bytes": (C.c_size_t, [C.POINTER(Append8Args)]),
+    "fa_block_table": (C.c_int, [C.POINTER(BlockTableArgs), C.c_void_p]),
+    "fa_block_table_checked": (C.c_int, [C.POINTER(BlockTableArgs), C.POINTER(C.c_uint32), C.c_void_p]),
     "fa_quantize_k_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                      C.c_int32, C.c_void_p]),
     "fa_fwd_int8": (C.c_int, [C.POINTER(Int8Args), C.c_void_p]),
@@ -150,7 +185,7 @@ def lib():
             fn = getattr(l, name)
             fn.restype = res
             fn.argtypes = args
-        for which, st in ((0, AttnArgs), (1, DecodeArgs), (2, Int8Args), (3, RotaryArgs)):
+        for which, st in enumerate((AttnArgs, DecodeArgs, Int8Args, RotaryArgs, Cache8, Append8Args, BlockTableArgs)):
             if l.fa_sizeof_args(which) != C.sizeof(st):
                 raise RuntimeError(f"ABI mismatch for {st.__name__}: library "
                                    f"{l.fa_sizeof_args(which)} vs binding {C.sizeof(st)}")
@@ -221,3 +256,8 @@ def kernel_ready(t) -> bool:
     """True when `t` can be handed to the kernels as is: unit inner stride, 16-byte rows."""
     return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
             and all(s % 8 == 0 for s in t.stride()[:-1]))
+
+
+def codes_ready(t) -> bool:
+    """The same for a cache of 8-bit codes."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 16 == 0 for s in t.stride()[:-1])

@@ -169,6 +169,15 @@ size_t decode_workspace_bytes(const fa_decode_args&);
 size_t decode_checked_workspace_bytes(const fa_decode_args&);
 int decode_paged_static(const fa_decode_args&, cudaStream_t);
 size_t decode_static_scratch_bytes();
+int decode8_paged(const fa_decode_args&, const fa_cache8&, cudaStream_t);
+int decode8_paged_checked(const fa_decode_args&, const fa_cache8&, uint32_t*, cudaStream_t);
+size_t decode8_workspace_bytes(const fa_decode_args&);
+int decode8_counters(const fa_decode_args&);
+int append8(const fa_append8_args&, cudaStream_t);
+int append8_checked(const fa_append8_args&, uint32_t*, cudaStream_t);
+size_t append8_workspace_bytes(const fa_append8_args&);
+int block_table(const fa_block_table_args&, cudaStream_t);
+int block_table_checked(const fa_block_table_args&, uint32_t*, cudaStream_t);
 int quantize_k(const void*, int8_t*, float*, int64_t, int, cudaStream_t);
 int fwd_int8_mma(const fa_int8_args&, cudaStream_t);
 bool fwd_int8_sm100_supported(const fa_int8_args&);
@@ -466,6 +475,97 @@ int fa_decode_paged_checked(const fa_decode_args* a, uint32_t* failed, void* str
   return decode_paged_checked(*a, failed, reinterpret_cast<cudaStream_t>(stream));
 }
 
+static bool mult16(const int64_t* s, int n) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] % 16 != 0) return false;
+  return true;
+}
+static int validate_cache8(const fa_cache8& c, int page_size, int num_pages, const void* k_cache, const void* v_cache, const int64_t* ks,
+                           const int64_t* vs) {
+  FA_REQUIRE(c.code == FA_CODE_INT8 || c.code == FA_CODE_E4M3, "code must be FA_CODE_INT8 or FA_CODE_E4M3");
+  FA_REQUIRE(c.block >= 1 && c.block <= 1024, "a scale block has 1 to 1024 tokens (got %d)", c.block);
+  FA_REQUIRE(page_size > 0 && page_size % c.block == 0, "the page size must be a multiple of the scale block");
+  FA_REQUIRE(num_pages >= 0, "negative size");
+  FA_REQUIRE(k_cache && v_cache && c.k_scale && c.v_scale, "8-bit caches and their scales are required");
+  FA_REQUIRE(aligned16(k_cache) && aligned16(v_cache) && mult16(ks, 3) && mult16(vs, 3), "cache rows must be 16-byte aligned");
+  return FA_OK;
+}
+static int validate_decode8(const fa_decode_args* a, const fa_cache8* c) {
+  if (int r = validate_decode(a)) return r;
+  FA_REQUIRE(c != nullptr, "cache is NULL");
+  if (a->batch == 0 || a->seqlen_q == 0) return FA_OK;
+  return validate_cache8(*c, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride);
+}
+int fa_decode_paged8(const fa_decode_args* a, const fa_cache8* c, void* stream) {
+  if (int r = validate_decode8(a, c)) return r;
+  if (int r = ensure_device(a->device)) return r;
+  return decode8_paged(*a, *c, reinterpret_cast<cudaStream_t>(stream));
+}
+int fa_decode_paged8_checked(const fa_decode_args* a, const fa_cache8* c, uint32_t* failed, void* stream) {
+  if (int r = validate_decode8(a, c)) return r;
+  FA_REQUIRE(failed != nullptr, "failed is NULL");
+  if (int r = ensure_device(a->device)) return r;
+  return decode8_paged_checked(*a, *c, failed, reinterpret_cast<cudaStream_t>(stream));
+}
+size_t fa_decode8_workspace_bytes(const fa_decode_args* a, const fa_cache8* c) {
+  if (a == nullptr || c == nullptr || a->heads_kv <= 0 || a->heads_q <= 0 || a->page_size <= 0) return 0;
+  return decode8_workspace_bytes(*a);
+}
+int32_t fa_decode8_counters(const fa_decode_args* a, const fa_cache8* c) {
+  if (a == nullptr || c == nullptr || a->heads_kv <= 0 || a->heads_q <= 0 || a->page_size <= 0) return 0;
+  return decode8_counters(*a);
+}
+
+static int validate_append8(const fa_append8_args* a) {
+  FA_REQUIRE(a != nullptr, "args is NULL");
+  FA_REQUIRE(a->dtype == FA_F16 || a->dtype == FA_BF16, "dtype must be FA_F16 or FA_BF16");
+  FA_REQUIRE(a->tokens >= 0 && a->tokens <= INT32_MAX && a->heads > 0, "negative or too large a size");
+  FA_REQUIRE(a->head_dim == 16 || a->head_dim == 32 || a->head_dim == 64 || a->head_dim == 128 || a->head_dim == 256,
+             "head dimension must be one of 16, 32, 64, 128, or 256 (got %d)", a->head_dim);
+  if (a->tokens == 0) return FA_OK;
+  FA_REQUIRE(a->k && a->v && a->slots, "k, v and slots are required");
+  FA_REQUIRE(aligned16(a->k) && aligned16(a->v) && mult8(a->k_stride, 2) && mult8(a->v_stride, 2), "k/v rows must be 16-byte aligned");
+  FA_REQUIRE(a->workspace == nullptr || aligned16(a->workspace), "workspace must be 16-byte aligned");
+  return validate_cache8(a->cache, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride);
+}
+int fa_append8(const fa_append8_args* a, void* stream) {
+  if (int r = validate_append8(a)) return r;
+  if (int r = ensure_device(a->device)) return r;
+  return append8(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+int fa_append8_checked(const fa_append8_args* a, uint32_t* failed, void* stream) {
+  if (int r = validate_append8(a)) return r;
+  FA_REQUIRE(failed != nullptr, "failed is NULL");
+  if (int r = ensure_device(a->device)) return r;
+  return append8_checked(*a, failed, reinterpret_cast<cudaStream_t>(stream));
+}
+size_t fa_append8_workspace_bytes(const fa_append8_args* a) {
+  return a == nullptr || a->num_pages < 0 ? 0 : append8_workspace_bytes(*a);
+}
+
+static int validate_block_table(const fa_block_table_args* a) {
+  FA_REQUIRE(a != nullptr, "args is NULL");
+  FA_REQUIRE(a->batch >= 0 && a->num_free >= 0 && a->table_pages >= 0 && a->table_stride >= 0, "negative size");
+  FA_REQUIRE(a->num_slots >= 0 && a->num_slots <= INT32_MAX && a->num_free <= INT32_MAX, "too many slots or pages");
+  FA_REQUIRE(a->page_size > 0, "page_size must be positive");
+  FA_REQUIRE(a->cu_seqlens && a->pages_used && (a->slots || a->num_slots == 0), "slots, cu_seqlens and pages_used are required");
+  FA_REQUIRE(a->batch == 0 || (a->cache_seqlens && a->new_lens), "cache_seqlens and new_lens are required");
+  FA_REQUIRE(a->batch == 0 || a->table_pages == 0 || a->block_table, "block_table is required");
+  FA_REQUIRE(a->num_free == 0 || a->free_pages, "free_pages is required");
+  return FA_OK;
+}
+int fa_block_table(const fa_block_table_args* a, void* stream) {
+  if (int r = validate_block_table(a)) return r;
+  if (int r = ensure_device(a->device)) return r;
+  return block_table(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+int fa_block_table_checked(const fa_block_table_args* a, uint32_t* failed, void* stream) {
+  if (int r = validate_block_table(a)) return r;
+  FA_REQUIRE(failed != nullptr, "failed is NULL");
+  if (int r = ensure_device(a->device)) return r;
+  return block_table_checked(*a, failed, reinterpret_cast<cudaStream_t>(stream));
+}
+
 int fa_varlen_check(const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int64_t total_q, int64_t total_k, int32_t k_at_most,
                     int64_t max_q, int64_t max_k, int32_t device, int32_t* ticket, void* stream) {
   FA_REQUIRE(cu_q != nullptr && cu_k != nullptr && ticket != nullptr && batch >= 0, "cu_seqlens and ticket are required");
@@ -693,6 +793,9 @@ size_t fa_sizeof_args(int which) {
     case 1: return sizeof(fa_decode_args);
     case 2: return sizeof(fa_int8_args);
     case 3: return sizeof(fa_rotary_args);
+    case 4: return sizeof(fa_cache8);
+    case 5: return sizeof(fa_append8_args);
+    case 6: return sizeof(fa_block_table_args);
   }
   return 0;
 }

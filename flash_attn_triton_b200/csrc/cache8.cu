@@ -1,0 +1,125 @@
+// Calls on the 8-bit KV cache: value checks, append, attention.  One launch where nothing is appended and the tables are small, else the
+// append (which then makes the checks) and the attention behind it.
+#include "cache8_host.h"
+#include "cache_dev.cuh"
+#include "check_words.h"
+
+namespace fa {
+
+int decode8_int8(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
+int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
+int decode8_resident(int head_dim, int unit_rows);
+int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st);
+
+namespace {
+
+constexpr size_t kAlign = 16;
+size_t aligned(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+int unit_rows_of(const fa_decode_args& a) { return a.seqlen_q * (a.heads_q / a.heads_kv) <= 8 ? 8 : 16; }
+
+// How a call is run.  Workspace: pieces, counters if the caller brings none, the word with the result of the checks.
+struct Plan {
+  int unit_rows;
+  DecodeGeom geo;
+  size_t piece_bytes, counter_bytes;
+  int counters;
+  bool append, inside;                 // the first kernel makes the checks, in every CTA
+  size_t word_at() const { return aligned(piece_bytes) + aligned(counter_bytes); }
+  size_t bytes() const { return word_at() + kAlign; }
+};
+
+Plan plan_of(const fa_decode_args& a) {
+  Plan p;
+  p.unit_rows = unit_rows_of(a);
+  const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
+  const int groups = (int)((rows + p.unit_rows - 1) / p.unit_rows);
+  p.geo = decode_geometry(a, groups, decode8_resident(a.head_dim, p.unit_rows));
+  p.piece_bytes = p.geo.splits == 1 ? 0 : (size_t)p.geo.shares * a.seqlen_q * a.heads_q * (a.head_dim + 1) * sizeof(float);
+  p.counters = p.piece_bytes ? a.batch * a.heads_kv * groups : 0;
+  p.counter_bytes = a.counters ? 0 : (size_t)p.counters * sizeof(uint32_t);
+  p.append = a.k_new != nullptr;
+  p.inside = (int64_t)a.batch * (a.block_table ? a.block_table_stride : 1) <= kInlineCheck;
+  return p;
+}
+
+bool empty(const fa_decode_args& a) { return a.batch <= 0 || a.seqlen_q <= 0 || a.heads_q <= 0 || a.heads_kv <= 0; }
+
+// host: word for the checks or null; *queued is set once a kernel that writes it is on the stream.
+int run(const fa_decode_args& args, const fa_cache8& c, const Plan& plan, uint32_t* host, bool* queued, cudaStream_t st) {
+  fa_decode_args a = args;
+  char* ws = static_cast<char*>(a.workspace);
+  uint32_t* word = reinterpret_cast<uint32_t*>(ws + plan.word_at());
+  if (plan.counters && a.counters == nullptr) {
+    a.counters = reinterpret_cast<uint32_t*>(ws + aligned(plan.piece_bytes));
+    const cudaError_t e = cudaMemsetAsync(a.counters, 0, plan.counter_bytes, st);
+    if (e != cudaSuccess) {
+      set_error("decode8: cudaMemsetAsync: %s", cudaGetErrorString(e));
+      return FA_ERR_LAUNCH;
+    }
+  }
+  const bool check = host != nullptr, first = check && !plan.inside;
+  if (first) {
+    if (int r = launch_decode_check(a, host, word, st)) return r;
+    *queued = true;
+  }
+  if (plan.append) {
+    const bool here = check && plan.inside;
+    if (int r = append8_launch(append_of(a, c), &a, a.dtype, c.code, a.device, here ? host : nullptr, check ? word : nullptr, here, st)) return r;
+    if (here) *queued = true;
+  }
+  const bool behind = plan.append || first;
+  const DecodeCheck chk = {check && plan.inside && !plan.append ? host : nullptr, check && behind ? word : nullptr};
+  const ScoreCfg cfg = make_score_cfg(a.softmax_scale, 0.f, a.causal, a.window_left, a.window_right, a.alibi_slopes != nullptr);
+  const int r = c.code == FA_CODE_INT8 ? decode8_int8(a, c, cfg, plan.unit_rows, plan.geo, chk, behind, st)
+                                       : decode8_e4m3(a, c, cfg, plan.unit_rows, plan.geo, chk, behind, st);
+  if (check && r == FA_OK) *queued = true;
+  return r;
+}
+
+int refused(const fa_decode_args& a, const Plan& plan) {
+  if (a.workspace == nullptr || a.workspace_bytes < plan.bytes()) {
+    set_error("decode8 workspace too small: need %zu bytes, got %zu", plan.bytes(), a.workspace_bytes);
+    return FA_ERR_WORKSPACE;
+  }
+  FA_REQUIRE(a.counters == nullptr || a.num_counters >= plan.counters, "decode8: too few counters");
+  return FA_OK;
+}
+
+}  // namespace
+
+size_t decode8_workspace_bytes(const fa_decode_args& a) { return empty(a) ? 0 : plan_of(a).bytes(); }
+int decode8_counters(const fa_decode_args& a) { return empty(a) ? 0 : plan_of(a).counters; }
+
+int decode8_paged(const fa_decode_args& a, const fa_cache8& c, cudaStream_t st) {
+  if (empty(a)) return FA_OK;
+  const Plan plan = plan_of(a);
+  if (int r = refused(a, plan)) return r;
+  return run(a, c, plan, nullptr, nullptr, st);
+}
+
+int decode8_paged_checked(const fa_decode_args& a, const fa_cache8& c, uint32_t* failed, cudaStream_t st) {
+  *failed = 0;
+  if (empty(a)) return FA_OK;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    set_error("value checks cannot run while the stream is being captured; turn them off with set_validation(False)");
+    return FA_ERR_LAUNCH;
+  }
+  const Plan plan = plan_of(a);
+  if (int r = refused(a, plan)) return r;
+  uint32_t* host = nullptr;
+  const int slot = take_check_word(false, a.device, &host);
+  if (slot < 0) return FA_ERR_LAUNCH;
+  bool queued = false;
+  int r = run(a, c, plan, host, &queued, st);
+  if (queued) {
+    const int w = await_check_word(slot, failed, st);
+    if (r == FA_OK) r = w;
+  }
+  give_check_word(slot, queued);
+  return r;
+}
+
+}  // namespace fa

@@ -56,6 +56,15 @@ struct Abi {
   int32_t (*decode_counters)(const fa_decode_args*);
   size_t (*decode_workspace)(const fa_decode_args*);
   size_t (*decode_checked_workspace)(const fa_decode_args*);
+  int (*decode8)(const fa_decode_args*, const fa_cache8*, void*);
+  int (*decode8_checked)(const fa_decode_args*, const fa_cache8*, uint32_t*, void*);
+  size_t (*decode8_workspace)(const fa_decode_args*, const fa_cache8*);
+  int32_t (*decode8_counters)(const fa_decode_args*, const fa_cache8*);
+  int (*append8)(const fa_append8_args*, void*);
+  int (*append8_checked)(const fa_append8_args*, uint32_t*, void*);
+  size_t (*append8_workspace)(const fa_append8_args*);
+  int (*block_table)(const fa_block_table_args*, void*);
+  int (*block_table_checked)(const fa_block_table_args*, uint32_t*, void*);
   PyObject* check;   // _native.check(status, what): raises the Python exception of a status
 };
 Abi g_abi = {};
@@ -718,8 +727,23 @@ Tensor decode_counters(const at::Device& dev, cudaStream_t stream) {
   return pool->front().words;
 }
 
+// The scales of an 8-bit cache (pages, blocks of a page, heads), whose codes are in `cache`.
+fa_cache8 cache8_of(const Tensor& cache, const Tensor& k_scale, const Tensor& v_scale) {
+  fa_cache8 c;
+  memset(&c, 0, sizeof(c));
+  c.code = cache.scalar_type() == at::kChar ? FA_CODE_INT8 : FA_CODE_E4M3;
+  c.block = (int)(cache.size(1) / k_scale.size(1));
+  c.k_scale = static_cast<float*>(k_scale.data_ptr());
+  c.v_scale = static_cast<float*>(v_scale.data_ptr());
+  for (int i = 0; i < 3; ++i) {
+    c.ks_stride[i] = k_scale.stride(i);
+    c.vs_stride[i] = v_scale.stride(i);
+  }
+  return c;
+}
+
 // kvcache(q, k_cache, v_cache, k_new, v_new, cos, sin, seqlens, batch_idx, leftpad, block_table, scale, causal, wl, wr,
-//         interleaved, alibi, num_splits, checks) -> out, or the mask of the value checks that failed
+//         interleaved, alibi, num_splits, checks, k_scale, v_scale) -> out, or the mask of the value checks that failed
 PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a{args, n};
@@ -736,6 +760,7 @@ PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor alibi = a.tensor_or_none();
   p.num_splits = (int)a.integer();
   const bool checks = a.truth();
+  Tensor k_scale = a.tensor_or_none(), v_scale = a.tensor_or_none();
 
   c10::cuda::CUDAGuard guard(q.device());
   at::AutoDispatchBelowADInplaceOrView below;
@@ -775,12 +800,15 @@ PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   if (alibi.defined()) p.alibi_slopes = alibi.const_data_ptr<float>();
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const bool coded = k_scale.defined();
+  fa_cache8 c8;
+  if (coded) c8 = cache8_of(kc, k_scale, v_scale);
   Tensor ws, ctr;
-  if (const size_t need = checks ? g_abi.decode_checked_workspace(&p) : g_abi.decode_workspace(&p)) {
+  if (const size_t need = coded ? g_abi.decode8_workspace(&p, &c8) : checks ? g_abi.decode_checked_workspace(&p) : g_abi.decode_workspace(&p)) {
     ws = empty_cuda({(int64_t)need}, at::kByte, dev);
     p.workspace = ws.data_ptr();
     p.workspace_bytes = need;
-    const int words = g_abi.decode_counters(&p);
+    const int words = coded ? g_abi.decode8_counters(&p, &c8) : g_abi.decode_counters(&p);
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     if (words <= kCounterWords && cudaStreamIsCapturing(st, &cap) == cudaSuccess) {
       // a captured call keeps counters of its own, zeroed inside the graph
@@ -794,13 +822,108 @@ PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   int status;
   if (checks) {
     pybind11::gil_scoped_release nogil;
-    status = g_abi.decode_checked(&p, &failed, st);
+    status = coded ? g_abi.decode8_checked(&p, &c8, &failed, st) : g_abi.decode_checked(&p, &failed, st);
   } else {
-    status = g_abi.decode(&p, st);
+    status = coded ? g_abi.decode8(&p, &c8, st) : g_abi.decode(&p, st);
   }
-  check(status, "fa_decode_paged");
+  check(status, coded ? "fa_decode_paged8" : "fa_decode_paged");
   if (failed) return PyLong_FromUnsignedLong(failed);
   return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// append8(k, v, k_cache, v_cache, slots, k_scale, v_scale, checks) -> the mask of the value checks that failed
+PyObject* py_append8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  Tensor k = a.tensor(), v = a.tensor(), kc = a.tensor(), vc = a.tensor(), slots = a.tensor(), k_scale = a.tensor(), v_scale = a.tensor();
+  const bool checks = a.truth();
+  c10::cuda::CUDAGuard guard(k.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto dev = k.device();
+  k = prep(k);
+  v = prep(v);
+  fa_append8_args p;
+  memset(&p, 0, sizeof(p));
+  p.dtype = k.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_F16;
+  p.device = dev.index();
+  p.tokens = k.size(0); p.heads = (int)k.size(1); p.head_dim = (int)k.size(2);
+  p.k = k.data_ptr(); p.v = v.data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    p.k_stride[i] = k.stride(i);
+    p.v_stride[i] = v.stride(i);
+  }
+  const View vkc = view_of(kc, kBSHD, -1, 0), vvc = view_of(vc, kBSHD, -1, 0);
+  p.k_cache = vkc.p; p.v_cache = vvc.p;
+  set_strides(p.kc_stride, vkc); set_strides(p.vc_stride, vvc);
+  p.page_size = (int)vkc.rows; p.num_pages = (int)vkc.batch;
+  p.slots = slots.const_data_ptr<int64_t>();
+  p.cache = cache8_of(kc, k_scale, v_scale);
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  uint32_t failed = 0;
+  int status;
+  Tensor ws;
+  if (checks) {
+    const size_t need = g_abi.append8_workspace(&p);
+    if (need) {
+      ws = empty_cuda({(int64_t)need}, at::kByte, dev);
+      p.workspace = ws.data_ptr();
+      p.workspace_bytes = need;
+    }
+    pybind11::gil_scoped_release nogil;
+    status = g_abi.append8_checked(&p, &failed, st);
+  } else {
+    status = g_abi.append8(&p, st);
+  }
+  check(status, "fa_append8");
+  return PyLong_FromUnsignedLong(failed);
+  END_HANDLE_TH_ERRORS
+}
+
+// block_table(cache_seqlens, new_lens, free_pages, block_table, page_size, num_slots, checks)
+//   -> (slots, cu_seqlens, pages_used), or the mask of the value checks that failed
+PyObject* py_block_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  Tensor seqlens = a.tensor(), fresh = a.tensor(), free_pages = a.tensor(), table = a.tensor();
+  fa_block_table_args p;
+  memset(&p, 0, sizeof(p));
+  p.page_size = (int)a.integer();
+  p.num_slots = a.integer();
+  const bool checks = a.truth();
+  c10::cuda::CUDAGuard guard(table.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto dev = table.device();
+  p.device = dev.index();
+  p.batch = (int)table.size(0);
+  p.cache_seqlens = seqlens.const_data_ptr<int32_t>();
+  p.new_lens = fresh.const_data_ptr<int32_t>();
+  p.free_pages = free_pages.const_data_ptr<int32_t>();
+  p.num_free = free_pages.numel();
+  p.block_table = table.data_ptr<int32_t>();
+  p.table_stride = table.stride(0);
+  p.table_pages = (int)table.size(1);
+  Tensor slots = empty_cuda({p.num_slots}, at::kLong, dev), cu = empty_cuda({p.batch + 1}, at::kInt, dev), used = empty_cuda({}, at::kInt, dev);
+  p.slots = slots.data_ptr<int64_t>();
+  p.cu_seqlens = cu.data_ptr<int32_t>();
+  p.pages_used = used.data_ptr<int32_t>();
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  uint32_t failed = 0;
+  int status;
+  if (checks) {
+    pybind11::gil_scoped_release nogil;
+    status = g_abi.block_table_checked(&p, &failed, st);
+  } else {
+    status = g_abi.block_table(&p, st);
+  }
+  check(status, "fa_block_table");
+  if (failed) return PyLong_FromUnsignedLong(failed);
+  PyObject* out = PyTuple_New(3);
+  if (out == nullptr) throw python_error();
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(slots));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(cu));
+  PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(used));
+  return out;
   END_HANDLE_TH_ERRORS
 }
 
@@ -840,6 +963,15 @@ PyObject* py_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_abi.decode_counters = (decltype(g_abi.decode_counters))get("fa_decode_counters");
   g_abi.decode_workspace = (decltype(g_abi.decode_workspace))get("fa_decode_workspace_bytes");
   g_abi.decode_checked_workspace = (decltype(g_abi.decode_checked_workspace))get("fa_decode_checked_workspace_bytes");
+  g_abi.decode8 = (decltype(g_abi.decode8))get("fa_decode_paged8");
+  g_abi.decode8_checked = (decltype(g_abi.decode8_checked))get("fa_decode_paged8_checked");
+  g_abi.decode8_workspace = (decltype(g_abi.decode8_workspace))get("fa_decode8_workspace_bytes");
+  g_abi.decode8_counters = (decltype(g_abi.decode8_counters))get("fa_decode8_counters");
+  g_abi.append8 = (decltype(g_abi.append8))get("fa_append8");
+  g_abi.append8_checked = (decltype(g_abi.append8_checked))get("fa_append8_checked");
+  g_abi.append8_workspace = (decltype(g_abi.append8_workspace))get("fa_append8_workspace_bytes");
+  g_abi.block_table = (decltype(g_abi.block_table))get("fa_block_table");
+  g_abi.block_table_checked = (decltype(g_abi.block_table_checked))get("fa_block_table_checked");
   Py_INCREF(chk);
   Py_XDECREF(g_abi.check);
   g_abi.check = chk;
@@ -855,6 +987,8 @@ PyMethodDef g_methods[] = {
     {"varlen_check", FAST(py_varlen_check), "value checks of a packed call"},
     {"backward", FAST(py_backward), "gradients from a forward's output and LSE"},
     {"kvcache", FAST(py_kvcache), "append to a KV cache and attend to it"},
+    {"append8", FAST(py_append8), "packed tokens into an 8-bit KV cache"},
+    {"block_table", FAST(py_block_table), "pages, slots and cu_seqlens of a step"},
     {"int8", FAST(py_int8), "INT8 scores forward"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fa_host", "host path of the attention kernels", -1, g_methods};

@@ -257,11 +257,111 @@ def _as_i32(x, device):
     return torch.as_tensor(x, device=device).to(torch.int32).flatten().contiguous()
 
 
+_CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
+
+
+def _check_coded_cache(k_cache, v_cache, k_scale, v_scale):
+    """An 8-bit cache (pages, page_size, heads, dim) and its scales (pages, blocks, heads); the caches have the same shape."""
+    if k_cache.dtype not in _CODE_DTYPES or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_scale and v_scale go with KV caches that are both torch.int8 or both torch.float8_e4m3fn")
+    if k_scale is None or v_scale is None:
+        raise ValueError("KV caches in 8 bits need k_scale and v_scale")
+    pages, page_size, heads, _ = k_cache.shape
+    for scale in (k_scale, v_scale):
+        if scale.dtype != torch.float32 or scale.device != k_cache.device:
+            raise ValueError("k_scale and v_scale must be float32 tensors on the device of the caches")
+        if scale.ndim != 3 or scale.shape[0] != pages or scale.shape[2] != heads or scale.shape != k_scale.shape:
+            raise ValueError("k_scale and v_scale must have shape (pages, blocks, nheads_k)")
+    blocks = k_scale.shape[1]
+    if blocks == 0 or page_size % blocks or not 1 <= page_size // blocks <= 1024:
+        raise ValueError("the blocks of k_scale and v_scale must divide a page into equal parts of 1 to 1024 tokens")
+    if not (N.codes_ready(k_cache) and N.codes_ready(v_cache)):
+        raise ValueError("KV caches must have a unit head-dim stride and 16-byte aligned rows")
+
+
+def kvcache_append(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale):
+    """Write packed new tokens into an 8-bit KV cache, in place.
+
+    k, v (tokens, nheads_k, d) fp16 or bf16; caches (num_pages, page_size, nheads_k, d) torch.int8 or torch.float8_e4m3fn
+    with scales (num_pages, blocks, nheads_k) fp32, as in flash_attn_with_kvcache; slot_mapping (tokens,) integers:
+    token i goes to row slot % page_size of page slot // page_size, a negative slot (padding) nowhere.  build_block_table
+    makes such slots.
+
+    Blocks fill from their first row on: the rows of a block before the first one that a call writes are tokens that it keeps, and
+    a call that writes its first row starts the block's scale afresh.  The scale is the largest magnitude of the
+    block so far over 127 (int8) or 448 (e4m3); where new tokens raise it, the codes of the tokens that stay are rounded again.
+    A NaN or infinity among the tokens of a block goes to its scale.  The tokens that a call brings for one block
+    follow one another, in the order of their slots.
+
+    With value checks on, a slot behind the cache or a block that is written in two places raises ValueError and
+    nothing is written; off (see set_validation), such slots are passed over, and such a block has the codes of either."""
+    if k.ndim != 3 or v.shape != k.shape:
+        raise ValueError("k and v must have shape (tokens, nheads_k, headdim)")
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape (num_pages, page_size, nheads_k, headdim)")
+    if not (k.is_cuda and v.is_cuda and k_cache.is_cuda and v_cache.is_cuda):
+        raise ValueError("All tensors must be CUDA tensors")
+    if k.device != v.device or k.device != k_cache.device or k.device != v_cache.device:
+        raise ValueError("k, v and the KV caches must be on the same device")
+    if k.dtype not in _KERNEL_DTYPES or v.dtype != k.dtype:
+        raise ValueError("kvcache_append supports matching FP16 or BF16 tensors")
+    if k.shape[1:] != k_cache.shape[2:]:
+        raise ValueError("new k/v tensors are incompatible with the cache")
+    _check_head_dim(k.shape[2])
+    if k.shape[1] == 0:
+        raise ValueError("new k/v tensors need at least one head")
+    _check_coded_cache(k_cache, v_cache, k_scale, v_scale)
+    if slot_mapping.ndim != 1 or slot_mapping.shape[0] != k.shape[0] or slot_mapping.dtype not in (torch.int32, torch.int64):
+        raise ValueError("slot_mapping must hold one integer slot per token")
+    slots = slot_mapping.to(device=k.device, dtype=torch.int64).contiguous()
+    failed = N.host().append8(k, v, k_cache, v_cache, slots, k_scale, v_scale, _VALIDATE)
+    if failed:
+        raise ValueError(("slot_mapping contains a slot behind the cache",
+                          "slot_mapping returns to a block: its tokens must follow one another")[(failed & -failed).bit_length() - 1])
+
+
+def build_block_table(cache_seqlens, new_lens, free_pages, block_table, page_size, num_tokens):
+    """Pages and slots for the new tokens of a step, on the GPU: request b has cache_seqlens[b] tokens in the cache and gets
+    new_lens[b] more (0 is allowed).
+
+    Pages are taken from free_pages in order and entered into block_table (batch, max_pages) int32, in place: entries
+    [ceil(old / page_size), ceil((old + new) / page_size)) of each row; the others stay.  Returns
+      slot_mapping (num_tokens,) int64   slots of the new tokens, request by request, -1 behind the last one
+      cu_seqlens (batch + 1,) int32      where the new tokens of each request begin
+      pages_used () int32                how many of free_pages were taken
+    num_tokens is a number that the host knows to be enough, so that the call does not wait for the lengths; what comes after
+    (kvcache_append, a captured graph of a fixed size) passes over the slots of -1.
+
+    With value checks on, lengths that do not fit raise ValueError; off (see set_validation), they leave the table as it was,
+    all slots -1 and pages_used -1."""
+    if block_table.ndim != 2 or block_table.dtype != torch.int32 or not block_table.is_cuda:
+        raise ValueError("block_table must be a CUDA tensor (batch, max_num_pages) of int32")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table must have rows of unit stride")
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("the rows of block_table must not overlap")
+    page_size, num_tokens = int(page_size), int(num_tokens)
+    if not 0 < page_size < 2 ** 31:
+        raise ValueError("page_size must be positive")
+    if not 0 <= num_tokens < 2 ** 31:
+        raise ValueError("num_tokens must be non-negative and below 2 ** 31")
+    device = block_table.device
+    old, new, free = (_as_i32(x, device) for x in (cache_seqlens, new_lens, free_pages))
+    if old.numel() != block_table.shape[0] or new.numel() != block_table.shape[0]:
+        raise ValueError("cache_seqlens and new_lens must contain one length per row of block_table")
+    made = N.host().block_table(old, new, free, block_table, page_size, num_tokens, _VALIDATE)
+    if isinstance(made, int):
+        raise ValueError(("cache_seqlens and new_lens must not be negative", "the new tokens exceed num_tokens",
+                          "free_pages has too few pages for the new tokens",
+                          "a request exceeds its row of block_table")[(made & -made).bit_length() - 1])
+    return made
+
+
 def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None, rotary_sin=None,
                             cache_seqlens=None, cache_batch_idx=None, cache_leftpad=None,
                             block_table=None, softmax_scale=None, causal=False,
                             window_size=(-1, -1), rotary_interleaved=True, alibi_slopes=None,
-                            num_splits=0):
+                            num_splits=0, k_scale=None, v_scale=None):
     """Attention against a KV cache, optionally appending new k/v first (in place) with
     rotary embedding applied to the new keys and to q.
 
@@ -272,6 +372,12 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     last seqlen_q positions of the sequence after the append; causal, window and ALiBi are
     measured from there (also without `causal`: the reference only shifts the causal mask,
     flash_attn_interface.py:523).  `num_splits` (0 = automatic) is an extra tuning knob.
+
+    A cache may be held in 8 bits: k_cache and v_cache are then torch.int8 or torch.float8_e4m3fn codes of the same
+    shapes, and k_scale, v_scale fp32 tensors (batch_cache or num_pages, blocks, nheads_k) with one scale per head and
+    block of capacity / blocks (page_size / blocks) consecutive tokens, at most 1024; a value is code * scale.  q, k
+    and v stay 16-bit.  New tokens are quantised as `kvcache_append` does it, and the attention is to what the cache
+    then holds.
 
     With value checks on (the default) the kernel makes them first (page indices in range, lengths
     fit the cache and the rotary tables) and the call waits for that one flag, not for the attention;
@@ -306,14 +412,17 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         raise ValueError("q and KV cache dimensions are incompatible")
     if dev != k_cache.device or dev != v_cache.device:
         raise ValueError("q and KV caches must be on the same device")
-    if dtype != k_cache.dtype or dtype != v_cache.dtype:
+    coded = k_cache.dtype in _CODE_DTYPES
+    if coded or k_scale is not None or v_scale is not None:
+        _check_coded_cache(k_cache, v_cache, k_scale, v_scale)
+    elif dtype != k_cache.dtype or dtype != v_cache.dtype:
         raise ValueError("q and KV caches must have the same dtype")
     if dtype not in _KERNEL_DTYPES:
         raise ValueError("flash_attn_with_kvcache supports FP16 and BF16 tensors")
     _check_head_dim(head_dim)
     if heads_kv == 0 or heads_q % heads_kv != 0:
         raise ValueError("The number of query heads must be divisible by KV heads")
-    if not (N.kernel_ready(k_cache) and N.kernel_ready(v_cache)):
+    if not coded and not (N.kernel_ready(k_cache) and N.kernel_ready(v_cache)):
         raise ValueError("KV caches must have a unit head-dim stride and 16-byte aligned rows")
     rows = None
     if cache_batch_idx is not None:
@@ -361,7 +470,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(head_dim)
     out = N.host().kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, lengths, rows, pads, block_table, softmax_scale,
-                           causal, window_size[0], window_size[1], rotary_interleaved, alibi, num_splits, _VALIDATE)
+                           causal, window_size[0], window_size[1], rotary_interleaved, alibi, num_splits, _VALIDATE, k_scale, v_scale)
     if isinstance(out, int):
         raise ValueError(_cache_value_errors(lengths_error)[(out & -out).bit_length() - 1])
     return out

@@ -294,6 +294,96 @@ int fa_decode_paged_static(const fa_decode_args* args, void* stream);
 size_t fa_decode_static_scratch_bytes(void);
 
 /*
+ * KV cache in 8 bits.  A cache holds codes (pages, page_size, heads_kv, head_dim) of one byte, rows 16-byte aligned, and one fp32
+ * scale per block of `block` consecutive tokens (it divides page_size) and head; a value is code * scale.
+ *
+ * Appending to a block: with `kept` tokens of the sequence already in it, its scale s and the new tokens' largest magnitude a,
+ *   need = a / Q  (Q = 127 or 448; below the smallest normal number: 0),  s' = max(kept ? s : 0, need),  inv = s' > 0 ? 1 / s' : 0
+ *   new codes  rn(x * inv);   kept codes, where s' > s,  rn(code * (s * inv));   all in IEEE fp32, rounded half to even.
+ * A NaN or an infinity among the new tokens goes to the scale, so that the values of that block and head are NaN or infinite until the
+ * block is started again.
+ *
+ * fa_decode_paged8: fa_decode_paged on such a cache; the call's cache pointers are the codes', its cache strides are in codes.  The
+ * new tokens are appended first, and the attention is to what the cache then holds.  dtype is q's, the new tokens' and o's.
+ * Workspace and counters: fa_decode8_workspace_bytes(), fa_decode8_counters().
+ */
+typedef enum fa_code { FA_CODE_INT8 = 0, FA_CODE_E4M3 = 1 } fa_code;
+typedef struct fa_cache8 {
+  int32_t code, block; /* block: 1 to 1024 tokens */
+  float* k_scale;
+  float* v_scale;
+  int64_t ks_stride[3], vs_stride[3]; /* (page, block of the page, head) */
+} fa_cache8;
+
+int fa_decode_paged8(const fa_decode_args* args, const fa_cache8* cache, void* stream);
+/* With the value checks of fa_decode_paged_checked. */
+int fa_decode_paged8_checked(const fa_decode_args* args, const fa_cache8* cache, uint32_t* failed, void* stream);
+size_t fa_decode8_workspace_bytes(const fa_decode_args* args, const fa_cache8* cache);
+int32_t fa_decode8_counters(const fa_decode_args* args, const fa_cache8* cache);
+
+/*
+ * Packed new tokens into an 8-bit cache by slot: token i goes to row slots[i] % page_size of page slots[i] / page_size; a negative
+ * slot, or one outside the cache, is passed over.  The tokens of one block follow one another in the call and in the block, and the
+ * block's rows before the first of them are taken for tokens that it keeps.
+ */
+typedef struct fa_append8_args {
+  int32_t dtype, device; /* of k and v */
+  int32_t heads, head_dim;
+  int64_t tokens;
+  const void* k;
+  const void* v;
+  int64_t k_stride[2], v_stride[2]; /* (token, head) */
+  void* k_cache;
+  void* v_cache;
+  int64_t kc_stride[3], vc_stride[3]; /* (page, row, head) */
+  int32_t page_size, num_pages;
+  const int64_t* slots;
+  fa_cache8 cache;
+  void* workspace; /* fa_append8_checked only: fa_append8_workspace_bytes() */
+  size_t workspace_bytes;
+} fa_append8_args;
+typedef enum fa_append8_check {
+  FA_SLOT_RANGE = 1, /* no slot lies behind the cache */
+  FA_SLOT_TWICE = 2  /* the tokens of every block follow one another */
+} fa_append8_check;
+int fa_append8(const fa_append8_args* args, void* stream);
+/* With value checks: `failed` receives those that did not hold; if any did not, nothing was written.  Returns as soon as the checks
+ * have run, while the tokens may still be on their way.  Not for streams under capture. */
+int fa_append8_checked(const fa_append8_args* args, uint32_t* failed, void* stream);
+size_t fa_append8_workspace_bytes(const fa_append8_args* args);
+
+/*
+ * Pages, slots and cu_seqlens of a step: request b holds cache_seqlens[b] tokens and gets new_lens[b] more.  Pages for them are taken
+ * from free_pages in order; entries [ceil(old / page), ceil((old + new) / page)) of its row of block_table are written, others stay.
+ *   slots[i]      slot of new token i (the tokens of the requests one after another); -1 for i from the last one on
+ *   cu_seqlens    (batch + 1) exclusive sums of new_lens;  pages_used[0]: pages taken
+ * A step that fails a check below changes no table: slots are -1, pages_used is -1, cu_seqlens zero.
+ */
+typedef struct fa_block_table_args {
+  int32_t device, batch, page_size;
+  const int32_t* cache_seqlens;
+  const int32_t* new_lens;
+  const int32_t* free_pages;
+  int64_t num_free;
+  int32_t* block_table;
+  int64_t table_stride; /* of a row */
+  int32_t table_pages;  /* entries of a row */
+  int64_t num_slots;
+  int64_t* slots;
+  int32_t* cu_seqlens;
+  int32_t* pages_used;
+} fa_block_table_args;
+typedef enum fa_block_table_check {
+  FA_TABLE_LENGTHS = 1, /* no length is negative */
+  FA_TABLE_SLOTS = 2,   /* the new tokens fit num_slots */
+  FA_TABLE_FREE = 4,    /* there are pages enough */
+  FA_TABLE_ROW = 8      /* every request fits its row of the table */
+} fa_block_table_check;
+int fa_block_table(const fa_block_table_args* args, void* stream);
+/* Waits for the checks (not for the tables); not for streams under capture. */
+int fa_block_table_checked(const fa_block_table_args* args, uint32_t* failed, void* stream);
+
+/*
  * Per-key-token INT8 quantisation: k (rows, head_dim) fp16 contiguous ->
  * k8 (rows, head_dim) int8, s_k (rows) fp32, with
  *   s = max(absmax, 1)/127;  code = round_half_away(k * (1/s))  in IEEE fp32,
@@ -416,7 +506,8 @@ int fa_debug_set_wait_status(int32_t device, int32_t code);
 int fa_mma_peak_probe(int32_t device, int32_t kind, int32_t iters, void* stream);
 /* sizeof of an argument block as this library was compiled: 0 = fa_attn_args,
  * 1 = fa_decode_args, 2 = fa_int8_args.  Lets a foreign-language binding check its
- * struct layout before the first call.  3 = fa_rotary_args. */
+ * struct layout before the first call.  3 = fa_rotary_args, 4 = fa_cache8, 5 = fa_append8_args,
+ * 6 = fa_block_table_args. */
 size_t fa_sizeof_args(int which);
 
 #ifdef __cplusplus
