@@ -8,7 +8,7 @@ namespace fa {
 
 int decode8_int8(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
 int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
-int decode8_resident(int head_dim, int unit_rows);
+DecodeGeom decode8_geometry(const fa_decode_args& a, int unit_rows, int row_groups);
 int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st);
 
 namespace {
@@ -34,7 +34,7 @@ Plan plan_of(const fa_decode_args& a) {
   p.unit_rows = unit_rows_of(a);
   const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
   const int groups = (int)((rows + p.unit_rows - 1) / p.unit_rows);
-  p.geo = decode_geometry(a, groups, decode8_resident(a.head_dim, p.unit_rows));
+  p.geo = decode8_geometry(a, p.unit_rows, groups);
   p.piece_bytes = p.geo.splits == 1 ? 0 : (size_t)p.geo.shares * a.seqlen_q * a.heads_q * (a.head_dim + 1) * sizeof(float);
   p.counters = p.piece_bytes ? a.batch * a.heads_kv * groups : 0;
   p.counter_bytes = a.counters ? 0 : (size_t)p.counters * sizeof(uint32_t);

@@ -4,17 +4,19 @@
 
 namespace fa {
 
-// Every code of either kind is a 16-bit float exactly: integers up to 127, or 4 significant bits from 2^-9 to 448.  (The products are
+// Every code of either kind is a 16-bit float exactly: whole numbers up to 255, or 4 significant bits from 2^-9 to 448.  (The products are
 // therefore taken in fp16 whatever the type of the queries; bf16 queries are brought into its range by a power of two.)
 template <int kCode> struct Code;
 
 template <> struct Code<FA_CODE_INT8> {
   static constexpr float kLargest = 127.f;
-  // 0x6400 | u is 1024 + u in fp16 (u = code + 128): one byte permutation and one subtraction per pair
+  // A byte in the low half of a 16-bit float is u * 2^-24 (u = code + 128): one byte permutation per pair.  The products are then
+  // 2^-24 of the true ones and too large by those with kBias.
+  static constexpr float kUnit = 0x1p-24f;
+  static constexpr uint32_t kBias = 0x00800080u;
   static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t sel) {
     uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0x64646464u), "r"(sel));
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sel));
     return r;
   }
   // bytes (0, 1) and (2, 3) of x as pairs
@@ -44,6 +46,8 @@ template <> struct Code<FA_CODE_INT8> {
 
 template <> struct Code<FA_CODE_E4M3> {
   static constexpr float kLargest = 448.f;
+  static constexpr float kUnit = 1.f;
+  static constexpr uint32_t kBias = 0u;
   static __device__ __forceinline__ uint32_t pair(uint16_t x) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(x));

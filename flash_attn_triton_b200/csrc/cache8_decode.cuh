@@ -11,7 +11,9 @@
 //   the 4 neighbouring codes that it is given as columns (2t, 2t+1, 2t+8, 2t+9) and the queries are arranged to match.  For V the
 //   transposing form gives a lane 2 dims of 2 keys; one byte permutation sorts them by dim, and rows g and g + 8 of the product are dims
 //   2g and 2g + 1.
-//   Scales travel with their tile: 32 words per warp and stage by 4-byte cp.async.
+//   int8 codes go to the tensor cores as (code + 128) * 2^-24, which is a byte permutation; what the 128 adds is the same for all keys of
+//   a row in the scores, where the accumulators start from its negative, and a product with a constant in the outputs.
+//   Scales travel with their tile, by 4-byte cp.async.
 //   Bound.  HBM: one byte per code.
 #pragma once
 #include <atomic>
@@ -25,31 +27,48 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int byt
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
+}
+
 template <int D, int kRows> struct Decode8 {
-  static constexpr int P = D == 16 ? 16 : D + 16;      // bytes of a staged row: 8 rows of ldmatrix meet 8 bank groups
-  static constexpr int NS = 3, QP = D + 8, OP = D + 4;
-  static constexpr size_t ring = (size_t)2 * NS * kTile * P;
-  static constexpr size_t scales = (size_t)NS * 4 * 32 * 4;
+  static constexpr int kKeys = D == 256 ? 16 : 32;     // of a warp's tile
+  static constexpr int kTile8 = 4 * kKeys;
+  static constexpr int P = D;                          // bytes of a staged row
+  static constexpr int NS = D == 128 && kRows == 8 ? 2 : 3, QP = D + 8, OP = D + 4;
+  static constexpr size_t ring = (size_t)2 * NS * kTile8 * P;
+  static constexpr size_t scales = (size_t)NS * 4 * 2 * kKeys * 4;
+  // Query fragments stay in registers, their rows pass through the last stage of the ring (two CTAs per SM would not fit otherwise); where
+  // there are too many, they are read again for each tile.
+  static constexpr bool kQueriesHeld = D * kRows < 4096;
   static constexpr size_t q_bytes = (size_t)kRows * QP * 2;
-  static constexpr size_t smem = ring + scales + q_bytes + 4 * kRows * 2 * 4;
+  static constexpr size_t q_at = kQueriesHeld ? ring / NS * (NS - 1) : ring + scales;
+  static constexpr size_t rows_at = ring + scales + (kQueriesHeld ? 0 : q_bytes);
+  static constexpr size_t smem = rows_at + 4 * kRows * 2 * 4;
   static_assert((size_t)4 * kRows * OP * 4 <= ring, "the warps' outputs, over the ring");
-  // CTAs per SM: accumulators and query fragments are D * kRows * 3 / 64 registers
-  static constexpr int kCtas = D * kRows <= 1024 ? 4 : D * kRows <= 2048 ? 3 : 2;
-  static constexpr int kResident = D == 256 ? 2 : kCtas;
+  static_assert(!kQueriesHeld || q_bytes <= ring / NS, "the queries, over a stage");
+  static constexpr int kResident = D <= 64 || (D == 128 && kRows == 8) ? 3 : 2;   // CTAs per SM
+  // 16-byte chunks of a row lie in another order, so that 8 rows of ldmatrix meet 8 bank groups: chunk c is at c ^ turn(row).
+  static constexpr int kChunks = D / 16;
+  static __device__ __forceinline__ int turn(int row) {
+    return kChunks >= 8 ? row & 7 : kChunks == 4 ? (row >> 1) & 3 : kChunks == 2 ? (row >> 2) & 1 : 0;
+  }
 };
+constexpr int kLongest8 = 32;          // tiles of the largest piece that is still run in one wave of CTAs
 
 // Sequence b after the append: keys the cache holds of it, positions of its tokens, the tiles that any query row sees.
 struct Seq8 {
   int keys, len, lo, nt;
 };
+template <int kTile8>
 __device__ __forceinline__ Seq8 seq8(const fa_decode_args& p, const ScoreCfg& cfg, int max_tiles, int b) {
   Seq8 s;
   const int cap = seq_capacity(p, b);
   s.len = max(0, min(p.cache_seqlens[b], cap)) + (p.k_new ? p.seqlen_new : 0);
   s.keys = min(s.len, cap);
   const int first = cfg.wl >= 0 ? min(max(0, s.len - p.seqlen_q - cfg.wl), s.keys) : 0;
-  s.lo = first / kTile;
-  s.nt = min(max(1, (s.keys + kTile - 1) / kTile - s.lo), max_tiles);
+  s.lo = first / kTile8;
+  s.nt = min(max(1, (s.keys + kTile8 - 1) / kTile8 - s.lo), max_tiles);
   return s;
 }
 
@@ -60,13 +79,14 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   using SM = Decode8<D, kRows>;
   using C = Code<kCode>;
   constexpr int P = SM::P, QP = SM::QP, NT = 128, NS = SM::NS, OP = SM::OP, NB = kRows / 8;
-  constexpr int CPR = D / 16, RPW = 32 / CPR, PASSES = RPW >= 16 ? 1 : 16 / RPW;     // a warp's loads: 16 rows of CPR 16-byte chunks
+  constexpr int KW = SM::kKeys, KB = KW / 16, kTile8 = SM::kTile8;
+  constexpr int CPR = D / 16, RPW = 32 / CPR < KW ? 32 / CPR : KW, PASSES = KW / RPW;  // a warp's loads: KW rows of CPR 16-byte chunks
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  unsigned char* ring = smem_raw;                // [stage][warp][K, V][16][P]
+  unsigned char* ring = smem_raw;                // [stage][warp][K, V][KW][P]
   float* sO = reinterpret_cast<float*>(smem_raw); // over the ring, when it is done with: 4 x kRows x OP
-  float* sS = reinterpret_cast<float*>(smem_raw + SM::ring);                       // [stage][warp][K, V][16]
-  __half* sQ = reinterpret_cast<__half*>(smem_raw + SM::ring + SM::scales);        // kRows x QP
-  float* sM = reinterpret_cast<float*>(smem_raw + SM::ring + SM::scales + SM::q_bytes); // 4 x kRows
+  float* sS = reinterpret_cast<float*>(smem_raw + SM::ring);                       // [stage][warp][K, V][KW]
+  __half* sQ = reinterpret_cast<__half*>(smem_raw + SM::q_at);                     // kRows x QP
+  float* sM = reinterpret_cast<float*>(smem_raw + SM::rows_at);                    // 4 x kRows
   float* sL = sM + 4 * kRows;                    // 4 x kRows
   __shared__ uint32_t sMost[4];
 
@@ -88,83 +108,104 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   // Behind the append or the checks (a programmatic launch): what the caller brought may be read before they are done, the cache and
   // their result may not.
   Piece piece;
-  const bool work = piece_of(geo, p.batch, share, U, lane, [&](int i) { return seq8(p, cfg, geo.max_tiles, i).nt; }, piece);
+  const bool work = piece_of<kLongest8>(geo, p.batch, share, U, lane, [&](int i) { return seq8<kTile8>(p, cfg, geo.max_tiles, i).nt; }, piece);
   if (behind) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!work || (chk.dev && *chk.dev)) return;
   const int b = piece.b, parts = piece.parts, base = piece.base, count = piece.count;
-  const Seq8 w = seq8(p, cfg, geo.max_tiles, b);
+  const Seq8 w = seq8<kTile8>(p, cfg, geo.max_tiles, b);
   const int len = w.len, keys = w.keys, tile0 = w.lo + piece.tile0;
 
   // ---- loading --------------------------------------------------------------------------
   const int lc = (lane % CPR) * 16, lr = lane / CPR;        // this lane's 16-byte column and first row
-  const bool one_page = p.block_table == nullptr || geo.page_shift >= 4;   // a warp's 16 keys lie inside one page
   const int pad = p.cache_leftpad ? max(0, p.cache_leftpad[b]) : 0;
   const int* table = p.block_table ? p.block_table + (int64_t)b * p.block_table_stride : nullptr;
-  int page = table ? 0 : (p.cache_batch_idx ? p.cache_batch_idx[b] : b);
+  const bool whole = table == nullptr || p.page_size % 16 == 0;       // 16 keys lie inside one page
+  int page[KB], row16[KB];                                  // of each 16 keys of the next tile
   int ld = tile0;                                           // next tile to load
   auto ld_page = [&]() {                                    // read one tile ahead of its use
-    if (table && one_page) {
-      const int key = ld * kTile + warp * 16;
-      if (key < keys) page = table[key >> geo.page_shift];
-    }
-  };
-  // page and row of a key
-  auto where = [&](int key, int& pg, int& row) {
-    if (one_page) {
-      pg = page;
-      row = table ? key & (p.page_size - 1) : key + pad;
-    } else {
-      const int pi = divided(key, p.page_size, geo.page_shift);
-      row = key - pi * p.page_size;
-      pg = table[pi];
+#pragma unroll
+    for (int h = 0; h < KB; ++h) {
+      const int key = ld * kTile8 + warp * KW + h * 16;
+      const int pi = table ? divided(key, p.page_size, geo.page_shift) : 0;
+      page[h] = table == nullptr ? (p.cache_batch_idx ? p.cache_batch_idx[b] : b) : key < keys ? table[pi] : 0;
+      row16[h] = table ? key - pi * p.page_size : key + pad;
     }
   };
   const unsigned char* kb = static_cast<const unsigned char*>(p.k_cache) + (int64_t)hk * p.kc_stride[2] + lc;
   const unsigned char* vb = static_cast<const unsigned char*>(p.v_cache) + (int64_t)hk * p.vc_stride[2] + lc;
-  // lanes 0-15: scales of K, lanes 16-31: of V
-  const float* sb = (lane < 16 ? c8.k_scale + (int64_t)hk * c8.ks_stride[2] : c8.v_scale + (int64_t)hk * c8.vs_stride[2]);
-  const int64_t sb_page = lane < 16 ? c8.ks_stride[0] : c8.vs_stride[0], sb_block = lane < 16 ? c8.ks_stride[1] : c8.vs_stride[1];
-  ld_page();
+  const float* ksb = c8.k_scale + (int64_t)hk * c8.ks_stride[2];
+  const float* vsb = c8.v_scale + (int64_t)hk * c8.vs_stride[2];
+  if (whole) ld_page();
   auto load_tile = [&](int st) {
     if (ld == tile0 + count) return;
-    const int key00 = ld * kTile + warp * 16;
-    {
-      const int key = key00 + (lane & 15);
-      const bool in = key < keys;
-      int pg = 0, row = 0;
-      if (in) where(key, pg, row);
-      cp_async4(smem_u32(sS + (st * 4 + warp) * 32 + lane), sb + pg * sb_page + divided(row, c8.block, block_shift) * sb_block, in ? 4 : 0);
-    }
-    if (RPW <= 16 || lr < 16) {
-      unsigned char* dK = ring + (size_t)((st * 4 + warp) * 2 * 16 + lr) * P + lc;
-      unsigned char* dV = dK + 16 * P;
-      const int key0 = key00 + lr;
-      if (one_page) {
-        int pg, row0;
-        where(key0, pg, row0);
-        const unsigned char* ks = kb + (int64_t)pg * p.kc_stride[0] + (int64_t)row0 * p.kc_stride[1];
-        const unsigned char* vs = vb + (int64_t)pg * p.vc_stride[0] + (int64_t)row0 * p.vc_stride[1];
-        const int64_t kstep = RPW * p.kc_stride[1], vstep = RPW * p.vc_stride[1];
+    const int key00 = ld * kTile8 + warp * KW;
+    // (row at + lr; at is a multiple of a power of two above lr)
+    const uint32_t dK = smem_u32(ring) + (uint32_t)((st * 4 + warp) * 2 * KW + lr) * P, dV = dK + KW * P;
+    auto column = [&](int at) { return (uint32_t)(lc ^ (SM::turn(lr) << 4) ^ (SM::turn(at) << 4)); };
+    float* dS = sS + (st * 4 + warp) * 2 * KW;
+    if (whole) {
+      if (KW == 32 || lane < KW) {
+        const int h = KB > 1 ? lane >> 4 : 0;
+        const int pg = KB > 1 && h ? page[KB - 1] : page[0], row = (KB > 1 && h ? row16[KB - 1] : row16[0]) + (lane & 15);
+        const int blk = divided(row, c8.block, block_shift), bytes = key00 + lane < keys ? 4 : 0;
+        cp_async4(smem_u32(dS + lane), bytes ? ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1] : ksb, bytes);
+        cp_async4(smem_u32(dS + KW + lane), bytes ? vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1] : vsb, bytes);
+      }
+      const bool all = key00 + KW <= keys;
+      if (RPW <= 16) {                 // a pass lies inside 16 keys
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          const int bytes = key0 + i * RPW < keys ? 16 : 0;      // rows past the last key are zero-filled
-          cp_async16(smem_u32(dK + i * RPW * P), bytes ? ks + i * kstep : kb, bytes);
-          cp_async16(smem_u32(dV + i * RPW * P), bytes ? vs + i * vstep : vb, bytes);
+        for (int h = 0; h < KB; ++h) {
+          const unsigned char* ks = kb + (int64_t)page[h] * p.kc_stride[0] + (int64_t)(row16[h] + lr) * p.kc_stride[1];
+          const unsigned char* vs = vb + (int64_t)page[h] * p.vc_stride[0] + (int64_t)(row16[h] + lr) * p.vc_stride[1];
+          const int64_t kstep = RPW * p.kc_stride[1], vstep = RPW * p.vc_stride[1];
+#pragma unroll
+          for (int i = 0; i < PASSES / KB; ++i) {
+            const int at = (h * (PASSES / KB) + i) * RPW;
+            if (all) {
+              cp_async16(dK + at * P + column(at), ks);
+              cp_async16(dV + at * P + column(at), vs);
+            } else {                   // rows past the last key are zero-filled
+              const int bytes = key00 + at + lr < keys ? 16 : 0;
+              cp_async16(dK + at * P + column(at), bytes ? ks : kb, bytes);
+              cp_async16(dV + at * P + column(at), bytes ? vs : vb, bytes);
+            }
+            ks += kstep;
+            vs += vstep;
+          }
         }
-      } else {
-#pragma unroll
+      } else if (lr < KW) {            // one pass takes them all
+        const bool up = KB > 1 && lr >= 16;
+        const int pg = up ? page[KB - 1] : page[0], row = (up ? row16[KB - 1] : row16[0]) + (lr & 15), bytes = key00 + lr < keys ? 16 : 0;
+        cp_async16(dK + column(0), bytes ? kb + (int64_t)pg * p.kc_stride[0] + (int64_t)row * p.kc_stride[1] : kb, bytes);
+        cp_async16(dV + column(0), bytes ? vb + (int64_t)pg * p.vc_stride[0] + (int64_t)row * p.vc_stride[1] : vb, bytes);
+      }
+    } else {                           // pages of any size: every row is looked up
+      auto where = [&](int key, int& pg, int& row) {
+        const int pi = divided(key, p.page_size, geo.page_shift);
+        row = key - pi * p.page_size;
+        pg = table[pi];
+      };
+      if (KW == 32 || lane < KW) {
+        int pg = 0, row = 0;
+        const int bytes = key00 + lane < keys ? 4 : 0;
+        if (bytes) where(key00 + lane, pg, row);
+        const int blk = divided(row, c8.block, block_shift);
+        cp_async4(smem_u32(dS + lane), ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1], bytes);
+        cp_async4(smem_u32(dS + KW + lane), vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1], bytes);
+      }
+      if (lr < KW) {
+#pragma unroll 1
         for (int i = 0; i < PASSES; ++i) {
-          const int key = key0 + i * RPW;
-          const int bytes = key < keys ? 16 : 0;
+          const int key = key00 + i * RPW + lr, bytes = key < keys ? 16 : 0;
           int pg = 0, row = 0;
           if (bytes) where(key, pg, row);
-          cp_async16(smem_u32(dK + i * RPW * P), kb + (int64_t)pg * p.kc_stride[0] + (int64_t)row * p.kc_stride[1], bytes);
-          cp_async16(smem_u32(dV + i * RPW * P), vb + (int64_t)pg * p.vc_stride[0] + (int64_t)row * p.vc_stride[1], bytes);
+          cp_async16(dK + i * RPW * P + column(i * RPW), kb + (int64_t)pg * p.kc_stride[0] + (int64_t)row * p.kc_stride[1], bytes);
+          cp_async16(dV + i * RPW * P + column(i * RPW), vb + (int64_t)pg * p.vc_stride[0] + (int64_t)row * p.vc_stride[1], bytes);
         }
       }
     }
     ++ld;
-    ld_page();
+    if (whole) ld_page();
   };
 
 #pragma unroll
@@ -231,15 +272,31 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
     }
   }
   __syncthreads();
-  uint32_t bq[NB][D / 16][2];
+  auto query = [&](int n, int kk) { return *reinterpret_cast<const uint2*>(sQ + (n * 8 + g) * QP + kk * 16 + 4 * t); };
+  uint2 bq[NB][SM::kQueriesHeld ? D / 16 : 1];
+  if (SM::kQueriesHeld) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) bq[n][SM::kQueriesHeld ? kk : 0] = query(n, kk);
+    }
+    __syncthreads();                             // the stage is free
+  }
+  // the scores of a tile start from what the bias of its codes adds to them
+  float s0[NB][2];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+    if (C::kBias) {
+      const uint32_t less = C::kBias | 0x80008000u, a[4] = {less, less, less, less};
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const uint2 x = *reinterpret_cast<const uint2*>(sQ + (n * 8 + g) * QP + kk * 16 + 4 * t);
-      bq[n][kk][0] = x.x;
-      bq[n][kk][1] = x.y;
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint2 x = SM::kQueriesHeld ? bq[n][SM::kQueriesHeld ? kk : 0] : query(n, kk);
+        mma16816<__half>(c, a, x.x, x.y);
+      }
     }
+    s0[n][0] = c[0];
+    s0[n][1] = c[1];
   }
   // this thread's score columns: query rows 8 n + 2 t and 8 n + 2 t + 1
   int qpos[NB][2];
@@ -255,81 +312,107 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
     }
   }
   const int qmin = len - p.seqlen_q + rg * kRows / G, qmax = len - p.seqlen_q + min(rg * kRows + kRows - 1, R - 1) / G;
-  float o[NB][D / 16][4];
+  float o[NB][D / 16][4], ob[NB][4];             // ob: the bias of the codes, weighted
   float mrow[NB][2], lrow[NB][2];                // M; sums of this lane's keys
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    ob[n][0] = ob[n][1] = ob[n][2] = ob[n][3] = 0.f;
     mrow[n][0] = mrow[n][1] = -INFINITY;
     lrow[n][0] = lrow[n][1] = 0.f;
   }
+  const float kmul = qinv * (1.f / C::kUnit);
 
   for (int ti = 0; ti < count; ++ti) {
-    const int keyw = (tile0 + ti) * kTile + warp * 16;   // this warp's first key
+    const int keyw = (tile0 + ti) * kTile8 + warp * KW;  // this warp's first key
     cp_async_wait<NS - 2>();
     __syncwarp();
     load_tile(stage == 0 ? NS - 1 : stage - 1);
     cp_async_commit();
-    unsigned char* tK = ring + (size_t)(stage * 4 + warp) * 2 * 16 * P;
-    unsigned char* tV = tK + 16 * P;
-    const float* tS = sS + (stage * 4 + warp) * 32;
+    // this lane's row and chunk of both tiles for ldmatrix
+    const uint32_t tK = smem_u32(ring) + (uint32_t)(stage * 4 + warp) * 2 * KW * P + (lane & 15) * P, tV = tK + KW * P;
+    const uint32_t turned = (uint32_t)((D > 16 ? lane >> 4 : 0) ^ SM::turn(lane & 15)) << 4;
+    const float* tS = sS + (stage * 4 + warp) * 2 * KW;
     if (++stage == NS) stage = 0;
     if (keyw >= keys) continue;
-    const float ks[2] = {tS[g] * qinv, tS[g + 8] * qinv}, vs[2] = {tS[16 + g], tS[24 + g]};
-    // log2 of the V scales; a block of zeros has a small one
-    const float lv[2] = {__log2f(fmaxf(vs[0], 0x1p-60f)), __log2f(fmaxf(vs[1], 0x1p-60f))};
-
-    // ---- S^T = K Q^T: keys keyw + g and keyw + g + 8 ------------------------------------
-    float s[NB][4];
+    // scales of this lane's keys keyw + 16 h + g and + 8; log2 of those of V: a block of zeros has a small one
+    float ks[KB][2], vs[KB][2], lv[KB][2];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int h = 0; h < KB; ++h) {
 #pragma unroll
-    for (int kk = 0; kk < (D + 31) / 32; ++kk) {
-      uint32_t r[4];
-      ldsm_x4(smem_u32(tK + (lane & 15) * P + kk * 32 + (D > 16 ? (lane >> 4) * 16 : 0)), r[0], r[1], r[2], r[3]);
-#pragma unroll
-      for (int half = 0; half < (D > 16 ? 2 : 1); ++half) {
-        uint32_t a[4];
-        C::neighbours(r[2 * half], a[0], a[2]);
-        C::neighbours(r[2 * half + 1], a[1], a[3]);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) mma16816<__half>(s[n], a, bq[n][2 * kk + half][0], bq[n][2 * kk + half][1]);
+      for (int j = 0; j < 2; ++j) {
+        ks[h][j] = tS[h * 16 + j * 8 + g] * kmul;
+        vs[h][j] = tS[KW + h * 16 + j * 8 + g];
+        lv[h][j] = __log2f(fmaxf(vs[h][j], 0x1p-60f));
       }
     }
-    // ---- softmax --------------------------------------------------------------------------
-    const bool full = !cfg.has_alibi && keyw + 16 <= keys && (!cfg.causal || keyw + 15 <= qmin) &&
-                      (cfg.wl < 0 || keyw >= qmax - cfg.wl) && (cfg.wr < 0 || keyw + 15 <= qmin + cfg.wr);
-    if (full) {
-      const float mul[2] = {ks[0] * cfg.scale_log2, ks[1] * cfg.scale_log2};
+
+    // ---- S^T = K Q^T ----------------------------------------------------------------------
+    float s[KB][NB][4];
+#pragma unroll
+    for (int h = 0; h < KB; ++h) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] *= mul[e >> 1];
+        s[h][n][0] = s[h][n][2] = s0[n][0];
+        s[h][n][1] = s[h][n][3] = s0[n][1];
       }
-    } else {
+    }
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
+    for (int kk = 0; kk < (D + 31) / 32; ++kk) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = e & 1, key = keyw + g + (e >> 1) * 8;
-          float th;
-          const float v = score_log2(cfg, slope[n][i], s[n][e] * ks[e >> 1], qpos[n][i], key, th);
-          s[n][e] = visible(cfg, qpos[n][i], key, keys) ? v : -INFINITY;
+      for (int h = 0; h < KB; ++h) {
+        uint32_t r[4];
+        ldsm_x4(tK + h * 16 * P + (turned ^ (kk * 32)), r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int half = 0; half < (D > 16 ? 2 : 1); ++half) {
+          uint32_t a[4];
+          C::neighbours(r[2 * half], a[0], a[2]);
+          C::neighbours(r[2 * half + 1], a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const uint2 x = SM::kQueriesHeld ? bq[n][SM::kQueriesHeld ? 2 * kk + half : 0] : query(n, 2 * kk + half);
+            mma16816<__half>(s[h][n], a, x.x, x.y);
+          }
         }
       }
     }
-    float mx[NB][2];
+    // ---- softmax --------------------------------------------------------------------------
+    const bool full = !cfg.has_alibi && keyw + KW <= keys && (!cfg.causal || keyw + KW - 1 <= qmin) &&
+                      (cfg.wl < 0 || keyw >= qmax - cfg.wl) && (cfg.wr < 0 || keyw + KW - 1 <= qmin + cfg.wr);
+    if (full) {
+#pragma unroll
+      for (int h = 0; h < KB; ++h) {
+        const float mul[2] = {ks[h][0] * cfg.scale_log2, ks[h][1] * cfg.scale_log2};
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[h][n][e] *= mul[e >> 1];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < KB; ++h) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = e & 1, j = e >> 1, key = keyw + h * 16 + j * 8 + g;
+            float th;
+            const float v = score_log2(cfg, slope[n][i], s[h][n][e] * ks[h][j], qpos[n][i], key, th);
+            const bool seen = visible(cfg, qpos[n][i], key, keys);
+            s[h][n][e] = seen ? v : -INFINITY;
+          }
+        }
+      }
+    }
     bool grow = false;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
+    for (int h = 0; h < KB; ++h) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float m = fmaxf(s[n][i] + lv[0], s[n][2 + i] + lv[1]);
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        mx[n][i] = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        grow |= mx[n][i] > mrow[n][i];
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) grow |= s[h][n][e] + lv[h][e >> 1] > mrow[n][e & 1];
       }
     }
     if (__any_sync(0xffffffffu, grow)) {
@@ -338,9 +421,15 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
         float alpha[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bool up = mx[n][i] > mrow[n][i];
-          alpha[i] = up ? exp2f(mrow[n][i] - mx[n][i]) : 1.f;    // from -inf: 0
-          if (up) mrow[n][i] = mx[n][i];
+          float m = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < KB; ++h) m = fmax3(m, s[h][n][i] + lv[h][0], s[h][n][2 + i] + lv[h][1]);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          const bool up = m > mrow[n][i];
+          alpha[i] = up ? exp2f(mrow[n][i] - m) : 1.f;           // from -inf: 0
+          if (up) mrow[n][i] = m;
           lrow[n][i] *= alpha[i];
         }
 #pragma unroll
@@ -348,35 +437,50 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
           o[n][db][0] *= alpha[0]; o[n][db][1] *= alpha[1];
           o[n][db][2] *= alpha[0]; o[n][db][3] *= alpha[1];
         }
+        ob[n][0] *= alpha[0]; ob[n][1] *= alpha[1];
       }
     }
-    uint32_t pb[NB][2];
+    uint32_t pb[KB][NB][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
+      // no finite score yet: exponents relative to 0, so that -inf gives 0 and NaN stays NaN
+      const float m[2] = {mrow[n][0] == -INFINITY ? 0.f : mrow[n][0], mrow[n][1] == -INFINITY ? 0.f : mrow[n][1]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // no finite score yet: exponents relative to 0, so that -inf gives 0 and NaN stays NaN
-        const float m = mrow[n][e & 1] == -INFINITY ? 0.f : mrow[n][e & 1];
-        const float pe = ex2(s[n][e] - m);
-        lrow[n][e & 1] += pe;
-        s[n][e] = pe == 0.f ? 0.f : pe * vs[e >> 1];             // a hidden key weighs 0 whatever its scale is
+      for (int h = 0; h < KB; ++h) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pe = ex2(s[h][n][e] - m[e & 1]);
+          lrow[n][e & 1] += pe;
+          s[h][n][e] = !full && pe == 0.f ? 0.f : pe * vs[h][e >> 1];      // a hidden key weighs 0 whatever its scale is
+        }
+        // P^T[key][row] as the accumulator holds it -> B fragment [keys] x [rows]
+        pb[h][n][0] = transpose_8x8(Elem<__half>::pack(s[h][n][0], s[h][n][1]));
+        pb[h][n][1] = transpose_8x8(Elem<__half>::pack(s[h][n][2], s[h][n][3]));
       }
-      // P^T[key][row] as the accumulator holds it -> B fragment [keys] x [rows]
-      pb[n][0] = transpose_8x8(Elem<__half>::pack(s[n][0], s[n][1]));
-      pb[n][1] = transpose_8x8(Elem<__half>::pack(s[n][2], s[n][3]));
     }
     // ---- O^T += V^T P^T -----------------------------------------------------------------
+    if (C::kBias) {
+      const uint32_t a[4] = {C::kBias, C::kBias, C::kBias, C::kBias};
+#pragma unroll
+      for (int h = 0; h < KB; ++h) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) mma16816<__half>(ob[n], a, pb[h][n][0], pb[h][n][1]);
+      }
+    }
 #pragma unroll
     for (int d2 = 0; d2 < (D + 31) / 32; ++d2) {
-      uint32_t r[4];
-      ldsm_x4_t(smem_u32(tV + (lane & 15) * P + d2 * 32 + (D > 16 ? (lane >> 4) * 16 : 0)), r[0], r[1], r[2], r[3]);
 #pragma unroll
-      for (int half = 0; half < (D > 16 ? 2 : 1); ++half) {
-        uint32_t a[4];
-        C::alternate(r[2 * half], a[0], a[1]);
-        C::alternate(r[2 * half + 1], a[2], a[3]);
+      for (int h = 0; h < KB; ++h) {
+        uint32_t r[4];
+        ldsm_x4_t(tV + h * 16 * P + (turned ^ (d2 * 32)), r[0], r[1], r[2], r[3]);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) mma16816<__half>(o[n][2 * d2 + half], a, pb[n][0], pb[n][1]);
+        for (int half = 0; half < (D > 16 ? 2 : 1); ++half) {
+          uint32_t a[4];
+          C::alternate(r[2 * half], a[0], a[1]);
+          C::alternate(r[2 * half + 1], a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) mma16816<__half>(o[n][2 * d2 + half], a, pb[h][n][0], pb[h][n][1]);
+        }
       }
     }
   }
@@ -403,10 +507,11 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
     for (int i = 0; i < 2; ++i) {
       const int r = n * 8 + 2 * t + i;
       const float mstar = fmaxf(fmaxf(sM[r], sM[kRows + r]), fmaxf(sM[2 * kRows + r], sM[3 * kRows + r]));
-      const float wgt = mstar == -INFINITY ? 0.f : exp2f(mrow[n][i] - mstar);
+      const float wgt = mstar == -INFINITY ? 0.f : exp2f(mrow[n][i] - mstar) * (1.f / C::kUnit);
 #pragma unroll
       for (int db = 0; db < D / 16; ++db)
-        *reinterpret_cast<float2*>(sO + (warp * kRows + r) * OP + db * 16 + 2 * g) = make_float2(wgt * o[n][db][i], wgt * o[n][db][2 + i]);
+        *reinterpret_cast<float2*>(sO + (warp * kRows + r) * OP + db * 16 + 2 * g) = 
+            make_float2(wgt * (o[n][db][i] - ob[n][i]), wgt * (o[n][db][2 + i] - ob[n][i]));
     }
   }
   __syncthreads();

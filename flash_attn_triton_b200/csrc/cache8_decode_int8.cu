@@ -9,13 +9,15 @@ int decode8_int8(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cf
                             : launch_decode8<__half, FA_CODE_INT8>(a, c, cfg, unit_rows, g, chk, behind, st);
 }
 
-// CTAs per SM that a kernel is compiled for.
-int decode8_resident(int head_dim, int unit_rows) {
+DecodeGeom decode8_geometry(const fa_decode_args& a, int unit_rows, int row_groups) {
   auto of = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    return unit_rows == 8 ? Decode8<D, 8>::kResident : Decode8<D, 16>::kResident;
+    using S8 = Decode8<D, 8>;
+    using S16 = Decode8<D, 16>;
+    static_assert(S8::kTile8 == S16::kTile8, "");
+    return decode_geometry(a, row_groups, unit_rows == 8 ? S8::kResident : S16::kResident, S8::kTile8, kLongest8);
   };
-  switch (head_dim) {
+  switch (a.head_dim) {
     case 16: return of(std::integral_constant<int, 16>{});
     case 32: return of(std::integral_constant<int, 32>{});
     case 64: return of(std::integral_constant<int, 64>{});
