@@ -155,10 +155,12 @@ int bwd_dq_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int bwd_dkdv_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int fwd_alt_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int fwd_alt_sm100_status();
+int cache8_chunk_status();
 int fwd_duo_sm100_status();
 int64_t dropout_bits_words(int, int);
 int dropout_bits(const fa_attn_args&, const ScoreCfg&, uint32_t*, cudaStream_t);
 int fwd_alt_sm100_clear_status();
+int cache8_chunk_clear_status();
 int fwd_duo_sm100_clear_status();
 int decode_paged(const fa_decode_args&, cudaStream_t);
 int decode_paged_checked(const fa_decode_args&, uint32_t*, cudaStream_t);
@@ -720,6 +722,7 @@ int fa_device_wait_status(int device) {
   if (s == 0) s = bwd_sm100_status();
   if (s == 0) s = fwd_alt_sm100_status();
   if (s == 0) s = fwd_duo_sm100_status();
+  if (s == 0) s = cache8_chunk_status();
   if (s == 0) s = host_wait_status(device);
   if (s != 0 && device >= 0 && device < 1024) g_host_wait[device] = s;   // remembered for the launchers
   return s;
@@ -736,6 +739,7 @@ int fa_device_wait_clear(int device) {
   bwd_sm100_clear_status();
   fwd_alt_sm100_clear_status();
   fwd_duo_sm100_clear_status();
+  cache8_chunk_clear_status();
   // a launch whose CTAs gave up has not put its pair of counters back to zero; the next one to get the pair would skip items
   void* queues = nullptr;
   e = cudaGetSymbolAddress(&queues, g_work_queues);

@@ -1,7 +1,8 @@
-// Calls on the 8-bit KV cache: value checks, append, attention.  One launch where nothing is appended and the tables are small, else the
-// append (which then makes the checks) and the attention behind it.
+// Calls on the 8-bit KV cache: value checks, append, attention.  A decode step is one launch where nothing is appended and the tables are
+// small, else the append (which then makes the checks) and the attention behind it.
 #include "cache8_host.h"
 #include "cache_dev.cuh"
+#include "cache_geo.cuh"
 #include "check_words.h"
 
 namespace fa {
@@ -9,6 +10,7 @@ namespace fa {
 int decode8_int8(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
 int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
 DecodeGeom decode8_geometry(const fa_decode_args& a, int unit_rows, int row_groups);
+int cache8_chunk(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
 int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st);
 
 namespace {
@@ -20,8 +22,10 @@ int unit_rows_of(const fa_decode_args& a) { return a.seqlen_q * (a.heads_q / a.h
 
 // How a call is run.  Workspace: pieces, counters if the caller brings none, the word with the result of the checks.
 struct Plan {
-  int unit_rows;
+  bool chunk;
+  int unit_rows;                       // decode
   DecodeGeom geo;
+  int pack_log2, parts, capacity;      // chunk
   size_t piece_bytes, counter_bytes;
   int counters;
   bool append, inside;                 // the first kernel makes the checks, in every CTA
@@ -29,17 +33,44 @@ struct Plan {
   size_t bytes() const { return word_at() + kAlign; }
 };
 
+// A chunk: more than 16 query rows per KV head.  The decode kernel would read the cache once per 16 rows; the tcgen05 kernel takes 128 at a
+// time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128: 690 -> 265 us).
+bool plan_chunk(const fa_decode_args& a, Plan& p) {
+  const int G = a.heads_q / a.heads_kv;
+  if (a.num_splits != 0 || (int64_t)a.seqlen_q * G <= 16 || a.softmax_scale < 0.f) return false;
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
+  if (a.block_table && a.page_size % 16 != 0) return false;          // 16 keys are looked up at a time
+  p.pack_log2 = 0;
+  if ((G & (G - 1)) == 0 && G <= 64)
+    while ((1 << p.pack_log2) < G) ++p.pack_log2;
+  const int64_t cap = a.block_table ? (int64_t)a.block_table_stride * a.page_size : a.page_size;
+  const int64_t mtiles = (((int64_t)a.seqlen_q << p.pack_log2) + 127) / 128;
+  const int64_t units = (int64_t)a.batch * (a.heads_q >> p.pack_log2) * mtiles;
+  if (units > (1 << 28) || cap > (1 << 30)) return false;
+  p.capacity = (int)cap;
+  // pieces of at least four key tiles, only while the units leave SMs idle
+  const int64_t fill = sm_count(a.device) / units, most = (cap + 511) / 512;
+  p.parts = (int)(fill < most ? fill : most);
+  if (p.parts < 1) p.parts = 1;
+  p.counters = p.parts > 1 ? (int)units : 0;
+  p.piece_bytes = p.parts > 1 ? (size_t)units * p.parts * 128 * (a.head_dim + 1) * sizeof(float) : 0;
+  return true;
+}
+
 Plan plan_of(const fa_decode_args& a) {
-  Plan p;
-  p.unit_rows = unit_rows_of(a);
-  const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
-  const int groups = (int)((rows + p.unit_rows - 1) / p.unit_rows);
-  p.geo = decode8_geometry(a, p.unit_rows, groups);
-  p.piece_bytes = p.geo.splits == 1 ? 0 : (size_t)p.geo.shares * a.seqlen_q * a.heads_q * (a.head_dim + 1) * sizeof(float);
-  p.counters = p.piece_bytes ? a.batch * a.heads_kv * groups : 0;
+  Plan p = {};
+  p.chunk = plan_chunk(a, p);
+  if (!p.chunk) {
+    p.unit_rows = unit_rows_of(a);
+    const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
+    const int groups = (int)((rows + p.unit_rows - 1) / p.unit_rows);
+    p.geo = decode8_geometry(a, p.unit_rows, groups);
+    p.piece_bytes = p.geo.splits == 1 ? 0 : (size_t)p.geo.shares * a.seqlen_q * a.heads_q * (a.head_dim + 1) * sizeof(float);
+    p.counters = p.piece_bytes ? a.batch * a.heads_kv * groups : 0;
+  }
   p.counter_bytes = a.counters ? 0 : (size_t)p.counters * sizeof(uint32_t);
   p.append = a.k_new != nullptr;
-  p.inside = (int64_t)a.batch * (a.block_table ? a.block_table_stride : 1) <= kInlineCheck;
+  p.inside = (int64_t)a.batch * (a.block_table ? a.block_table_stride : 1) <= kInlineCheck && (p.append || !p.chunk);
   return p;
 }
 
@@ -69,8 +100,29 @@ int run(const fa_decode_args& args, const fa_cache8& c, const Plan& plan, uint32
     if (here) *queued = true;
   }
   const bool behind = plan.append || first;
-  const DecodeCheck chk = {check && plan.inside && !plan.append ? host : nullptr, check && behind ? word : nullptr};
   const ScoreCfg cfg = make_score_cfg(a.softmax_scale, 0.f, a.causal, a.window_left, a.window_right, a.alibi_slopes != nullptr);
+  if (plan.chunk) {
+    CacheGeo geo = {};
+    geo.seqlens = a.cache_seqlens;
+    geo.table = a.block_table;
+    geo.table_stride = a.block_table_stride;
+    geo.batch_idx = a.cache_batch_idx;
+    geo.leftpad = a.cache_leftpad;
+    geo.page_size = a.page_size;
+    geo.page_log2 = page_shift_of(a);
+    geo.box_rows = 128;                // keys that one copy brings: they lie inside one page
+    while (a.block_table && a.page_size % geo.box_rows != 0) geo.box_rows /= 2;
+    geo.n_new = plan.append ? a.seqlen_new : 0;
+    geo.tokens = a.seqlen_q;
+    geo.pack_log2 = plan.pack_log2;
+    geo.parts = plan.parts;
+    geo.capacity = plan.capacity;
+    geo.ws = reinterpret_cast<float*>(ws);
+    geo.counters = a.counters;
+    geo.bad = check ? word : nullptr;
+    return cache8_chunk(a, c, geo, cfg, st);
+  }
+  const DecodeCheck chk = {check && plan.inside && !plan.append ? host : nullptr, check && behind ? word : nullptr};
   const int r = c.code == FA_CODE_INT8 ? decode8_int8(a, c, cfg, plan.unit_rows, plan.geo, chk, behind, st)
                                        : decode8_e4m3(a, c, cfg, plan.unit_rows, plan.geo, chk, behind, st);
   if (check && r == FA_OK) *queued = true;
@@ -78,6 +130,12 @@ int run(const fa_decode_args& args, const fa_cache8& c, const Plan& plan, uint32
 }
 
 int refused(const fa_decode_args& a, const Plan& plan) {
+  if (plan.chunk)
+    if (const int code = host_wait_status(a.device)) {
+      set_error("fa_decode_paged8: a bounded device-side wait ran out earlier on device %d (code %d); the tcgen05 kernels "
+                "stay off until fa_device_wait_clear()", a.device, code);
+      return FA_ERR_DEVICE_WAIT;
+    }
   if (a.workspace == nullptr || a.workspace_bytes < plan.bytes()) {
     set_error("decode8 workspace too small: need %zu bytes, got %zu", plan.bytes(), a.workspace_bytes);
     return FA_ERR_WORKSPACE;

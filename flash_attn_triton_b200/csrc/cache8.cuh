@@ -31,6 +31,14 @@ template <> struct Code<FA_CODE_INT8> {
     a = pair(x, 0x4240);
     b = pair(x, 0x4341);
   }
+  // bytes (0, 1) and (2, 3) as they are, without the factor and the bias: 0x6400 | u is 1024 + u
+  static __device__ __forceinline__ void integers(uint32_t x, uint32_t& a, uint32_t& b) {
+    x ^= 0x80808080u;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(a) : "r"(x), "r"(0x64646464u), "r"(0x4140u));
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(b) : "r"(x), "r"(0x64646464u), "r"(0x4342u));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(0x64806480u));
+  }
   // four codes of x[i] * m.  Adding 1.5 * 2^23 leaves the number rounded half to even in the low byte.
   static __device__ __forceinline__ uint32_t four(float a, float b, float c, float d, float m) {
     const float magic = 12582912.f;
@@ -57,6 +65,7 @@ template <> struct Code<FA_CODE_E4M3> {
     a = pair((uint16_t)x);
     b = pair((uint16_t)(x >> 16));
   }
+  static __device__ __forceinline__ void integers(uint32_t x, uint32_t& a, uint32_t& b) { neighbours(x, a, b); }
   static __device__ __forceinline__ void alternate(uint32_t x, uint32_t& a, uint32_t& b) {
     neighbours(__byte_perm(x, 0u, 0x3120), a, b);
   }
@@ -73,6 +82,13 @@ template <> struct Code<FA_CODE_E4M3> {
     f[0] = p.x; f[1] = p.y; f[2] = q.x; f[3] = q.y;
   }
 };
+
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
+}
 
 // log2 of a power of two, else -1
 inline int log2_of(int n) {

@@ -23,14 +23,6 @@
 
 namespace fa {
 
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(bytes));
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
-}
-
 template <int D, int kRows> struct Decode8 {
   static constexpr int kKeys = D == 256 ? 16 : 32;     // of a warp's tile
   static constexpr int kTile8 = 4 * kKeys;

@@ -418,7 +418,7 @@ inline PFN_encodeTiled get_encode_tiled() {
 // 128-byte swizzle: box0 * elem_bytes must be 128.
 inline bool encode_tmap(CUtensorMap* out, const void* base, int elem_bytes, int rank,
                         const uint64_t* dims, const uint64_t* strides_bytes /* rank-1 */,
-                        const uint32_t* box) {
+                        const uint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return false;
   cuuint64_t gd[5];
@@ -432,7 +432,7 @@ inline bool encode_tmap(CUtensorMap* out, const void* base, int elem_bytes, int 
   for (int i = 0; i < rank - 1; ++i) gs[i] = strides_bytes[i];
   CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUresult r = enc(out, dt, (cuuint32_t)rank, const_cast<void*>(base), gd, gs, bx, es,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
