@@ -115,8 +115,10 @@ struct Tile {
 
 }  // namespace
 
-// T: type of q and o.  kAlibi: with slopes.
-template <typename T, int kCode, int D, bool kAlibi>
+// T: type of q and o.  kAlibi: with slopes.  kFine: a scale for each key of a tile; else every 16 keys have one scale (blocks of a multiple of
+// 16 tokens, no left padding), which goes into the exponent's FMA and stays in registers.  With one per key, read from shared memory by every
+// thread, a call took FINE us where it now takes COARSE (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128).
+template <typename T, int kCode, int D, bool kAlibi, bool kFine>
 __global__ void __launch_bounds__(kThreads, 1)
 cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmO, const fa_decode_args p, const fa_cache8 c8, const int block_shift,
@@ -373,8 +375,13 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         pg = page_of(j + 2);
         const int sb = j % kScaleBufs;
         if (!wait_bar(&sh->sc_empty[sb], ((j / kScaleBufs) & 1) ^ 1, sh, 14)) break;
-        *reinterpret_cast<float4*>(&sh->ks[sb][lane * 4]) = k4;
-        *reinterpret_cast<float4*>(&sh->vs[sb][lane * 4]) = v4;
+        if (kFine) {
+          *reinterpret_cast<float4*>(&sh->ks[sb][lane * 4]) = k4;
+          *reinterpret_cast<float4*>(&sh->vs[sb][lane * 4]) = v4;
+        } else if ((lane & 3) == 0) {
+          sh->ks[sb][lane >> 2] = k4.x;
+          sh->vs[sb][lane >> 2] = v4.x;
+        }
         float m = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -552,65 +559,74 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (!ok) break;
       tc_fence_after();
 
-      // ---- the 128 scores of this row into registers -------------------------------------
-      uint32_t r[4][32];
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + cc * 32, r[cc]);
-      tmem_wait_ld();
-
-      // ---- times the scales of the keys; masked tiles and ALiBi go on to the log2 domain ------
-      const bool prescaled = kAlibi || masked;
-      const float smul = kAlibi ? qinv : prescaled ? cfg.scale_log2 * qinv : 1.f;
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(&sh->ks[sb][cc * 32 + i]);
-          const float2 a = f2mul(make_float2(__uint_as_float(r[cc][i]), __uint_as_float(r[cc][i + 1])), make_float2(k4.x, k4.y));
-          const float2 b = f2mul(make_float2(__uint_as_float(r[cc][i + 2]), __uint_as_float(r[cc][i + 3])), make_float2(k4.z, k4.w));
-          r[cc][i] = __float_as_uint(a.x);
-          r[cc][i + 1] = __float_as_uint(a.y);
-          r[cc][i + 2] = __float_as_uint(b.x);
-          r[cc][i + 3] = __float_as_uint(b.y);
-        }
-      }
+      // The scores are read twice, 32 columns at a time: for the maximum, and for the exponentials (P of columns cc overwrites columns that
+      // have been read).  All 128 of a row do not fit beside the rest in what 512 threads have: 512 bytes of them were spilled, and a
+      // tile's exponentials took 4200 cycles.
+      const bool prescaled = kAlibi || masked;           // masked tiles and ALiBi go to the log2 domain at once
+      ColMask cm;
       if (prescaled) {
-        ColMask cm;
         int vk_lo, vk_hi;
         visible_k_interval(cfg, qpos, w.keys, vk_lo, vk_hi);
         cm = make_col_mask(vk_lo - k0, vk_hi - k0);
-        const float dist0 = (float)(qpos - k0);
-        const FeatK fk = feat_k<false>(cfg, slope);
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 v = f2mul(make_float2(__uint_as_float(r[cc][i]), __uint_as_float(r[cc][i + 1])), make_float2(smul, smul));
-            if (kAlibi)
-              v = score_unit_feat2<false, true, true>(fk, v, make_float2(dist0 - (float)(cc * 32 + i), dist0 - (float)(cc * 32 + i + 1)));
-            r[cc][i] = __float_as_uint(col_visible(cm, cc * 32 + i) ? v.x : -INFINITY);
-            r[cc][i + 1] = __float_as_uint(col_visible(cm, cc * 32 + i + 1) ? v.y : -INFINITY);
-          }
-        }
       }
-      const float mul = prescaled ? 1.f : cfg.scale_log2 * qinv;
+      const float f = cfg.scale_log2 * qinv, dist0 = (float)(qpos - k0), tilt = slope * FA_LOG2E;
+      // Columns cc * 32 + i in place, ready to be multiplied by mg (of each 16 keys) and exponentiated.
+      auto prepare = [&](auto log2_tag, int cc, uint32_t (&r)[32], float2& mg) {
+        if (kFine) {
+          mg = make_float2(f, f);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(&sh->ks[sb][cc * 32 + i]);
+            const float2 a = f2mul(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(k4.x, k4.y));
+            const float2 b = f2mul(make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), make_float2(k4.z, k4.w));
+            r[i] = __float_as_uint(a.x);
+            r[i + 1] = __float_as_uint(a.y);
+            r[i + 2] = __float_as_uint(b.x);
+            r[i + 3] = __float_as_uint(b.y);
+          }
+        } else {
+          mg = f2mul(*reinterpret_cast<const float2*>(&sh->ks[sb][cc * 2]), make_float2(f, f));
+        }
+        if constexpr (decltype(log2_tag)::value) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float v = __uint_as_float(r[i]) * (i < 16 ? mg.x : mg.y);
+            if (kAlibi) v = fmaf(-tilt, fabsf(dist0 - (float)(cc * 32 + i)), v);
+            r[i] = __float_as_uint(col_visible(cm, cc * 32 + i) ? v : -INFINITY);
+          }
+          mg = make_float2(1.f, 1.f);
+        }
+      };
 
       // ---- row maximum of t + log2 vs, vs by its largest of 16 keys -----------------------------
+      // (each pass is compiled apart for the tiles that go to the log2 domain first: what most tiles run stays small)
       float mx = -INFINITY;
-      {
-        const float4 l0 = *reinterpret_cast<const float4*>(&sh->lv[sb][0]), l1 = *reinterpret_cast<const float4*>(&sh->lv[sb][4]);
-        const float lv[8] = {l0.x, l0.y, l0.z, l0.w, l1.x, l1.y, l1.z, l1.w};
+      auto largest = [&](auto log2_tag) {
+        uint32_t ra[32], rb[32];
+        tmem_ld32(tS, ra);
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const uint32_t* v = &r[g >> 1][(g & 1) * 16];
-          float m[5];
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t (&cur)[32] = (cc & 1) ? rb : ra;
+          uint32_t (&nxt)[32] = (cc & 1) ? ra : rb;
+          tmem_wait_ld();
+          if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, nxt);
+          float2 mg;
+          prepare(log2_tag, cc, cur, mg);
+          const float2 lv = *reinterpret_cast<const float2*>(&sh->lv[sb][cc * 2]);
 #pragma unroll
-          for (int i = 0; i < 5; ++i)
-            m[i] = fmax3(__uint_as_float(v[3 * i]), __uint_as_float(v[3 * i + 1]), __uint_as_float(v[3 * i + 2]));
-          const float most = fmaxf(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], __uint_as_float(v[15])));
-          mx = fmaxf(mx, fmaf(most, mul, lv[g]));
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t* v = &cur[g * 16];
+            float m[5];
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+              m[i] = fmax3(__uint_as_float(v[3 * i]), __uint_as_float(v[3 * i + 1]), __uint_as_float(v[3 * i + 2]));
+            const float most = fmaxf(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], __uint_as_float(v[15])));
+            mx = fmaxf(mx, fmaf(most, g ? mg.y : mg.x, g ? lv.y : lv.x));
+          }
         }
-      }
+      };
+      if (prescaled) largest(std::true_type{});
+      else largest(std::false_type{});
 
       // ---- the maximum the exponents are relative to, settled in tile order ---------------
       float m_use;
@@ -652,19 +668,31 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const float m_safe = (m_use == -INFINITY) ? 0.f : m_use;
 
       // ---- p = exp2(t - M), row sum, p vs -> TMEM in place over S ----------------------------
-      const float2 mul2 = make_float2(mul, mul), nm2 = make_float2(-m_safe, -m_safe);
+      const float2 nm2 = make_float2(-m_safe, -m_safe);
       float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto weigh = [&](auto mask_tag) {
-        constexpr bool kMask = decltype(mask_tag)::value;
+      auto weigh = [&](auto log2_tag) {
+        constexpr bool kMask = decltype(log2_tag)::value;
+        uint32_t ra[32], rb[32];
+        tmem_ld32(tS, ra);
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
+          uint32_t (&cur)[32] = (cc & 1) ? rb : ra;
+          uint32_t (&nxt)[32] = (cc & 1) ? ra : rb;
+          tmem_wait_ld();
+          if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, nxt);
+          float2 mg, v16 = make_float2(0.f, 0.f);        // scales of V of the two 16 keys
+          prepare(log2_tag, cc, cur, mg);
+          if (!kFine) v16 = *reinterpret_cast<const float2*>(&sh->vs[sb][cc * 2]);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 v4 = *reinterpret_cast<const float4*>(&sh->vs[sb][cc * 32 + i]);
+            float4 v4;
+            if (kFine) v4 = *reinterpret_cast<const float4*>(&sh->vs[sb][cc * 32 + i]);
+            else v4.x = v4.y = v4.z = v4.w = i < 16 ? v16.x : v16.y;
+            const float2 mul2 = i < 16 ? make_float2(mg.x, mg.x) : make_float2(mg.y, mg.y);
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
-              const float2 a = f2fma(make_float2(__uint_as_float(r[cc][i + e]), __uint_as_float(r[cc][i + e + 1])), mul2, nm2);
+              const float2 a = f2fma(make_float2(__uint_as_float(cur[i + e]), __uint_as_float(cur[i + e + 1])), mul2, nm2);
               const float2 pe = make_float2(ex2(a.x), ex2(a.y));
               acc2[e >> 1] = f2add(acc2[e >> 1], pe);
               float2 wt = f2mul(pe, e ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
@@ -683,7 +711,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           }
         }
       };
-      if (masked) weigh(std::true_type{});
+      if (prescaled) weigh(std::true_type{});
       else weigh(std::false_type{});
       sum = (acc2[0].x + acc2[0].y) + (acc2[1].x + acc2[1].y);
       tmem_wait_st();
@@ -835,7 +863,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 // ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
-template <typename T, int kCode, int D, bool kAlibi>
+template <typename T, int kCode, int D, bool kAlibi, bool kFine>
 static int launch_chunk8(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
   const int pack = 1 << geo.pack_log2;
   CUtensorMap tm[3];
@@ -853,7 +881,7 @@ static int launch_chunk8(const fa_decode_args& d, const fa_cache8& c, const Cach
     set_error("cache8_chunk: cuTensorMapEncodeTiled failed");
     return FA_ERR_LAUNCH;
   }
-  auto kern = cache8_chunk_kernel<T, kCode, D, kAlibi>;
+  auto kern = cache8_chunk_kernel<T, kCode, D, kAlibi, kFine>;
   constexpr int smem = CCfg<D>::kSmemBytes;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
@@ -878,7 +906,10 @@ static int launch_chunk8(const fa_decode_args& d, const fa_cache8& c, const Cach
 
 template <typename T, int kCode, int D>
 static int launch_chunk8_dim(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
-  return cfg.has_alibi ? launch_chunk8<T, kCode, D, true>(d, c, geo, cfg, st) : launch_chunk8<T, kCode, D, false>(d, c, geo, cfg, st);
+  // (with ALiBi, which is rare, there is the general kernel alone)
+  if (cfg.has_alibi) return launch_chunk8<T, kCode, D, true, true>(d, c, geo, cfg, st);
+  return c.block % 16 != 0 || geo.leftpad != nullptr ? launch_chunk8<T, kCode, D, false, true>(d, c, geo, cfg, st)
+                                                     : launch_chunk8<T, kCode, D, false, false>(d, c, geo, cfg, st);
 }
 template <typename T, int kCode>
 static int launch_chunk8_code(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
