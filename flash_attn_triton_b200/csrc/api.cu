@@ -156,11 +156,13 @@ int bwd_dkdv_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int fwd_alt_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int fwd_alt_sm100_status();
 int cache8_chunk_status();
+int cache8_pair_status();
 int fwd_duo_sm100_status();
 int64_t dropout_bits_words(int, int);
 int dropout_bits(const fa_attn_args&, const ScoreCfg&, uint32_t*, cudaStream_t);
 int fwd_alt_sm100_clear_status();
 int cache8_chunk_clear_status();
+int cache8_pair_clear_status();
 int fwd_duo_sm100_clear_status();
 int decode_paged(const fa_decode_args&, cudaStream_t);
 int decode_paged_checked(const fa_decode_args&, uint32_t*, cudaStream_t);
@@ -173,8 +175,8 @@ int decode_paged_static(const fa_decode_args&, cudaStream_t);
 size_t decode_static_scratch_bytes();
 int decode8_paged(const fa_decode_args&, const fa_cache8&, cudaStream_t);
 int decode8_paged_checked(const fa_decode_args&, const fa_cache8&, uint32_t*, cudaStream_t);
-size_t decode8_workspace_bytes(const fa_decode_args&);
-int decode8_counters(const fa_decode_args&);
+size_t decode8_workspace_bytes(const fa_decode_args&, const fa_cache8&);
+int decode8_counters(const fa_decode_args&, const fa_cache8&);
 int append8(const fa_append8_args&, cudaStream_t);
 int append8_checked(const fa_append8_args&, uint32_t*, cudaStream_t);
 size_t append8_workspace_bytes(const fa_append8_args&);
@@ -511,11 +513,11 @@ int fa_decode_paged8_checked(const fa_decode_args* a, const fa_cache8* c, uint32
 }
 size_t fa_decode8_workspace_bytes(const fa_decode_args* a, const fa_cache8* c) {
   if (a == nullptr || c == nullptr || a->heads_kv <= 0 || a->heads_q <= 0 || a->page_size <= 0) return 0;
-  return decode8_workspace_bytes(*a);
+  return decode8_workspace_bytes(*a, *c);
 }
 int32_t fa_decode8_counters(const fa_decode_args* a, const fa_cache8* c) {
   if (a == nullptr || c == nullptr || a->heads_kv <= 0 || a->heads_q <= 0 || a->page_size <= 0) return 0;
-  return decode8_counters(*a);
+  return decode8_counters(*a, *c);
 }
 
 static int validate_append8(const fa_append8_args* a) {
@@ -723,6 +725,7 @@ int fa_device_wait_status(int device) {
   if (s == 0) s = fwd_alt_sm100_status();
   if (s == 0) s = fwd_duo_sm100_status();
   if (s == 0) s = cache8_chunk_status();
+  if (s == 0) s = cache8_pair_status();
   if (s == 0) s = host_wait_status(device);
   if (s != 0 && device >= 0 && device < 1024) g_host_wait[device] = s;   // remembered for the launchers
   return s;
@@ -740,6 +743,7 @@ int fa_device_wait_clear(int device) {
   fwd_alt_sm100_clear_status();
   fwd_duo_sm100_clear_status();
   cache8_chunk_clear_status();
+  cache8_pair_clear_status();
   // a launch whose CTAs gave up has not put its pair of counters back to zero; the next one to get the pair would skip items
   void* queues = nullptr;
   e = cudaGetSymbolAddress(&queues, g_work_queues);

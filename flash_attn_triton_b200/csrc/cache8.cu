@@ -11,6 +11,7 @@ int decode8_int8(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, 
 int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
 DecodeGeom decode8_geometry(const fa_decode_args& a, int unit_rows, int row_groups);
 int cache8_chunk(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
+int cache8_pair(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
 int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st);
 
 namespace {
@@ -22,7 +23,7 @@ int unit_rows_of(const fa_decode_args& a) { return a.seqlen_q * (a.heads_q / a.h
 
 // How a call is run.  Workspace: pieces, counters if the caller brings none, the word with the result of the checks.
 struct Plan {
-  bool chunk;
+  bool chunk, pair;                    // pair: 256 query rows per CTA
   int unit_rows;                       // decode
   DecodeGeom geo;
   int pack_log2, parts, capacity;      // chunk
@@ -35,7 +36,7 @@ struct Plan {
 
 // A chunk: more than 16 query rows per KV head.  The decode kernel would read the cache once per 16 rows; the tcgen05 kernel takes 128 at a
 // time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128: 690 -> 265 us).
-bool plan_chunk(const fa_decode_args& a, Plan& p) {
+bool plan_chunk(const fa_decode_args& a, const fa_cache8& c, Plan& p) {
   const int G = a.heads_q / a.heads_kv;
   if (a.num_splits != 0 || (int64_t)a.seqlen_q * G <= 16 || a.softmax_scale < 0.f) return false;
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
@@ -44,22 +45,25 @@ bool plan_chunk(const fa_decode_args& a, Plan& p) {
   if ((G & (G - 1)) == 0 && G <= 64)
     while ((1 << p.pack_log2) < G) ++p.pack_log2;
   const int64_t cap = a.block_table ? (int64_t)a.block_table_stride * a.page_size : a.page_size;
-  const int64_t mtiles = (((int64_t)a.seqlen_q << p.pack_log2) + 127) / 128;
+  const int64_t rows = (int64_t)a.seqlen_q << p.pack_log2;
+  p.pair = a.head_dim <= 128 && rows > 128 && a.alibi_slopes == nullptr && a.cache_leftpad == nullptr && c.block % 16 == 0;
+  const int per_cta = p.pair ? 256 : 128;
+  const int64_t mtiles = (rows + per_cta - 1) / per_cta;
   const int64_t units = (int64_t)a.batch * (a.heads_q >> p.pack_log2) * mtiles;
   if (units > (1 << 28) || cap > (1 << 30)) return false;
   p.capacity = (int)cap;
-  // pieces of at least four key tiles, only while the units leave SMs idle
-  const int64_t fill = sm_count(a.device) / units, most = (cap + 511) / 512;
+  // pieces of at least four key tiles, only while the units do not fill the SMs twice (chunk_pieces() has how many there are)
+  const int64_t sms = sm_count(a.device), fill = units >= 2 * sms ? 1 : sms / units > 4 ? sms / units : 4, most = (cap + 511) / 512;
   p.parts = (int)(fill < most ? fill : most);
   if (p.parts < 1) p.parts = 1;
   p.counters = p.parts > 1 ? (int)units : 0;
-  p.piece_bytes = p.parts > 1 ? (size_t)units * p.parts * 128 * (a.head_dim + 1) * sizeof(float) : 0;
+  p.piece_bytes = p.parts > 1 ? (size_t)units * p.parts * per_cta * (a.head_dim + 1) * sizeof(float) : 0;
   return true;
 }
 
-Plan plan_of(const fa_decode_args& a) {
+Plan plan_of(const fa_decode_args& a, const fa_cache8& c) {
   Plan p = {};
-  p.chunk = plan_chunk(a, p);
+  p.chunk = plan_chunk(a, c, p);
   if (!p.chunk) {
     p.unit_rows = unit_rows_of(a);
     const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
@@ -116,11 +120,12 @@ int run(const fa_decode_args& args, const fa_cache8& c, const Plan& plan, uint32
     geo.tokens = a.seqlen_q;
     geo.pack_log2 = plan.pack_log2;
     geo.parts = plan.parts;
+    geo.sms = sm_count(a.device);
     geo.capacity = plan.capacity;
     geo.ws = reinterpret_cast<float*>(ws);
     geo.counters = a.counters;
     geo.bad = check ? word : nullptr;
-    return cache8_chunk(a, c, geo, cfg, st);
+    return plan.pair ? cache8_pair(a, c, geo, cfg, st) : cache8_chunk(a, c, geo, cfg, st);
   }
   const DecodeCheck chk = {check && plan.inside && !plan.append ? host : nullptr, check && behind ? word : nullptr};
   const int r = c.code == FA_CODE_INT8 ? decode8_int8(a, c, cfg, plan.unit_rows, plan.geo, chk, behind, st)
@@ -146,12 +151,12 @@ int refused(const fa_decode_args& a, const Plan& plan) {
 
 }  // namespace
 
-size_t decode8_workspace_bytes(const fa_decode_args& a) { return empty(a) ? 0 : plan_of(a).bytes(); }
-int decode8_counters(const fa_decode_args& a) { return empty(a) ? 0 : plan_of(a).counters; }
+size_t decode8_workspace_bytes(const fa_decode_args& a, const fa_cache8& c) { return empty(a) ? 0 : plan_of(a, c).bytes(); }
+int decode8_counters(const fa_decode_args& a, const fa_cache8& c) { return empty(a) ? 0 : plan_of(a, c).counters; }
 
 int decode8_paged(const fa_decode_args& a, const fa_cache8& c, cudaStream_t st) {
   if (empty(a)) return FA_OK;
-  const Plan plan = plan_of(a);
+  const Plan plan = plan_of(a, c);
   if (int r = refused(a, plan)) return r;
   return run(a, c, plan, nullptr, nullptr, st);
 }
@@ -165,7 +170,7 @@ int decode8_paged_checked(const fa_decode_args& a, const fa_cache8& c, uint32_t*
     set_error("value checks cannot run while the stream is being captured; turn them off with set_validation(False)");
     return FA_ERR_LAUNCH;
   }
-  const Plan plan = plan_of(a);
+  const Plan plan = plan_of(a, c);
   if (int r = refused(a, plan)) return r;
   uint32_t* host = nullptr;
   const int slot = take_check_word(false, a.device, &host);

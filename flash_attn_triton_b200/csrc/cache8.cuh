@@ -1,6 +1,7 @@
 // Codes of the 8-bit KV cache: to 16-bit floats for the tensor cores, and from floats.
 #pragma once
 #include "cache_dev.cuh"
+#include "cache_geo.cuh"
 
 namespace fa {
 
@@ -98,5 +99,23 @@ inline int log2_of(int n) {
   return s;
 }
 __device__ __forceinline__ int divided(int x, int n, int shift) { return shift >= 0 ? x >> shift : x / n; }
+
+// Chunks of tokens: pieces that `all` key tiles of a unit are cut into.  A piece has the tiles that an SM would have if all work were
+// shared evenly, so that sequences longer than that do not set the time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128, 256
+// rows per CTA: 235 us in whole units, SPLIT cut).  Every warp works it out from the lengths; units: of a sequence.
+__device__ __forceinline__ int chunk_pieces(const fa_decode_args& p, const ScoreCfg& cfg, const CacheGeo& geo, int units, int all, int lane) {
+  if (geo.parts == 1) return 1;
+  int64_t tiles = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int cap = seq_capacity(p, b);
+    int keys = min(max(0, min(geo.seqlens[b], cap)) + geo.n_new, cap);
+    if (cfg.wl >= 0) keys = min(keys, cfg.wl + geo.tokens + 127);
+    tiles += (keys + 127) / 128;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+  const int even = max(4, (int)((tiles * units + geo.sms - 1) / geo.sms));
+  return max(1, min(min(geo.parts, all), (all + even - 1) / even));
+}
 
 }  // namespace fa

@@ -19,7 +19,6 @@
 
 #include "cache8.cuh"
 #include "cache8_host.h"
-#include "cache_geo.cuh"
 #include "sm100.cuh"
 
 namespace fa {
@@ -178,7 +177,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     visible_key_range(cfg, tq_min, tq_max, w.keys, klo, khi);
     const int lo = klo / kBN, hi = (khi + kBN - 1) / kBN;
     const int all = khi > klo ? hi - lo : 0;
-    w.parts = max(1, min(geo.parts, all));
+    w.parts = chunk_pieces(p, cfg, geo, (p.heads_q >> geo.pack_log2) * ((w.rows + kBM - 1) / kBM), all, lane);
     if (w.part >= w.parts) return;
     const int first = (int)((int64_t)w.part * all / w.parts), last = (int)((int64_t)(w.part + 1) * all / w.parts);
     w.n_hi = lo + last;

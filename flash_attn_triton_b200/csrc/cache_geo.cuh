@@ -17,6 +17,7 @@ struct CacheGeo {
   int tokens;              // query tokens of a sequence
   int pack_log2;           // query heads packed into the rows of a tile
   int parts;               // pieces the keys of a sequence are cut into, at most
+  int sms;                 // 8-bit cache: what a piece is sized for
   int capacity;            // keys a sequence can hold
   float* ws;               // pieces: fp32 outputs, then their base-2 LSEs
   uint32_t* counters;      // per unit, zero
