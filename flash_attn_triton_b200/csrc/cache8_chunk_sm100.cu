@@ -369,6 +369,14 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       scales_of(0, pg);
       pg = page_of(1);
       for (int j = 0; j < nt; ++j) {
+        // A scale of V that is no number or infinite goes to the scores instead, which the mask takes out where the key is hidden
+        // (0 times either would not be 0).
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(fabsf(vs[i]) <= 3.4e38f)) {
+            ks[i] = NAN;
+            vs[i] = 0.f;
+          }
         const float4 k4 = make_float4(ks[0], ks[1], ks[2], ks[3]), v4 = make_float4(vs[0], vs[1], vs[2], vs[3]);
         scales_of(j + 1, pg);
         pg = page_of(j + 2);
@@ -558,49 +566,43 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (!ok) break;
       tc_fence_after();
 
-      // The scores are read twice, 32 columns at a time: for the maximum, and for the exponentials (P of columns cc overwrites columns that
-      // have been read).  All 128 of a row do not fit beside the rest in what 512 threads have: 512 bytes of them were spilled, and a
-      // tile's exponentials took 4200 cycles.
-      const bool prescaled = kAlibi || masked;           // masked tiles and ALiBi go to the log2 domain at once
-      ColMask cm;
-      if (prescaled) {
+      // ---- scores times the scales of the keys: mg of each 16 keys turns them into the log2 domain.  Tiles with a mask, with ALiBi or with
+      // a scale per key go there at once, through tensor memory in a rolled loop: copies of the passes below for them cost the code that every
+      // tile runs 14 % (instruction cache).
+      const bool masked_or_fine = kAlibi || kFine || masked;
+      const float f = cfg.scale_log2 * qinv;
+      if (masked_or_fine) {
         int vk_lo, vk_hi;
         visible_k_interval(cfg, qpos, w.keys, vk_lo, vk_hi);
-        cm = make_col_mask(vk_lo - k0, vk_hi - k0);
-      }
-      const float f = cfg.scale_log2 * qinv, dist0 = (float)(qpos - k0), tilt = slope * FA_LOG2E;
-      // Columns cc * 32 + i in place, ready to be multiplied by mg (of each 16 keys) and exponentiated.
-      auto prepare = [&](auto log2_tag, int cc, uint32_t (&r)[32], float2& mg) {
-        if (kFine) {
-          mg = make_float2(f, f);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(&sh->ks[sb][cc * 32 + i]);
-            const float2 a = f2mul(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), make_float2(k4.x, k4.y));
-            const float2 b = f2mul(make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), make_float2(k4.z, k4.w));
-            r[i] = __float_as_uint(a.x);
-            r[i + 1] = __float_as_uint(a.y);
-            r[i + 2] = __float_as_uint(b.x);
-            r[i + 3] = __float_as_uint(b.y);
-          }
-        } else {
-          mg = f2mul(*reinterpret_cast<const float2*>(&sh->ks[sb][cc * 2]), make_float2(f, f));
-        }
-        if constexpr (decltype(log2_tag)::value) {
+        const float tilt = slope * FA_LOG2E;
+#pragma unroll 1
+        for (int cc = 0; cc < 4; ++cc) {
+          const ColMask cm = make_col_mask(vk_lo - k0 - cc * 32, vk_hi - k0 - cc * 32);
+          const float2 k2 = *reinterpret_cast<const float2*>(&sh->ks[sb][kFine ? 0 : cc * 2]);
+          const float dist0 = (float)(qpos - k0 - cc * 32);
+          uint32_t ra[32];
+          tmem_ld32(tS + cc * 32, ra);
+          tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            float v = __uint_as_float(r[i]) * (i < 16 ? mg.x : mg.y);
-            if (kAlibi) v = fmaf(-tilt, fabsf(dist0 - (float)(cc * 32 + i)), v);
-            r[i] = __float_as_uint(col_visible(cm, cc * 32 + i) ? v : -INFINITY);
+            float v = __uint_as_float(ra[i]) * (kFine ? sh->ks[sb][cc * 32 + i] : i < 16 ? k2.x : k2.y) * f;
+            if (kAlibi) v = fmaf(-tilt, fabsf(dist0 - (float)i), v);
+            ra[i] = __float_as_uint(col_visible(cm, i) ? v : -INFINITY);
           }
-          mg = make_float2(1.f, 1.f);
+          tmem_st32(tS + cc * 32, ra);
         }
+        tmem_wait_st();
+      }
+      auto factors = [&](int cc) {
+        return masked_or_fine ? make_float2(1.f, 1.f) : f2mul(*reinterpret_cast<const float2*>(&sh->ks[sb][cc * 2]), make_float2(f, f));
       };
 
       // ---- row maximum of t + log2 vs, vs by its largest of 16 keys -----------------------------
-      // (each pass is compiled apart for the tiles that go to the log2 domain first: what most tiles run stays small)
+      // The scores are read twice, 32 columns at a time: for the maximum, and for the exponentials (P of columns cc overwrites columns that
+      // have been read).  All 128 of a row do not fit beside the rest in what 512 threads have: 512 bytes of them were spilled, and a
+      // tile's exponentials took 4200 cycles.
       float mx = -INFINITY;
-      auto largest = [&](auto log2_tag) {
+      {
         uint32_t ra[32], rb[32];
         tmem_ld32(tS, ra);
 #pragma unroll
@@ -609,9 +611,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           uint32_t (&nxt)[32] = (cc & 1) ? ra : rb;
           tmem_wait_ld();
           if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, nxt);
-          float2 mg;
-          prepare(log2_tag, cc, cur, mg);
-          const float2 lv = *reinterpret_cast<const float2*>(&sh->lv[sb][cc * 2]);
+          const float2 mg = factors(cc), lv = *reinterpret_cast<const float2*>(&sh->lv[sb][cc * 2]);
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             const uint32_t* v = &cur[g * 16];
@@ -623,9 +623,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             mx = fmaxf(mx, fmaf(most, g ? mg.y : mg.x, g ? lv.y : lv.x));
           }
         }
-      };
-      if (prescaled) largest(std::true_type{});
-      else largest(std::false_type{});
+      }
 
       // ---- the maximum the exponents are relative to, settled in tile order ---------------
       float m_use;
@@ -650,7 +648,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           tc_fence_after();
           if (need) alpha = exp2f(m_old - mx);
           if (need) sh->mref[row_in_tile] = mx;
-#pragma unroll
+#pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t ro[32];
             tmem_ld32(tO + cc * 32, ro);
@@ -669,8 +667,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       // ---- p = exp2(t - M), row sum, p vs -> TMEM in place over S ----------------------------
       const float2 nm2 = make_float2(-m_safe, -m_safe);
       float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto weigh = [&](auto log2_tag) {
-        constexpr bool kMask = decltype(log2_tag)::value;
+      {
         uint32_t ra[32], rb[32];
         tmem_ld32(tS, ra);
 #pragma unroll
@@ -679,8 +676,8 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           uint32_t (&nxt)[32] = (cc & 1) ? ra : rb;
           tmem_wait_ld();
           if (cc < 3) tmem_ld32(tS + (cc + 1) * 32, nxt);
-          float2 mg, v16 = make_float2(0.f, 0.f);        // scales of V of the two 16 keys
-          prepare(log2_tag, cc, cur, mg);
+          const float2 mg = factors(cc);
+          float2 v16 = make_float2(0.f, 0.f);            // scales of V of the two 16 keys
           if (!kFine) v16 = *reinterpret_cast<const float2*>(&sh->vs[sb][cc * 2]);
           uint32_t pk[16];
 #pragma unroll
@@ -694,11 +691,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               const float2 a = f2fma(make_float2(__uint_as_float(cur[i + e]), __uint_as_float(cur[i + e + 1])), mul2, nm2);
               const float2 pe = make_float2(ex2(a.x), ex2(a.y));
               acc2[e >> 1] = f2add(acc2[e >> 1], pe);
-              float2 wt = f2mul(pe, e ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
-              if (kMask) {               // a hidden key weighs 0 whatever its scale is
-                wt.x = pe.x == 0.f ? 0.f : wt.x;
-                wt.y = pe.y == 0.f ? 0.f : wt.y;
-              }
+              const float2 wt = f2mul(pe, e ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
               pk[(i + e) >> 1] = Elem<__half>::pack(wt.x, wt.y);
             }
           }
@@ -709,9 +702,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             mbar_arrive(smem_u32(&sh->p_half[buf]));
           }
         }
-      };
-      if (prescaled) weigh(std::true_type{});
-      else weigh(std::false_type{});
+      }
       sum = (acc2[0].x + acc2[0].y) + (acc2[1].x + acc2[1].y);
       tmem_wait_st();
       tc_fence_before();
@@ -735,8 +726,8 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       l_all = sh->lrun[row_in_tile];
     }
     if (!failed) {
-      const float inv = l_all > 0.f ? 1.f / l_all : 0.f;
-      const float lse = l_all > 0.f ? m_fin + log2f(l_all) : -INFINITY;
+      const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+      const float lse = l_all == 0.f ? -INFINITY : m_fin + log2f(l_all);
       const bool row_ok = row < w.rows;
       const bool piece = w.parts > 1;
       const int64_t slot = blockIdx.x;
