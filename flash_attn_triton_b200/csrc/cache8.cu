@@ -74,7 +74,9 @@ Plan plan_of(const fa_decode_args& a, const fa_cache8& c) {
   }
   p.counter_bytes = a.counters ? 0 : (size_t)p.counters * sizeof(uint32_t);
   p.append = a.k_new != nullptr;
-  p.inside = (int64_t)a.batch * (a.block_table ? a.block_table_stride : 1) <= kInlineCheck && (p.append || !p.chunk);
+  // (an append has few CTAs: 16 x 84 entries, checked by a kernel of its own in front, cost a step of 45 us 5 of them)
+  p.inside = (int64_t)a.batch * (a.block_table ? a.block_table_stride : 1) <= (p.append ? 4 * kInlineCheck : kInlineCheck) &&
+             (p.append || !p.chunk);
   return p;
 }
 

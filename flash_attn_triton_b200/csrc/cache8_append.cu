@@ -73,7 +73,7 @@ struct Run {
 
 // kSlots: packed tokens; else those of the cache call d.  g.per_y (head, key or value) per CTA along y, 2^g.warps_log2 warps for one.
 template <typename T, int kCode, bool kSlots>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
     cache8_append_kernel(const Append8 p, const fa_decode_args d, const AppendGeom g, uint32_t* host, uint32_t* dev, bool check_here) {
   using C = Code<kCode>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -169,13 +169,16 @@ __global__ void __launch_bounds__(kThreads, 2)
                            (int64_t)at.row * p.c_stride[which][1] + h * p.c_stride[which][2];
     const int64_t code_stride = p.c_stride[which][1];
     const bool rotate = !kSlots && which == 0 && d.rotary_cos != nullptr;
-    auto load = [&](int j) {
-      const int row = j >> dshift, col = (j & ((1 << dshift) - 1)) * 8;
-      const T* src = x + row * row_stride;
+    // piece gl + k * gsize of a lane: the same column, gsize >> dshift rows on
+    const int row0 = gl >> dshift, col = (gl & ((1 << dshift) - 1)) * 8, rstep = gsize >> dshift;
+    const T* xl = x + row0 * row_stride + col;
+    const int64_t xstep = rstep * row_stride;
+    auto load = [&](int k) {
       if (rotate)
-        return rotary_chunk<T, true>(src, col, reinterpret_cast<const T*>(d.rotary_cos), reinterpret_cast<const T*>(d.rotary_sin), pos + row,
-                                     d.rotary_dim, d.rotary_interleaved, d.rotary_seqlen);
-      return *reinterpret_cast<const uint4*>(src + col);
+        return rotary_chunk<T, true>(xl - col + k * xstep, col, reinterpret_cast<const T*>(d.rotary_cos),
+                                     reinterpret_cast<const T*>(d.rotary_sin), pos + row0 + k * rstep, d.rotary_dim, d.rotary_interleaved,
+                                     d.rotary_seqlen);
+      return *reinterpret_cast<const uint4*>(xl + k * xstep);
     };
     // bit patterns without their sign order magnitudes, NaN above infinity above numbers
     uint32_t most = 0u;
@@ -186,12 +189,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
       const int j = gl + k * gsize;
-      held[k] = j < pieces ? load(j) : make_uint4(0u, 0u, 0u, 0u);
+      held[k] = j < pieces ? load(k) : make_uint4(0u, 0u, 0u, 0u);
     }
     const float old = run.kept > 0 ? *scale : 0.f;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) widen(held[k]);
-    for (int j = gl + kHeld * gsize; j < pieces; j += gsize) widen(load(j));
+    for (int k = kHeld; gl + k * gsize < pieces; ++k) widen(load(k));
     most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
     if (wlog > 0) {
       if (lane == 0) part[turn][warp] = most;
@@ -204,18 +207,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (need < 1.17549435e-38f) need = 0.f;
     const float now = old != old ? old : (need > old || need != need) ? need : old;
     const float inv = now > 0.f ? __frcp_rn(now) : now != now ? now : 0.f;
-    auto store = [&](int j, const uint4& v) {
-      const int row = j >> dshift, col = (j & ((1 << dshift) - 1)) * 8;
+    unsigned char* cl = codes + row0 * code_stride + col;
+    const int64_t cstep = rstep * code_stride;
+    auto store = [&](int k, const uint4& v) {
       const float2 a = Elem<T>::unpack(v.x), b = Elem<T>::unpack(v.y), c = Elem<T>::unpack(v.z), e = Elem<T>::unpack(v.w);
-      *reinterpret_cast<uint2*>(codes + row * code_stride + col) =
-          make_uint2(C::four(a.x, a.y, b.x, b.y, inv), C::four(c.x, c.y, e.x, e.y, inv));
+      *reinterpret_cast<uint2*>(cl + k * cstep) = make_uint2(C::four(a.x, a.y, b.x, b.y, inv), C::four(c.x, c.y, e.x, e.y, inv));
     };
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int j = gl + k * gsize;
-      if (j < pieces) store(j, held[k]);
-    }
-    for (int j = gl + kHeld * gsize; j < pieces; j += gsize) store(j, load(j));
+    for (int k = 0; k < kHeld; ++k)
+      if (gl + k * gsize < pieces) store(k, held[k]);
+    for (int k = kHeld; gl + k * gsize < pieces; ++k) store(k, load(k));
     if (run.kept > 0 && now > old) {
       const float m = __fmul_rn(old, inv);
       for (int j = gl; j < run.kept << (dshift - 1); j += gsize) {
@@ -296,12 +297,15 @@ static AppendGeom append_geometry(const Append8& p, int device) {
   g.warps_log2 = 0;
   while (g.warps_log2 < 3 && pieces > (32ll * kHeld << g.warps_log2)) ++g.warps_log2;
   const int groups = 8 >> g.warps_log2;
+  // A CTA per block and few heads where the tokens are few (a span shorter than a block leaves CTAs without a run, which is cheap as
+  // long as all run at once), all heads of a block where there are more blocks than CTAs.  2048 tokens, 8 heads of 128, blocks of 64: 30 us
+  // with spans of 2 tokens and all heads, FEW now; 25 k tokens: 52, MORE.
+  int64_t ny = (2 * p.heads + groups - 1) / groups;
   const int64_t most = p.block > 32 ? (p.block < kSpanMost ? p.block : kSpanMost) : 32;
   g.span = 1;
-  while (g.span * 2 <= most && (p.tokens + 2 * g.span - 1) / (2 * g.span) >= ctas) g.span *= 2;
+  while (g.span * 2 <= most && (p.tokens + 2 * g.span - 1) / (2 * g.span) * ny >= ctas) g.span *= 2;
   const int64_t nx = (p.tokens + g.span - 1) / g.span;
-  int64_t ny = (2 * p.heads + groups - 1) / groups;
-  if (nx * ny > ctas) ny = nx >= ctas ? 1 : (ctas + nx - 1) / nx;
+  while (ny > 1 && nx * ny > 4 * ctas) ny = (ny + 1) / 2;
   g.per_y = (int)((2 * p.heads + ny - 1) / ny);
   g.grid_x = (unsigned)nx;
   g.grid_y = (unsigned)((2 * p.heads + g.per_y - 1) / g.per_y);

@@ -406,12 +406,30 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       constexpr int QC = D / 8, NQ = kRows * QC / 256, kAtOnce = NQ < 8 ? NQ : 8;
       const T* cos = reinterpret_cast<const T*>(p.rotary_cos);
       const T* sin = reinterpret_cast<const T*>(p.rotary_sin);
+      // (rows past the last one read it and are cleared behind the loads: a branch around each load put them one behind the other, 8 us)
       auto load = [&](int k) {
-        const int i = k * 256 + tid, r = w.m0 + i / QC, d = i % QC * 8;
-        if (r >= w.rows) return make_uint4(0u, 0u, 0u, 0u);
+        const int i = k * 256 + tid, r = min(w.m0 + i / QC, w.rows - 1), d = i % QC * 8;
         const int tok = r >> geo.pack_log2, h = w.h + (r & ((1 << geo.pack_log2) - 1));
         const T* row = reinterpret_cast<const T*>(p.q) + w.b * p.q_stride[0] + tok * p.q_stride[1] + (int64_t)h * p.q_stride[2];
+        if (cos == nullptr) return *reinterpret_cast<const uint4*>(row + d);
         return rotary_chunk<T, true>(row, d, cos, sin, w.pos0 + tok + w.pad, p.rotary_dim, p.rotary_interleaved, p.rotary_seqlen);
+      };
+      auto load_all = [&](int k0, uint4* to) {
+        if (cos == nullptr) {
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) to[k] = load(k0 + k);
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < kAtOnce; ++k) {
+            const uint4 v = load(k0 + k);
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e)
+              if (e == k) to[e] = v;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          if (w.m0 + ((k0 + k) * 256 + tid) / QC >= w.rows) to[k] = make_uint4(0u, 0u, 0u, 0u);
       };
       auto store = [&](int k, uint4 v, float mul) {
         const int i = k * 256 + tid, r = i / QC, c = i % QC;
@@ -430,8 +448,7 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (std::is_same<T, __nv_bfloat16>::value) {
         uint32_t most = 0u;
         for (int k0 = NQ - kAtOnce; k0 >= 0; k0 -= kAtOnce) {        // the first ones stay
-#pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) held[k] = load(k0 + k);
+          load_all(k0, held);
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k) {
             const uint32_t* x = reinterpret_cast<const uint32_t*>(&held[k]);
@@ -455,8 +472,7 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       }
       for (int k0 = 0; k0 < NQ; k0 += kAtOnce) {
         if (k0 > 0 || !std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) held[k] = load(k0 + k);
+          load_all(k0, held);
         }
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) store(k0 + k, held[k], qmul);
