@@ -16,7 +16,7 @@ namespace fa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 4;          // slots of a thread, at least
+constexpr int kPerThread = 4;          // slots of a thread at a time
 
 struct Sums {
   int64_t tokens, pages;
@@ -127,26 +127,54 @@ __global__ void __launch_bounds__(kThreads) block_table_kernel(const fa_block_ta
       left -= taken;
     }
   }
-  for (int64_t i = from; i < p.num_slots; i += step) {
-    int64_t slot = -1;
-    if (i < all.tokens) {
-      const int s = stretch_of(first_token, (int)i);
-      int left = (int)i - first_token[s], b = s * per, pages = first_page[s];
-      for (;; ++b) {
-        const int64_t old = p.cache_seqlens[b];
-        const int fresh = p.new_lens[b], have = (int)pages_of(old);
-        if (left < fresh) {
-          const int64_t pos = old + left;
-          const int pi = (int)(page_shift >= 0 ? pos >> page_shift : pos / p.page_size);
-          const int page = pi < have ? p.block_table[(int64_t)b * p.table_stride + pi] : p.free_pages[pages + pi - have];
-          slot = (int64_t)page * p.page_size + (pos - (int64_t)pi * p.page_size);
-          break;
+  // kPerThread slots of a thread follow one another: one bisection for them
+  const bool pairs = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0;
+  for (int64_t i0 = from * kPerThread; i0 < p.num_slots; i0 += step * kPerThread) {
+    int64_t slot[kPerThread];
+    int left = 0, b = 0, fresh = 0, have = 0, first = 0;
+    int64_t old = 0;
+    const int n = (int)max((int64_t)0, min((int64_t)kPerThread, all.tokens - i0));
+    auto enter = [&]() {                         // request b; `first`: where its pages begin among the free ones
+      old = p.cache_seqlens[b];
+      fresh = p.new_lens[b];
+      have = (int)pages_of(old);
+    };
+    auto leave = [&]() {
+      left -= fresh;
+      first += (int)pages_of(old + fresh) - have;
+      ++b;
+    };
+    if (n > 0) {
+      const int s = stretch_of(first_token, (int)i0);
+      left = (int)i0 - first_token[s];
+      b = s * per;
+      first = first_page[s];
+      enter();
+    }
+#pragma unroll
+    for (int e = 0; e < kPerThread; ++e) {
+      slot[e] = -1;
+      if (e < n) {
+        while (left >= fresh) {
+          leave();
+          enter();
         }
-        left -= fresh;
-        pages += (int)pages_of(old + fresh) - have;
+        const int64_t pos = old + left;
+        const int pi = (int)(page_shift >= 0 ? pos >> page_shift : pos / p.page_size);
+        const int page = pi < have ? p.block_table[(int64_t)b * p.table_stride + pi] : p.free_pages[first + pi - have];
+        slot[e] = (int64_t)page * p.page_size + (pos - (int64_t)pi * p.page_size);
+        ++left;
       }
     }
-    p.slots[i] = slot;
+#pragma unroll
+    for (int e = 0; e < kPerThread; e += 2) {
+      if (pairs && i0 + e + 1 < p.num_slots) {
+        *reinterpret_cast<longlong2*>(p.slots + i0 + e) = make_longlong2(slot[e], slot[e + 1]);
+      } else {
+        if (i0 + e < p.num_slots) p.slots[i0 + e] = slot[e];
+        if (i0 + e + 1 < p.num_slots) p.slots[i0 + e + 1] = slot[e + 1];
+      }
+    }
   }
 }
 

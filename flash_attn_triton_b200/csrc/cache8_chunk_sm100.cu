@@ -477,7 +477,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     // ---- Q: rotated, to fp16 (bf16: times the power of two that brings the largest element of the tile to [2^14, 2^15)), swizzled
     float qinv = 1.f;
     {
-      constexpr int QC = D / 8, NQ = kBM * QC / 256, kAtOnce = NQ < 8 ? NQ : 8;
+      constexpr int QC = D / 8, NQ = kBM * QC / 256, kAtOnce = NQ < 16 ? NQ : 16;
       const T* cos = reinterpret_cast<const T*>(p.rotary_cos);
       const T* sin = reinterpret_cast<const T*>(p.rotary_sin);
       // (rows past the last one read it and are cleared behind the loads: a branch around each load put them one behind the other, 8 us)
