@@ -484,6 +484,11 @@ static bool mult16(const int64_t* s, int n) {
     if (s[i] % 16 != 0) return false;
   return true;
 }
+static bool below_64g(const int64_t* s, int n) {       // strides in 16 bytes are held in 32 bits
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0 || s[i] >= (int64_t)1 << 36) return false;
+  return true;
+}
 static int validate_cache8(const fa_cache8& c, int page_size, int num_pages, const void* k_cache, const void* v_cache, const int64_t* ks,
                            const int64_t* vs) {
   FA_REQUIRE(c.code == FA_CODE_INT8 || c.code == FA_CODE_E4M3, "code must be FA_CODE_INT8 or FA_CODE_E4M3");
@@ -492,6 +497,7 @@ static int validate_cache8(const fa_cache8& c, int page_size, int num_pages, con
   FA_REQUIRE(num_pages >= 0, "negative size");
   FA_REQUIRE(k_cache && v_cache && c.k_scale && c.v_scale, "8-bit caches and their scales are required");
   FA_REQUIRE(aligned16(k_cache) && aligned16(v_cache) && mult16(ks, 3) && mult16(vs, 3), "cache rows must be 16-byte aligned");
+  FA_REQUIRE(below_64g(ks, 3) && below_64g(vs, 3), "cache strides must not be negative and must be below 64 GiB");
   return FA_OK;
 }
 static int validate_decode8(const fa_decode_args* a, const fa_cache8* c) {

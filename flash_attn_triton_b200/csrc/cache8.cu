@@ -7,9 +7,9 @@
 
 namespace fa {
 
-int decode8_int8(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
-int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const DecodeGeom&, const DecodeCheck&, bool, cudaStream_t);
-DecodeGeom decode8_geometry(const fa_decode_args& a, int unit_rows, int row_groups);
+int decode8_int8(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const Geom8&, const DecodeCheck&, bool, cudaStream_t);
+int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, const Geom8&, const DecodeCheck&, bool, cudaStream_t);
+Geom8 decode8_geometry(const fa_decode_args& a, const fa_cache8& c, int unit_rows, int row_groups);
 int cache8_chunk(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
 int cache8_pair(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
 int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st);
@@ -25,7 +25,7 @@ int unit_rows_of(const fa_decode_args& a) { return a.seqlen_q * (a.heads_q / a.h
 struct Plan {
   bool chunk, pair;                    // pair: 256 query rows per CTA
   int unit_rows;                       // decode
-  DecodeGeom geo;
+  Geom8 geo;
   int pack_log2, parts, capacity;      // chunk
   size_t piece_bytes, counter_bytes;
   int counters;
@@ -68,8 +68,8 @@ Plan plan_of(const fa_decode_args& a, const fa_cache8& c) {
     p.unit_rows = unit_rows_of(a);
     const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
     const int groups = (int)((rows + p.unit_rows - 1) / p.unit_rows);
-    p.geo = decode8_geometry(a, p.unit_rows, groups);
-    p.piece_bytes = p.geo.splits == 1 ? 0 : (size_t)p.geo.shares * a.seqlen_q * a.heads_q * (a.head_dim + 1) * sizeof(float);
+    p.geo = decode8_geometry(a, c, p.unit_rows, groups);
+    p.piece_bytes = p.geo.splits == 1 ? 0 : (size_t)p.geo.rows * a.seqlen_q * a.heads_q * (a.head_dim + 1) * sizeof(float);
     p.counters = p.piece_bytes ? a.batch * a.heads_kv * groups : 0;
   }
   p.counter_bytes = a.counters ? 0 : (size_t)p.counters * sizeof(uint32_t);

@@ -1,5 +1,6 @@
 // Codes of the 8-bit KV cache: to 16-bit floats for the tensor cores, and from floats.
 #pragma once
+#include "cache8_host.h"
 #include "cache_dev.cuh"
 #include "cache_geo.cuh"
 
@@ -98,6 +99,8 @@ inline int log2_of(int n) {
   while ((1 << s) < n) ++s;
   return s;
 }
+// x / n for 0 <= x < 2^31 by one product: m = ceil(2^(31 + l) / n) with 2^l >= n is too large by less than n / 2^31 of itself.
+__device__ __forceinline__ int divided(int x, const Div32& d) { return (int)(((uint64_t)(uint32_t)x * d.m) >> d.shift); }
 __device__ __forceinline__ int divided(int x, int n, int shift) { return shift >= 0 ? x >> shift : x / n; }
 
 // Chunks of tokens: pieces that `all` key tiles of a unit are cut into.  A piece has the tiles that an SM would have if all work were

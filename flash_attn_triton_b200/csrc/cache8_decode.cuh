@@ -3,8 +3,8 @@
 //
 //   Mathematics.  With codes k8, v8 and scales ks, vs of the block a key j is in:
 //     t_j = scale * ks_j * (q . k8_j),   out = sum_j p_j vs_j v8_j / sum_j p_j,   p_j = 2^(t_j - M).
-//   M is the running maximum of t_j + log2 vs_j, so that the weights p_j vs_j that go to the tensor cores as fp16 are at most about 1,
-//   however much the scales of the blocks differ; the sum of the p_j is in fp32, whose range takes the offset.
+//   M follows the maximum of t_j + log2 vs_j (at most 8 behind), so that the weights p_j vs_j that go to the tensor cores as fp16 are at most
+//   2^8, however much the scales of the blocks differ; the sum of the p_j is in fp32, whose range takes the offset.
 //   Operands.  Codes are fp16 exactly.  bf16 queries are multiplied by the power of two that brings the largest of a unit to [2^14, 2^15);
 //   elements more than 2^32 below it lose bits, nothing else does.
 //   Fragments.  Both tiles are read by ldmatrix in units of two bytes.  The head dimension of q . k8 may come in any order: a lane takes
@@ -14,6 +14,7 @@
 //   int8 codes go to the tensor cores as (code + 128) * 2^-24, which is a byte permutation; what the 128 adds is the same for all keys of
 //   a row in the scores, where the accumulators start from its negative, and a product with a constant in the outputs.
 //   Scales travel with their tile, by 4-byte cp.async.
+//   Split: see the ranges in the kernel.
 //   Bound.  HBM: one byte per code.
 #pragma once
 #include <atomic>
@@ -46,7 +47,21 @@ template <int D, int kRows> struct Decode8 {
     return kChunks >= 8 ? row & 7 : kChunks == 4 ? (row >> 1) & 3 : kChunks == 2 ? (row >> 2) & 1 : 0;
   }
 };
-constexpr int kLongest8 = 32;          // tiles of the largest piece that is still run in one wave of CTAs
+constexpr int kLongest8 = 32;          // tiles of the largest range that is still run in one wave of CTAs
+constexpr float kRaise = 8.f;          // log2 of the largest weight that the maximum is not raised for
+constexpr int kWaves8 = 4;             // waves of CTAs beyond that
+// Ranges that the `all` tiles of a unit are cut into, of U units; the host's grid is for a full cache.
+__host__ __device__ __forceinline__ int ranges8(int resident, int U, int64_t all, int longest) {
+  const int once = resident / U;
+  if (once == 0 || all > (int64_t)kLongest8 * once) {
+    const int n = kWaves8 * resident / U;
+    return (int)(n < 1 ? 1 : n < all ? n : all);
+  }
+  const float most = ceilf(sqrtf(7.f * longest));
+  const int size = (int)ceilf((float)longest / most);
+  const int64_t n = (all + size - 1) / size;
+  return (int)(n < once ? n : once);
+}
 
 // Sequence b after the append: keys the cache holds of it, positions of its tokens, the tiles that any query row sees.
 struct Seq8 {
@@ -66,7 +81,7 @@ __device__ __forceinline__ Seq8 seq8(const fa_decode_args& p, const ScoreCfg& cf
 
 template <typename T, int kCode, int D, int kRows>
 __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
-    decode8_kernel(const fa_decode_args p, const fa_cache8 c8, const int block_shift, const ScoreCfg cfg, const DecodeGeom geo,
+    decode8_kernel(const fa_decode_args p, const fa_cache8 c8, const ScoreCfg cfg, const Geom8 geo,
                    const DecodeCheck chk, const bool behind) {
   using SM = Decode8<D, kRows>;
   using C = Code<kCode>;
@@ -97,15 +112,67 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   const int u = blockIdx.x % U, share = blockIdx.x / U;
   const int hk = u / geo.row_groups, rg = u % geo.row_groups;
 
+  // ---- this CTA's range of tiles -----------------------------------------------------------------
+  // The tiles of the unit in all sequences, one after another, are cut into n equal ranges, however the sequences lie in them: one wave of
+  // CTAs while that needs no more than kLongest8 tiles each (but no sequence is cut into more than sqrt(7 nt) pieces), else kWaves8
+  // full waves.  (Pieces of equal size within each sequence left the last wave partly empty: 20 sequences with a window of 4095, 16 heads
+  // over 4 of 256: 54 us, RANGES now; 64 of 1024 to 32768, 32 over 8 of 128: 397, RANGES.)  Every warp works its range out; lane i sums
+  // the sequences [i per, (i + 1) per).
+  auto tiles = [&](int i) { return seq8<kTile8>(p, cfg, geo.max_tiles, i).nt; };
+  int b = 0, n = 1;                              // sequence; ranges
+  int64_t all = 0, off = 0, pos = 0, end = 0;    // tiles in all; before sequence b; the range that is left
+  if (geo.splits == 0) {
+    const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
+    int sum = 0, longest = 0;
+    for (int i = b0; i < b1; ++i) {
+      const int nt = tiles(i);
+      sum += nt;
+      longest = max(longest, nt);
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    all = __shfl_sync(0xffffffffu, inc, 31);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    n = ranges8(geo.resident, U, all, longest);
+    if (share < n) {
+      pos = share * all / n;
+      end = (share + 1) * all / n;
+      const int src = __ffs(__ballot_sync(0xffffffffu, pos >= inc - sum && pos < inc)) - 1;
+      b = __shfl_sync(0xffffffffu, b0, src);
+      off = __shfl_sync(0xffffffffu, inc - sum, src);
+      for (;; ++b) {
+        const int nt = tiles(b);
+        if (pos < off + nt) break;
+        off += nt;
+      }
+    }
+  } else {
+    // pieces of equal size of sequence b; a range is one of them
+    b = share / geo.splits;
+    const int nt = tiles(b), part = share - b * geo.splits;
+    n = min(geo.splits, nt);
+    all = nt;
+    if (part < n) {
+      pos = (int64_t)part * nt / n;
+      end = (int64_t)(part + 1) * nt / n;
+    }
+  }
   // Behind the append or the checks (a programmatic launch): what the caller brought may be read before they are done, the cache and
   // their result may not.
-  Piece piece;
-  const bool work = piece_of<kLongest8>(geo, p.batch, share, U, lane, [&](int i) { return seq8<kTile8>(p, cfg, geo.max_tiles, i).nt; }, piece);
   if (behind) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!work || (chk.dev && *chk.dev)) return;
-  const int b = piece.b, parts = piece.parts, base = piece.base, count = piece.count;
+  if (chk.dev && *chk.dev) return;
+
+  for (; pos < end; __syncthreads()) {
   const Seq8 w = seq8<kTile8>(p, cfg, geo.max_tiles, b);
-  const int len = w.len, keys = w.keys, tile0 = w.lo + piece.tile0;
+  const int len = w.len, keys = w.keys, tile0 = w.lo + (int)(pos - off), count = (int)(min(end, off + w.nt) - pos);
+  // pieces of the sequence: the ranges that it lies in; they have rows first, first + 1, ... of the workspace
+  const int64_t in0 = geo.splits ? 0 : ((off + 1) * n + all - 1) / all - 1, in1 = geo.splits ? n - 1 : ((off + w.nt) * n + all - 1) / all - 1;
+  const int parts = (int)(in1 - in0) + 1;
+  const int64_t first = geo.splits ? (int64_t)b * geo.splits : in0 + b, mine = geo.splits ? share : share + b;
 
   // ---- loading --------------------------------------------------------------------------
   const int lc = (lane % CPR) * 16, lr = lane / CPR;        // this lane's 16-byte column and first row
@@ -118,96 +185,103 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
 #pragma unroll
     for (int h = 0; h < KB; ++h) {
       const int key = ld * kTile8 + warp * KW + h * 16;
-      const int pi = table ? divided(key, p.page_size, geo.page_shift) : 0;
+      const int pi = table ? divided(key, geo.page) : 0;
       page[h] = table == nullptr ? (p.cache_batch_idx ? p.cache_batch_idx[b] : b) : key < keys ? table[pi] : 0;
       row16[h] = table ? key - pi * p.page_size : key + pad;
     }
   };
   const unsigned char* kb = static_cast<const unsigned char*>(p.k_cache) + (int64_t)hk * p.kc_stride[2] + lc;
   const unsigned char* vb = static_cast<const unsigned char*>(p.v_cache) + (int64_t)hk * p.vc_stride[2] + lc;
+  // Addresses by products of 32 bits into 64: with general strides and divisions the loads were 400 of the 780 instructions of a tile, and
+  // the step over 2 GB of cache took 400 us instead of LEAN.
+  auto row_of = [&](bool value, int pg, int row) {
+    const uint64_t at = (uint64_t)(uint32_t)pg * (value ? geo.v_page : geo.k_page) + (uint64_t)(uint32_t)row * (value ? geo.v_row : geo.k_row);
+    return (value ? vb : kb) + at * 16;
+  };
   const float* ksb = c8.k_scale + (int64_t)hk * c8.ks_stride[2];
   const float* vsb = c8.v_scale + (int64_t)hk * c8.vs_stride[2];
   if (whole) ld_page();
-  auto load_tile = [&](int st) {
-    if (ld == tile0 + count) return;
-    const int key00 = ld * kTile8 + warp * KW;
-    // (row at + lr; at is a multiple of a power of two above lr)
-    const uint32_t dK = smem_u32(ring) + (uint32_t)((st * 4 + warp) * 2 * KW + lr) * P, dV = dK + KW * P;
-    auto column = [&](int at) { return (uint32_t)(lc ^ (SM::turn(lr) << 4) ^ (SM::turn(at) << 4)); };
-    float* dS = sS + (st * 4 + warp) * 2 * KW;
-    if (whole) {
-      if (KW == 32 || lane < KW) {
-        const int h = KB > 1 ? lane >> 4 : 0;
-        const int pg = KB > 1 && h ? page[KB - 1] : page[0], row = (KB > 1 && h ? row16[KB - 1] : row16[0]) + (lane & 15);
-        const int blk = divided(row, c8.block, block_shift), bytes = key00 + lane < keys ? 4 : 0;
-        cp_async4(smem_u32(dS + lane), bytes ? ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1] : ksb, bytes);
-        cp_async4(smem_u32(dS + KW + lane), bytes ? vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1] : vsb, bytes);
-      }
-      const bool all = key00 + KW <= keys;
-      if (RPW <= 16) {                 // a pass lies inside 16 keys
+  // Keys (with the scales of both) or values of tile `ld` to a stage, as a cp.async group of their own: a stage's keys make room for
+  // keys ahead as soon as the scores are computed.  With a group and a wait per tile there was a third less on its way: MEASURED.
+  auto load_half = [&](int st, bool value) {
+    if (ld < tile0 + count) {
+      const int key00 = ld * kTile8 + warp * KW;
+      // (row at + lr; at is a multiple of a power of two above lr)
+      const uint32_t dst = smem_u32(ring) + (uint32_t)(((st * 4 + warp) * 2 + value) * KW + lr) * P;
+      auto column = [&](int at) { return (uint32_t)(lc ^ (SM::turn(lr) << 4) ^ (SM::turn(at) << 4)); };
+      const unsigned char* base = value ? vb : kb;
+      float* dS = sS + (st * 4 + warp) * 2 * KW;
+      if (whole) {
+        if (!value && (KW == 32 || lane < KW)) {
+          const int h = KB > 1 ? lane >> 4 : 0;
+          const int pg = KB > 1 && h ? page[KB - 1] : page[0], row = (KB > 1 && h ? row16[KB - 1] : row16[0]) + (lane & 15);
+          const int blk = divided(row, geo.block), bytes = key00 + lane < keys ? 4 : 0;
+          cp_async4(smem_u32(dS + lane), bytes ? ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1] : ksb, bytes);
+          cp_async4(smem_u32(dS + KW + lane), bytes ? vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1] : vsb, bytes);
+        }
+        const bool all_in = key00 + KW <= keys;
+        if (RPW <= 16) {               // a pass lies inside 16 keys
 #pragma unroll
-        for (int h = 0; h < KB; ++h) {
-          const unsigned char* ks = kb + (int64_t)page[h] * p.kc_stride[0] + (int64_t)(row16[h] + lr) * p.kc_stride[1];
-          const unsigned char* vs = vb + (int64_t)page[h] * p.vc_stride[0] + (int64_t)(row16[h] + lr) * p.vc_stride[1];
-          const int64_t kstep = RPW * p.kc_stride[1], vstep = RPW * p.vc_stride[1];
+          for (int h = 0; h < KB; ++h) {
+            const unsigned char* src = row_of(value, page[h], row16[h] + lr);
+            const uint32_t step = (value ? geo.v_row : geo.k_row) * RPW;
 #pragma unroll
-          for (int i = 0; i < PASSES / KB; ++i) {
-            const int at = (h * (PASSES / KB) + i) * RPW;
-            if (all) {
-              cp_async16(dK + at * P + column(at), ks);
-              cp_async16(dV + at * P + column(at), vs);
-            } else {                   // rows past the last key are zero-filled
-              const int bytes = key00 + at + lr < keys ? 16 : 0;
-              cp_async16(dK + at * P + column(at), bytes ? ks : kb, bytes);
-              cp_async16(dV + at * P + column(at), bytes ? vs : vb, bytes);
+            for (int i = 0; i < PASSES / KB; ++i) {
+              const int at = (h * (PASSES / KB) + i) * RPW;
+              const unsigned char* x = src + (uint64_t)step * (16 * i);
+              if (all_in) {
+                cp_async16(dst + at * P + column(at), x);
+              } else {                 // rows past the last key are zero-filled
+                const int bytes = key00 + at + lr < keys ? 16 : 0;
+                cp_async16(dst + at * P + column(at), bytes ? x : base, bytes);
+              }
             }
-            ks += kstep;
-            vs += vstep;
+          }
+        } else if (lr < KW) {          // one pass takes them all
+          const bool up = KB > 1 && lr >= 16;
+          const int pg = up ? page[KB - 1] : page[0], row = (up ? row16[KB - 1] : row16[0]) + (lr & 15), bytes = key00 + lr < keys ? 16 : 0;
+          cp_async16(dst + column(0), bytes ? row_of(value, pg, row) : base, bytes);
+        }
+      } else {                         // pages of any size: every row is looked up
+        auto where = [&](int key, int& pg, int& row) {
+          const int pi = divided(key, geo.page);
+          row = key - pi * p.page_size;
+          pg = table[pi];
+        };
+        if (!value && (KW == 32 || lane < KW)) {
+          int pg = 0, row = 0;
+          const int bytes = key00 + lane < keys ? 4 : 0;
+          if (bytes) where(key00 + lane, pg, row);
+          const int blk = divided(row, geo.block);
+          cp_async4(smem_u32(dS + lane), ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1], bytes);
+          cp_async4(smem_u32(dS + KW + lane), vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1], bytes);
+        }
+        if (lr < KW) {
+#pragma unroll 1
+          for (int i = 0; i < PASSES; ++i) {
+            const int key = key00 + i * RPW + lr, bytes = key < keys ? 16 : 0;
+            int pg = 0, row = 0;
+            if (bytes) where(key, pg, row);
+            cp_async16(dst + i * RPW * P + column(i * RPW), row_of(value, pg, row), bytes);
           }
         }
-      } else if (lr < KW) {            // one pass takes them all
-        const bool up = KB > 1 && lr >= 16;
-        const int pg = up ? page[KB - 1] : page[0], row = (up ? row16[KB - 1] : row16[0]) + (lr & 15), bytes = key00 + lr < keys ? 16 : 0;
-        cp_async16(dK + column(0), bytes ? kb + (int64_t)pg * p.kc_stride[0] + (int64_t)row * p.kc_stride[1] : kb, bytes);
-        cp_async16(dV + column(0), bytes ? vb + (int64_t)pg * p.vc_stride[0] + (int64_t)row * p.vc_stride[1] : vb, bytes);
       }
-    } else {                           // pages of any size: every row is looked up
-      auto where = [&](int key, int& pg, int& row) {
-        const int pi = divided(key, p.page_size, geo.page_shift);
-        row = key - pi * p.page_size;
-        pg = table[pi];
-      };
-      if (KW == 32 || lane < KW) {
-        int pg = 0, row = 0;
-        const int bytes = key00 + lane < keys ? 4 : 0;
-        if (bytes) where(key00 + lane, pg, row);
-        const int blk = divided(row, c8.block, block_shift);
-        cp_async4(smem_u32(dS + lane), ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1], bytes);
-        cp_async4(smem_u32(dS + KW + lane), vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1], bytes);
-      }
-      if (lr < KW) {
-#pragma unroll 1
-        for (int i = 0; i < PASSES; ++i) {
-          const int key = key00 + i * RPW + lr, bytes = key < keys ? 16 : 0;
-          int pg = 0, row = 0;
-          if (bytes) where(key, pg, row);
-          cp_async16(dK + i * RPW * P + column(i * RPW), kb + (int64_t)pg * p.kc_stride[0] + (int64_t)row * p.kc_stride[1], bytes);
-          cp_async16(dV + i * RPW * P + column(i * RPW), vb + (int64_t)pg * p.vc_stride[0] + (int64_t)row * p.vc_stride[1], bytes);
-        }
+      if (value) {
+        ++ld;
+        if (whole) ld_page();
       }
     }
-    ++ld;
-    if (whole) ld_page();
+    cp_async_commit();
   };
 
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
-    load_tile(i);
-    cp_async_commit();
+    load_half(i, false);
+    load_half(i, true);
   }
 
   float* ws_o = reinterpret_cast<float*>(p.workspace);
-  float* ws_l = ws_o + (int64_t)(gridDim.x / U) * p.heads_kv * R * D;
+  float* ws_l = ws_o + (int64_t)geo.rows * p.heads_kv * R * D;
   int stage = 0;
 
   // ---- Q rows (rotary fused) -> shared memory as fp16 -> B fragments held in registers ------------
@@ -315,19 +389,24 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
     lrow[n][0] = lrow[n][1] = 0.f;
   }
   const float kmul = qinv * (1.f / C::kUnit);
+  load_half(NS - 1, false);                      // (the queries went through this stage)
+  load_half(NS - 1, true);
 
   for (int ti = 0; ti < count; ++ti) {
     const int keyw = (tile0 + ti) * kTile8 + warp * KW;  // this warp's first key
-    cp_async_wait<NS - 2>();
+    cp_async_wait<2 * NS - 1>();
     __syncwarp();
-    load_tile(stage == 0 ? NS - 1 : stage - 1);
-    cp_async_commit();
     // this lane's row and chunk of both tiles for ldmatrix
     const uint32_t tK = smem_u32(ring) + (uint32_t)(stage * 4 + warp) * 2 * KW * P + (lane & 15) * P, tV = tK + KW * P;
     const uint32_t turned = (uint32_t)((D > 16 ? lane >> 4 : 0) ^ SM::turn(lane & 15)) << 4;
     const float* tS = sS + (stage * 4 + warp) * 2 * KW;
+    const int here = stage;
     if (++stage == NS) stage = 0;
-    if (keyw >= keys) continue;
+    if (keyw >= keys) {                          // (the last tile)
+      cp_async_commit();
+      cp_async_commit();
+      continue;
+    }
     // scales of this lane's keys keyw + 16 h + g and + 8; log2 of those of V: a block of zeros has a small one
     float ks[KB][2], vs[KB][2], lv[KB][2];
 #pragma unroll
@@ -369,6 +448,8 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
         }
       }
     }
+    __syncwarp();
+    load_half(here, false);
     // ---- softmax --------------------------------------------------------------------------
     const bool full = !cfg.has_alibi && keyw + KW <= keys && (!cfg.causal || keyw + KW - 1 <= qmin) &&
                       (cfg.wl < 0 || keyw >= qmax - cfg.wl) && (cfg.wr < 0 || keyw + KW - 1 <= qmin + cfg.wr);
@@ -398,13 +479,14 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
         }
       }
     }
+    // Raised only where a weight would pass 2^kRaise: of 8 rows one has a new maximum in more than half of the tiles of a range.
     bool grow = false;
 #pragma unroll
     for (int h = 0; h < KB; ++h) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) grow |= s[h][n][e] + lv[h][e >> 1] > mrow[n][e & 1];
+        for (int e = 0; e < 4; ++e) grow |= s[h][n][e] + (lv[h][e >> 1] - kRaise) > mrow[n][e & 1];
       }
     }
     if (__any_sync(0xffffffffu, grow)) {
@@ -451,6 +533,8 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
       }
     }
     // ---- O^T += V^T P^T -----------------------------------------------------------------
+    cp_async_wait<2 * NS - 1>();
+    __syncwarp();
     if (C::kBias) {
       const uint32_t a[4] = {C::kBias, C::kBias, C::kBias, C::kBias};
 #pragma unroll
@@ -475,6 +559,8 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
         }
       }
     }
+    __syncwarp();
+    load_half(here, true);
   }
 
   // ---- merge the 4 warps (each saw a quarter of every tile) -----------------------------------
@@ -510,7 +596,7 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
 
   // ---- output, or a piece of it -----------------------------------------------------------
   // workspace: the R query rows of every (piece, kv head), not padded to units
-  const int64_t ws_row = ((int64_t)share * p.heads_kv + hk) * R + rg * kRows;
+  const int64_t ws_row = (mine * p.heads_kv + hk) * R + rg * kRows;
   for (int i = tid; i < kRows * (D / 4); i += NT) {
     const int r = i / (D / 4), c4 = (i % (D / 4)) * 4;
     const int gr = rg * kRows + r;
@@ -558,15 +644,21 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
       for (int i = tid; i < rows * (D / 4); i += NT) {
         const int r = i / (D / 4), gr = rg * kRows + r;
         const int sq = gr / G, h = hk * G + gr % G;
-        merge_pieces<T, D>(ws_o, ws_l, ((int64_t)base * p.heads_kv + hk) * R + gr, (int64_t)p.heads_kv * R, parts, (i % (D / 4)) * 4,
+        merge_pieces<T, D>(ws_o, ws_l, (first * p.heads_kv + hk) * R + gr, (int64_t)p.heads_kv * R, parts, (i % (D / 4)) * 4,
                            reinterpret_cast<T*>(p.o) + b * p.o_stride[0] + sq * p.o_stride[1] + (int64_t)h * p.o_stride[2]);
       }
     }
   }
+  // the next sequence of the range
+  cp_async_wait<0>();
+  pos += count;
+  off += w.nt;
+  ++b;
+  }
 }
 
 template <typename T, int kCode, int D, int kRows>
-static int launch_decode8_rows(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cfg, const DecodeGeom& g, const DecodeCheck& chk,
+static int launch_decode8_rows(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cfg, const Geom8& g, const DecodeCheck& chk,
                                bool behind, cudaStream_t st) {
   auto kern = decode8_kernel<T, kCode, D, kRows>;
   const size_t smem = Decode8<D, kRows>::smem;
@@ -582,7 +674,7 @@ static int launch_decode8_rows(const fa_decode_args& a, const fa_cache8& c, cons
   }
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr;
-  lc.gridDim = dim3((unsigned)g.shares * a.heads_kv * g.row_groups);
+  lc.gridDim = dim3((unsigned)g.ranges * a.heads_kv * g.row_groups);
   lc.blockDim = dim3(128);
   lc.dynamicSmemBytes = smem;
   lc.stream = st;
@@ -592,19 +684,19 @@ static int launch_decode8_rows(const fa_decode_args& a, const fa_cache8& c, cons
     lc.attrs = &attr;
     lc.numAttrs = 1;
   }
-  cudaLaunchKernelEx(&lc, kern, a, c, log2_of(c.block), cfg, g, chk, behind);
+  cudaLaunchKernelEx(&lc, kern, a, c, cfg, g, chk, behind);
   return check_launch("decode8");
 }
 
 template <typename T, int kCode, int D>
-static int launch_decode8_dim(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cfg, int unit_rows, const DecodeGeom& g,
+static int launch_decode8_dim(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cfg, int unit_rows, const Geom8& g,
                               const DecodeCheck& chk, bool behind, cudaStream_t st) {
   return unit_rows == 8 ? launch_decode8_rows<T, kCode, D, 8>(a, c, cfg, g, chk, behind, st)
                         : launch_decode8_rows<T, kCode, D, 16>(a, c, cfg, g, chk, behind, st);
 }
 
 template <typename T, int kCode>
-static int launch_decode8(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cfg, int unit_rows, const DecodeGeom& g,
+static int launch_decode8(const fa_decode_args& a, const fa_cache8& c, const ScoreCfg& cfg, int unit_rows, const Geom8& g,
                           const DecodeCheck& chk, bool behind, cudaStream_t st) {
   switch (a.head_dim) {
     case 16: return launch_decode8_dim<T, kCode, 16>(a, c, cfg, unit_rows, g, chk, behind, st);

@@ -25,6 +25,30 @@ struct AppendGeom {
   unsigned grid_x, grid_y;
 };
 
+// A division by n that kernels make by a product.
+struct Div32 {
+  uint32_t m;
+  int shift;
+};
+inline Div32 div_by(int n) {
+  int l = 0;
+  while ((1ll << l) < n) ++l;
+  const int shift = 31 + l;
+  return Div32{(uint32_t)(((1ull << shift) + (uint64_t)n - 1) / (uint64_t)n), shift};
+}
+
+// Decode: how a call is cut, and where its cache lies (strides in 16 bytes: an address is then two 32-bit products).
+struct Geom8 {
+  int ranges;      // CTAs per unit
+  int rows;        // of the workspace: pieces
+  int splits;      // 0: ranges sized on the device; else that many pieces of every sequence
+  int resident;    // CTAs the GPU runs at a time
+  int max_tiles;   // tiles of a full cache
+  int row_groups;  // ceil(seqlen_q * group / rows of a unit)
+  Div32 page, block;
+  uint32_t k_page, k_row, v_page, v_row;
+};
+
 Append8 append_of(const fa_decode_args& call, const fa_cache8& cache);
 // call: a cache call (null: packed tokens).  host, dev, check_here: value checks as in cache_append_kernel.
 int append8_launch(const Append8& p, const fa_decode_args* call, int dtype, int code, int device, uint32_t* host, uint32_t* dev,

@@ -227,8 +227,7 @@ __device__ __forceinline__ SeqTiles seq_tiles(const fa_decode_args& p, const Sco
 struct Piece {
   int b, tile0, count, parts, base;
 };
-// kLongest: largest piece that is still run in one wave; kCost: a tile's time over that of a piece in the merge.
-template <int kLongest = kOneWave, int kCost = 7, typename Tiles>
+template <typename Tiles>
 __device__ __forceinline__ bool piece_of(const DecodeGeom& geo, int batch, int share, int U, int lane, Tiles tiles, Piece& out) {
   int b, parts, base;
   if (geo.splits == 0) {
@@ -249,11 +248,11 @@ __device__ __forceinline__ bool piece_of(const DecodeGeom& geo, int batch, int s
       mine = 0;
       for (int i = b0; i < b1; ++i) mine += (tiles(i) + size - 1) / size;
     };
-    if (size > kLongest) {
-      size = max(kLongest / 2, (int)((work + kWaves * geo.resident - 1) / (kWaves * geo.resident)));
+    if (size > kOneWave) {
+      size = max(kOneWave / 2, (int)((work + kWaves * geo.resident - 1) / (kWaves * geo.resident)));
       count_pieces();
     } else {
-      size = max(size, (int)ceilf((float)longest / ceilf(sqrtf((float)kCost * longest))));
+      size = max(size, (int)ceilf((float)longest / ceilf(sqrtf(7.f * longest))));
       for (; size < longest; size += max(1, size >> 3)) {
         count_pieces();
         if (__reduce_add_sync(0xffffffffu, mine) * U <= geo.resident) break;
@@ -369,11 +368,11 @@ inline int page_shift_of(const fa_decode_args& a) {
 //     bandwidth).
 // An explicit num_splits, and batches too large to sum in every warp, cut every sequence into the
 // same number of pieces.
-inline DecodeGeom decode_geometry(const fa_decode_args& a, int row_groups, int ctas_per_sm, int tile = kTile, int longest = kOneWave) {
+inline DecodeGeom decode_geometry(const fa_decode_args& a, int row_groups, int ctas_per_sm) {
   DecodeGeom g;
   g.row_groups = row_groups;
   const int64_t cap = a.block_table ? (int64_t)a.block_table_stride * a.page_size : a.page_size;
-  const int64_t nt = cap > 0 ? (cap + tile - 1) / tile : 1;
+  const int64_t nt = cap > 0 ? (cap + kTile - 1) / kTile : 1;
   const int64_t U = (int64_t)a.heads_kv * g.row_groups;
   g.max_tiles = (int)nt;
   g.splits = 0;
@@ -383,7 +382,7 @@ inline DecodeGeom decode_geometry(const fa_decode_args& a, int row_groups, int c
     g.shares = a.batch * g.splits;
   } else {
     const int64_t most = a.batch * nt, whole = a.batch;
-    int64_t n = most * U <= (int64_t)longest * g.resident ? g.resident / U : kWaves * g.resident / U + 1;
+    int64_t n = most * U <= (int64_t)kOneWave * g.resident ? g.resident / U : kWaves * g.resident / U + 1;
     n += whole;                                // rounding up adds less than a piece per sequence
     g.shares = (int)(n < most ? n : most);
   }
