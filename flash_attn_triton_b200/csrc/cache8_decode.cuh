@@ -219,7 +219,6 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
           cp_async4(smem_u32(dS + lane), bytes ? ksb + pg * c8.ks_stride[0] + blk * c8.ks_stride[1] : ksb, bytes);
           cp_async4(smem_u32(dS + KW + lane), bytes ? vsb + pg * c8.vs_stride[0] + blk * c8.vs_stride[1] : vsb, bytes);
         }
-        const bool all_in = key00 + KW <= keys;
         if (RPW <= 16) {               // a pass lies inside 16 keys
 #pragma unroll
           for (int h = 0; h < KB; ++h) {
@@ -229,12 +228,7 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
             for (int i = 0; i < PASSES / KB; ++i) {
               const int at = (h * (PASSES / KB) + i) * RPW;
               const unsigned char* x = src + (uint64_t)step * (16 * i);
-              if (all_in) {
-                cp_async16(dst + at * P + column(at), x);
-              } else {                 // rows past the last key are zero-filled
-                const int bytes = key00 + at + lr < keys ? 16 : 0;
-                cp_async16(dst + at * P + column(at), bytes ? x : base, bytes);
-              }
+              cp_async16(dst + at * P + column(at), x, key00 + at + lr < keys ? 16 : 0);     // zeros past the last key
             }
           }
         } else if (lr < KW) {          // one pass takes them all
