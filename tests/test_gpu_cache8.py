@@ -268,6 +268,136 @@ def test_attend_hidden_scales_do_not_reach_a_row():
     assert ((out - want).abs() <= ref.tolerance(want, weight, F16, 100, 10.0)).all()
 
 
+def rotated(x, positions, cos, sin, interleaved):
+    """Rotary embedding of x (batch, tokens, heads, dim), every product and sum rounded to its type."""
+    n = cos.shape[1] * 2
+    c, s = cos[positions][:, :, None], sin[positions][:, :, None]
+    part, rest = x[..., :n], x[..., n:]
+    a, b = (part[..., 0::2], part[..., 1::2]) if interleaved else part.chunk(2, -1)
+    ra, rb = a * c - b * s, a * s + b * c
+    out = torch.stack([ra, rb], -1).flatten(-2) if interleaved else torch.cat([ra, rb], -1)
+    return torch.cat([out, rest], -1)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("interleaved,share", [(True, 1.0), (False, 1.0), (False, 0.5)])
+@pytest.mark.parametrize("n,heads,dim,dtype", [(1, 8, 128, BF16), (3, 4, 64, F16), (20, 8, 128, BF16), (90, 8, 64, F16), (25, 4, 256, BF16)])
+def test_attend_rotary(n, heads, dim, dtype, interleaved, share, code):
+    """New keys are rotated before they are quantised, the queries as they are read; scales and caches with strides of their own."""
+    page, old, hk = 32, [45, 130], 2
+    table, pool = make_table(6, [x + n for x in old], page)
+    kc, ks = make_cache(61, pool, page, hk, dim, code, 2)
+    vc, vs = make_cache(62, pool, page, hk, dim, code, 2)
+    both = torch.stack([ref.bits(kc), ref.bits(vc)], 2).to(DEV).view(code)          # (pages, page, 2, heads, dim)
+    scales = torch.stack([ks, vs]).permute(0, 3, 1, 2).contiguous().to(DEV).permute(0, 2, 3, 1)
+    qkv = rand(63, 2, n, heads + 2 * hk, dim).to(dtype)
+    q, k, v = qkv.split([heads, hk, hk], 2)
+    angle = rand(64, 240, int(dim * share) // 2)
+    cos, sin = torch.cos(angle).to(dtype), torch.sin(angle).to(dtype)
+    dq, dk, dv = qkv.to(DEV).split([heads, hk, hk], 2)
+    out = fa().flash_attn_with_kvcache(dq, both[:, :, 0], both[:, :, 1], dk, dv, cos.to(DEV), sin.to(DEV), cache_seqlens=torch.tensor(old, device=DEV),
+                                       block_table=table.to(DEV), causal=True, rotary_interleaved=interleaved, k_scale=scales[0], v_scale=scales[1])
+    at = torch.tensor(old)[:, None] + torch.arange(n)
+    ref.append_call(rotated(k, at, cos, sin, interleaved), kc, ks, old, table=table)
+    ref.append_call(v, vc, vs, old, table=table)
+    same_cache(both[:, :, 0].contiguous(), kc)
+    same_cache(both[:, :, 1].contiguous(), vc)
+    assert torch.equal(scales[0].cpu(), ks) and torch.equal(scales[1].cpu(), vs)
+    vv = ref.values(vc, vs)
+    want, weight = ref.attend(rotated(q, at, cos, sin, interleaved), ref.values(kc, ks), vv, [x + n for x in old], causal=True, table=table)
+    assert ((out.double().cpu() - want).abs() <= ref.tolerance(want, weight, dtype, 220, float(vv.abs().max()))).all()
+
+
+@pytest.mark.parametrize("n,heads,dim,blocks", [(1, 2, 64, 1), (40, 4, 64, 1), (90, 8, 128, 1), (24, 4, 256, 1), (40, 4, 64, 2)])
+def test_attend_scales_that_are_no_numbers(n, heads, dim, blocks):
+    """Rows that see a block of NaN or infinite scale are no numbers; rows that do not (before it, or past it by the window) are as without
+    it, and so are rows in front of codes of NaN behind the end."""
+    page, old, hk = 16, [160 + n, 75 + n], 2
+    table, pool = make_table(7, old, page)
+    for spoil_v in (False, True):
+        kc, ks = make_cache(71, pool, page, hk, dim, E4M3, blocks)
+        vc, vs = make_cache(72, pool, page, hk, dim, E4M3, blocks)
+        q = rand(73, 2, n, heads, dim).to(F16)
+        (vs if spoil_v else ks)[table[0, 5], 0, 0] = math.inf if spoil_v else math.nan    # keys 80 on of sequence 0, head 0
+        for b, length in enumerate(old):
+            if length % page:
+                kc.view(torch.int8)[table[b, length // page], length % page:] = 0x7f
+                vc.view(torch.int8)[table[b, length // page], length % page:] = 0x7f
+        clean_k, clean_v = ks.nan_to_num(0.01), torch.where(torch.isfinite(vs), vs, 0.01)
+        for window in ((-1, -1), (60, 0)):
+            want, weight = ref.attend(q, ref.values(kc, clean_k).nan_to_num(), ref.values(vc, clean_v).nan_to_num(), old, causal=True, window=window,
+                                      table=table)
+            out = fa().flash_attn_with_kvcache(q.to(DEV), kc.to(DEV), vc.to(DEV), cache_seqlens=torch.tensor(old, device=DEV), block_table=table.to(DEV),
+                                               causal=True, window_size=window, k_scale=ks.to(DEV), v_scale=vs.to(DEV)).double().cpu()
+            rows = 16 // blocks
+            at = torch.arange(old[0] - n, old[0])
+            sees = (at >= 80) & ((at - window[0] < 80 + rows) if window[0] >= 0 else True)
+            spoilt = torch.zeros(2, n, heads, dtype=torch.bool)
+            spoilt[0, :, :heads // hk] = sees[:, None]
+            fine = ((out - want).abs() <= ref.tolerance(want, weight, F16, 300, 10.0)).all(-1)
+            assert fine[~spoilt].all()
+            assert not torch.isfinite(out[spoilt]).any()
+
+
+@pytest.mark.parametrize("batch,n,dim", [(600, 1, 64), (600, 2, 32), (40, 20, 64), (33, 70, 128)])
+def test_attend_large_batches(batch, n, dim):
+    run_attend(8, [(37 * i) % 70 for i in range(batch)], n, True, 4, 2, dim, 16, 1, BF16, E4M3, causal=True)
+
+
+def test_offsets_past_32_bits():
+    """Pages beyond 4 GiB of codes: tables, append, a decode step and chunks."""
+    page, heads, dim, blocks = 256, 8, 256, 4
+    pages = 9000                                       # 4.7e9 codes in each cache
+    kc = torch.empty(pages, page, heads, dim, dtype=torch.int8, device=DEV)
+    vc = torch.empty_like(kc)
+    ks, vs = (torch.full((pages, blocks, heads), float("nan"), device=DEV) for _ in range(2))
+    table = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    free = torch.tensor([8999, 4095, 8192, 8191, 8900], dtype=torch.int32, device=DEV)
+    lens = [300, 77]
+    slots, _, used = fa().build_block_table(torch.zeros(2, device=DEV), torch.tensor(lens, device=DEV), free, table, page, sum(lens))
+    assert int(used) == 3 and slots.max().item() > 2 ** 21
+    k, v = rand(81, sum(lens), heads, dim).to(BF16), rand(82, sum(lens), heads, dim).to(BF16)
+    fa().kvcache_append(k.to(DEV), v.to(DEV), kc, vc, slots, ks, vs)
+    small = torch.tensor([[0, 1, 4], [2, 3, 4]])       # the same pages of a small cache
+    p_kc, p_vc = (torch.zeros(5, page, heads, dim, dtype=torch.int8) for _ in range(2))
+    p_ks, p_vs = (torch.full((5, blocks, heads), float("nan")) for _ in range(2))
+    at = torch.cat([torch.arange(300), 2 * page + torch.arange(77)])
+    ref.append_slots(k, p_kc, p_ks, at)
+    ref.append_slots(v, p_vc, p_vs, at)
+    order = table[:, :2].flatten().long().cpu()[[0, 1, 2]]
+    assert torch.equal(kc[order.to(DEV)].cpu()[0], p_kc[0]) and torch.equal(ks[order.to(DEV)].cpu()[:2, 0], p_ks[:2, 0])
+    table[1, 1:], table[0, 2] = 8191, 8900
+    for n in (1, 20, 150):
+        q = rand(83 + n, 2, n, 16, dim).to(BF16)
+        kn, vn = rand(84 + n, 2, n, heads, dim).to(BF16), rand(85 + n, 2, n, heads, dim).to(BF16)
+        out = fa().flash_attn_with_kvcache(q.to(DEV), kc, vc, kn.to(DEV), vn.to(DEV), cache_seqlens=torch.tensor(lens, device=DEV), block_table=table,
+                                           causal=True, k_scale=ks, v_scale=vs)
+        place = dict(table=small)
+        ref.append_call(kn, p_kc, p_ks, lens, **place)
+        ref.append_call(vn, p_vc, p_vs, lens, **place)
+        lens = [x + n for x in lens]
+        vv = ref.values(p_vc, p_vs)
+        want, weight = ref.attend(q, ref.values(p_kc, p_ks), vv, lens, causal=True, **place)
+        assert ((out.double().cpu() - want).abs() <= ref.tolerance(want, weight, BF16, max(lens), 4.0)).all()
+
+
+def test_chunks_stay_off_after_a_wait_ran_out():
+    from flash_attn_triton_b200 import _native as N
+    kc, ks = (t.to(DEV) for t in make_cache(95, 4, 64, 2, 64, INT8, 1))
+    q = torch.zeros(1, 40, 4, 64, dtype=F16, device=DEV)
+    call = lambda q: fa().flash_attn_with_kvcache(q, kc, kc, cache_seqlens=torch.tensor([50], device=DEV), cache_batch_idx=torch.zeros(1, device=DEV),
+                                                  k_scale=ks, v_scale=ks)
+    dev = torch.cuda.current_device()
+    assert N.lib().fa_debug_set_wait_status(dev, 31) == 0
+    try:
+        with pytest.raises(N.DeviceWaitError):
+            call(q)
+        call(q[:, :1])                                 # decode waits for nothing
+    finally:
+        assert N.lib().fa_device_wait_clear(dev) == 0
+    call(q)
+
+
 def test_attend_scales_far_apart():
     """Blocks whose scales differ by 2^30: what a row sees of small values, where its weight is on them, keeps its precision."""
     page, dim = 16, 64
