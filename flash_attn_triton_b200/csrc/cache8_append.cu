@@ -20,6 +20,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kHeld = 8;               // 16-byte pieces that a lane holds; a larger share of a block is read twice
 constexpr int kSpanMost = 256, kBlockMost = 1024;
+constexpr int kHeadWords = 4;          // of the value checks, in front of the bits of the blocks
 
 // Row of a slot: page, block of the page, row of the block.
 struct Place {
@@ -238,40 +239,30 @@ __global__ void __launch_bounds__(kThreads, 3)
 }
 
 // ---------------------------------------------------------------------------------------
-// value checks of packed tokens: claims[block] = first token of a run in it, then looked at again
+// value checks of packed tokens: a run takes the bit of its block, and finds it taken where the call writes the block in two places
 // ---------------------------------------------------------------------------------------
-__device__ __forceinline__ int64_t block_of_slot(const Append8& p, int64_t s) {
-  const Place w = place_of(p, s);
-  return w.page * (p.page_size / p.block) + w.block;
-}
-__device__ __forceinline__ void claim_blocks(const Append8& p, int32_t* claims, int64_t from, int64_t step) {
-  for (int64_t t = from; t < p.tokens; t += step) {
-    const int64_t s = slot_of(p, t);
-    if (s >= 0 && !carries_on(p, t, s)) claims[block_of_slot(p, s)] = (int32_t)t;
+// words: result, CTAs that are done, then the bits; zero before the launch, or by the one CTA of a small call itself.
+__global__ void __launch_bounds__(1024) append8_check_kernel(const Append8 p, uint32_t* words, int64_t bit_words, uint32_t* host) {
+  uint32_t* bits = words + kHeadWords;
+  if (gridDim.x == 1) {
+    for (int64_t i = threadIdx.x; i < bit_words; i += 1024) bits[i] = 0u;
+    __syncthreads();
   }
-}
-__device__ __forceinline__ uint32_t verify_claims(const Append8& p, const int32_t* claims, int64_t from, int64_t step) {
   uint32_t bad = 0;
-  for (int64_t t = from; t < p.tokens; t += step) {
+  for (int64_t t = (int64_t)blockIdx.x * 1024 + threadIdx.x; t < p.tokens; t += (int64_t)gridDim.x * 1024) {
     const int64_t s = slot_of(p, t);
-    if (s < 0 && p.slots[t] >= 0) bad |= FA_SLOT_RANGE;
-    if (s >= 0 && !carries_on(p, t, s) && claims[block_of_slot(p, s)] != (int32_t)t) bad |= FA_SLOT_TWICE;
+    if (s < 0) {
+      if (p.slots[t] >= 0) bad |= FA_SLOT_RANGE;
+    } else if (!carries_on(p, t, s)) {
+      const Place w = place_of(p, s);
+      const int64_t block = w.page * (p.page_size / p.block) + w.block;
+      const uint32_t bit = 1u << (block & 31);
+      if (atomicOr(bits + (block >> 5), bit) & bit) bad |= FA_SLOT_TWICE;
+    }
   }
-  return bad;
-}
-// One CTA does both; else the grid claims, and verifies in a second launch whose last CTA answers.  words: result, CTAs that are done.
-__global__ void __launch_bounds__(1024) append8_check_kernel(const Append8 p, int32_t* claims, uint32_t* words, uint32_t* host, int phase) {
-  const int64_t from = (int64_t)blockIdx.x * 1024 + threadIdx.x, step = (int64_t)gridDim.x * 1024;
-  if (phase != 2) claim_blocks(p, claims, from, step);
-  if (phase == 1) {
-    if (from == 0) words[0] = words[1] = 0u;
-    return;
-  }
-  __syncthreads();
-  const uint32_t bad = verify_claims(p, claims, from, step);
   const uint32_t all = (__syncthreads_or(bad & FA_SLOT_RANGE) ? FA_SLOT_RANGE : 0u) | (__syncthreads_or(bad & FA_SLOT_TWICE) ? FA_SLOT_TWICE : 0u);
   if (threadIdx.x != 0) return;
-  if (phase == 0) {
+  if (gridDim.x == 1) {
     words[0] = all;
     *reinterpret_cast<volatile uint32_t*>(host) = all | kCheckDone;
   } else {
@@ -394,12 +385,12 @@ Append8 append_of(const fa_decode_args& a, const fa_cache8& c) {
   return p;
 }
 
-constexpr size_t kWordsBytes = 16;     // of the value checks, in front of the claims
-constexpr int64_t kOneCta = 4096;      // tokens up to which one CTA makes the checks
+constexpr int64_t kOneCta = 4096;      // tokens, and words of bits, up to which one CTA makes the checks
 
+static int64_t bit_words(const fa_append8_args& a) { return ((int64_t)a.num_pages * (a.page_size / a.cache.block) + 31) / 32; }
 size_t append8_workspace_bytes(const fa_append8_args& a) {
   if (a.tokens <= 0 || a.cache.block <= 0 || a.page_size <= 0) return 0;
-  return kWordsBytes + (size_t)a.num_pages * (a.page_size / a.cache.block) * sizeof(int32_t);
+  return (kHeadWords + (size_t)bit_words(a)) * sizeof(uint32_t);
 }
 
 int append8(const fa_append8_args& a, cudaStream_t st) {
@@ -422,24 +413,24 @@ int append8_checked(const fa_append8_args& a, uint32_t* failed, cudaStream_t st)
     return FA_ERR_WORKSPACE;
   }
   uint32_t* words = static_cast<uint32_t*>(a.workspace);
-  int32_t* claims = reinterpret_cast<int32_t*>(static_cast<char*>(a.workspace) + kWordsBytes);
   const Append8 p = append_of(a);
   uint32_t* host = nullptr;
   const int slot = take_check_word(false, a.device, &host);
   if (slot < 0) return FA_ERR_LAUNCH;
   int r = FA_OK;
-  if (a.tokens <= kOneCta) {
-    append8_check_kernel<<<1, 1024, 0, st>>>(p, claims, words, host, 0);
-    r = check_launch("append8_check");
-  } else {
-    const int64_t need_ctas = (a.tokens + 2047) / 2048, fit = 2ll * sm_count(a.device);
-    const unsigned grid = (unsigned)(need_ctas < fit ? need_ctas : fit);
-    append8_check_kernel<<<grid, 1024, 0, st>>>(p, claims, words, host, 1);
-    r = check_launch("append8_check");
-    if (r == FA_OK) {
-      append8_check_kernel<<<grid, 1024, 0, st>>>(p, claims, words, host, 2);
-      r = check_launch("append8_check");
+  unsigned grid = 1;
+  if (a.tokens > kOneCta || bit_words(a) > kOneCta) {
+    const int64_t ctas = (a.tokens + 2047) / 2048, fit = 2ll * sm_count(a.device);
+    grid = (unsigned)(ctas < 2 ? 2 : ctas < fit ? ctas : fit);
+    const cudaError_t e = cudaMemsetAsync(words, 0, need, st);
+    if (e != cudaSuccess) {
+      set_error("append8: cudaMemsetAsync: %s", cudaGetErrorString(e));
+      r = FA_ERR_LAUNCH;
     }
+  }
+  if (r == FA_OK) {
+    append8_check_kernel<<<grid, 1024, 0, st>>>(p, words, bit_words(a), host);
+    r = check_launch("append8_check");
   }
   const bool queued = r == FA_OK;
   if (r == FA_OK) r = append8_launch(p, nullptr, a.dtype, a.cache.code, a.device, nullptr, words, false, st);
