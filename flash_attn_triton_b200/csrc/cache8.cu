@@ -35,7 +35,7 @@ struct Plan {
 };
 
 // A chunk: more than 16 query rows per KV head.  The decode kernel would read the cache once per 16 rows; the tcgen05 kernel takes 128 at a
-// time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128: 690 -> 265 us).
+// time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128: 690 us, 200).
 bool plan_chunk(const fa_decode_args& a, const fa_cache8& c, Plan& p) {
   const int G = a.heads_q / a.heads_kv;
   if (a.num_splits != 0 || (int64_t)a.seqlen_q * G <= 16 || a.softmax_scale < 0.f) return false;

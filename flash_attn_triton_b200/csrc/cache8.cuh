@@ -104,8 +104,9 @@ __device__ __forceinline__ int divided(int x, const Div32& d) { return (int)(((u
 __device__ __forceinline__ int divided(int x, int n, int shift) { return shift >= 0 ? x >> shift : x / n; }
 
 // Chunks of tokens: pieces that `all` key tiles of a unit are cut into.  A piece has the tiles that an SM would have if all work were
-// shared evenly, so that sequences longer than that do not set the time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128, 256
-// rows per CTA: 235 us in whole units, SPLIT cut).  Every warp works it out from the lengths; units: of a sequence.
+// shared evenly, so that sequences longer than that do not set the time (32 heads over 8 of 128, whole units -> cut: 100 tokens behind
+// 30000 563 -> 146 us, 3 x 256 behind 300 to 30000 571 -> 534, 4 x 256 behind 1024 to 8192 197 -> 201).  Every warp works it out from
+// the lengths; units: of a sequence.
 __device__ __forceinline__ int chunk_pieces(const fa_decode_args& p, const ScoreCfg& cfg, const CacheGeo& geo, int units, int all, int lane) {
   if (geo.parts == 1) return 1;
   int64_t tiles = 0;

