@@ -241,6 +241,46 @@ def test_attend(case, dtype, code):
     run_attend(1000 + case, dtype=dtype, code=code, **ATTENDS[case])
 
 
+CHUNKS = [
+    # one query tile per CTA, then two; contiguous caches shorter than a tile of keys, rows and pads of their own
+    dict(old=[20, 7], n=40, append=True, heads=4, heads_kv=2, dim=64, page=72, blocks=9, causal=True, paged=False),
+    dict(old=[20, 0], n=70, append=True, heads=8, heads_kv=2, dim=128, page=96, blocks=6, causal=True, paged=False),
+    dict(old=[100, 300, 9], n=70, append=True, heads=8, heads_kv=2, dim=64, page=512, blocks=32, causal=True, paged=False, rows=[3, 0, 2]),
+    dict(old=[100, 300, 9], n=70, append=True, heads=8, heads_kv=2, dim=128, page=512, blocks=4, causal=True, paged=False, rows=[3, 0, 2],
+         leftpad=[0, 17, 130]),
+    # rows ahead of the sequence see nothing
+    dict(old=[10, 45], n=40, append=0, heads=4, heads_kv=2, dim=64, page=16, blocks=1, causal=True),
+    dict(old=[10, 85, 0], n=80, append=0, heads=8, heads_kv=2, dim=128, page=16, blocks=1, causal=True),
+    dict(old=[0, 0], n=80, append=0, heads=8, heads_kv=2, dim=64, page=16, blocks=1),
+    # windows, to the right too
+    dict(old=[200, 90], n=40, append=0, heads=4, heads_kv=2, dim=128, page=32, blocks=2, window_size=(30, 2)),
+    dict(old=[400, 290], n=90, append=True, heads=8, heads_kv=2, dim=64, page=32, blocks=2, window_size=(100, 3)),
+    dict(old=[700, 290], n=90, append=True, heads=8, heads_kv=2, dim=128, page=128, blocks=1, causal=True, window_size=(150, 0)),
+    # no mask, keys past the last one in the tile; groups that are no power of two; a scale per key; a scale of 0
+    dict(old=[129, 383], n=65, append=True, heads=6, heads_kv=2, dim=64, page=48, blocks=3),
+    dict(old=[250, 31], n=200, append=True, heads=3, heads_kv=1, dim=128, page=80, blocks=5, causal=True),
+    dict(old=[100], n=50, append=True, heads=4, heads_kv=1, dim=256, page=16, blocks=16, causal=True),
+    dict(old=[100, 600], n=70, append=True, heads=4, heads_kv=1, dim=64, page=16, blocks=1, causal=True, softmax_scale=0.0),
+    # few units: keys in pieces
+    dict(old=[3000], n=33, append=True, heads=4, heads_kv=1, dim=64, page=64, blocks=4, causal=True),
+    dict(old=[2500, 100], n=33, append=True, heads=8, heads_kv=1, dim=128, page=256, blocks=2, causal=True),
+    dict(old=[1500], n=20, append=True, heads=1, heads_kv=1, dim=256, page=128, blocks=1, causal=True),
+]
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("case", range(len(CHUNKS)))
+def test_attend_chunks(case, dtype, code):
+    run_attend(2000 + 100 * case, dtype=dtype, code=code, **CHUNKS[case])
+
+
+@pytest.mark.parametrize("n,heads", [(1, 4), (30, 4), (90, 8)])
+def test_attend_large_scores(n, heads):
+    """Scores up to 60: the maximum moves a lot, and one key takes nearly all."""
+    run_attend(9, [300, 70], n, True, heads, 2, 64, 16, 1, F16, INT8, causal=True, q_gain=15.0)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_attend_alibi(n):
     slopes = torch.tensor([[0.5, 0.1, 0.03, 0.0], [0.2, 0.2, 0.01, 1.0]], device=DEV)
