@@ -6,9 +6,9 @@
 //   head stay in registers between the maximum and the codes and are read once.
 //   Split.  A run is the tokens of a call that fall into one block.  A CTA looks at `span` tokens, lists the runs that begin among
 //   them, and its warps take (run, head, key or value) one by one; 1 to 8 warps share one by the size of a block, so that each lane
-//   has at most kHeld 16-byte pieces of it.  Nothing is left to atomics: a block belongs to one run, and a run and head to one group of warps.
-//   Measured: 302 k tokens of 8 heads of 128, int8, blocks of 32: 342 us, 5.4 TB/s of 6.5 (issue active 63 %: rounding and packing are 13
-//   instructions per element); 22 k, e4m3, blocks of 64: 34 us (floor 21); 32 single tokens: 5.5 us, all latency.
+//   has at most 8 or 16 16-byte pieces of it.  Nothing is left to atomics: a block belongs to one run, and a run and head to one group of warps.
+//   Measured: 302 k tokens of 8 heads of 128, int8, blocks of 32: 318 us, 5.8 TB/s of 6.5 (rounding and packing are 13 instructions
+//   per element); 22 k, e4m3, blocks of 64: 34 us (floor 21); 32 single tokens: 5.5 us, all latency.
 #include <type_traits>
 
 #include "cache8.cuh"
@@ -20,7 +20,6 @@ namespace fa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeld = 8;               // 16-byte pieces that a lane holds; a larger share of a block is read twice
 constexpr int kSpanMost = 256, kBlockMost = 1024;
 constexpr int kHeadWords = 4;          // of the value checks, in front of the bits of the blocks
 
@@ -75,8 +74,9 @@ struct Run {
 }  // namespace
 
 // kSlots: packed tokens; else those of the cache call d.  g.per_y (head, key or value) per CTA along y, 2^g.warps_log2 warps for one.
-template <typename T, int kCode, bool kSlots>
-__global__ void __launch_bounds__(kThreads, 3)
+// kHeld: 16-byte pieces that a lane holds; a larger share of a block is read twice.
+template <typename T, int kCode, bool kSlots, int kHeld>
+__global__ void __launch_bounds__(kThreads, kHeld == 8 ? 4 : 2)
     cache8_append_kernel(const Append8 p, const fa_decode_args d, const AppendGeom g, uint32_t* host, uint32_t* dev, bool check_here) {
   using C = Code<kCode>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -287,8 +287,12 @@ static AppendGeom append_geometry(const Append8& p, int device) {
   // warps of a (run, head): as many as hold a full block
   const int longest = (int)(p.longest_run < p.block ? p.longest_run : p.block);
   const int64_t pieces = (int64_t)longest * (p.head_dim / 8);
+  // 8 pieces per lane and four CTAs per SM, except where 16 let one warp hold a block (no barrier: 302 k tokens of 8 heads of 128 in blocks
+  // of 32, 350 -> 338 us) or 8 warps one that is read twice otherwise (blocks of 256: 210 -> 163); else they only cost CTAs (blocks of 64:
+  // 48 -> 50; of 16: 46 -> 59).
+  g.held = (pieces > 256 && pieces <= 512) || pieces > 2048 ? 16 : 8;
   g.warps_log2 = 0;
-  while (g.warps_log2 < 3 && pieces > (32ll * kHeld << g.warps_log2)) ++g.warps_log2;
+  while (g.warps_log2 < 3 && pieces > (32ll * g.held << g.warps_log2)) ++g.warps_log2;
   const int groups = 8 >> g.warps_log2;
   // A CTA per block and few heads where the tokens are few (a span shorter than a block leaves CTAs without a run, which is cheap as
   // long as all run at once), all heads of a block where there are more blocks than CTAs.  2048 tokens, 8 heads of 128, blocks of 64: 30 us
@@ -312,8 +316,10 @@ int append8_launch(const Append8& p, const fa_decode_args* call, int dtype, int 
   if (call) d = *call;
   auto go = [&](auto* t, auto c, auto slots) {
     using T = std::remove_pointer_t<decltype(t)>;
-    cache8_append_kernel<T, decltype(c)::value, decltype(slots)::value>
-        <<<dim3(g.grid_x, g.grid_y), kThreads, 0, st>>>(p, d, g, host, dev, check_here);
+    constexpr int kCode = decltype(c)::value;
+    constexpr bool kSlots = decltype(slots)::value;
+    auto kern = g.held == 8 ? cache8_append_kernel<T, kCode, kSlots, 8> : cache8_append_kernel<T, kCode, kSlots, 16>;
+    kern<<<dim3(g.grid_x, g.grid_y), kThreads, 0, st>>>(p, d, g, host, dev, check_here);
   };
   auto by_source = [&](auto* t, auto c) {
     if (call) go(t, c, std::false_type{});

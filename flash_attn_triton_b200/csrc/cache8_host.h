@@ -21,7 +21,7 @@ struct Append8 {
 };
 struct AppendGeom {
   int span;                            // tokens whose runs a CTA takes
-  int per_y, warps_log2;
+  int per_y, warps_log2, held;
   unsigned grid_x, grid_y;
 };
 
