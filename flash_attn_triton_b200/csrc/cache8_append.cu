@@ -76,7 +76,7 @@ struct Run {
 // kSlots: packed tokens; else those of the cache call d.  g.per_y (head, key or value) per CTA along y, 2^g.warps_log2 warps for one.
 // kHeld: 16-byte pieces that a lane holds; a larger share of a block is read twice.
 template <typename T, int kCode, bool kSlots, int kHeld>
-__global__ void __launch_bounds__(kThreads, kHeld == 8 ? 4 : 2)
+__global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
     cache8_append_kernel(const Append8 p, const fa_decode_args d, const AppendGeom g, uint32_t* host, uint32_t* dev, bool check_here) {
   using C = Code<kCode>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 8 ? 4 : 2)
       __threadfence_system();
     }
     if (bad) return;
-  } else if (dev && *dev) {
+  } else if (!kSlots && dev && *dev) {
     return;
   }
   __shared__ Run runs[kSpanMost];
@@ -141,6 +141,11 @@ __global__ void __launch_bounds__(kThreads, kHeld == 8 ? 4 : 2)
     }
   }
   __syncthreads();
+  if (kSlots && dev) {
+    // behind the checks (a programmatic launch): the runs were listed meanwhile (a call of 22 k tokens 46 us, 42.5)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (*dev) return;
+  }
 
   // ---- (run, head, key or value) by groups of warps ---------------------------------------------
   const int wlog = g.warps_log2, group = warp >> wlog, groups = 8 >> wlog;
@@ -245,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 8 ? 4 : 2)
 // ---------------------------------------------------------------------------------------
 // words: result, CTAs that are done, then the bits; zero before the launch, or by the one CTA of a small call itself.
 __global__ void __launch_bounds__(1024) append8_check_kernel(const Append8 p, uint32_t* words, int64_t bit_words, uint32_t* host) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   uint32_t* bits = words + kHeadWords;
   if (gridDim.x == 1) {
     for (int64_t i = threadIdx.x; i < bit_words; i += 1024) bits[i] = 0u;
@@ -319,7 +325,16 @@ int append8_launch(const Append8& p, const fa_decode_args* call, int dtype, int 
     constexpr int kCode = decltype(c)::value;
     constexpr bool kSlots = decltype(slots)::value;
     auto kern = g.held == 8 ? cache8_append_kernel<T, kCode, kSlots, 8> : cache8_append_kernel<T, kCode, kSlots, 16>;
-    kern<<<dim3(g.grid_x, g.grid_y), kThreads, 0, st>>>(p, d, g, host, dev, check_here);
+    cudaLaunchConfig_t lc = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    lc.gridDim = dim3(g.grid_x, g.grid_y);
+    lc.blockDim = dim3(kThreads);
+    lc.stream = st;
+    lc.attrs = &attr;
+    lc.numAttrs = kSlots && dev ? 1 : 0;
+    cudaLaunchKernelEx(&lc, kern, p, d, g, host, dev, check_here);
   };
   auto by_source = [&](auto* t, auto c) {
     if (call) go(t, c, std::false_type{});
@@ -428,7 +443,7 @@ int append8_checked(const fa_append8_args& a, uint32_t* failed, cudaStream_t st)
   int r = FA_OK;
   unsigned grid = 1;
   if (a.tokens > kOneCta || bit_words(a) > kOneCta) {
-    const int64_t ctas = (a.tokens + 2047) / 2048, fit = 2ll * sm_count(a.device);
+    const int64_t ctas = (a.tokens + 1023) / 1024, fit = 2ll * sm_count(a.device);
     grid = (unsigned)(ctas < 2 ? 2 : ctas < fit ? ctas : fit);
     const cudaError_t e = cudaMemsetAsync(words, 0, need, st);
     if (e != cudaSuccess) {
