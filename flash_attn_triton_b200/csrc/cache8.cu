@@ -12,6 +12,8 @@ int decode8_e4m3(const fa_decode_args&, const fa_cache8&, const ScoreCfg&, int, 
 Geom8 decode8_geometry(const fa_decode_args& a, const fa_cache8& c, int unit_rows, int row_groups);
 int cache8_chunk(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
 int cache8_pair(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
+int cache8_chunk_pieces(int head_dim);
+int cache8_pair_pieces(int head_dim);
 int launch_decode_check(const fa_decode_args& a, uint32_t* host, uint32_t* dev, cudaStream_t st);
 
 namespace {
@@ -52,9 +54,12 @@ bool plan_chunk(const fa_decode_args& a, const fa_cache8& c, Plan& p) {
   const int64_t units = (int64_t)a.batch * (a.heads_q >> p.pack_log2) * mtiles;
   if (units > (1 << 28) || cap > (1 << 30)) return false;
   p.capacity = (int)cap;
-  // pieces of at least four key tiles, only while the units do not fill the SMs twice (chunk_pieces() has how many there are)
+  // pieces of at least four key tiles, only while the units do not fill the SMs twice (chunk_pieces() has how many there are), and no more
+  // than a merge has room for the weights of (pairs: 144; one unit alone would have a piece per SM)
   const int64_t sms = sm_count(a.device), fill = units >= 2 * sms ? 1 : sms / units > 4 ? sms / units : 4, most = (cap + 511) / 512;
+  const int64_t room = p.pair ? cache8_pair_pieces(a.head_dim) : cache8_chunk_pieces(a.head_dim);
   p.parts = (int)(fill < most ? fill : most);
+  if (p.parts > room) p.parts = (int)room;
   if (p.parts < 1) p.parts = 1;
   p.counters = p.parts > 1 ? (int)units : 0;
   p.piece_bytes = p.parts > 1 ? (size_t)units * p.parts * per_cta * (a.head_dim + 1) * sizeof(float) : 0;

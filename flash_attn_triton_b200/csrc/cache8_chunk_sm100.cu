@@ -51,6 +51,8 @@ template <int D> struct CCfg {
   static constexpr int kShared = kRawAt + kRaw * kRawBytes;
   static constexpr int kSmemBytes = kShared + 1024 /*align slack*/ + 6144 /*CShared*/;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+  // Pieces of the keys, at most: a merge keeps a weight per piece and row over both rings.
+  static constexpr int kPieces = (kShared - kQBytes) / (kBM * (int)sizeof(float));
 };
 
 struct CShared {
@@ -807,7 +809,7 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           __threadfence();
           const int64_t s0 = (int64_t)(blockIdx.x / geo.parts) * geo.parts;
           const int rows = min(kBM, w.rows - w.m0);
-          // weights of the pieces per row, over the ring (every K/V tile has been read)
+          // weights of the pieces per row, over the rings (every K/V tile has been read); w.parts <= geo.parts <= C::kPieces
           float* wt = reinterpret_cast<float*>(tiles + C::kQBytes);
           if (tid < rows) {
             float m = -INFINITY, sum = 0.f;
@@ -871,6 +873,10 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 // ---------------------------------------------------------------------------------------
 template <typename T, int kCode, int D, bool kAlibi, bool kFine>
 static int launch_chunk8(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
+  if (geo.parts > CCfg<D>::kPieces) {
+    set_error("cache8_chunk: %d pieces, %d at most", geo.parts, CCfg<D>::kPieces);
+    return FA_ERR_LAUNCH;
+  }
   const int pack = 1 << geo.pack_log2;
   CUtensorMap tm[3];
   // codes as they lie, no swizzle: their readers are threads
@@ -934,6 +940,10 @@ int cache8_chunk(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& ge
                                   : launch_chunk8_code<__nv_bfloat16, FA_CODE_E4M3>(d, c, geo, cfg, st);
   return c.code == FA_CODE_INT8 ? launch_chunk8_code<__half, FA_CODE_INT8>(d, c, geo, cfg, st)
                                 : launch_chunk8_code<__half, FA_CODE_E4M3>(d, c, geo, cfg, st);
+}
+
+int cache8_chunk_pieces(int head_dim) {
+  return head_dim == 64 ? CCfg<64>::kPieces : head_dim == 128 ? CCfg<128>::kPieces : CCfg<256>::kPieces;
 }
 
 int cache8_chunk_status() {

@@ -48,6 +48,8 @@ template <int D> struct PCfg {
   static constexpr int kShared = kRawAt + kRaw * kRawBytes;
   static constexpr int kSmemBytes = kShared + 1024 /*align slack*/ + 2048 /*PShared*/;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+  // Pieces of the keys, at most: a merge keeps a weight per piece and row over both rings.
+  static constexpr int kPieces = (kShared - 2 * kQBytes) / (kRows * (int)sizeof(float));
 };
 
 struct PShared {
@@ -681,7 +683,7 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           __threadfence();
           const int64_t p0 = (int64_t)(blockIdx.x / geo.parts) * geo.parts;
           const int rows = min(kRows, w.rows - w.m0);
-          // weights of the pieces per row, over the ring (every K/V tile has been read)
+          // weights of the pieces per row, over the rings (every K/V tile has been read); w.parts <= geo.parts <= C::kPieces
           float* wt = reinterpret_cast<float*>(tiles + 2 * C::kQBytes);
           if (tid < rows) {
             float m = -INFINITY, sum = 0.f;
@@ -745,6 +747,10 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 // ---------------------------------------------------------------------------------------
 template <typename T, int kCode, int D>
 static int launch_pair8(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
+  if (geo.parts > PCfg<D>::kPieces) {
+    set_error("cache8_pair: %d pieces, %d at most", geo.parts, PCfg<D>::kPieces);
+    return FA_ERR_LAUNCH;
+  }
   const int pack = 1 << geo.pack_log2;
   CUtensorMap tm[3];
   // codes as they lie, no swizzle: their readers are threads
@@ -794,6 +800,8 @@ static int launch_pair8_of(const fa_decode_args& d, const fa_cache8& c, const Ca
 int cache8_pair(const fa_decode_args& d, const fa_cache8& c, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
   return d.dtype == FA_BF16 ? launch_pair8_of<__nv_bfloat16>(d, c, geo, cfg, st) : launch_pair8_of<__half>(d, c, geo, cfg, st);
 }
+
+int cache8_pair_pieces(int head_dim) { return head_dim == 64 ? PCfg<64>::kPieces : PCfg<128>::kPieces; }
 
 int cache8_pair_status() {
   int v = 0;
