@@ -214,7 +214,14 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
     float need = __fdiv_rn(Elem<T>::to_f(*reinterpret_cast<const T*>(&bits)), C::kLargest);
     if (need < 1.17549435e-38f) need = 0.f;
     const float now = old != old ? old : (need > old || need != need) ? need : old;
-    const float inv = now > 0.f ? __frcp_rn(now) : now != now ? now : 0.f;
+    // A scale that is no number or infinite makes every value of the block and head one that is none: its new codes are 0, since e4m3 codes of
+    // NaN would reach rows that do not see the key (0 times NaN in the products).
+    const bool spoilt = !(now <= 3.402823466e38f);
+    const float inv = now > 0.f && !spoilt ? __frcp_rn(now) : 0.f;
+    if (spoilt) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) held[k] = make_uint4(0u, 0u, 0u, 0u);
+    }
     unsigned char* cl = codes + row0 * code_stride + col;
     const int64_t cstep = rstep * code_stride;
     auto store = [&](int k, const uint4& v) {
@@ -224,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
       if (gl + k * gsize < pieces) store(k, held[k]);
-    for (int k = kHeld; gl + k * gsize < pieces; ++k) store(k, load(k));
+    for (int k = kHeld; gl + k * gsize < pieces; ++k) store(k, spoilt ? make_uint4(0u, 0u, 0u, 0u) : load(k));
     if (run.kept > 0 && now > old) {
       const float m = __fmul_rn(old, inv);
       for (int j = gl; j < run.kept << (dshift - 1); j += gsize) {

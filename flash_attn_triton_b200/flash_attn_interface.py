@@ -290,7 +290,8 @@ def kvcache_append(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale):
     Blocks fill from their first row on: the rows of a block before the first one that a call writes are tokens that it keeps, and
     a call that writes its first row starts the block's scale afresh.  The scale is the largest magnitude of the
     block so far over 127 (int8) or 448 (e4m3); where new tokens raise it, the codes of the tokens that stay are rounded again.
-    A NaN or infinity among the tokens of a block goes to its scale.  The tokens that a call brings for one block
+    A NaN or infinity among the tokens of a block goes to its scale, which makes the values of that block and head NaN and those of
+    no other; its new codes are 0 then.  The tokens that a call brings for one block
     follow one another, in the order of their slots.
 
     With value checks on, a slot behind the cache or a block that is written in two places raises ValueError and
@@ -375,7 +376,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
 
     A cache may be held in 8 bits: k_cache and v_cache are then torch.int8 or torch.float8_e4m3fn codes of the same
     shapes, and k_scale, v_scale fp32 tensors (batch_cache or num_pages, blocks, nheads_k) with one scale per head and
-    block of capacity / blocks (page_size / blocks) consecutive tokens, at most 1024; a value is code * scale.  q, k
+    block of capacity / blocks (page_size / blocks) consecutive tokens, at most 1024; a value is code * scale.  Codes are numbers
+    (no e4m3 NaN, which an append never writes) wherever a sequence has keys.  q, k
     and v stay 16-bit.  New tokens are quantised as `kvcache_append` does it, and the attention is to what the cache
     then holds.
 

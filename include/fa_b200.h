@@ -300,8 +300,10 @@ size_t fa_decode_static_scratch_bytes(void);
  * Appending to a block: with `kept` tokens of the sequence already in it, its scale s and the new tokens' largest magnitude a,
  *   need = a / Q  (Q = 127 or 448; below the smallest normal number: 0),  s' = max(kept ? s : 0, need),  inv = s' > 0 ? 1 / s' : 0
  *   new codes  rn(x * inv);   kept codes, where s' > s,  rn(code * (s * inv));   all in IEEE fp32, rounded half to even.
- * A NaN or an infinity among the new tokens goes to the scale, so that the values of that block and head are NaN or infinite until the
- * block is started again.
+ * A NaN or an infinity among the new tokens goes to the scale, so that the values of that block and head are NaN until the block is
+ * started again; while the scale is no finite number, new codes are 0.
+ * Codes are numbers: a NaN of e4m3 (0x7f, 0xff), which an append never writes, in a key that a sequence holds may also reach rows that do
+ * not see the key.  In rows of the cache that no sequence holds, any code will do.
  *
  * fa_decode_paged8: fa_decode_paged on such a cache; the call's cache pointers are the codes', its cache strides are in codes.  The
  * new tokens are appended first, and the attention is to what the cache then holds.  dtype is q's, the new tokens' and o's.

@@ -1,8 +1,12 @@
-"""KV cache in 8 bits, beside test_gpu_cache8.py: many pieces of one sequence."""
+"""KV cache in 8 bits, beside test_gpu_cache8.py: many pieces of one sequence, tokens that are no numbers."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_cache8 import BF16, E4M3, F16, INT8, run_attend
+import cache8_reference as ref
+from test_gpu_cache8 import BF16, E4M3, F16, INT8, fa, make_cache, make_table, rand, run_attend
+from util import DEV
 
 pytestmark = pytest.mark.gpu
 
@@ -16,3 +20,78 @@ def test_chunk_of_one_unit_behind_a_long_context(dim, dtype, code, old):
     torch.cuda.synchronize()
     assert N.lib().fa_device_wait_status(torch.cuda.current_device()) == 0
     run_attend(12, [100], 32, True, 8, 1, dim, 256, 1, dtype, code, causal=True)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_append_writes_no_codes_of_nan(bad, code):
+    """Tokens that are no numbers: codes of 0 under a scale of NaN or infinity, by slot, for blocks that one lane holds and larger ones;
+    tokens that come behind them too, until the block is started again."""
+    for page, dim in ((16, 32), (1024, 64)):
+        kc, ks = make_cache(21, 2, page, 2, dim, code, 1)
+        x = rand(22, page - 4, 2, dim).to(BF16)
+        x[3, 1, 5] = bad
+        kd, vd, ksd, vsd = kc.to(DEV), kc.to(DEV), ks.to(DEV), ks.to(DEV)
+        fa().kvcache_append(x.to(DEV), x.to(DEV), kd, vd, torch.arange(page, 2 * page - 4, device=DEV), ksd, vsd)
+        more = rand(23, 2, 2, dim).to(BF16)
+        fa().kvcache_append(more.to(DEV), more.to(DEV), kd, vd, torch.arange(2 * page - 4, 2 * page - 2, device=DEV), ksd, vsd)
+        for codes, scale in ((kd, ksd), (vd, vsd)):
+            codes, scale = codes.cpu(), scale.cpu()
+            assert (ref.bits(codes)[1, :page - 2, 1] == 0).all() and not math.isfinite(scale[1, 0, 1])
+            assert ref.values(codes, scale)[1, :page - 2, 1].isnan().all() and torch.isfinite(ref.values(codes, scale)[1, :page - 2, 0]).all()
+            assert torch.equal(ref.bits(codes)[0], ref.bits(kc)[0])
+
+
+SPOILT = [
+    # query tokens, heads, dim, page, blocks: decode, one query tile per CTA, two; a scale per key (blocks of 4)
+    (3, 4, 64, 16, 1),
+    (8, 4, 256, 32, 2),
+    (40, 4, 64, 16, 1),
+    (40, 4, 128, 16, 4),
+    (40, 4, 256, 16, 1),
+    (100, 8, 64, 16, 1),
+    (100, 8, 128, 32, 2),
+]
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("new", [False, True], ids=["cached", "new"])
+@pytest.mark.parametrize("case", range(len(SPOILT)))
+def test_tokens_that_are_no_numbers_spoil_the_rows_that_see_them(case, new, bad, code):
+    """A NaN or infinity among the cached values, whose block the window of most rows has passed, or among the new ones, where earlier
+    rows do not see its block: those rows, in one tile of keys with it, are as without it."""
+    n, heads, dim, page, blocks = SPOILT[case]
+    hk, size = 2, page // blocks
+    first = 208 if new else 100 // size * size         # of the block
+    old = [208 - min(8, n // 2), 61]
+    window = (-1, -1) if new else (94 if n <= 8 else 100, 0)
+    table, pool = make_table(31, [x + n for x in old], page)
+    k, v = (rand(32 + i, 2, old[0] + n, hk, dim).to(F16) for i in range(2))
+    clean = v.clone()
+    v[0, first + 1, 0, 3] = bad
+    slots = torch.cat([torch.tensor([int(table[b, p // page]) * page + p % page for p in range(old[b])]) for b in range(2)])
+    cached = lambda x: torch.cat([x[b, :old[b]] for b in range(2)])
+    added = lambda x: torch.stack([x[b, old[b]:old[b] + n] for b in range(2)])
+    q = rand(34, 2, n, heads, dim).to(F16)
+    kc, vc = (torch.zeros(pool, page, hk, dim, dtype=torch.int8, device=DEV).view(code) for _ in range(2))
+    ks, vs = (torch.zeros(pool, blocks, hk, device=DEV) for _ in range(2))
+    fa().kvcache_append(cached(k).to(DEV), cached(v).to(DEV), kc, vc, slots.to(DEV), ks, vs)
+    out = fa().flash_attn_with_kvcache(q.to(DEV), kc, vc, added(k).to(DEV), added(v).to(DEV), cache_seqlens=torch.tensor(old, device=DEV),
+                                       block_table=table.to(DEV), causal=True, window_size=window, k_scale=ks, v_scale=vs).double().cpu()
+    # with a number in that place
+    pk, pv = (torch.zeros(pool, page, hk, dim, dtype=torch.int8).view(code) for _ in range(2))
+    pks, pvs = torch.zeros(pool, blocks, hk), torch.zeros(pool, blocks, hk)
+    for x, codes, scale in ((k, pk, pks), (clean, pv, pvs)):
+        ref.append_slots(cached(x), codes, scale, slots)
+        ref.append_call(added(x), codes, scale, old, table=table)
+    lens = [x + n for x in old]
+    want, weight = ref.attend(q, ref.values(pk, pks), ref.values(pv, pvs), lens, causal=True, window=window, table=table)
+    at = torch.arange(old[0], lens[0])
+    sees = (at >= first) & ((at - window[0] < first + size) if window[0] >= 0 else True)
+    spoilt = torch.zeros(2, n, heads, dtype=torch.bool)
+    spoilt[0, :, :heads // hk] = sees[:, None]
+    assert (~sees).any() and (sees.any() or not new)
+    fine = ((out - want).abs() <= ref.tolerance(want, weight, F16, max(lens), 10.0)).all(-1)
+    assert fine[~spoilt].all()
+    assert not torch.isfinite(out[spoilt]).any()
