@@ -8,7 +8,7 @@
 //   warps 12-15      converters: a unit of codes to fp16, into the swizzled ring that the MMAs read
 //
 // Mathematics.  As in cache8_decode.cuh: t_j = scale * ks_j * (q . k8_j), weights 2^(t_j - M) * vs_j rounded to fp16, sums of 2^(t_j - M) in
-// fp32.  M is the largest of (maximum of t over 16 keys + log2 of the largest vs of the 16), so no weight is above 2^cfg.rescale_at.  The
+// fp32.  M is the largest t + log2 vs of the keys that the row sees, so no weight is above 2^cfg.rescale_at.  The
 // codes are fp16 exactly and the scales stay out of the products: ks multiplies the scores, vs the probabilities, in fp32.
 // Bound.  Per tile of 128 x 128 scores the tensor pipe has 16 * head_dim / 128 * 64 cycles, the exponentials 1024; a converter thread
 // turns 2 x head_dim codes into halves meanwhile.  (With cp.async by the converter threads themselves, asking for a unit took them
@@ -49,7 +49,7 @@ template <int D> struct CCfg {
   static constexpr int kQBytes = kBM * D * 2;
   static constexpr int kRawAt = kQBytes + kStages * kUnitBytes;
   static constexpr int kShared = kRawAt + kRaw * kRawBytes;
-  static constexpr int kSmemBytes = kShared + 1024 /*align slack*/ + 6144 /*CShared*/;
+  static constexpr int kSmemBytes = kShared + 1024 /*align slack*/ + 8192 /*CShared*/;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
   // Pieces of the keys, at most: a merge keeps a weight per piece and row over both rings.
   static constexpr int kPieces = (kShared - kQBytes) / (kBM * (int)sizeof(float));
@@ -76,9 +76,9 @@ struct CShared {
   float lrun[kBM];         // row sums, up to the tile before the last one each group has settled
   alignas(16) float ks[kScaleBufs][kBN];
   alignas(16) float vs[kScaleBufs][kBN];
-  alignas(16) float lv[kScaleBufs][kBN / 16];   // log2 of the largest vs of 16 keys
+  alignas(16) float lv[kScaleBufs][kBN];        // log2 of vs, of each key (kFine) or of 16
 };
-static_assert(sizeof(CShared) <= 6144, "CShared must fit its reserve");
+static_assert(sizeof(CShared) <= 8192, "CShared must fit its reserve");
 
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, CShared* sh, int code) {
   return bounded_wait(bar, parity, &sh->abort_flag, &g_cache8_chunk_status, code);
@@ -387,14 +387,14 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (kFine) {
           *reinterpret_cast<float4*>(&sh->ks[sb][lane * 4]) = k4;
           *reinterpret_cast<float4*>(&sh->vs[sb][lane * 4]) = v4;
+          auto log2_of_scale = [](float v) { return __log2f(fmaxf(v, 0x1p-60f)); };
+          *reinterpret_cast<float4*>(&sh->lv[sb][lane * 4]) =
+              make_float4(log2_of_scale(v4.x), log2_of_scale(v4.y), log2_of_scale(v4.z), log2_of_scale(v4.w));
         } else if ((lane & 3) == 0) {
           sh->ks[sb][lane >> 2] = k4.x;
           sh->vs[sb][lane >> 2] = v4.x;
+          sh->lv[sb][lane >> 2] = __log2f(fmaxf(v4.x, 0x1p-60f));
         }
-        float m = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        if ((lane & 3) == 0) sh->lv[sb][lane >> 2] = __log2f(fmaxf(m, 0x1p-60f));
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh->sc_full[sb]));
       }
@@ -586,9 +586,11 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
       // ---- scores times the scales of the keys: mg of each 16 keys turns them into the log2 domain.  Tiles with a mask, with ALiBi or with
       // a scale per key go there at once, through tensor memory in a rolled loop: copies of the passes below for them cost the code that every
-      // tile runs 14 % (instruction cache).
+      // tile runs 14 % (instruction cache).  With a scale per key the maximum is taken there too, over the keys that the row sees: a key
+      // that it does not see, or sees with a low score, may have a scale of V far above theirs.
       const bool masked_or_fine = kAlibi || kFine || masked;
       const float f = cfg.scale_log2 * qinv;
+      float mx = -INFINITY;                              // row maximum of t + log2 vs
       if (masked_or_fine) {
         int vk_lo, vk_hi;
         visible_k_interval(cfg, qpos, w.keys, vk_lo, vk_hi);
@@ -605,7 +607,9 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           for (int i = 0; i < 32; ++i) {
             float v = __uint_as_float(ra[i]) * (kFine ? sh->ks[sb][cc * 32 + i] : i < 16 ? k2.x : k2.y) * f;
             if (kAlibi) v = fmaf(-tilt, fabsf(dist0 - (float)i), v);
-            ra[i] = __float_as_uint(col_visible(cm, i) ? v : -INFINITY);
+            v = col_visible(cm, i) ? v : -INFINITY;
+            ra[i] = __float_as_uint(v);
+            if (kFine) mx = fmaxf(mx, v + sh->lv[sb][cc * 32 + i]);
           }
           tmem_st32(tS + cc * 32, ra);
         }
@@ -615,12 +619,11 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         return masked_or_fine ? make_float2(1.f, 1.f) : f2mul(*reinterpret_cast<const float2*>(&sh->ks[sb][cc * 2]), make_float2(f, f));
       };
 
-      // ---- row maximum of t + log2 vs, vs by its largest of 16 keys -----------------------------
+      // ---- row maximum, vs and mg by 16 keys ------------------------------------------------------
       // The scores are read twice, 32 columns at a time: for the maximum, and for the exponentials (P of columns cc overwrites columns that
       // have been read).  All 128 of a row do not fit beside the rest in what 512 threads have: 512 bytes of them were spilled, and a
       // tile's exponentials took 4200 cycles.
-      float mx = -INFINITY;
-      {
+      if (!kFine) {
         uint32_t ra[32], rb[32];
         tmem_ld32(tS, ra);
 #pragma unroll

@@ -1,4 +1,5 @@
-"""KV cache in 8 bits, beside test_gpu_cache8.py: many pieces of one sequence, tokens that are no numbers."""
+"""KV cache in 8 bits, beside test_gpu_cache8.py: many pieces of one sequence, tokens that are no numbers, scales
+far apart in chunks."""
 import math
 
 import pytest
@@ -95,3 +96,35 @@ def test_tokens_that_are_no_numbers_spoil_the_rows_that_see_them(case, new, bad,
     fine = ((out - want).abs() <= ref.tolerance(want, weight, F16, max(lens), 10.0)).all(-1)
     assert fine[~spoilt].all()
     assert not torch.isfinite(out[spoilt]).any()
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("n,heads,dim,blocks,leftpad", [(40, 4, 64, 16, 0), (40, 4, 128, 4, 0), (30, 4, 256, 2, 0), (40, 4, 64, 1, 5), (100, 8, 128, 16, 0),
+                                                        (40, 4, 64, 1, 0), (100, 8, 64, 1, 0)])
+def test_chunk_with_scales_far_apart(n, heads, dim, blocks, leftpad, code):
+    """Keys whose scales of V are 2^30 above their neighbours', hidden from the earlier rows of the chunk: what those rows see keeps its
+    precision."""
+    page, hk = 16, 2
+    size, old = page // blocks, [160, 75]              # lengths that include the chunk
+    paged = leftpad == 0
+    table, pool = make_table(41, old, page)
+    if not paged:
+        table, pool, page, blocks = None, 2, 192, 12   # the same 16 keys per scale, but not in line with tiles of 16
+    place = dict(table=table) if paged else dict(leftpad=torch.tensor([leftpad, 0]))
+    kc, ks = make_cache(42, pool, page, hk, dim, code, blocks)
+    vc, vs = make_cache(43, pool, page, hk, dim, code, blocks)
+    q = rand(44, 2, n, heads, dim).to(F16)
+    # the block of key 140 of sequence 0 has large values
+    at = 140 + leftpad
+    row = (int(table[0, at // page]), at % page // (page // blocks)) if paged else (0, at // (page // blocks))
+    vs[row] *= 2.0 ** 30
+    first = 140 // size * size if paged else at // 16 * 16 - leftpad
+    want, weight = ref.attend(q, ref.values(kc, ks), ref.values(vc, vs), old, causal=True, **place)
+    d = lambda t: None if t is None else t.to(DEV)
+    out = fa().flash_attn_with_kvcache(d(q), d(kc), d(vc), cache_seqlens=torch.tensor(old, device=DEV), block_table=d(table),
+                                       cache_leftpad=d(place.get("leftpad")), causal=True, k_scale=d(ks), v_scale=d(vs)).double().cpu()
+    sees = torch.zeros(2, n, dtype=torch.bool)
+    sees[0] = torch.arange(old[0] - n, old[0]) >= first
+    assert sees.any() and (~sees[0]).any()
+    tol = ref.tolerance(want, weight, F16, max(old), 6.0)        # (no value of the others is above 3.5 * 1.6)
+    assert ((out - want).abs() <= tol)[~sees].all()
