@@ -1,7 +1,7 @@
 // New keys and values into the 8-bit KV cache: packed tokens by slot, or the new tokens of a cache call.
 //
-//   Mathematics.  For each block of tokens and head: need = largest |x| / Q, s' = max(s, need), codes rn(x / s'), and where the scale
-//   grows the codes that the block keeps are rounded again to it.  (fa_b200.h has the exact form.)
+//   Mathematics.  For each block of tokens and head: need = largest |x| / Q, s' = s where |s| >= need, else need, codes rn(x / s'), and where
+//   the scale grows the codes that the block keeps are rounded again to it.  (fa_b200.h has the exact form.)
 //   Bound.  HBM: 2 bytes read and 1 written per element.  A sum over rows is not needed, only a maximum, so the values of a block and
 //   head stay in registers between the maximum and the codes and are read once.
 //   Split.  A run is the tokens of a call that fall into one block.  A CTA looks at `span` tokens, lists the runs that begin among
@@ -213,11 +213,12 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
     const unsigned short bits = (unsigned short)most;
     float need = __fdiv_rn(Elem<T>::to_f(*reinterpret_cast<const T*>(&bits)), C::kLargest);
     if (need < 1.17549435e-38f) need = 0.f;
-    const float now = old != old ? old : (need > old || need != need) ? need : old;
+    const bool raised = need > fabsf(old);
+    const float now = old != old ? old : raised || need != need ? need : old;
     // A scale that is no number or infinite makes every value of the block and head one that is none: its new codes are 0, since e4m3 codes of
     // NaN would reach rows that do not see the key (0 times NaN in the products).
-    const bool spoilt = !(now <= 3.402823466e38f);
-    const float inv = now > 0.f && !spoilt ? __frcp_rn(now) : 0.f;
+    const bool spoilt = !(fabsf(now) <= 3.402823466e38f);
+    const float inv = now != 0.f && !spoilt ? __frcp_rn(now) : 0.f;
     if (spoilt) {
 #pragma unroll
       for (int k = 0; k < kHeld; ++k) held[k] = make_uint4(0u, 0u, 0u, 0u);
@@ -232,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
     for (int k = 0; k < kHeld; ++k)
       if (gl + k * gsize < pieces) store(k, held[k]);
     for (int k = kHeld; gl + k * gsize < pieces; ++k) store(k, spoilt ? make_uint4(0u, 0u, 0u, 0u) : load(k));
-    if (run.kept > 0 && now > old) {
-      const float m = __fmul_rn(old, inv);
+    if (run.kept > 0 && raised) {
+      const float m = __fmul_rn(old, inv), least = m < 0.f ? -127.f : -128.f;            // int8: -128 has no opposite
       for (int j = gl; j < run.kept << (dshift - 1); j += gsize) {
         const int row = j >> (dshift - 1), col = (j & ((1 << (dshift - 1)) - 1)) * 16;
         uint4* q = reinterpret_cast<uint4*>(codes - (int64_t)(row + 1) * code_stride + col);
@@ -243,6 +244,10 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
         for (int k = 0; k < 4; ++k) {
           float f[4];
           C::floats(w[k], f);
+          if (kCode == FA_CODE_INT8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = fmaxf(f[e], least);
+          }
           w[k] = C::four(f[0], f[1], f[2], f[3], m);
         }
         *q = v;

@@ -8,7 +8,7 @@
 //   warps 12-15      converters: a unit of codes to fp16, into the swizzled ring that the MMAs read
 //
 // Mathematics.  As in cache8_decode.cuh: t_j = scale * ks_j * (q . k8_j), weights 2^(t_j - M) * vs_j rounded to fp16, sums of 2^(t_j - M) in
-// fp32.  M is the largest t + log2 vs of the keys that the row sees, so no weight is above 2^cfg.rescale_at.  The
+// fp32.  M is the largest t + log2 |vs| of the keys that the row sees, so no weight is above 2^cfg.rescale_at.  The
 // codes are fp16 exactly and the scales stay out of the products: ks multiplies the scores, vs the probabilities, in fp32.
 // Bound.  Per tile of 128 x 128 scores the tensor pipe has 16 * head_dim / 128 * 64 cycles, the exponentials 1024; a converter thread
 // turns 2 x head_dim codes into halves meanwhile.  (With cp.async by the converter threads themselves, asking for a unit took them
@@ -76,7 +76,7 @@ struct CShared {
   float lrun[kBM];         // row sums, up to the tile before the last one each group has settled
   alignas(16) float ks[kScaleBufs][kBN];
   alignas(16) float vs[kScaleBufs][kBN];
-  alignas(16) float lv[kScaleBufs][kBN];        // log2 of vs, of each key (kFine) or of 16
+  alignas(16) float lv[kScaleBufs][kBN];        // log2 of |vs|, of each key (kFine) or of 16
 };
 static_assert(sizeof(CShared) <= 8192, "CShared must fit its reserve");
 
@@ -387,13 +387,13 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (kFine) {
           *reinterpret_cast<float4*>(&sh->ks[sb][lane * 4]) = k4;
           *reinterpret_cast<float4*>(&sh->vs[sb][lane * 4]) = v4;
-          auto log2_of_scale = [](float v) { return __log2f(fmaxf(v, 0x1p-60f)); };
+          auto log2_of_scale = [](float v) { return __log2f(fmaxf(fabsf(v), 0x1p-60f)); };
           *reinterpret_cast<float4*>(&sh->lv[sb][lane * 4]) =
               make_float4(log2_of_scale(v4.x), log2_of_scale(v4.y), log2_of_scale(v4.z), log2_of_scale(v4.w));
         } else if ((lane & 3) == 0) {
           sh->ks[sb][lane >> 2] = k4.x;
           sh->vs[sb][lane >> 2] = v4.x;
-          sh->lv[sb][lane >> 2] = __log2f(fmaxf(v4.x, 0x1p-60f));
+          sh->lv[sb][lane >> 2] = __log2f(fmaxf(fabsf(v4.x), 0x1p-60f));
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh->sc_full[sb]));
@@ -580,6 +580,10 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 
       const int sb = j % kScaleBufs;
       ok = wait_bar(&sh->sc_full[sb], (j / kScaleBufs) & 1, sh, 29);
+      if (!kFine) {                                      // a negative scale of K, see below
+        const float4 a = *reinterpret_cast<const float4*>(&sh->ks[sb][0]), b = *reinterpret_cast<const float4*>(&sh->ks[sb][4]);
+        masked |= fminf(fminf(fminf(a.x, a.y), fminf(a.z, a.w)), fminf(fminf(b.x, b.y), fminf(b.z, b.w))) < 0.f;
+      }
       ok = ok && wait_bar(&sh->s_full[buf], par, sh, 31 + x);
       if (!ok) break;
       tc_fence_after();
@@ -587,10 +591,11 @@ cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       // ---- scores times the scales of the keys: mg of each 16 keys turns them into the log2 domain.  Tiles with a mask, with ALiBi or with
       // a scale per key go there at once, through tensor memory in a rolled loop: copies of the passes below for them cost the code that every
       // tile runs 14 % (instruction cache).  With a scale per key the maximum is taken there too, over the keys that the row sees: a key
-      // that it does not see, or sees with a low score, may have a scale of V far above theirs.
+      // that it does not see, or sees with a low score, may have a scale of V far above theirs.  So do tiles with a negative scale of K, whose
+      // largest score has the smallest product.
       const bool masked_or_fine = kAlibi || kFine || masked;
       const float f = cfg.scale_log2 * qinv;
-      float mx = -INFINITY;                              // row maximum of t + log2 vs
+      float mx = -INFINITY;                              // row maximum of t + log2 |vs|
       if (masked_or_fine) {
         int vk_lo, vk_hi;
         visible_k_interval(cfg, qpos, w.keys, vk_lo, vk_hi);

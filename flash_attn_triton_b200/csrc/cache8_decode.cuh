@@ -3,7 +3,7 @@
 //
 //   Mathematics.  With codes k8, v8 and scales ks, vs of the block a key j is in:
 //     t_j = scale * ks_j * (q . k8_j),   out = sum_j p_j vs_j v8_j / sum_j p_j,   p_j = 2^(t_j - M).
-//   M is the running maximum of t_j + log2 vs_j, so that the weights p_j vs_j that go to the tensor cores as fp16 are at most about 1,
+//   M is the running maximum of t_j + log2 |vs_j|, so that the weights p_j vs_j that go to the tensor cores as fp16 are at most about 1,
 //   however much the scales of the blocks differ; the sum of the p_j is in fp32, whose range takes the offset.
 //   Operands.  Codes are fp16 exactly.  bf16 queries are multiplied by the power of two that brings the largest of a unit to [2^14, 2^15);
 //   elements more than 2^32 below it lose bits, nothing else does.
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
       for (int j = 0; j < 2; ++j) {
         ks[h][j] = tS[h * 16 + j * 8 + g] * kmul;
         vs[h][j] = tS[KW + h * 16 + j * 8 + g];
-        lv[h][j] = __log2f(fmaxf(vs[h][j], 0x1p-60f));
+        lv[h][j] = __log2f(fmaxf(fabsf(vs[h][j]), 0x1p-60f));
       }
     }
 

@@ -70,7 +70,7 @@ struct PShared {
   uint32_t qmost[8];
   alignas(16) float ks[kScaleBufs][kBN / 16];   // scales of each 16 keys
   alignas(16) float vs[kScaleBufs][kBN / 16];
-  alignas(16) float lv[kScaleBufs][kBN / 16];   // log2 of those of V
+  alignas(16) float lv[kScaleBufs][kBN / 16];   // log2 of the magnitude of those of V
 };
 static_assert(sizeof(PShared) <= 2048, "PShared must fit its reserve");
 
@@ -327,7 +327,7 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
             if (!ok) break;
             if (lane < 16) (of_v ? sh->vs[sb] : sh->ks[sb])[lane & 7] = now;
-            if (of_v && lane < 16) sh->lv[sb][lane & 7] = __log2f(fmaxf(now, 0x1p-60f));
+            if (of_v && lane < 16) sh->lv[sb][lane & 7] = __log2f(fmaxf(fabsf(now), 0x1p-60f));
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->sc_full[sb]));
           }
@@ -503,18 +503,20 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (cfg.wr >= 0) masked |= (k0 + kBN - 1 > sq_min + cfg.wr);
       const int sb = j % kScaleBufs;
       ok = wait_bar(&sh->sc_full[sb], (j / kScaleBufs) & 1, sh, 29);
-      ok = ok && wait_bar(&sh->s_full[x], j & 1, sh, 31 + x);
       if (!ok) break;
-      tc_fence_after();
-
       // mg of each 16 keys turns their scores into the log2 domain.  Masked tiles go there at once, through tensor memory in a rolled loop:
-      // with copies of the passes below for them, the code that every tile runs was slower by 14 % (instruction cache).
+      // with copies of the passes below for them, the code that every tile runs was slower by 14 % (instruction cache).  So do tiles with a
+      // negative scale of K, whose largest score has the smallest product (seen before the scores are there, it costs nothing).
       float mg[8];
       {
         const float4 a = *reinterpret_cast<const float4*>(&sh->ks[sb][0]), b = *reinterpret_cast<const float4*>(&sh->ks[sb][4]);
         mg[0] = a.x * f; mg[1] = a.y * f; mg[2] = a.z * f; mg[3] = a.w * f;
         mg[4] = b.x * f; mg[5] = b.y * f; mg[6] = b.z * f; mg[7] = b.w * f;
+        masked |= fminf(fminf(fminf(a.x, a.y), fminf(a.z, a.w)), fminf(fminf(b.x, b.y), fminf(b.z, b.w))) < 0.f;
       }
+      ok = wait_bar(&sh->s_full[x], j & 1, sh, 31 + x);
+      if (!ok) break;
+      tc_fence_after();
       if (masked) {
         int vk_lo, vk_hi;
         visible_k_interval(cfg, qpos, w.keys, vk_lo, vk_hi);
@@ -543,7 +545,7 @@ cache8_pair_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + cc * 32, r[cc]);
       tmem_wait_ld();
 
-      // ---- row maximum of t + log2 vs -----------------------------------------------------------
+      // ---- row maximum of t + log2 |vs| -----------------------------------------------------------
       float mx = -INFINITY;
       {
         const float4 a = *reinterpret_cast<const float4*>(&sh->lv[sb][0]), b = *reinterpret_cast<const float4*>(&sh->lv[sb][4]);

@@ -298,8 +298,9 @@ size_t fa_decode_static_scratch_bytes(void);
  * scale per block of `block` consecutive tokens (it divides page_size) and head; a value is code * scale.
  *
  * Appending to a block: with `kept` tokens of the sequence already in it, its scale s and the new tokens' largest magnitude a,
- *   need = a / Q  (Q = 127 or 448; below the smallest normal number: 0),  s' = max(kept ? s : 0, need),  inv = s' > 0 ? 1 / s' : 0
- *   new codes  rn(x * inv);   kept codes, where s' > s,  rn(code * (s * inv));   all in IEEE fp32, rounded half to even.
+ *   need = a / Q  (Q = 127 or 448; below the smallest normal number: 0),  s' = kept && |s| >= need ? s : need,  inv = s' ? 1 / s' : 0
+ *   new codes  rn(x * inv);   kept codes, where need > |s|,  rn(code * (s * inv));   all in IEEE fp32, rounded half to even.
+ * An append makes no negative scales, but a caller's may be (a kept code of -128 counts as -127 where its sign changes).
  * A NaN or an infinity among the new tokens goes to the scale, so that the values of that block and head are NaN until the block is
  * started again; while the scale is no finite number, new codes are 0.
  * Codes are numbers: a NaN of e4m3 (0x7f, 0xff), which an append never writes, in a key that a sequence holds may also reach rows that do

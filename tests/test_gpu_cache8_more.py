@@ -1,5 +1,5 @@
 """KV cache in 8 bits, beside test_gpu_cache8.py: many pieces of one sequence, tokens that are no numbers, scales
-far apart in chunks."""
+far apart in chunks, negative scales."""
 import math
 
 import pytest
@@ -128,3 +128,61 @@ def test_chunk_with_scales_far_apart(n, heads, dim, blocks, leftpad, code):
     assert sees.any() and (~sees[0]).any()
     tol = ref.tolerance(want, weight, F16, max(old), 6.0)        # (no value of the others is above 3.5 * 1.6)
     assert ((out - want).abs() <= tol)[~sees].all()
+
+
+def signs(seed, scale):
+    """The scales, about half of them negative."""
+    return torch.where(rand(seed, *scale.shape) < 0, -scale, scale)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("n,heads,dim,blocks,window", [(1, 4, 64, 1, -1), (4, 8, 128, 16, -1), (3, 4, 256, 1, 50), (40, 4, 64, 1, -1), (40, 4, 128, 4, -1),
+                                                       (40, 4, 256, 1, 90), (100, 8, 64, 1, -1), (100, 8, 128, 1, 120)])
+def test_attend_negative_scales(n, heads, dim, blocks, window, code):
+    page, hk, old = 16, 2, [500, 260]                  # whole tiles of keys in front of the rows, and ones with a mask
+    table, pool = make_table(51, old, page)
+    kc, ks = make_cache(52, pool, page, hk, dim, code, blocks)
+    vc, vs = make_cache(53, pool, page, hk, dim, code, blocks)
+    ks, vs = signs(54, ks), signs(55, vs)
+    q = (2 * rand(56, 2, n, heads, dim)).to(F16)
+    want, weight = ref.attend(q, ref.values(kc, ks), ref.values(vc, vs), old, causal=True, window=(window, 0) if window >= 0 else (-1, -1), table=table)
+    out = fa().flash_attn_with_kvcache(q.to(DEV), kc.to(DEV), vc.to(DEV), cache_seqlens=torch.tensor(old, device=DEV), block_table=table.to(DEV),
+                                       causal=True, window_size=(window, 0) if window >= 0 else (-1, -1), k_scale=ks.to(DEV), v_scale=vs.to(DEV))
+    assert ((out.double().cpu() - want).abs() <= ref.tolerance(want, weight, F16, max(old), 6.0)).all()
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+def test_append_to_blocks_of_negative_scale(code):
+    """The sign stays where the magnitude does; where new tokens raise it, kept codes change sign."""
+    page, dim, heads, pages = 16, 32, 4, 5
+    kc, ks = make_cache(61, pages, page, heads, dim, code, 1)
+    if code == INT8:
+        kc[:, 3] = -128
+    ks = signs(62, ks)
+    assert (ks < 0).any() and (ks > 0).any()
+    ks[1, 0, 0], ks[2, 0, 1] = -math.inf, 0.0
+    slots = torch.tensor([p * page + r for p in range(pages) for r in range(5, 9)])
+    x = rand(63, len(slots), heads, dim).to(F16)
+    x[:8] *= 0.1                                       # below what the scales allow, then above
+    x[12:] *= 9
+    want, wants = kc.clone(), ks.clone()
+    for p in range(pages):
+        new = x[4 * p:4 * p + 4].float()
+        for h in range(heads):
+            old, need = ks[p, 0, h], new[:, h].abs().max() / torch.tensor(ref.LARGEST[code])
+            now = old if old.abs() >= need else need
+            inv = 1 / now if now != 0 and now.isfinite() else torch.zeros(())
+            if need > old.abs():
+                held = kc[p, :5, h].float()
+                want[p, :5, h] = ref.coded((held.clamp(min=-127.0) if old < 0 and code == INT8 else held) * (old * inv), code)
+            want[p, 5:9, h] = ref.coded(new[:, h] * inv if now.isfinite() else torch.zeros(4, dim), code)      # (0, not -0, under an infinite scale)
+            wants[p, 0, h] = now
+    kd, vd, ksd, vsd = kc.to(DEV), kc.to(DEV), ks.to(DEV), ks.to(DEV)
+    fa().kvcache_append(x.to(DEV), x.to(DEV), kd, vd, slots.to(DEV), ksd, vsd)
+    for codes, scale in ((kd, ksd), (vd, vsd)):
+        assert torch.equal(ref.bits(codes.cpu()), ref.bits(want)) and torch.equal(scale.cpu(), wants)
+    fine = wants.isfinite() & (wants != 0)             # and the new values are within half a step
+    held, size = ref.values(want, wants)[:, 5:9], wants.abs().double()[:, :, :, None]
+    half = size / 2 if code == INT8 else torch.maximum(x.double().view(pages, 4, heads, dim).abs() * 2.0 ** -4, size * 2.0 ** -10)
+    err = (held - x.double().view(pages, 4, heads, dim)).abs()
+    assert (err <= half * (1 + 1e-5))[fine.expand(-1, 4, -1)].all()
