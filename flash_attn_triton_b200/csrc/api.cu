@@ -11,6 +11,7 @@
 
 #include "common.cuh"
 #include "queue_slots.h"
+#include "strided.h"
 
 namespace fa {
 
@@ -500,11 +501,25 @@ static int validate_cache8(const fa_cache8& c, int page_size, int num_pages, con
   FA_REQUIRE(below_64g(ks, 3) && below_64g(vs, 3), "cache strides must not be negative and must be below 64 GiB");
   return FA_OK;
 }
+// What an append writes: codes and scales of keys and values, each of them a place of its own.
+static int validate_written8(const fa_cache8& c, int page_size, int num_pages, int heads, int head_dim, void* k_cache, void* v_cache,
+                             const int64_t* ks, const int64_t* vs) {
+  const int64_t rows[3] = {num_pages, page_size, heads}, blocks[3] = {num_pages, page_size / c.block, heads};
+  const Strided k = strided(k_cache, head_dim, 1, rows, ks), v = strided(v_cache, head_dim, 1, rows, vs);
+  FA_REQUIRE(!may_overlap_itself(k) && !may_overlap_itself(v) && !may_overlap(k, v),
+             "k_cache and v_cache must not overlap, nor rows of them, where tokens are appended");
+  const Strided k_scale = strided(c.k_scale, 4, 4, blocks, c.ks_stride), v_scale = strided(c.v_scale, 4, 4, blocks, c.vs_stride);
+  FA_REQUIRE(!may_overlap_itself(k_scale) && !may_overlap_itself(v_scale) && !may_overlap(k_scale, v_scale),
+             "k_scale and v_scale must not overlap, nor elements of them, where tokens are appended");
+  return FA_OK;
+}
 static int validate_decode8(const fa_decode_args* a, const fa_cache8* c) {
   if (int r = validate_decode(a)) return r;
   FA_REQUIRE(c != nullptr, "cache is NULL");
   if (a->batch == 0 || a->seqlen_q == 0) return FA_OK;
-  return validate_cache8(*c, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride);
+  if (int r = validate_cache8(*c, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride)) return r;
+  if (a->k_new == nullptr) return FA_OK;
+  return validate_written8(*c, a->page_size, a->num_pages, a->heads_kv, a->head_dim, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride);
 }
 int fa_decode_paged8(const fa_decode_args* a, const fa_cache8* c, void* stream) {
   if (int r = validate_decode8(a, c)) return r;
@@ -536,7 +551,8 @@ static int validate_append8(const fa_append8_args* a) {
   FA_REQUIRE(a->k && a->v && a->slots, "k, v and slots are required");
   FA_REQUIRE(aligned16(a->k) && aligned16(a->v) && mult8(a->k_stride, 2) && mult8(a->v_stride, 2), "k/v rows must be 16-byte aligned");
   FA_REQUIRE(a->workspace == nullptr || aligned16(a->workspace), "workspace must be 16-byte aligned");
-  return validate_cache8(a->cache, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride);
+  if (int r = validate_cache8(a->cache, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride)) return r;
+  return validate_written8(a->cache, a->page_size, a->num_pages, a->heads, a->head_dim, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride);
 }
 int fa_append8(const fa_append8_args* a, void* stream) {
   if (int r = validate_append8(a)) return r;

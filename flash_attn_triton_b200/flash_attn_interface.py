@@ -292,7 +292,7 @@ def kvcache_append(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale):
     block so far over 127 (int8) or 448 (e4m3); where new tokens raise it, the codes of the tokens that stay are rounded again.
     A NaN or infinity among the tokens of a block goes to its scale, which makes the values of that block and head NaN and those of
     no other; its new codes are 0 then.  The tokens that a call brings for one block
-    follow one another, in the order of their slots.
+    follow one another, in the order of their slots.  Caches and scales must not overlap, nor elements of them.
 
     With value checks on, a slot behind the cache or a block that is written in two places raises ValueError and
     nothing is written; off (see set_validation), such slots are passed over, and such a block has the codes of either."""
@@ -379,7 +379,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     block of capacity / blocks (page_size / blocks) consecutive tokens, at most 1024; a value is code * scale.  Codes are numbers
     (no e4m3 NaN, which an append never writes) wherever a sequence has keys.  q, k
     and v stay 16-bit.  New tokens are quantised as `kvcache_append` does it, and the attention is to what the cache
-    then holds.
+    then holds; caches and scales that overlap (an expanded scale, one tensor for keys and values) are for calls without them.
 
     With value checks on (the default) the kernel makes them first (page indices in range, lengths
     fit the cache and the rotary tables) and the call waits for that one flag, not for the attention;

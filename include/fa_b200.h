@@ -306,6 +306,8 @@ size_t fa_decode_static_scratch_bytes(void);
  * Codes are numbers: a NaN of e4m3 (0x7f, 0xff), which an append never writes, in a key that a sequence holds may also reach rows that do
  * not see the key.  In rows of the cache that no sequence holds, any code will do.
  *
+ * Where tokens are appended, caches and scales are written: strides of 0, one tensor for keys and values and the like are refused then.
+ *
  * fa_decode_paged8: fa_decode_paged on such a cache; the call's cache pointers are the codes', its cache strides are in codes.  The
  * new tokens are appended first, and the attention is to what the cache then holds.  dtype is q's, the new tokens' and o's.
  * Workspace and counters: fa_decode8_workspace_bytes(), fa_decode8_counters().

@@ -186,3 +186,32 @@ def test_append_to_blocks_of_negative_scale(code):
     half = size / 2 if code == INT8 else torch.maximum(x.double().view(pages, 4, heads, dim).abs() * 2.0 ** -4, size * 2.0 ** -10)
     err = (held - x.double().view(pages, 4, heads, dim)).abs()
     assert (err <= half * (1 + 1e-5))[fine.expand(-1, 4, -1)].all()
+
+
+def test_overlapping_caches_and_scales():
+    """Read, they are what they hold; calls that append refuse them and write nothing."""
+    page, hk, dim, pool = 16, 2, 64, 4
+    kc, ks = (t.to(DEV) for t in make_cache(71, pool, page, hk, dim, INT8, 1))
+    vc, vs = kc.clone(), ks.clone()
+    one = torch.full((1, 1, 1), 0.02, device=DEV).expand(pool, 1, hk)
+    q = rand(72, 1, 1, 4, dim).to(F16).to(DEV)
+    new = rand(73, 1, 1, hk, dim).to(F16).to(DEV)
+    lens, rows = torch.tensor([7], device=DEV), torch.tensor([2], device=DEV)
+    call = lambda kc=kc, vc=vc, ks=ks, vs=vs, k=None: fa().flash_attn_with_kvcache(q, kc, vc, k, k, cache_seqlens=lens, cache_batch_idx=rows, k_scale=ks,
+                                                                                 v_scale=vs)
+    flat = one.contiguous()
+    assert torch.equal(call(ks=one, vs=one), call(ks=flat, vs=flat.clone()))
+    assert torch.equal(call(vc=kc, vs=ks), call())
+    before = [t.clone() for t in (kc, vc, ks, vs, one)]
+    slots = torch.arange(3, device=DEV)
+    packed = rand(74, 3, hk, dim).to(F16).to(DEV)
+    for bad in (dict(ks=one), dict(vs=one), dict(ks=flat, vs=flat), dict(vc=kc), dict(kc=kc[:1].expand(pool, -1, -1, -1)), dict(ks=ks, vs=ks)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            call(**bad, k=new)
+        t = {**dict(kc=kc, vc=vc, ks=ks, vs=vs), **bad}
+        with pytest.raises(ValueError, match="must not overlap"):
+            fa().kvcache_append(packed, packed, t["kc"], t["vc"], slots, t["ks"], t["vs"])
+    assert all(torch.equal(a, b) for a, b in zip((kc, vc, ks, vs, one), before))
+    call(k=new)
+    fa().kvcache_append(packed, packed, kc, vc, slots, ks, vs)
+    assert not torch.equal(kc, before[0])
