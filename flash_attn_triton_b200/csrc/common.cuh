@@ -87,8 +87,10 @@ __host__ __device__ inline ScoreCfg make_score_cfg(float scale, float softcap, i
   c.softcap = softcap;
   c.inv_softcap = softcap > 0.f ? 1.f / softcap : 0.f;
   c.causal = causal;
-  c.wl = wl;
-  c.wr = wr;
+  // wider than any sequence, and position +- window stays inside 32 bits
+  constexpr int kWidest = 1 << 30;
+  c.wl = wl < kWidest ? wl : kWidest;
+  c.wr = wr < kWidest ? wr : kWidest;
   c.has_alibi = alibi ? 1 : 0;
   c.bias = nullptr;
   c.bias_stride[0] = c.bias_stride[1] = c.bias_stride[2] = c.bias_stride[3] = 0;

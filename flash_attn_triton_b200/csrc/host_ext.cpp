@@ -21,6 +21,7 @@
 
 #include <string.h>
 
+#include <algorithm>
 #include <array>
 #include <list>
 #include <mutex>
@@ -483,6 +484,8 @@ struct Args {
     TORCH_CHECK_TYPE(THPVariable_Check(o), "expected a tensor or None");
     return THPVariable_Unpack(o);
   }
+  // a window's bound: of any size, -1 or less is open
+  int window() { return (int)std::max<int64_t>(-1, std::min<int64_t>(integer(), INT32_MAX)); }
   int64_t integer() {
     const long long x = PyLong_AsLongLong(next());
     if (x == -1 && PyErr_Occurred()) throw python_error();
@@ -503,8 +506,8 @@ struct Args {
 void score_params(Args& a, Params& c) {
   c.scale = a.real();
   c.causal = a.truth();
-  c.wl = (int)a.integer();
-  c.wr = (int)a.integer();
+  c.wl = a.window();
+  c.wr = a.window();
   c.softcap = a.real();
   c.alibi = a.tensor_or_none();
 }
@@ -754,8 +757,8 @@ PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   memset(&p, 0, sizeof(p));
   p.softmax_scale = (float)a.real();
   p.causal = a.truth();
-  p.window_left = (int)a.integer();
-  p.window_right = (int)a.integer();
+  p.window_left = a.window();
+  p.window_right = a.window();
   p.rotary_interleaved = a.truth();
   Tensor alibi = a.tensor_or_none();
   p.num_splits = (int)a.integer();
