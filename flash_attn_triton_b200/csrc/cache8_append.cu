@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
       const int j = gl + k * gsize;
       held[k] = j < pieces ? load(k) : make_uint4(0u, 0u, 0u, 0u);
     }
-    const float old = run.kept > 0 ? *scale : 0.f;
+    float old = run.kept > 0 ? *scale : 0.f;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) widen(held[k]);
     for (int k = kHeld; gl + k * gsize < pieces; ++k) widen(load(k));
@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, kHeld == 16 ? 2 : kSlots ? 4 : 3)
     const unsigned short bits = (unsigned short)most;
     float need = __fdiv_rn(Elem<T>::to_f(*reinterpret_cast<const T*>(&bits)), C::kLargest);
     if (need < 1.17549435e-38f) need = 0.f;
+    if (fabsf(old) < 1.17549435e-38f) old = 0.f;          // (its reciprocal may be infinite)
     const bool raised = need > fabsf(old);
     const float now = old != old ? old : raised || need != need ? need : old;
     // A scale that is no number or infinite makes every value of the block and head one that is none: its new codes are 0, since e4m3 codes of

@@ -298,7 +298,7 @@ size_t fa_decode_static_scratch_bytes(void);
  * scale per block of `block` consecutive tokens (it divides page_size) and head; a value is code * scale.
  *
  * Appending to a block: with `kept` tokens of the sequence already in it, its scale s and the new tokens' largest magnitude a,
- *   need = a / Q  (Q = 127 or 448; below the smallest normal number: 0),  s' = kept && |s| >= need ? s : need,  inv = s' ? 1 / s' : 0
+ *   need = a / Q  (Q = 127 or 448; it and |s| below the smallest normal number: 0),  s' = kept && |s| >= need ? s : need,  inv = s' ? 1 / s' : 0
  *   new codes  rn(x * inv);   kept codes, where need > |s|,  rn(code * (s * inv));   all in IEEE fp32, rounded half to even.
  * An append makes no negative scales, but a caller's may be (a kept code of -128 counts as -127 where its sign changes).
  * A NaN or an infinity among the new tokens goes to the scale, so that the values of that block and head are NaN until the block is

@@ -215,3 +215,21 @@ def test_overlapping_caches_and_scales():
     call(k=new)
     fa().kvcache_append(packed, packed, kc, vc, slots, ks, vs)
     assert not torch.equal(kc, before[0])
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+def test_append_to_blocks_of_tiny_scale(code):
+    """A caller's scale below the smallest normal number counts as 0: zeros and tiny tokens get codes of 0 (not 0 times an infinite reciprocal)."""
+    page, dim, heads = 16, 32, 3
+    kc, ks = make_cache(81, 4, page, heads, dim, code, 1)
+    ks[1, 0], ks[2, 0] = 1e-40, -1e-45
+    slots = torch.tensor([p * page + r for p in (1, 2, 3) for r in (5, 6)])
+    x = rand(82, 6, heads, dim).to(BF16)
+    x[:4, 0], x[:4, 1] = 0.0, 1e-38
+    kd, vd, ksd, vsd = kc.to(DEV), kc.to(DEV), ks.to(DEV), ks.to(DEV)
+    fa().kvcache_append(x.to(DEV), x.to(DEV), kd, vd, slots.to(DEV), ksd, vsd)
+    want, wants = kc.clone(), torch.where(ks.abs() < ref.TINY, 0.0, ks)
+    ref.append_slots(x, want, wants, slots)
+    for codes, scale in ((kd, ksd), (vd, vsd)):
+        assert torch.equal(ref.bits(codes.cpu()), ref.bits(want)) and torch.equal(scale.cpu(), wants)
+    assert (wants[1:3, 0, :2] == 0).all() and (want.float()[1:3, 5:7, :2] == 0).all()
