@@ -226,11 +226,11 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
 #pragma unroll
           for (int h = 0; h < KB; ++h) {
             const unsigned char* src = row_of(value, page[h], row16[h] + lr);
-            const uint32_t step = (value ? geo.v_row : geo.k_row) * RPW;
+            const uint64_t unit = value ? geo.v_row : geo.k_row;                 // (of 16 bytes, up to 2^32 - 1: products of them are wider)
 #pragma unroll
             for (int i = 0; i < PASSES / KB; ++i) {
               const int at = (h * (PASSES / KB) + i) * RPW;
-              const unsigned char* x = src + (uint64_t)step * (16 * i);
+              const unsigned char* x = src + unit * (uint32_t)(16 * RPW * i);
               cp_async16(dst + at * P + column(at), x, key00 + at + lr < keys ? 16 : 0);     // zeros past the last key
             }
           }

@@ -233,3 +233,27 @@ def test_append_to_blocks_of_tiny_scale(code):
     for codes, scale in ((kd, ksd), (vd, vsd)):
         assert torch.equal(ref.bits(codes.cpu()), ref.bits(want)) and torch.equal(scale.cpu(), wants)
     assert (wants[1:3, 0, :2] == 0).all() and (want.float()[1:3, 5:7, :2] == 0).all()
+
+
+def test_rows_far_apart():
+    """Rows of a cache 32 GiB apart: an offset of two of them, in units of 16 bytes, passes 32 bits."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 80 * 2 ** 30:
+        pytest.skip("needs 64 GiB")
+    dim, rows, far = 256, 3, 2 ** 35
+    memory = torch.empty(2 * far + 4096, dtype=torch.int8, device=DEV)
+    wide = memory.as_strided((1, rows, 1, dim), (16, far, 256, 1))
+    near, scale = make_cache(91, 1, rows, 1, dim, INT8, 1)
+    other, oscale = make_cache(92, 1, rows, 1, dim, INT8, 1)
+    wide.copy_(near)
+    q = rand(93, 1, 1, 2, dim).to(F16).to(DEV)
+    for spread_v in (False, True):
+        pair = lambda x, y: (y, x) if spread_v else (x, y)
+        outs = []
+        for x in (wide, near.to(DEV)):
+            k, v = pair(x, other.to(DEV))
+            ks, vs = pair(scale.to(DEV), oscale.to(DEV))
+            outs.append(fa().flash_attn_with_kvcache(q, k, v, cache_seqlens=torch.tensor([rows], device=DEV), k_scale=ks, v_scale=vs))
+        assert torch.equal(*outs)
+    del memory, wide
+    torch.cuda.empty_cache()
