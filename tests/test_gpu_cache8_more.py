@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import cache8_reference as ref
-from test_gpu_cache8 import BF16, E4M3, F16, INT8, fa, make_cache, make_table, rand, run_attend
+from test_gpu_cache8 import BF16, E4M3, F16, INT8, fa, make_cache, make_table, rand, run_attend, same_cache
 from util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -257,3 +257,110 @@ def test_rows_far_apart():
         assert torch.equal(*outs)
     del memory, wide
     torch.cuda.empty_cache()
+
+
+def test_offsets_past_32_bits_all_that_is_written():
+    """Pages beyond 4 GiB of codes: after a packed append and after each call, codes and scales of every page that the tables name."""
+    page, heads, dim, blocks, pages = 256, 8, 256, 4, 9000     # 4.7e9 codes in each cache
+    far = torch.tensor([8999, 4095, 8192, 8191, 8900])
+    kc = torch.empty(pages, page, heads, dim, dtype=torch.int8, device=DEV)
+    vc = torch.empty_like(kc)
+    ks, vs = (torch.full((pages, blocks, heads), float("nan"), device=DEV) for _ in range(2))
+    kc[far], vc[far] = 0, 0
+    table, small = far[torch.tensor([[0, 1, 4], [2, 3, 4]])].to(torch.int32), torch.tensor([[0, 1, 4], [2, 3, 4]])
+    plain = [torch.zeros(5, page, heads, dim, dtype=torch.int8) for _ in range(2)] + [torch.full((5, blocks, heads), float("nan")) for _ in range(2)]
+
+    def compare():
+        for got, want in zip((kc, vc, ks, vs), plain):
+            assert torch.equal(got[far.to(DEV)].cpu().nan_to_num(-1) if want.is_floating_point() else got[far.to(DEV)].cpu(),
+                               want.nan_to_num(-1) if want.is_floating_point() else want)
+
+    lens = [300, 77]
+    place = lambda t: torch.cat([t[b, torch.arange(n) // page].long() * page + torch.arange(n) % page for b, n in enumerate(lens)])
+    slots = place(table)
+    k, v = rand(101, sum(lens), heads, dim).to(BF16), rand(102, sum(lens), heads, dim).to(BF16)
+    fa().kvcache_append(k.to(DEV), v.to(DEV), kc, vc, slots.to(DEV), ks, vs)
+    ref.append_slots(k, plain[0], plain[2], place(small))
+    ref.append_slots(v, plain[1], plain[3], place(small))
+    compare()
+    for n in (1, 20, 150):
+        q, kn, vn = rand(103 + n, 2, n, 16, dim).to(BF16), rand(104 + n, 2, n, heads, dim).to(BF16), rand(105 + n, 2, n, heads, dim).to(BF16)
+        fa().flash_attn_with_kvcache(q.to(DEV), kc, vc, kn.to(DEV), vn.to(DEV), cache_seqlens=torch.tensor(lens, device=DEV), block_table=table.to(DEV),
+                                     causal=True, k_scale=ks, v_scale=vs)
+        ref.append_call(kn, plain[0], plain[2], lens, table=small)
+        ref.append_call(vn, plain[1], plain[3], lens, table=small)
+        compare()
+        lens = [x + n for x in lens]
+
+
+GROUPS = [
+    # query heads over KV heads that are no power of two apart, one token to more than a tile of rows
+    (28, 4, 1), (28, 4, 2), (28, 4, 3), (28, 4, 30), (40, 8, 1), (40, 8, 3), (40, 8, 4), (10, 2, 27), (7, 1, 150),
+    # rows around the limits of the kernels: 8, 16 and 128 per KV head
+    (8, 1, 1), (9, 1, 1), (8, 1, 2), (17, 1, 1), (16, 1, 8), (43, 1, 3), (16, 2, 16), (16, 2, 17),
+]
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("heads,hk,n", GROUPS)
+def test_attend_groups(heads, hk, n, code):
+    for dim, dtype in ((64, BF16), (128, F16)):
+        run_attend(heads + n, [90, 333], n, True, heads, hk, dim, 32, 2, dtype, code, causal=True)
+
+
+def steps(seed, dim, heads, hk, n, old, page=32):
+    """A call on caches of its own: (function of nothing -> (out, codes, scales), tensors that it reads)."""
+    table, pool = make_table(seed, [x + n for x in old], page)
+    kc, ks = (t.to(DEV) for t in make_cache(seed + 1, pool, page, hk, dim, E4M3, 1))
+    vc, vs = (t.to(DEV) for t in make_cache(seed + 2, pool, page, hk, dim, E4M3, 1))
+    start = [t.clone() for t in (kc, vc, ks, vs)]
+    q, k, v = (rand(seed + 3 + i, len(old), n, h, dim).to(F16).to(DEV) for i, h in enumerate((heads, hk, hk)))
+    lens, tab = torch.tensor(old, dtype=torch.int32, device=DEV), table.to(DEV)
+
+    def call():
+        for t, s in zip((kc, vc, ks, vs), start):
+            t.copy_(s)
+        out = fa().flash_attn_with_kvcache(q, kc, vc, k, v, cache_seqlens=lens, block_table=tab, causal=True, k_scale=ks, v_scale=vs)
+        return [out, kc.view(torch.int8).clone(), vc.view(torch.int8).clone(), ks.clone(), vs.clone()]
+    return call, (q, k, v)
+
+
+PATHS = [(64, 8, 2, 1, [3000, 70]), (256, 4, 2, 4, [900, 900]), (64, 4, 1, 33, [3000]), (256, 2, 1, 40, [2000, 10]), (128, 8, 1, 40, [6000])]
+
+
+@pytest.mark.parametrize("case", range(len(PATHS)))
+def test_calls_repeat_themselves(case):
+    """The same call gives the same bits, each of its pieces merged in their order whichever CTA comes last."""
+    call, _ = steps(110 + 10 * case, *PATHS[case])
+    first = call()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, call()))
+
+
+def test_graphs_and_streams_at_once():
+    """Two captured calls with pieces to merge, replayed at the same time on two streams beside eager calls: as alone."""
+    made = [steps(210 + 10 * i, 64, 4, 1, 33, [3000 + 7 * i]) for i in range(2)] + [steps(240, 128, 8, 1, 40, [2500])]
+    fa().set_validation(False)
+    try:
+        alone = [call() for call, _ in made]
+        side = [torch.cuda.Stream() for _ in range(2)]
+        graphs, outs = [], []
+        for (call, _), stream in zip(made, side):
+            with torch.cuda.stream(stream):
+                call()
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                outs.append(call())
+            graphs.append(g)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for g, stream in zip(graphs, side):
+                with torch.cuda.stream(stream):
+                    g.replay()
+            eager = made[2][0]()
+        torch.cuda.synchronize()
+        for got, want in zip(outs + [eager], alone):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    finally:
+        fa().set_validation(True)
