@@ -364,3 +364,36 @@ def test_graphs_and_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(got, want))
     finally:
         fa().set_validation(True)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("n,heads,dim,blocks", [(1, 4, 64, 1), (4, 8, 256, 1), (40, 4, 64, 1), (40, 4, 128, 4), (40, 4, 256, 1), (100, 8, 64, 1),
+                                                (100, 8, 128, 1)])
+def test_largest_weight_is_not_rounded(n, heads, dim, blocks, code):
+    """fp16: one value in a cache of zeros, whose key has a row's largest score by up to 2^7.  Its weight is exactly 1 relative to the row's
+    maximum, so the output is off by its own rounding and by fp32 (2^-15 of it, see cache8_reference.tolerance) alone.  Maxima are of
+    score + log2 scale: blocks of zeros with scores of 0 have scales up to 1.6 / 0.3 = 2^2.4 of that value's, so rows of low scores may have
+    one of them as the maximum, and a weight that is rounded (half a step more)."""
+    page, hk, length = 16, 2, 300 + n
+    table, pool = make_table(121, [length], page)
+    kc, vc = (torch.zeros(pool, page, hk, dim, dtype=torch.int8).view(torch.int8) for _ in range(2))
+    key = rand(122, hk, dim).sign()
+    kc[table[0, 1], 4] = (64 * key).to(torch.int8)     # key 20: behind tiles of keys with scores of 0
+    vc[table[0, 1], 4] = (rand(123, hk, dim) * 25).round().clamp(-100, 100).to(torch.int8)
+    kc, vc = (ref.coded(x.float(), code) for x in (kc, vc))
+    _, ks = make_cache(124, pool, page, hk, dim, code, blocks)
+    _, vs = make_cache(125, pool, page, hk, dim, code, blocks)
+    # score u of row r, head h: 0.5 to 5 in natural units, q as fp16 holds it
+    u = torch.linspace(0.5, 5.0, n * heads).view(1, n, heads, 1)
+    block = 4 // (page // blocks)
+    unit = (64 * dim ** 0.5 * ks[table[0, 1], block])[None, None, :].repeat_interleave(heads // hk, -1)[..., None]
+    q = (u * key.repeat_interleave(heads // hk, 0) / unit).to(F16)
+    want, weight = ref.attend(q, ref.values(kc, ks), ref.values(vc, vs), [length], causal=True, table=table)
+    out = fa().flash_attn_with_kvcache(q.to(DEV), kc.to(DEV), vc.to(DEV), cache_seqlens=torch.tensor([length], device=DEV), block_table=table.to(DEV),
+                                       causal=True, k_scale=ks.to(DEV), v_scale=vs.to(DEV)).double().cpu()
+    half = torch.finfo(F16).eps / 2 * want.abs() + torch.finfo(F16).smallest_normal * 2.0 ** -11
+    others = vs[table[0].long()].amax(dim=(0, 1))      # of a head
+    leads = u[..., 0] - 0.01 > torch.log(others / vs[table[0, 1], block])[None, None].repeat_interleave(heads // hk, -1)
+    assert leads.sum() > leads.numel() // 2
+    rounded = torch.where(leads, 0.0, 2.0 ** -11)[..., None]
+    assert ((out - want).abs() <= half + (2.0 ** -15 + rounded) * weight).all()
