@@ -37,7 +37,11 @@ struct Plan {
 };
 
 // A chunk: more than 16 query rows per KV head.  The decode kernel would read the cache once per 16 rows; the tcgen05 kernel takes 128 at a
-// time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128: 690 us, 200).
+// time (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128: 669 us, 199).  Near the border, without an append, 4 sequences of those lengths,
+// heads of 64 / 128, tcgen05 against decode units: 24 rows 43 / 47 us against 35 / 42, 48 rows 44 / 50 against 41 / 51, 64 rows 44 / 51 against
+// 48 / 59; 32 sequences: 171 / 194 against 146 / 200, 171 / 194 against 195 / 269, 172 / 195 against 242 / 336.  So decode units would gain up to
+// a fifth at 17 to 32 rows.  They would gain more where the group is no power of two, whose heads do not share a tile: 28 heads over 4, 3 tokens
+// (21 rows) 100 / 113 against 26 / 36, 8 tokens (56 rows) 101 / 114 against 35 / 41.
 bool plan_chunk(const fa_decode_args& a, const fa_cache8& c, Plan& p) {
   const int G = a.heads_q / a.heads_kv;
   if (a.num_splits != 0 || (int64_t)a.seqlen_q * G <= 16 || a.softmax_scale < 0.f) return false;

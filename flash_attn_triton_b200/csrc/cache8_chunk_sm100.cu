@@ -118,7 +118,7 @@ struct Tile {
 
 // T: type of q and o.  kAlibi: with slopes.  kFine: a scale for each key of a tile; else every 16 keys have one scale (blocks of a multiple of
 // 16 tokens, no left padding), which goes into the exponent's FMA and stays in registers.  With one per key, read from shared memory by every
-// thread, a call took 250 us where it now takes 232 (4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128).
+// thread, a call of 4 x 256 tokens behind 1024 to 8192, 32 heads over 8 of 128, takes 250 us and 195 with one per 16; heads of 256: 404, 356.
 template <typename T, int kCode, int D, bool kAlibi, bool kFine>
 __global__ void __launch_bounds__(kThreads, 1)
 cache8_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,

@@ -15,8 +15,8 @@
 //   a row in the scores, where the accumulators start from its negative, and a product with a constant in the outputs.
 //   Scales travel with their tile, by 4-byte cp.async.
 //   Split: see the ranges in the kernel.
-//   Bound.  HBM: one byte per code.  Measured: 64 sequences of 1024 to 32768, 32 heads over 8 of 128, int8: 392 us, 5.2 TB/s of 6.5.  What is
-//   left is the chain of a tile with 12 warps per SM: 790 instructions for 32 keys, issue active 49 %; with the loads taken out of the loop
+//   Bound.  HBM: one byte per code.  Measured: 64 sequences of 1024 to 32768, 32 heads over 8 of 128: 386 us (int8), 388 (e4m3), 5.3 TB/s of 6.5;
+//   heads of 64 282 us, 3.6 TB/s; whole calls over other inputs in turn 434 to 452 on three boxes.  What is left is the chain of a tile with 12 warps per SM: 790 instructions for 32 keys, issue active 49 %; with the loads taken out of the loop
 //   it takes 235 us, with all of them from L2 346.  A TMA copy per warp and tile in place of 16 cp.async was slower (437 us; heads of
 //   64: 425 instead of 295), so were 16 keys per warp and 16 warps (469), three stages and 8 warps (434).
 #pragma once
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   // The tiles of the unit in all sequences, one after another, are cut into n equal ranges, however the sequences lie in them: one wave of
   // CTAs while that needs no more than kLongest8 tiles each (but no sequence is cut into more than sqrt(7 nt) pieces), else kWaves8
   // full waves.  (Pieces of equal size within each sequence, as decode.cu has them, leave the last wave partly empty: 1 x 1900 tokens,
-  // 32 heads over 8 of 128: 30 us, 26 in ranges; batches that fill the GPU several times take as long either way.)  Every warp works its range out; lane i sums
+  // 32 heads over 8 of 128, calls with an append behind an L2 that was written over: 30 us, 26 in ranges; batches that fill the GPU several times take as long either way.)  Every warp works its range out; lane i sums
   // the sequences [i per, (i + 1) per).
   auto tiles = [&](int i) { return seq8<kTile8>(p, cfg, geo.max_tiles, i).nt; };
   int b = 0, n = 1;                              // sequence; ranges
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
   if (whole) ld_page();
   // Keys (with the scales of both) or values of tile `ld` to a stage; a tile is one cp.async group.  (Groups of their own for keys and values,
   // so that a stage's keys make room as soon as the scores are computed, had half as much again on its way and were 5 to 10 % slower:
-  // 1 x 1900 tokens 26 -> 30 us, 64 of 1024 to 32768 with heads of 64 302 -> 319.)
+  // 1 x 1900 tokens, timed as above, 26 -> 30 us, 64 of 1024 to 32768 with heads of 64 302 -> 319.)
   auto load_half = [&](int st, bool value) {
     if (ld < tile0 + count) {
       const int key00 = ld * kTile8 + warp * KW;

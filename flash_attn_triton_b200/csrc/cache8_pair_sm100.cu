@@ -10,8 +10,9 @@
 // Tensor memory: S_0 | S_1 | O_0 | O_1.  P_x overwrites S_x, and Q_x K_(j+1)^T is issued behind P_x V_j, which reads it, in the in-order pipe.
 // With 12 warps the softmax warps have 216 registers, and all scores of a row fit (16 warps with one query tile: 184 and two readings).
 // Why two tiles: with one, the converters have 1100 (e4m3) to 1800 (int8) cycles of work for 1024 of the tensor pipe.  2 x 1537 tokens behind
-// 5000 to 11000, 32 heads over 8 of 128, int8: 1250 us with one, 770 with two (720 TFLOP/s); 4 x 256 behind 1024 to 8192: 232, 200.
-// Bound: the chain of a tile: 1.5 k cycles from the last of P to the next scores, 0.7 k load and maximum, 2.2 k exponentials and P; 5.2 k cycles
+// 5000 to 11000, 32 heads over 8 of 128, int8: fp16 1249 us with one, 856 with two (660 TFLOP/s of a call over other inputs in turn), bf16 1134,
+// 778; 16 x 64 behind 1024 to 8192, e4m3: 218, 210; 4 x 256: 195, 199.
+// Bound: the chain of a tile (fp16, before maxima were raised at once): 1.5 k cycles from the last of P to the next scores, 0.7 k load and maximum, 2.2 k exponentials and P; 5.2 k cycles
 // per two tiles of which the tensor pipe needs 2.0 k.  A quarter of the exponentials on the FMA pipe: 5 % slower (registers).
 // Every mbarrier wait is bounded; on timeout the CTA raises a status word, frees its tensor memory and returns.
 #include <cmath>

@@ -379,7 +379,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     block of capacity / blocks (page_size / blocks) consecutive tokens, at most 1024; a value is code * scale.  Codes are numbers
     (no e4m3 NaN, which an append never writes) wherever a sequence has keys.  q, k
     and v stay 16-bit.  New tokens are quantised as `kvcache_append` does it, and the attention is to what the cache
-    then holds; caches and scales that overlap (an expanded scale, one tensor for keys and values) are for calls without them.
+    then holds; caches and scales that overlap (an expanded scale, one tensor for keys and values) are for calls without them, and no two
+    sequences of a call append to one block.
 
     With value checks on (the default) the kernel makes them first (page indices in range, lengths
     fit the cache and the rotary tables) and the call waits for that one flag, not for the attention;
