@@ -27,19 +27,24 @@ template <> struct Code<FA_CODE_INT8> {
     a = pair(x, 0x4140);
     b = pair(x, 0x4342);
   }
-  // bytes (0, 2) and (1, 3)
-  static __device__ __forceinline__ void alternate(uint32_t x, uint32_t& a, uint32_t& b) {
-    x ^= 0x80808080u;
-    a = pair(x, 0x4240);
-    b = pair(x, 0x4341);
+  // bytes as they are, without the factor and the bias: 0x6400 | u is 1024 + u
+  static __device__ __forceinline__ uint32_t whole(uint32_t x, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0x64646464u), "r"(sel));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+    return r;
   }
-  // bytes (0, 1) and (2, 3) as they are, without the factor and the bias: 0x6400 | u is 1024 + u
+  // (0, 1) and (2, 3)
   static __device__ __forceinline__ void integers(uint32_t x, uint32_t& a, uint32_t& b) {
     x ^= 0x80808080u;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(a) : "r"(x), "r"(0x64646464u), "r"(0x4140u));
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(b) : "r"(x), "r"(0x64646464u), "r"(0x4342u));
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(0x64806480u));
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(0x64806480u));
+    a = whole(x, 0x4140);
+    b = whole(x, 0x4342);
+  }
+  // (0, 2) and (1, 3)
+  static __device__ __forceinline__ void alternate(uint32_t x, uint32_t& a, uint32_t& b) {
+    x ^= 0x80808080u;
+    a = whole(x, 0x4240);
+    b = whole(x, 0x4341);
   }
   // four codes of x[i] * m.  Adding 1.5 * 2^23 leaves the number rounded half to even in the low byte.
   static __device__ __forceinline__ uint32_t four(float a, float b, float c, float d, float m) {

@@ -11,8 +11,10 @@
 //   the 4 neighbouring codes that it is given as columns (2t, 2t+1, 2t+8, 2t+9) and the queries are arranged to match.  For V the
 //   transposing form gives a lane 2 dims of 2 keys; one byte permutation sorts them by dim, and rows g and g + 8 of the product are dims
 //   2g and 2g + 1.
-//   int8 codes go to the tensor cores as (code + 128) * 2^-24, which is a byte permutation; what the 128 adds is the same for all keys of
-//   a row in the scores, where the accumulators start from its negative, and a product with a constant in the outputs.
+//   int8 keys go to the tensor cores as (code + 128) * 2^-24, which is a byte permutation; what the 128 adds is the same for all keys of a row,
+//   and the accumulators start from its negative.  Values go as the codes themselves, one subtraction per pair more: 128 times the weights left
+//   the outputs off by 2^-21 of the largest value, however small they were (fp16, 120 k keys of equal weight: error 6.8e-4 of the outputs' rms
+//   instead of 2.9e-4; 64 sequences of 1024 to 32768: 427 -> 428 us, heads of 64 291 -> 296).
 //   Scales travel with their tile, by 4-byte cp.async.
 //   Split: see the ranges in the kernel.
 //   Bound.  HBM: one byte per code.  Measured: 64 sequences of 1024 to 32768, 32 heads over 8 of 128: 386 us (int8), 388 (e4m3), 5.3 TB/s of 6.5;
@@ -377,13 +379,12 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
     }
   }
   const int qmin = len - p.seqlen_q + rg * kRows / G, qmax = len - p.seqlen_q + min(rg * kRows + kRows - 1, R - 1) / G;
-  float o[NB][D / 16][4], ob[NB][4];             // ob: the bias of the codes, weighted
+  float o[NB][D / 16][4];
   float mrow[NB][2], lrow[NB][2];                // M; sums of this lane's keys
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-    ob[n][0] = ob[n][1] = ob[n][2] = ob[n][3] = 0.f;
     mrow[n][0] = mrow[n][1] = -INFINITY;
     lrow[n][0] = lrow[n][1] = 0.f;
   }
@@ -503,7 +504,6 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
           o[n][db][0] *= alpha[0]; o[n][db][1] *= alpha[1];
           o[n][db][2] *= alpha[0]; o[n][db][3] *= alpha[1];
         }
-        ob[n][0] *= alpha[0]; ob[n][1] *= alpha[1];
       }
     }
     uint32_t pb[KB][NB][2];
@@ -525,14 +525,6 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
       }
     }
     // ---- O^T += V^T P^T -----------------------------------------------------------------
-    if (C::kBias) {
-      const uint32_t a[4] = {C::kBias, C::kBias, C::kBias, C::kBias};
-#pragma unroll
-      for (int h = 0; h < KB; ++h) {
-#pragma unroll
-        for (int n = 0; n < NB; ++n) mma16816<__half>(ob[n], a, pb[h][n][0], pb[h][n][1]);
-      }
-    }
 #pragma unroll
     for (int d2 = 0; d2 < (D + 31) / 32; ++d2) {
 #pragma unroll
@@ -573,11 +565,10 @@ __global__ void __launch_bounds__(128, Decode8<D, kRows>::kResident)
     for (int i = 0; i < 2; ++i) {
       const int r = n * 8 + 2 * t + i;
       const float mstar = fmaxf(fmaxf(sM[r], sM[kRows + r]), fmaxf(sM[2 * kRows + r], sM[3 * kRows + r]));
-      const float wgt = mstar == -INFINITY ? 0.f : exp2f(mrow[n][i] - mstar) * (1.f / C::kUnit);
+      const float wgt = mstar == -INFINITY ? 0.f : exp2f(mrow[n][i] - mstar);
 #pragma unroll
       for (int db = 0; db < D / 16; ++db)
-        *reinterpret_cast<float2*>(sO + (warp * kRows + r) * OP + db * 16 + 2 * g) = 
-            make_float2(wgt * (o[n][db][i] - ob[n][i]), wgt * (o[n][db][2 + i] - ob[n][i]));
+        *reinterpret_cast<float2*>(sO + (warp * kRows + r) * OP + db * 16 + 2 * g) = make_float2(wgt * o[n][db][i], wgt * o[n][db][2 + i]);
     }
   }
   __syncthreads();

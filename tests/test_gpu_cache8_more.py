@@ -397,3 +397,26 @@ def test_largest_weight_is_not_rounded(n, heads, dim, blocks, code):
     assert leads.sum() > leads.numel() // 2
     rounded = torch.where(leads, 0.0, 2.0 ** -11)[..., None]
     assert ((out - want).abs() <= half + (2.0 ** -15 + rounded) * weight).all()
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("n,heads,dim", [(1, 4, 16), (1, 4, 64), (1, 8, 128), (1, 4, 256), (4, 4, 32), (4, 4, 64), (3, 4, 128), (4, 4, 256), (40, 4, 64),
+                                         (100, 4, 128)])
+def test_small_values_beside_a_heavy_zero(n, heads, dim, code):
+    """A key of value 0 has nearly all of the weight, the others 2^-13 of it and small values: the sums are as exact as those values ask for,
+    whatever a code is on the way (the tolerance of cache8_reference, whose largest value is 4)."""
+    page, hk, length = 16, 1, 64 + n
+    table, pool = make_table(131, [length], page)
+    kc = torch.zeros(pool, page, hk, dim)
+    vc = (rand(132, pool, page, hk, dim) * 2).round().clamp(-4, 4)
+    heavy = int(table[0, 0]), 3
+    key = rand(133, hk, dim).sign()
+    kc[heavy], vc[heavy] = 64 * key, 0.0
+    kc, vc = ref.coded(kc, code), ref.coded(vc, code)
+    ks = vs = torch.ones(pool, 1, hk)
+    q = (9.0 / (64 * dim ** 0.5) * key.expand(1, n, heads, dim)).to(F16)
+    want, weight = ref.attend(q, ref.values(kc, ks), ref.values(vc, vs), [length], causal=True, table=table)
+    out = fa().flash_attn_with_kvcache(q.to(DEV), kc.to(DEV), vc.to(DEV), cache_seqlens=torch.tensor([length], device=DEV), block_table=table.to(DEV),
+                                       causal=True, k_scale=ks.to(DEV), v_scale=vs.to(DEV)).double().cpu()
+    assert weight.max() < 0.08                         # (no more than 163 others of 2^-13 each, values up to 4)
+    assert ((out - want).abs() <= ref.tolerance(want, weight, F16, length, 4.0)).all()
