@@ -12,8 +12,8 @@ template <int kCode> struct Code;
 
 template <> struct Code<FA_CODE_INT8> {
   static constexpr float kLargest = 127.f;
-  // A byte in the low half of a 16-bit float is u * 2^-24 (u = code + 128): one byte permutation per pair.  The products are then
-  // 2^-24 of the true ones and too large by those with kBias.
+  // Keys of the decode kernel (neighbours): a byte in the low half of a 16-bit float is u * 2^-24 (u = code + 128), one byte permutation per
+  // pair.  The products are then 2^-24 of the true ones and too large by those with kBias.
   static constexpr float kUnit = 0x1p-24f;
   static constexpr uint32_t kBias = 0x00800080u;
   static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t sel) {

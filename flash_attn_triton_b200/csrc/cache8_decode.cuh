@@ -17,9 +17,9 @@
 //   instead of 2.9e-4; 64 sequences of 1024 to 32768: 427 -> 428 us, heads of 64 291 -> 296).
 //   Scales travel with their tile, by 4-byte cp.async.
 //   Split: see the ranges in the kernel.
-//   Bound.  HBM: one byte per code.  Measured: 64 sequences of 1024 to 32768, 32 heads over 8 of 128: 386 us (int8), 388 (e4m3), 5.3 TB/s of 6.5;
-//   heads of 64 282 us, 3.6 TB/s; whole calls over other inputs in turn 434 to 452.  What is left is the chain of a tile with 12 warps per SM:
-//   790 instructions for 32 keys, issue active 49 %; with the loads taken out of the loop it takes 235 us, with all of them from L2 346.  A TMA
+//   Bound.  HBM: one byte per code.  Measured: 64 sequences of 1024 to 32768, 32 heads over 8 of 128: 386 to 398 us (int8 and
+//   e4m3), 5.2 TB/s of 6.5; heads of 64 285 us, 3.6 TB/s; whole calls over other inputs in turn 434 to 457.  What is left is the chain of a tile
+//   with 12 warps per SM: 840 instructions for 32 keys (int8), issue active about half; with the loads taken out of the loop it takes 235 us, with all of them from L2 346.  A TMA
 //   copy per warp and tile in place of 16 cp.async was slower (437 us; heads of 64: 425 instead of 295), so were 16 keys per warp and 16
 //   warps (469), three stages and 8 warps (434).
 #pragma once
