@@ -2,7 +2,8 @@
 
 Same eleven names as the reference's flash_attn_triton/__init__.py:6-18, plus
 `attention_int8` (which the reference keeps in triton_kernel/attention_kernel_int8.py) and the calls around a
-KV cache in 8 bits, `build_block_table` and `kvcache_append`.
+KV cache in 8 bits, `build_block_table` and `kvcache_append`, and those of decoding with trees of drafted tokens,
+`qk_norm_rotary`, `verify_draft_tree`, `kvcache_compact` and `release_pages`.
 """
 from .flash_attn_interface import (  # noqa: F401
     FlashAttention,
@@ -21,5 +22,6 @@ from .flash_attn_interface import (  # noqa: F401
     kvcache_append,
     set_validation,
 )
+from .drafting import kvcache_compact, qk_norm_rotary, release_pages, verify_draft_tree  # noqa: F401
 
 __version__ = "0.1.0"

@@ -61,6 +61,7 @@ class DecodeArgs(C.Structure):
         ("causal", C.c_int32), ("window_left", C.c_int32), ("window_right", C.c_int32),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("num_splits", C.c_int32),
         ("counters", C.c_void_p), ("num_counters", C.c_int32),
+        ("tree_mask", C.c_void_p), ("tree_stride", C.c_int64 * 2),
     ]
 
 
@@ -114,6 +115,51 @@ class BlockTableArgs(C.Structure):
     ]
 
 
+class VerifyArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("device", C.c_int32), ("batch", C.c_int32), ("nodes", C.c_int32), ("vocab", C.c_int64),
+        ("draft_tokens", C.c_void_p), ("token_stride", C.c_int64), ("parents", C.c_void_p), ("parent_stride", C.c_int64),
+        ("target", C.c_void_p), ("draft", C.c_void_p), ("target_stride", C.c_int64 * 2), ("draft_stride", C.c_int64 * 2),
+        ("accept", C.c_void_p), ("sample", C.c_void_p), ("path", C.c_void_p), ("num_accepted", C.c_void_p), ("next_token", C.c_void_p),
+    ]
+
+
+class CompactArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32), ("layers", C.c_int32), ("batch", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32),
+        ("k_cache", C.POINTER(C.c_void_p)), ("v_cache", C.POINTER(C.c_void_p)), ("kc_stride", _I64x3), ("vc_stride", _I64x3),
+        ("page_size", C.c_int32), ("num_pages", C.c_int32), ("block_table", C.c_void_p), ("block_table_stride", C.c_int32),
+        ("cache_batch_idx", C.c_void_p), ("cache_leftpad", C.c_void_p), ("cache_seqlens", C.c_void_p),
+        ("path", C.c_void_p), ("path_stride", C.c_int32), ("path_len", C.c_int32), ("num_accepted", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class ReleaseArgs(C.Structure):
+    _fields_ = [
+        ("device", C.c_int32), ("batch", C.c_int32), ("page_size", C.c_int32), ("held_lens", C.c_void_p), ("kept_lens", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int32), ("num_pages", C.c_int32),
+        ("pages", C.c_void_p), ("pages_released", C.c_void_p),
+    ]
+
+
+class QkNormArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("device", C.c_int32), ("batch", C.c_int32), ("seqlen", C.c_int32),
+        ("heads_q", C.c_int32), ("heads_kv", C.c_int32), ("head_dim", C.c_int32),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_stride", _I64x3), ("k_stride", _I64x3),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_wide", C.c_int32), ("table_wide", C.c_int32), ("eps", C.c_float),
+        ("cos", C.c_void_p), ("sin", C.c_void_p), ("rotary_dim", C.c_int32), ("rotary_seqlen", C.c_int32), ("interleaved", C.c_int32),
+        ("positions", C.c_void_p), ("pos_stride", C.c_int64 * 2),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("qo_stride", _I64x3), ("ko_stride", _I64x3),
+        ("d_qo", C.c_void_p), ("d_ko", C.c_void_p), ("d_qo_stride", _I64x3), ("d_ko_stride", _I64x3),
+        ("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_q_stride", _I64x3), ("d_k_stride", _I64x3),
+        ("d_q_weight", C.c_void_p), ("d_k_weight", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+COMPACT_LAYERS = 128
+
 EXPORTS = {
     "fa_fwd": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
     "fa_bwd_preprocess": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
@@ -148,6 +194,15 @@ EXPORTS = {
     "fa_append8_workspace_bytes": (C.c_size_t, [C.POINTER(Append8Args)]),
     "fa_block_table": (C.c_int, [C.POINTER(BlockTableArgs), C.c_void_p]),
     "fa_block_table_checked": (C.c_int, [C.POINTER(BlockTableArgs), C.POINTER(C.c_uint32), C.c_void_p]),
+    "fa_verify_draft_tree": (C.c_int, [C.POINTER(VerifyArgs), C.c_void_p]),
+    "fa_compact": (C.c_int, [C.POINTER(CompactArgs), C.c_void_p]),
+    "fa_compact_checked": (C.c_int, [C.POINTER(CompactArgs), C.POINTER(C.c_uint32), C.c_void_p]),
+    "fa_compact_workspace_bytes": (C.c_size_t, [C.POINTER(CompactArgs)]),
+    "fa_release_pages": (C.c_int, [C.POINTER(ReleaseArgs), C.c_void_p]),
+    "fa_release_pages_checked": (C.c_int, [C.POINTER(ReleaseArgs), C.POINTER(C.c_uint32), C.c_void_p]),
+    "fa_qk_norm": (C.c_int, [C.POINTER(QkNormArgs), C.c_void_p]),
+    "fa_qk_norm_bwd": (C.c_int, [C.POINTER(QkNormArgs), C.c_void_p]),
+    "fa_qk_norm_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(QkNormArgs)]),
     "fa_quantize_k_int8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32,
                                      C.c_int32, C.c_void_p]),
     "fa_fwd_int8": (C.c_int, [C.POINTER(Int8Args), C.c_void_p]),
@@ -185,7 +240,8 @@ def lib():
             fn = getattr(l, name)
             fn.restype = res
             fn.argtypes = args
-        for which, st in enumerate((AttnArgs, DecodeArgs, Int8Args, RotaryArgs, Cache8, Append8Args, BlockTableArgs)):
+        for which, st in enumerate((AttnArgs, DecodeArgs, Int8Args, RotaryArgs, Cache8, Append8Args, BlockTableArgs,
+                                    VerifyArgs, CompactArgs, ReleaseArgs, QkNormArgs)):
             if l.fa_sizeof_args(which) != C.sizeof(st):
                 raise RuntimeError(f"ABI mismatch for {st.__name__}: library "
                                    f"{l.fa_sizeof_args(which)} vs binding {C.sizeof(st)}")

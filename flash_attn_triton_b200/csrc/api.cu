@@ -182,6 +182,14 @@ int append8(const fa_append8_args&, cudaStream_t);
 int append8_checked(const fa_append8_args&, uint32_t*, cudaStream_t);
 size_t append8_workspace_bytes(const fa_append8_args&);
 int block_table(const fa_block_table_args&, cudaStream_t);
+int verify_draft_tree(const fa_verify_args&, cudaStream_t);
+int compact(const fa_compact_args&, cudaStream_t);
+int compact_checked(const fa_compact_args&, uint32_t*, cudaStream_t);
+size_t compact_workspace_bytes(const fa_compact_args&);
+int release_pages(const fa_release_args&, cudaStream_t);
+int release_pages_checked(const fa_release_args&, uint32_t*, cudaStream_t);
+int qk_norm(const fa_qk_norm_args&, bool backward, cudaStream_t);
+size_t qk_norm_bwd_workspace_bytes(const fa_qk_norm_args&);
 int block_table_checked(const fa_block_table_args&, uint32_t*, cudaStream_t);
 int quantize_k(const void*, int8_t*, float*, int64_t, int, cudaStream_t);
 int fwd_int8_mma(const fa_int8_args&, cudaStream_t);
@@ -459,6 +467,9 @@ static int validate_decode(const fa_decode_args* a) {
                "rotary tables exceed the head dimension");
     FA_REQUIRE(a->rotary_seqlen > 0, "rotary_seqlen must be the number of rows of the rotary tables");
   }
+  if (a->tree_mask)
+    FA_REQUIRE(a->window_left < 0 && a->window_right < 0 && !a->alibi_slopes && !a->rotary_cos,
+               "tree_mask cannot be combined with a window, ALiBi or rotary tables: the position of a node is not its slot");
   if (a->k_new) {
     FA_REQUIRE(a->seqlen_new > 0, "seqlen_new must be positive when k/v are given");
     FA_REQUIRE(aligned16(a->k_new) && aligned16(a->v_new) && mult8(a->kn_stride, 3) && mult8(a->vn_stride, 3),
@@ -516,6 +527,7 @@ static int validate_written8(const fa_cache8& c, int page_size, int num_pages, i
 static int validate_decode8(const fa_decode_args* a, const fa_cache8* c) {
   if (int r = validate_decode(a)) return r;
   FA_REQUIRE(c != nullptr, "cache is NULL");
+  FA_REQUIRE(a->tree_mask == nullptr, "tree_mask goes with 16-bit caches");
   if (a->batch == 0 || a->seqlen_q == 0) return FA_OK;
   if (int r = validate_cache8(*c, a->page_size, a->num_pages, a->k_cache, a->v_cache, a->kc_stride, a->vc_stride)) return r;
   if (a->k_new == nullptr) return FA_OK;
@@ -590,6 +602,116 @@ int fa_block_table_checked(const fa_block_table_args* a, uint32_t* failed, void*
   FA_REQUIRE(failed != nullptr, "failed is NULL");
   if (int r = ensure_device(a->device)) return r;
   return block_table_checked(*a, failed, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static bool any_dtype(int d) { return d == FA_F16 || d == FA_BF16 || d == FA_F32; }
+
+int fa_verify_draft_tree(const fa_verify_args* a, void* stream) {
+  FA_REQUIRE(a != nullptr, "args is NULL");
+  FA_REQUIRE(any_dtype(a->dtype), "dtype must be FA_F16, FA_BF16 or FA_F32");
+  FA_REQUIRE(a->batch >= 0 && a->batch <= INT32_MAX / 8, "negative or too large a batch");
+  FA_REQUIRE(a->nodes >= 1 && a->nodes <= 1024, "a tree has 1 to 1024 nodes (got %d)", a->nodes);
+  FA_REQUIRE(a->vocab >= 1 && a->vocab <= INT32_MAX, "the vocabulary must have 1 to 2^31 - 1 tokens");
+  if (a->batch == 0) return FA_OK;
+  FA_REQUIRE(a->draft_tokens && a->parents && a->target && a->draft && a->accept && a->sample && a->path && a->num_accepted && a->next_token,
+             "a pointer is NULL");
+  if (int r = ensure_device(a->device)) return r;
+  return verify_draft_tree(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static int validate_compact(const fa_compact_args* a) {
+  FA_REQUIRE(a != nullptr, "args is NULL");
+  FA_REQUIRE(a->layers >= 0 && a->layers <= FA_COMPACT_LAYERS, "a call has up to %d layers (got %d)", FA_COMPACT_LAYERS, a->layers);
+  FA_REQUIRE(a->batch >= 0 && a->heads > 0 && a->heads <= 1 << 20 && a->num_pages >= 0 && a->path_len >= 0 && a->path_stride >= 0,
+             "negative or too large a size");
+  FA_REQUIRE(a->head_dim == 16 || a->head_dim == 32 || a->head_dim == 64 || a->head_dim == 128 || a->head_dim == 256,
+             "head dimension must be one of 16, 32, 64, 128, or 256 (got %d)", a->head_dim);
+  if (a->batch == 0 || a->layers == 0) return FA_OK;
+  FA_REQUIRE(a->k_cache && a->v_cache && a->cache_seqlens && a->num_accepted && (a->path || a->path_len == 0), "a pointer is NULL");
+  FA_REQUIRE(a->page_size > 0, "page_size must be positive");
+  FA_REQUIRE(a->block_table == nullptr || a->block_table_stride > 0, "block_table_stride must be positive when a block table is given");
+  FA_REQUIRE(!(a->block_table && a->cache_batch_idx), "cache_batch_idx cannot be combined with paged KV caches");
+  FA_REQUIRE(!(a->block_table && a->cache_leftpad), "cache_leftpad cannot be combined with paged KV caches");
+  FA_REQUIRE(mult8(a->kc_stride, 3) && mult8(a->vc_stride, 3), "cache rows must be 16-byte aligned");
+  const int64_t rows[3] = {a->num_pages, a->page_size, a->heads};
+  for (int i = 0; i < a->layers; ++i) {
+    FA_REQUIRE(a->k_cache[i] && a->v_cache[i] && aligned16(a->k_cache[i]) && aligned16(a->v_cache[i]), "cache rows must be 16-byte aligned");
+    const Strided k = strided(a->k_cache[i], 2 * a->head_dim, 2, rows, a->kc_stride), v = strided(a->v_cache[i], 2 * a->head_dim, 2, rows, a->vc_stride);
+    FA_REQUIRE(i > 0 || (!may_overlap_itself(k) && !may_overlap_itself(v)), "rows of a cache must not overlap");
+    FA_REQUIRE(!may_overlap(k, v), "k_cache and v_cache must not overlap");
+    for (int j = 0; j < i; ++j)
+      FA_REQUIRE(a->k_cache[j] != a->k_cache[i] && a->v_cache[j] != a->v_cache[i] && a->k_cache[j] != a->v_cache[i] && a->v_cache[j] != a->k_cache[i],
+                 "the caches of the layers must not overlap");
+  }
+  return FA_OK;
+}
+int fa_compact(const fa_compact_args* a, void* stream) {
+  if (int r = validate_compact(a)) return r;
+  if (int r = ensure_device(a->device)) return r;
+  return compact(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+int fa_compact_checked(const fa_compact_args* a, uint32_t* failed, void* stream) {
+  if (int r = validate_compact(a)) return r;
+  FA_REQUIRE(failed != nullptr, "failed is NULL");
+  if (int r = ensure_device(a->device)) return r;
+  return compact_checked(*a, failed, reinterpret_cast<cudaStream_t>(stream));
+}
+size_t fa_compact_workspace_bytes(const fa_compact_args* a) {
+  return a == nullptr || a->batch < 0 || a->path_len < 0 ? 0 : compact_workspace_bytes(*a);
+}
+
+static int validate_release(const fa_release_args* a) {
+  FA_REQUIRE(a != nullptr, "args is NULL");
+  FA_REQUIRE(a->batch >= 0 && a->num_pages >= 0 && a->table_pages >= 0 && a->table_stride >= 0, "negative size");
+  FA_REQUIRE(a->page_size > 0, "page_size must be positive");
+  FA_REQUIRE(a->pages_released && (a->pages || a->num_pages == 0), "pages and pages_released are required");
+  FA_REQUIRE(a->batch == 0 || (a->held_lens && a->kept_lens), "held_lens and kept_lens are required");
+  FA_REQUIRE(a->batch == 0 || a->table_pages == 0 || a->block_table, "block_table is required");
+  return FA_OK;
+}
+int fa_release_pages(const fa_release_args* a, void* stream) {
+  if (int r = validate_release(a)) return r;
+  if (int r = ensure_device(a->device)) return r;
+  return release_pages(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+int fa_release_pages_checked(const fa_release_args* a, uint32_t* failed, void* stream) {
+  if (int r = validate_release(a)) return r;
+  FA_REQUIRE(failed != nullptr, "failed is NULL");
+  if (int r = ensure_device(a->device)) return r;
+  return release_pages_checked(*a, failed, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static int qk_norm_impl(const fa_qk_norm_args* a, bool backward, void* stream) {
+  FA_REQUIRE(a != nullptr, "args is NULL");
+  FA_REQUIRE(any_dtype(a->dtype), "dtype must be FA_F16, FA_BF16 or FA_F32");
+  FA_REQUIRE(a->batch >= 0 && a->seqlen >= 0 && a->heads_q > 0 && a->heads_kv >= 0 && a->heads_q <= 1 << 20 && a->heads_kv <= 1 << 20,
+             "negative or too large a size");
+  FA_REQUIRE(a->head_dim == 16 || a->head_dim == 32 || a->head_dim == 64 || a->head_dim == 128 || a->head_dim == 256,
+             "head dimension must be one of 16, 32, 64, 128, or 256 (got %d)", a->head_dim);
+  FA_REQUIRE((a->cos == nullptr) == (a->sin == nullptr), "rotary_cos and rotary_sin must be supplied together");
+  FA_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim % 2 == 0 && a->rotary_dim <= a->head_dim && a->rotary_seqlen >= 0,
+             "rotary tables exceed the head dimension");
+  if (a->batch > 0 && a->seqlen > 0) {
+    FA_REQUIRE(a->q && aligned16(a->q) && mult8(a->q_stride, 3), "rows of q must be 16-byte aligned");
+    FA_REQUIRE(a->heads_kv == 0 || (a->k && aligned16(a->k) && mult8(a->k_stride, 3)), "rows of k must be 16-byte aligned");
+    void* const out[2] = {backward ? a->d_q : a->q_out, backward ? a->d_k : a->k_out};
+    const int64_t* os[2] = {backward ? a->d_q_stride : a->qo_stride, backward ? a->d_k_stride : a->ko_stride};
+    for (int i = 0; i < (a->heads_kv ? 2 : 1); ++i) FA_REQUIRE(out[i] && aligned16(out[i]) && mult8(os[i], 3), "rows of the results must be 16-byte aligned");
+    if (backward) {
+      FA_REQUIRE(a->d_qo && aligned16(a->d_qo) && mult8(a->d_qo_stride, 3), "rows of the gradients must be 16-byte aligned");
+      FA_REQUIRE(a->heads_kv == 0 || (a->d_ko && aligned16(a->d_ko) && mult8(a->d_ko_stride, 3)), "rows of the gradients must be 16-byte aligned");
+      if (a->d_q_weight || a->d_k_weight)
+        FA_REQUIRE(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= qk_norm_bwd_workspace_bytes(*a), "workspace too small");
+    }
+  }
+  if (int r = ensure_device(a->device)) return r;
+  return qk_norm(*a, backward, reinterpret_cast<cudaStream_t>(stream));
+}
+int fa_qk_norm(const fa_qk_norm_args* a, void* stream) { return qk_norm_impl(a, false, stream); }
+int fa_qk_norm_bwd(const fa_qk_norm_args* a, void* stream) { return qk_norm_impl(a, true, stream); }
+size_t fa_qk_norm_bwd_workspace_bytes(const fa_qk_norm_args* a) {
+  if (a == nullptr || a->batch < 0 || a->seqlen < 0 || a->heads_q <= 0 || a->heads_kv < 0 || a->head_dim < 8 || a->head_dim > 256) return 0;
+  return qk_norm_bwd_workspace_bytes(*a);
 }
 
 int fa_varlen_check(const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int64_t total_q, int64_t total_k, int32_t k_at_most,
@@ -826,6 +948,10 @@ size_t fa_sizeof_args(int which) {
     case 4: return sizeof(fa_cache8);
     case 5: return sizeof(fa_append8_args);
     case 6: return sizeof(fa_block_table_args);
+    case 7: return sizeof(fa_verify_args);
+    case 8: return sizeof(fa_compact_args);
+    case 9: return sizeof(fa_release_args);
+    case 10: return sizeof(fa_qk_norm_args);
   }
   return 0;
 }

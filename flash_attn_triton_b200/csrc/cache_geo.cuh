@@ -22,6 +22,10 @@ struct CacheGeo {
   float* ws;               // pieces: fp32 outputs, then their base-2 LSEs
   uint32_t* counters;      // per unit, zero
   const uint32_t* bad;     // set by the value checks: do nothing
+  // A tree of drafted tokens, or null: (batch, tokens + 1, tree_words), bit j & 31 of word j >> 5: the row sees node j; the last row of a
+  // sequence: some row sees node j.  Bits from `tokens` on are 0.
+  const uint32_t* tree_bits;
+  int tree_words;
 };
 
 }  // namespace fa

@@ -33,6 +33,7 @@
 //   synchronisation took 150 us around a 16 us kernel), in decode_check_kernel otherwise.
 #include <sched.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <mutex>
@@ -75,7 +76,8 @@ template <int D, int kRows> struct DecodeSmem {
   static_assert((size_t)4 * kRows * OP * 4 <= ring, "the warps' outputs, over the ring");
 };
 
-template <typename T, int D, int kRows>
+// kTree: the last seqlen_q positions are nodes of a tree, and which of them a row sees is in p.tree_mask.
+template <typename T, int D, int kRows, bool kTree>
 __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     decode_kernel(const fa_decode_args p, const ScoreCfg cfg, const DecodeGeom geo, const DecodeCheck chk) {
   using SM = DecodeSmem<D, kRows>;
@@ -247,6 +249,8 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
       slope[n][i] = cfg.has_alibi ? p.alibi_slopes[b * p.heads_q + hk * G + gi] : 0.f;
     }
   }
+  const int tree0 = kTree ? len - p.seqlen_q : 0;        // the root's position
+  const uint8_t* seen = kTree ? p.tree_mask + b * p.tree_stride[0] : nullptr;
   const int qmin = len - p.seqlen_q + rg * kRows / G, qmax = len - p.seqlen_q + min(rg * kRows + kRows - 1, R - 1) / G;
   float o[NB][D / 16][4];
 #pragma unroll
@@ -292,6 +296,16 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
       }
       __syncwarp();
     }
+    // Nodes that no row sees (of a request that uses fewer than others) may hold anything: 0 times a NaN would be one.
+    if (kTree && keyw + 16 > tree0) {
+      const int node = keyw + (lane & 15) - tree0;
+      bool dead = node >= 0 && node < p.seqlen_q;
+      if (dead)
+        for (int i = 0; i < p.seqlen_q; ++i) dead = dead && seen[i * p.tree_stride[1] + node] == 0;
+      for (unsigned rest = __ballot_sync(0xffffffffu, dead) & 0xffffu; rest; rest &= rest - 1)
+        if (lane < CPR) *reinterpret_cast<uint4*>(tV + (__ffs(rest) - 1) * P + lane * 8) = make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
+    }
 
     // ---- S^T = K Q^T: keys keyw + g and keyw + g + 8 ------------------------------------
     float s[NB][4];
@@ -306,7 +320,7 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
     }
     // ---- softmax.  Plain scores that every row sees need no test per element; their scale goes
     // into the exponent's FMA --------------------------------------------------------------
-    const bool full = !cfg.has_alibi && keyw + 16 <= len && (!cfg.causal || keyw + 15 <= qmin) &&
+    const bool full = !cfg.has_alibi && keyw + 16 <= (kTree ? tree0 : len) && (!cfg.causal || keyw + 15 <= qmin) &&
                       (cfg.wl < 0 || keyw >= qmax - cfg.wl) && (cfg.wr < 0 || keyw + 15 <= qmin + cfg.wr);
     float mul = cfg.scale_log2;
     if (!full) {
@@ -318,7 +332,9 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
           const int i = e & 1, key = keyw + g + (e >> 1) * 8;
           float th;
           const float v = score_log2(cfg, slope[n][i], s[n][e], qpos[n][i], key, th);
-          s[n][e] = visible(cfg, qpos[n][i], key, len) ? v : -INFINITY;
+          bool ok = visible(cfg, qpos[n][i], key, len);
+          if (kTree && ok && key >= tree0) ok = seen[(qpos[n][i] - tree0) * p.tree_stride[1] + key - tree0] != 0;
+          s[n][e] = ok ? v : -INFINITY;
         }
       }
     }
@@ -492,9 +508,10 @@ constexpr int kAppendPerSm = 5;    // CTAs of 256 threads with 48 registers each
 // 16-byte chunk per thread and step, HBM-bound.  host / dev: value checks made by every CTA, see decode_kernel.
 // Index: of a chunk.  With 64-bit indices the five divisions of a thread were most of the kernel; and as every CTA makes the
 // checks, there are no more CTAs than run at a time (4 x 256 tokens of 32 heads over 8 of 128: 15.5 -> 10.9 us).
-template <typename T, typename Index>
+// kTree: the mask of the tree as bits to tree_bits, see CacheGeo.
+template <typename T, typename Index, bool kTree>
 __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const fa_decode_args p, T* q_out, int page_shift, uint32_t* host,
-                                                           uint32_t* dev, bool check_here) {
+                                                           uint32_t* dev, bool check_here, uint32_t* tree_bits) {
   if (check_here) {
     const uint32_t bad = decode_checks(p, threadIdx.x, 256);
     if (threadIdx.x == 0 && blockIdx.x == 0) {
@@ -505,6 +522,24 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
     if (bad) return;
   } else if (dev && *dev) {
     return;
+  }
+  if (kTree) {
+    // a warp has a word: of a node's row, or (row seqlen_q) of the nodes that any row sees
+    const int n = p.seqlen_q, words = (n + 31) >> 5, lane = threadIdx.x & 31;
+    const int64_t all = (int64_t)p.batch * (n + 1) * words;
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += (int64_t)gridDim.x * 8) {
+      const int64_t br = i / words;
+      const int w = (int)(i - br * words), b = (int)(br / (n + 1)), row = (int)(br - (int64_t)b * (n + 1)), j = w * 32 + lane;
+      const uint8_t* m = p.tree_mask + b * p.tree_stride[0] + j;
+      bool seen = false;
+      if (j < n) {
+        if (row < n) seen = m[row * p.tree_stride[1]] != 0;
+        else
+          for (int r = 0; r < n; ++r) seen |= m[r * p.tree_stride[1]] != 0;
+      }
+      const uint32_t bits = __ballot_sync(0xffffffffu, seen);
+      if (lane == 0) tree_bits[i] = bits;
+    }
   }
   const int D = p.head_dim, cpr_log2 = 31 - __clz(D / 8);      // (a power of two)
   const int n_new = p.k_new ? p.seqlen_new : 0;
@@ -545,7 +580,7 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
 
 struct ChunkPlan {
   int pack_log2, units, parts, capacity;
-  size_t q_bytes, piece_bytes;   // workspace: rotated queries, pieces, then the counters if the caller brings none
+  size_t q_bytes, piece_bytes;   // workspace: rotated queries or the bits of a tree's mask, pieces, then the counters if the caller brings none
 };
 // Whether a call is a chunk, and how it is cut.
 static bool chunk_plan(const fa_decode_args& a, ChunkPlan& c) {
@@ -570,6 +605,7 @@ static bool chunk_plan(const fa_decode_args& a, ChunkPlan& c) {
   c.parts = (int)(fill < most ? fill : most);
   if (c.parts < 1) c.parts = 1;
   c.q_bytes = a.rotary_cos ? (size_t)a.batch * a.seqlen_q * a.heads_q * a.head_dim * 2 : 0;
+  if (a.tree_mask) c.q_bytes = ((size_t)a.batch * (a.seqlen_q + 1) * ((a.seqlen_q + 31) / 32) * sizeof(uint32_t) + 15) / 16 * 16;
   c.piece_bytes = c.parts > 1 ? (size_t)c.units * c.parts * 128 * (a.head_dim + 1) * sizeof(float) : 0;
   return true;
 }
@@ -600,11 +636,11 @@ size_t decode_workspace_bytes(const fa_decode_args& a) {
   return pieces == 0 ? 0 : pieces + (a.counters ? 0 : (size_t)decode_num_counters(a) * sizeof(uint32_t));
 }
 
-template <typename T, int D, int kRows>
+template <typename T, int D, int kRows, bool kTree>
 static int launch_rows(const fa_decode_args& a, const ScoreCfg& cfg, const DecodeGeom& g, const DecodeCheck& chk,
                          cudaStream_t st) {
   const size_t smem = DecodeSmem<D, kRows>::fixed;
-  auto kern = decode_kernel<T, D, kRows>;
+  auto kern = decode_kernel<T, D, kRows, kTree>;
   // once per kernel and device: a step of one conversation is bounded by the host's part
   static std::atomic<uint64_t> prepared{0};
   const uint64_t bit = a.device < 64 ? 1ull << a.device : 0;
@@ -635,7 +671,8 @@ static int launch_rows(const fa_decode_args& a, const ScoreCfg& cfg, const Decod
 template <typename T, int D>
 static int launch_decode(const fa_decode_args& a, const ScoreCfg& cfg, const DecodeGeom& g, const DecodeCheck& chk,
                          cudaStream_t st) {
-  return decode_unit_rows(a) == 8 ? launch_rows<T, D, 8>(a, cfg, g, chk, st) : launch_rows<T, D, 16>(a, cfg, g, chk, st);
+  if (a.tree_mask) return decode_unit_rows(a) == 8 ? launch_rows<T, D, 8, true>(a, cfg, g, chk, st) : launch_rows<T, D, 16, true>(a, cfg, g, chk, st);
+  return decode_unit_rows(a) == 8 ? launch_rows<T, D, 8, false>(a, cfg, g, chk, st) : launch_rows<T, D, 16, false>(a, cfg, g, chk, st);
 }
 
 template <typename T>
@@ -721,18 +758,24 @@ static int chunk_run(const fa_decode_args& args, const ChunkPlan& c, uint32_t* h
       }
     }
   }
-  void* q_out = c.q_bytes ? ws : nullptr;
+  void* q_out = a.rotary_cos ? ws : nullptr;
+  uint32_t* tree_bits = a.tree_mask ? reinterpret_cast<uint32_t*>(ws) : nullptr;
+  geo.tree_bits = tree_bits;
+  geo.tree_words = (a.seqlen_q + 31) / 32;
   const int64_t chunks = ((q_out ? (int64_t)a.batch * a.seqlen_q * a.heads_q : 0) + 2ll * a.batch * geo.n_new * a.heads_kv) *
                          (a.head_dim / 8);
-  if (chunks > 0 || inside) {
-    const int64_t need = chunks > 0 ? (chunks + 255) / 256 : 1, fit = (int64_t)sm_count(a.device) * kAppendPerSm;
+  if (chunks > 0 || inside || tree_bits) {
+    int64_t need = chunks > 0 ? (chunks + 255) / 256 : 1;
+    if (tree_bits) need = std::max(need, ((int64_t)a.batch * (a.seqlen_q + 1) * geo.tree_words + 7) / 8);
+    const int64_t fit = (int64_t)sm_count(a.device) * kAppendPerSm;
     const unsigned grid = (unsigned)(need < fit ? need : fit);
     const int shift = page_shift_of(a);
     const bool small = chunks < (int64_t)1 << 31;
     auto append = [&](auto* q) {
       using T = std::remove_pointer_t<decltype(q)>;
-      auto kern = small ? cache_append_kernel<T, uint32_t> : cache_append_kernel<T, int64_t>;
-      kern<<<grid, 256, 0, st>>>(a, q, shift, host, dev, inside);
+      auto kern = tree_bits ? cache_append_kernel<T, int64_t, true>
+                  : small   ? cache_append_kernel<T, uint32_t, false> : cache_append_kernel<T, int64_t, false>;
+      kern<<<grid, 256, 0, st>>>(a, q, shift, host, dev, inside, tree_bits);
     };
     if (a.dtype == FA_BF16) append(static_cast<__nv_bfloat16*>(q_out));
     else append(static_cast<__half*>(q_out));

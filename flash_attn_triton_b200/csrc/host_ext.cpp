@@ -66,6 +66,15 @@ struct Abi {
   size_t (*append8_workspace)(const fa_append8_args*);
   int (*block_table)(const fa_block_table_args*, void*);
   int (*block_table_checked)(const fa_block_table_args*, uint32_t*, void*);
+  int (*verify)(const fa_verify_args*, void*);
+  int (*compact)(const fa_compact_args*, void*);
+  int (*compact_checked)(const fa_compact_args*, uint32_t*, void*);
+  size_t (*compact_workspace)(const fa_compact_args*);
+  int (*release)(const fa_release_args*, void*);
+  int (*release_checked)(const fa_release_args*, uint32_t*, void*);
+  int (*qk_norm)(const fa_qk_norm_args*, void*);
+  int (*qk_norm_bwd)(const fa_qk_norm_args*, void*);
+  size_t (*qk_norm_bwd_workspace)(const fa_qk_norm_args*);
   PyObject* check;   // _native.check(status, what): raises the Python exception of a status
 };
 Abi g_abi = {};
@@ -746,7 +755,7 @@ fa_cache8 cache8_of(const Tensor& cache, const Tensor& k_scale, const Tensor& v_
 }
 
 // kvcache(q, k_cache, v_cache, k_new, v_new, cos, sin, seqlens, batch_idx, leftpad, block_table, scale, causal, wl, wr,
-//         interleaved, alibi, num_splits, checks, k_scale, v_scale) -> out, or the mask of the value checks that failed
+//         interleaved, alibi, num_splits, checks, k_scale, v_scale, tree_mask) -> out, or the mask of the value checks that failed
 PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a{args, n};
@@ -763,7 +772,7 @@ PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor alibi = a.tensor_or_none();
   p.num_splits = (int)a.integer();
   const bool checks = a.truth();
-  Tensor k_scale = a.tensor_or_none(), v_scale = a.tensor_or_none();
+  Tensor k_scale = a.tensor_or_none(), v_scale = a.tensor_or_none(), tree = a.tensor_or_none();
 
   c10::cuda::CUDAGuard guard(q.device());
   at::AutoDispatchBelowADInplaceOrView below;
@@ -802,6 +811,11 @@ PyObject* py_kvcache(PyObject*, PyObject* const* args, Py_ssize_t n) {
     p.rotary_seqlen = (int)cos.size(0);
   }
   if (alibi.defined()) p.alibi_slopes = alibi.const_data_ptr<float>();
+  if (tree.defined()) {                              // (batch or 1, nodes, nodes) bool, rows of unit stride
+    p.tree_mask = static_cast<const uint8_t*>(tree.const_data_ptr());
+    p.tree_stride[0] = tree.size(0) == 1 ? 0 : tree.stride(0);
+    p.tree_stride[1] = tree.stride(1);
+  }
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   const bool coded = k_scale.defined();
   fa_cache8 c8;
@@ -930,6 +944,311 @@ PyObject* py_block_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
+  PyObject* out = PyTuple_New((Py_ssize_t)tensors.size());
+  if (out == nullptr) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  return out;
+}
+
+int dtype_of(const Tensor& t) {
+  return t.scalar_type() == at::kFloat ? FA_F32 : t.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_F16;
+}
+
+// verify(draft_tokens, parents, target, draft, accept, sample) -> (path, num_accepted, next_token)
+PyObject* py_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  Tensor tokens = a.tensor(), parents = a.tensor(), target = a.tensor(), draft = a.tensor(), accept = a.tensor(), sample = a.tensor();
+  c10::cuda::CUDAGuard guard(target.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto dev = target.device();
+  fa_verify_args p;
+  memset(&p, 0, sizeof(p));
+  p.dtype = dtype_of(target);
+  p.device = dev.index();
+  p.batch = (int)target.size(0); p.nodes = (int)target.size(1); p.vocab = target.size(2);
+  p.draft_tokens = tokens.const_data_ptr<int64_t>();
+  p.token_stride = tokens.stride(0);
+  p.parents = parents.const_data_ptr<int32_t>();
+  p.parent_stride = parents.dim() == 1 ? 0 : parents.stride(0);
+  p.target = target.const_data_ptr();
+  p.draft = draft.const_data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    p.target_stride[i] = target.stride(i);
+    p.draft_stride[i] = draft.stride(i);
+  }
+  p.accept = accept.const_data_ptr<float>();
+  p.sample = sample.const_data_ptr<float>();
+  Tensor path = empty_cuda({p.batch, p.nodes}, at::kInt, dev), count = empty_cuda({p.batch}, at::kInt, dev), next = empty_cuda({p.batch}, at::kLong, dev);
+  p.path = path.data_ptr<int32_t>();
+  p.num_accepted = count.data_ptr<int32_t>();
+  p.next_token = next.data_ptr<int64_t>();
+  check(g_abi.verify(&p, stream_of(target)), "fa_verify_draft_tree");
+  return tuple_of({path, count, next});
+  END_HANDLE_TH_ERRORS
+}
+
+// compact([k_cache], [v_cache], seqlens, path, num_accepted, block_table, batch_idx, leftpad, checks) -> the mask of the value checks that failed
+PyObject* py_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  PyObject* lists[2] = {a.next(), a.next()};
+  Tensor lens = a.tensor(), path = a.tensor(), accepted = a.tensor(), table = a.tensor_or_none(), idx = a.tensor_or_none(), pads = a.tensor_or_none();
+  const bool checks = a.truth();
+  void* caches[2][FA_COMPACT_LAYERS];
+  fa_compact_args p;
+  memset(&p, 0, sizeof(p));
+  Tensor first;
+  for (int w = 0; w < 2; ++w) {
+    TORCH_CHECK_TYPE(PyList_Check(lists[w]), "expected a list of tensors");
+    p.layers = (int)PyList_GET_SIZE(lists[w]);
+    TORCH_CHECK(p.layers <= FA_COMPACT_LAYERS, "too many layers for one call");
+    for (int i = 0; i < p.layers; ++i) {
+      PyObject* o = PyList_GET_ITEM(lists[w], i);
+      TORCH_CHECK_TYPE(THPVariable_Check(o), "expected a tensor");
+      const Tensor& t = THPVariable_Unpack(o);
+      caches[w][i] = t.data_ptr();
+      if (i == 0) {
+        first = t;
+        for (int d = 0; d < 3; ++d) (w ? p.vc_stride : p.kc_stride)[d] = t.stride(d);
+      }
+    }
+  }
+  c10::cuda::CUDAGuard guard(first.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto dev = first.device();
+  p.device = dev.index();
+  p.k_cache = caches[0];
+  p.v_cache = caches[1];
+  p.num_pages = (int)first.size(0); p.page_size = (int)first.size(1); p.heads = (int)first.size(2); p.head_dim = (int)first.size(3);
+  p.batch = (int)path.size(0);
+  if (table.defined()) {
+    p.block_table = table.const_data_ptr<int32_t>();
+    p.block_table_stride = (int)table.size(1);       // contiguous
+  }
+  if (idx.defined()) p.cache_batch_idx = idx.const_data_ptr<int32_t>();
+  if (pads.defined()) p.cache_leftpad = pads.const_data_ptr<int32_t>();
+  p.cache_seqlens = lens.const_data_ptr<int32_t>();
+  p.path = path.const_data_ptr<int32_t>();
+  p.path_stride = p.path_len = (int)path.size(1);    // contiguous
+  p.num_accepted = accepted.const_data_ptr<int32_t>();
+  void* st = stream_of(first);
+  uint32_t failed = 0;
+  int status;
+  Tensor ws;
+  if (checks) {
+    if (const size_t need = g_abi.compact_workspace(&p)) {
+      ws = empty_cuda({(int64_t)need}, at::kByte, dev);
+      p.workspace = ws.data_ptr();
+      p.workspace_bytes = need;
+    }
+    pybind11::gil_scoped_release nogil;
+    status = g_abi.compact_checked(&p, &failed, st);
+  } else {
+    status = g_abi.compact(&p, st);
+  }
+  check(status, "fa_compact");
+  return PyLong_FromUnsignedLong(failed);
+  END_HANDLE_TH_ERRORS
+}
+
+// release(held_lens, kept_lens, block_table, page_size, num_pages, checks) -> (pages, pages_released), or the mask of the value checks that failed
+PyObject* py_release(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  Tensor held = a.tensor(), kept = a.tensor(), table = a.tensor();
+  fa_release_args p;
+  memset(&p, 0, sizeof(p));
+  p.page_size = (int)a.integer();
+  p.num_pages = (int)a.integer();
+  const bool checks = a.truth();
+  c10::cuda::CUDAGuard guard(table.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto dev = table.device();
+  p.device = dev.index();
+  p.batch = (int)table.size(0);
+  p.held_lens = held.const_data_ptr<int32_t>();
+  p.kept_lens = kept.const_data_ptr<int32_t>();
+  p.block_table = table.const_data_ptr<int32_t>();
+  p.table_stride = table.stride(0);
+  p.table_pages = (int)table.size(1);
+  Tensor pages = empty_cuda({p.num_pages}, at::kInt, dev), count = empty_cuda({}, at::kInt, dev);
+  p.pages = pages.data_ptr<int32_t>();
+  p.pages_released = count.data_ptr<int32_t>();
+  void* st = stream_of(table);
+  uint32_t failed = 0;
+  int status;
+  if (checks) {
+    pybind11::gil_scoped_release nogil;
+    status = g_abi.release_checked(&p, &failed, st);
+  } else {
+    status = g_abi.release(&p, st);
+  }
+  check(status, "fa_release_pages");
+  if (failed) return PyLong_FromUnsignedLong(failed);
+  return tuple_of({pages, count});
+  END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------------------
+// norms of queries and keys with the rotation
+// ---------------------------------------------------------------------------------------
+// as the kernels read it; a copy also where a tensor is contiguous but begins between two 16-byte boundaries
+Tensor readable(const Tensor& t) { return kernel_ready(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+struct NormCall {
+  Tensor q, k, q_weight, k_weight, cos, sin, positions;        // q, k: (batch, seqlen, heads, dim) or (tokens, heads, dim)
+  double eps;
+  bool interleaved;
+};
+
+void norm_strides(int64_t* dst, const Tensor& t) {
+  const bool packed = t.dim() == 3;
+  dst[0] = packed ? 0 : t.stride(0);
+  dst[1] = t.stride(packed ? 0 : 1);
+  dst[2] = t.stride(packed ? 1 : 2);
+}
+
+void fill_norm(fa_qk_norm_args& p, const NormCall& c) {
+  memset(&p, 0, sizeof(p));
+  const bool packed = c.q.dim() == 3;
+  p.dtype = dtype_of(c.q);
+  p.device = c.q.device().index();
+  p.batch = packed ? 1 : (int)c.q.size(0);
+  p.seqlen = (int)c.q.size(packed ? 0 : 1);
+  p.heads_q = (int)c.q.size(-2); p.heads_kv = (int)c.k.size(-2); p.head_dim = (int)c.q.size(-1);
+  p.q = c.q.const_data_ptr();
+  p.k = c.k.const_data_ptr();
+  norm_strides(p.q_stride, c.q);
+  norm_strides(p.k_stride, c.k);
+  for (const Tensor* w : {&c.q_weight, &c.k_weight})
+    if (w->defined()) p.weight_wide = w->scalar_type() == at::kFloat;
+  if (c.q_weight.defined()) p.q_weight = c.q_weight.const_data_ptr();
+  if (c.k_weight.defined()) p.k_weight = c.k_weight.const_data_ptr();
+  p.eps = (float)c.eps;
+  if (c.cos.defined()) {
+    p.cos = c.cos.const_data_ptr();
+    p.sin = c.sin.const_data_ptr();
+    p.table_wide = c.cos.scalar_type() == at::kFloat;
+    p.rotary_dim = (int)c.cos.size(1) * 2;
+    p.rotary_seqlen = (int)c.cos.size(0);
+  }
+  p.interleaved = c.interleaved;
+  if (c.positions.defined()) {                                 // (tokens) or (batch or 1, seqlen)
+    p.positions = c.positions.const_data_ptr<int32_t>();
+    const bool rows = c.positions.dim() == 2;
+    p.pos_stride[0] = rows && c.positions.size(0) > 1 ? c.positions.stride(0) : 0;
+    p.pos_stride[1] = c.positions.stride(rows ? 1 : 0);
+  }
+}
+
+struct QkNormBackward : public Node {
+  SavedVariable saved[7];
+  double eps;
+  bool interleaved;
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    Tensor g[2];
+    for (int i = 0; i < 2; ++i) g[i] = grads[i].defined() ? grads[i] : input_metadata(i).zeros_like();
+    NormCall c;
+    Tensor* const members[7] = {&c.q, &c.k, &c.q_weight, &c.k_weight, &c.cos, &c.sin, &c.positions};
+    for (int i = 0; i < 7; ++i) *members[i] = saved[i].unpack();
+    c.eps = eps;
+    c.interleaved = interleaved;
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(c.q.device());
+    for (auto& t : g) t = readable(t);
+    fa_qk_norm_args p;
+    fill_norm(p, c);
+    p.d_qo = g[0].const_data_ptr();
+    p.d_ko = g[1].const_data_ptr();
+    norm_strides(p.d_qo_stride, g[0]);
+    norm_strides(p.d_ko_stride, g[1]);
+    const auto dev = c.q.device();
+    variable_list out(4);
+    out[0] = empty_cuda(c.q.sizes(), c.q.scalar_type(), dev);
+    out[1] = empty_cuda(c.k.sizes(), c.k.scalar_type(), dev);
+    p.d_q = out[0].mutable_data_ptr();
+    p.d_k = out[1].mutable_data_ptr();
+    norm_strides(p.d_q_stride, out[0]);
+    norm_strides(p.d_k_stride, out[1]);
+    if (c.q_weight.defined() && task_should_compute_output(2)) {
+      out[2] = empty_cuda(c.q_weight.sizes(), c.q_weight.scalar_type(), dev);
+      p.d_q_weight = out[2].mutable_data_ptr();
+    }
+    if (c.k_weight.defined() && task_should_compute_output(3)) {
+      out[3] = empty_cuda(c.k_weight.sizes(), c.k_weight.scalar_type(), dev);
+      p.d_k_weight = out[3].mutable_data_ptr();
+    }
+    Tensor ws;
+    if (p.d_q_weight || p.d_k_weight) {
+      p.workspace_bytes = g_abi.qk_norm_bwd_workspace(&p);
+      ws = empty_cuda({(int64_t)p.workspace_bytes}, at::kByte, dev);
+      p.workspace = ws.mutable_data_ptr();
+    }
+    check(g_abi.qk_norm_bwd(&p, stream_of(c.q)), "fa_qk_norm_bwd");
+    return out;
+  }
+  std::string name() const override { return "QkNormRotaryBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& s : saved) s.reset_data();
+  }
+};
+
+// qk_norm(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved) -> (q_out, k_out)
+PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  NormCall c;
+  c.q = a.tensor();
+  c.k = a.tensor();
+  c.q_weight = a.tensor_or_none();
+  c.k_weight = a.tensor_or_none();
+  c.cos = a.tensor_or_none();
+  c.sin = a.tensor_or_none();
+  c.positions = a.tensor_or_none();
+  c.eps = a.real();
+  c.interleaved = a.truth();
+  c10::cuda::CUDAGuard guard(c.q.device());
+  variable_list in = {c.q, c.k, c.q_weight, c.k_weight};
+  for (const auto& t : in)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "qk_norm_rotary has no forward-mode derivative");
+  std::shared_ptr<QkNormBackward> node;
+  if (at::GradMode::is_enabled() && torch::autograd::any_variable_requires_grad(in)) {
+    node = std::shared_ptr<QkNormBackward>(new QkNormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(in));
+  }
+  Tensor qo, ko;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c.q = readable(c.q);
+    c.k = readable(c.k);
+    const auto dev = c.q.device();
+    qo = empty_cuda(c.q.sizes(), c.q.scalar_type(), dev);
+    ko = empty_cuda(c.k.sizes(), c.k.scalar_type(), dev);
+    fa_qk_norm_args p;
+    fill_norm(p, c);
+    p.q_out = qo.mutable_data_ptr();
+    p.k_out = ko.mutable_data_ptr();
+    norm_strides(p.qo_stride, qo);
+    norm_strides(p.ko_stride, ko);
+    check(g_abi.qk_norm(&p, stream_of(c.q)), "fa_qk_norm");
+  }
+  if (node) {
+    torch::autograd::set_history({qo, ko}, node);
+    const Tensor* const members[7] = {&c.q, &c.k, &c.q_weight, &c.k_weight, &c.cos, &c.sin, &c.positions};
+    for (int i = 0; i < 7; ++i) node->saved[i] = SavedVariable(*members[i], false);
+    node->eps = c.eps;
+    node->interleaved = c.interleaved;
+  }
+  return tuple_of({qo, ko});
+  END_HANDLE_TH_ERRORS
+}
+
 // init({name: address}, check): addresses of the C functions, once per loaded library
 PyObject* py_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -975,6 +1294,15 @@ PyObject* py_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_abi.append8_workspace = (decltype(g_abi.append8_workspace))get("fa_append8_workspace_bytes");
   g_abi.block_table = (decltype(g_abi.block_table))get("fa_block_table");
   g_abi.block_table_checked = (decltype(g_abi.block_table_checked))get("fa_block_table_checked");
+  g_abi.verify = (decltype(g_abi.verify))get("fa_verify_draft_tree");
+  g_abi.compact = (decltype(g_abi.compact))get("fa_compact");
+  g_abi.compact_checked = (decltype(g_abi.compact_checked))get("fa_compact_checked");
+  g_abi.compact_workspace = (decltype(g_abi.compact_workspace))get("fa_compact_workspace_bytes");
+  g_abi.release = (decltype(g_abi.release))get("fa_release_pages");
+  g_abi.release_checked = (decltype(g_abi.release_checked))get("fa_release_pages_checked");
+  g_abi.qk_norm = (decltype(g_abi.qk_norm))get("fa_qk_norm");
+  g_abi.qk_norm_bwd = (decltype(g_abi.qk_norm_bwd))get("fa_qk_norm_bwd");
+  g_abi.qk_norm_bwd_workspace = (decltype(g_abi.qk_norm_bwd_workspace))get("fa_qk_norm_bwd_workspace_bytes");
   Py_INCREF(chk);
   Py_XDECREF(g_abi.check);
   g_abi.check = chk;
@@ -992,6 +1320,10 @@ PyMethodDef g_methods[] = {
     {"kvcache", FAST(py_kvcache), "append to a KV cache and attend to it"},
     {"append8", FAST(py_append8), "packed tokens into an 8-bit KV cache"},
     {"block_table", FAST(py_block_table), "pages, slots and cu_seqlens of a step"},
+    {"verify", FAST(py_verify), "verification of drafted tokens"},
+    {"compact", FAST(py_compact), "accepted tokens moved together in a KV cache"},
+    {"release", FAST(py_release), "pages that are no longer needed"},
+    {"qk_norm", FAST(py_qk_norm), "norms of queries and keys with the rotation"},
     {"int8", FAST(py_int8), "INT8 scores forward"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fa_host", "host path of the attention kernels", -1, g_methods};

@@ -362,7 +362,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
                             cache_seqlens=None, cache_batch_idx=None, cache_leftpad=None,
                             block_table=None, softmax_scale=None, causal=False,
                             window_size=(-1, -1), rotary_interleaved=True, alibi_slopes=None,
-                            num_splits=0, k_scale=None, v_scale=None):
+                            num_splits=0, k_scale=None, v_scale=None, tree_mask=None):
     """Attention against a KV cache, optionally appending new k/v first (in place) with
     rotary embedding applied to the new keys and to q.
 
@@ -381,6 +381,12 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     and v stay 16-bit.  New tokens are quantised as `kvcache_append` does it, and the attention is to what the cache
     then holds; caches and scales that overlap (an expanded scale, one tensor for keys and values) are for calls without them, and no two
     sequences of a call append to one block.
+
+    tree_mask: the query rows are the nodes of a tree of drafted tokens, the last seqlen_q tokens of the sequence after the append.  Bool,
+    (batch, seqlen_q, seqlen_q) or (seqlen_q, seqlen_q): row i sees node j where [.., i, j] is true -- itself and its ancestors, as a
+    rule -- and all tokens before the tree; with `causal`, only j <= i.  Rows of nodes that a request does not use may be all false
+    (they see the context alone; zeros without one), and what nodes hold that no row sees does not matter.  For 16-bit caches, without window, ALiBi
+    and rotary tables: a node's position is not its slot, see `qk_norm_rotary`.
 
     With value checks on (the default) the kernel makes them first (page indices in range, lengths
     fit the cache and the rotary tables) and the call waits for that one flag, not for the attention;
@@ -464,6 +470,12 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
             raise ValueError("rotary tables exceed the head dimension")
         rotary_cos = rotary_cos.to(device=dev, dtype=dtype).contiguous()
         rotary_sin = rotary_sin.to(device=dev, dtype=dtype).contiguous()
+    if tree_mask is not None:
+        tree_mask = _check_tree_mask(tree_mask, B, seqlen_q, dev)
+        if coded:
+            raise ValueError("tree_mask goes with FP16 and BF16 caches")
+        if window_size[0] >= 0 or window_size[1] >= 0 or alibi_slopes is not None or rotary_cos is not None:
+            raise ValueError("tree_mask cannot be combined with a window, ALiBi or rotary tables: the position of a node is not its slot")
     alibi = _normalise_alibi(alibi_slopes, B, heads_q, dev)
     if B == 0 or seqlen_q == 0:
         if _VALIDATE:
@@ -473,10 +485,22 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(head_dim)
     out = N.host().kvcache(q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, lengths, rows, pads, block_table, softmax_scale,
-                           causal, window_size[0], window_size[1], rotary_interleaved, alibi, num_splits, _VALIDATE, k_scale, v_scale)
+                           causal, window_size[0], window_size[1], rotary_interleaved, alibi, num_splits, _VALIDATE, k_scale, v_scale,
+                           tree_mask)
     if isinstance(out, int):
         raise ValueError(_cache_value_errors(lengths_error)[(out & -out).bit_length() - 1])
     return out
+
+
+def _check_tree_mask(mask, batch, nodes, device):
+    """(batch or 1, nodes, nodes) bool with rows of unit stride."""
+    if mask.dtype != torch.bool or mask.shape not in ((batch, nodes, nodes), (nodes, nodes)):
+        raise ValueError("tree_mask must be bool, (batch, seqlen_q, seqlen_q) or (seqlen_q, seqlen_q)")
+    if mask.device != device:
+        raise ValueError("tree_mask must be on the device of q")
+    if mask.ndim == 2:
+        mask = mask[None]
+    return mask if nodes <= 1 or mask.stride(2) == 1 else mask.contiguous()
 
 
 def _cache_value_errors(lengths_error):

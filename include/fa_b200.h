@@ -219,6 +219,13 @@ typedef struct fa_decode_args {
    * leaves the words zero again. */
   uint32_t* counters;
   int32_t num_counters;
+
+  /* A tree of drafted tokens, or NULL: the last seqlen_q positions after the append are its nodes, and query row i sees, of
+   * the keys there, those j with tree_mask[b * tree_stride[0] + i * tree_stride[1] + j] != 0 (bytes), besides all keys before them;
+   * with `causal`, only j <= i.  Values of nodes that no row sees are not read as numbers (they may be NaN).  16-bit caches;
+   * no window, ALiBi or rotary tables (the position of a node is not its slot). */
+  const uint8_t* tree_mask;
+  int64_t tree_stride[2];
 } fa_decode_args;
 
 int fa_decode_paged(const fa_decode_args* args, void* stream);
@@ -389,6 +396,138 @@ int fa_block_table(const fa_block_table_args* args, void* stream);
 int fa_block_table_checked(const fa_block_table_args* args, uint32_t* failed, void* stream);
 
 /*
+ * Verification of drafted tokens.  draft_tokens, parents (batch, nodes): the token of each node of a request's tree and the node before
+ * it (node 0 is the root, a token that is certain; a node whose parent is not an earlier one is not used).  target, draft (batch,
+ * nodes, vocab): the distribution of the token that follows each node, of the model that verifies and of the one that drafted; the children
+ * of a node were drawn from its draft distribution.  accept (batch, nodes), sample (batch): random numbers in [0, 1).
+ *   node = 0, c = 0, Z = 1;  for i = 1 .. nodes - 1 with parents[i] == node, x = draft_tokens[i]:
+ *     accept[i] * q(x) * Z < max(p(x) - c q(x), 0):  node = i, c = 0, Z = 1        (p, q: target and draft at `node`)
+ *     else                                           c += Z, Z = sum over v of max(p(v) - c q(v), 0)
+ *   path: the nodes visited, -1 behind them; num_accepted: how many, with the root
+ *   next_token: first v with r(0) + .. + r(v) > sample * sum r, r = max(p - c q, 0) (or max(p, 0) where that sums to 0); the last v with
+ *               r > 0 where rounding leaves none; -1 where the sum is 0 or no finite number
+ * Sums and products in 64 bits.  A token outside the vocabulary has p = q = 0.
+ */
+typedef struct fa_verify_args {
+  int32_t dtype, device; /* of target and draft: any fa_dtype */
+  int32_t batch, nodes;  /* nodes: 1 to 1024 */
+  int64_t vocab;         /* 1 to 2^31 - 1 */
+  const int64_t* draft_tokens;
+  int64_t token_stride; /* of a request; nodes follow one another */
+  const int32_t* parents;
+  int64_t parent_stride; /* 0: the same tree for all */
+  const void* target;
+  const void* draft;
+  int64_t target_stride[2], draft_stride[2]; /* (batch, node); the vocabulary is contiguous */
+  const float* accept;                       /* contiguous */
+  const float* sample;
+  int32_t* path; /* (batch, nodes) */
+  int32_t* num_accepted;
+  int64_t* next_token;
+} fa_verify_args;
+int fa_verify_draft_tree(const fa_verify_args* args, void* stream);
+
+/*
+ * Rows of accepted tokens moved together, in place, in the caches of all layers (16-bit types): for i < num_accepted[b], the row of
+ * position cache_seqlens[b] + i takes that of position cache_seqlens[b] + path[b][i]; path is ascending, so nothing is overwritten before
+ * it is read.  The caches of all layers have the same shape and strides, and none overlaps another.
+ * A request that fails a check below is passed over; _checked moves nothing then.
+ */
+#define FA_COMPACT_LAYERS 128 /* of one call */
+typedef struct fa_compact_args {
+  int32_t device, layers, batch, heads, head_dim;
+  void* const* k_cache; /* host arrays of `layers` device pointers */
+  void* const* v_cache;
+  int64_t kc_stride[3], vc_stride[3]; /* (page, row, head) */
+  int32_t page_size, num_pages;
+  const int32_t* block_table; /* as in fa_decode_args */
+  int32_t block_table_stride;
+  const int32_t* cache_batch_idx;
+  const int32_t* cache_leftpad;
+  const int32_t* cache_seqlens;
+  const int32_t* path; /* (batch, path_stride) */
+  int32_t path_stride, path_len;
+  const int32_t* num_accepted;
+  void* workspace; /* fa_compact_checked only: fa_compact_workspace_bytes() */
+  size_t workspace_bytes;
+} fa_compact_args;
+typedef enum fa_compact_check {
+  FA_COMPACT_COUNT = 1,   /* 0 <= num_accepted <= path_len */
+  FA_COMPACT_PATH = 2,    /* the accepted part of a path ascends from 0 or more */
+  FA_COMPACT_LENGTHS = 4, /* no length or left padding is negative, and the rows lie inside the cache */
+  FA_COMPACT_PAGES = 8    /* the pages and cache rows that are touched exist */
+} fa_compact_check;
+int fa_compact(const fa_compact_args* args, void* stream);
+/* Waits for the checks (not for the rows); not for streams under capture. */
+int fa_compact_checked(const fa_compact_args* args, uint32_t* failed, void* stream);
+size_t fa_compact_workspace_bytes(const fa_compact_args* args);
+
+/*
+ * Pages that requests no longer need: request b has pages for held_lens[b] tokens in its row of block_table and keeps those for
+ * kept_lens[b].  Entries [ceil(kept / page), ceil(held / page)) of the rows go to `pages`, row by row, -1 behind the last, and
+ * their number to pages_released[0].  The table stays as it is.  A call that fails a check writes -1 everywhere.
+ */
+typedef struct fa_release_args {
+  int32_t device, batch, page_size;
+  const int32_t* held_lens;
+  const int32_t* kept_lens;
+  const int32_t* block_table;
+  int64_t table_stride; /* of a row */
+  int32_t table_pages;  /* entries of a row */
+  int32_t num_pages;    /* room in pages */
+  int32_t* pages;
+  int32_t* pages_released;
+} fa_release_args;
+typedef enum fa_release_check {
+  FA_RELEASE_LENGTHS = 1, /* 0 <= kept <= held */
+  FA_RELEASE_ROW = 2,     /* every request fits its row of the table */
+  FA_RELEASE_ROOM = 4     /* the pages fit num_pages */
+} fa_release_check;
+int fa_release_pages(const fa_release_args* args, void* stream);
+int fa_release_pages_checked(const fa_release_args* args, uint32_t* failed, void* stream);
+
+/*
+ * RMS norm of every head of q and k, then the rotation by the token's position, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight;  out = y rotated as fa_rotary does it      in fp32, rounded once
+ * A token's table row is positions[b * s0 + t * s1], or t without positions; outside the table [0, rotary_seqlen) nothing is rotated.
+ * Backward (fa_qk_norm_bwd): d_qo, d_ko are the gradients of the outputs, d_q, d_k those of q and k; with g the gradient rotated back,
+ *   d_weight = sum over tokens and heads of g x r;  dx = r (g w - x r mean(g w x r)),   r = rsqrt(mean(x^2) + eps)
+ * Weights, their gradients and the tables: wide = 0: of dtype; else fp32.  The weight gradients' sums are in fp32 and always in the same order.
+ */
+typedef struct fa_qk_norm_args {
+  int32_t dtype, device; /* any fa_dtype */
+  int32_t batch, seqlen, heads_q, heads_kv, head_dim;
+  const void* q;
+  const void* k;
+  int64_t q_stride[3], k_stride[3]; /* (batch, row, head) */
+  const void* q_weight;             /* (head_dim), or NULL: ones */
+  const void* k_weight;
+  int32_t weight_wide, table_wide;
+  float eps;
+  const void* cos; /* (rotary_seqlen, rotary_dim / 2) contiguous; NULL: no rotation */
+  const void* sin;
+  int32_t rotary_dim, rotary_seqlen, interleaved;
+  const int32_t* positions;
+  int64_t pos_stride[2];
+  void* q_out; /* forward */
+  void* k_out;
+  int64_t qo_stride[3], ko_stride[3];
+  const void* d_qo; /* backward */
+  const void* d_ko;
+  int64_t d_qo_stride[3], d_ko_stride[3];
+  void* d_q;
+  void* d_k;
+  int64_t d_q_stride[3], d_k_stride[3];
+  void* d_q_weight; /* or NULL */
+  void* d_k_weight;
+  void* workspace; /* fa_qk_norm_bwd_workspace_bytes() */
+  size_t workspace_bytes;
+} fa_qk_norm_args;
+int fa_qk_norm(const fa_qk_norm_args* args, void* stream);
+int fa_qk_norm_bwd(const fa_qk_norm_args* args, void* stream);
+size_t fa_qk_norm_bwd_workspace_bytes(const fa_qk_norm_args* args);
+
+/*
  * Per-key-token INT8 quantisation: k (rows, head_dim) fp16 contiguous ->
  * k8 (rows, head_dim) int8, s_k (rows) fp32, with
  *   s = max(absmax, 1)/127;  code = round_half_away(k * (1/s))  in IEEE fp32,
@@ -512,7 +651,7 @@ int fa_mma_peak_probe(int32_t device, int32_t kind, int32_t iters, void* stream)
 /* sizeof of an argument block as this library was compiled: 0 = fa_attn_args,
  * 1 = fa_decode_args, 2 = fa_int8_args.  Lets a foreign-language binding check its
  * struct layout before the first call.  3 = fa_rotary_args, 4 = fa_cache8, 5 = fa_append8_args,
- * 6 = fa_block_table_args. */
+ * 6 = fa_block_table_args, 7 = fa_verify_args, 8 = fa_compact_args, 9 = fa_release_args, 10 = fa_qk_norm_args. */
 size_t fa_sizeof_args(int which);
 
 #ifdef __cplusplus
