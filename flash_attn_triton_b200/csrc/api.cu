@@ -156,12 +156,14 @@ int bwd_dq_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int bwd_dkdv_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int fwd_alt_sm100(const fa_attn_args&, const ScoreCfg&, cudaStream_t);
 int fwd_alt_sm100_status();
+int tree_sm100_status();
 int cache8_chunk_status();
 int cache8_pair_status();
 int fwd_duo_sm100_status();
 int64_t dropout_bits_words(int, int);
 int dropout_bits(const fa_attn_args&, const ScoreCfg&, uint32_t*, cudaStream_t);
 int fwd_alt_sm100_clear_status();
+int tree_sm100_clear_status();
 int cache8_chunk_clear_status();
 int cache8_pair_clear_status();
 int fwd_duo_sm100_clear_status();
@@ -867,6 +869,7 @@ int fa_device_wait_status(int device) {
   int s = fwd_sm100_status();
   if (s == 0) s = bwd_sm100_status();
   if (s == 0) s = fwd_alt_sm100_status();
+  if (s == 0) s = tree_sm100_status();
   if (s == 0) s = fwd_duo_sm100_status();
   if (s == 0) s = cache8_chunk_status();
   if (s == 0) s = cache8_pair_status();
@@ -885,6 +888,7 @@ int fa_device_wait_clear(int device) {
   fwd_sm100_clear_status();
   bwd_sm100_clear_status();
   fwd_alt_sm100_clear_status();
+  tree_sm100_clear_status();
   fwd_duo_sm100_clear_status();
   cache8_chunk_clear_status();
   cache8_pair_clear_status();

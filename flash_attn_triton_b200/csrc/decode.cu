@@ -50,6 +50,10 @@ namespace fa {
 int cache_attention_sm100(const fa_decode_args& d, const void* q, const int64_t* q_stride, const CacheGeo& geo,
                           const ScoreCfg& cfg, cudaStream_t st);
 
+int tree_sm100_ranges(const fa_decode_args& d, int pack_log2);
+size_t tree_sm100_piece_bytes(const fa_decode_args& d, int pack_log2);
+int tree_sm100(const fa_decode_args& d, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
+
 __global__ void __launch_bounds__(1024) decode_check_kernel(const fa_decode_args p, uint32_t* host, uint32_t* dev) {
   const uint32_t bad = decode_checks(p, threadIdx.x, blockDim.x);
   if (threadIdx.x == 0) {
@@ -524,6 +528,7 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
     return;
   }
   if (kTree) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the attention gets ready meanwhile
     // a warp has a word: of a node's row, or (row seqlen_q) of the nodes that any row sees
     const int n = p.seqlen_q, words = (n + 31) >> 5, lane = threadIdx.x & 31;
     const int64_t all = (int64_t)p.batch * (n + 1) * words;
@@ -533,9 +538,10 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
       const uint8_t* m = p.tree_mask + b * p.tree_stride[0] + j;
       bool seen = false;
       if (j < n) {
-        if (row < n) seen = m[row * p.tree_stride[1]] != 0;
+        // (causal: a row sees no node behind its own)
+        if (row < n) seen = m[row * p.tree_stride[1]] != 0 && !(p.causal && j > row);
         else
-          for (int r = 0; r < n; ++r) seen |= m[r * p.tree_stride[1]] != 0;
+          for (int r = p.causal ? j : 0; r < n; ++r) seen |= m[r * p.tree_stride[1]] != 0;
       }
       const uint32_t bits = __ballot_sync(0xffffffffu, seen);
       if (lane == 0) tree_bits[i] = bits;
@@ -582,10 +588,14 @@ struct ChunkPlan {
   int pack_log2, units, parts, capacity;
   size_t q_bytes, piece_bytes;   // workspace: rotated queries or the bits of a tree's mask, pieces, then the counters if the caller brings none
 };
+#ifndef FA_TREE_ROWS
+#define FA_TREE_ROWS 16
+#endif
+constexpr int kTreeRows = FA_TREE_ROWS;   // query rows per KV head up to which a tree stays with decode_kernel
 // Whether a call is a chunk, and how it is cut.
 static bool chunk_plan(const fa_decode_args& a, ChunkPlan& c) {
   const int G = a.heads_q / a.heads_kv;
-  if (a.num_splits != 0 || a.seqlen_q * G <= 16 || a.softmax_scale < 0.f) return false;
+  if (a.num_splits != 0 || a.seqlen_q * G <= (a.tree_mask ? kTreeRows : 16) || a.softmax_scale < 0.f) return false;
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
   if (a.block_table) {       // a tile of 128 keys is whole pages, or lies inside one
     const bool pow2 = (a.page_size & (a.page_size - 1)) == 0;
@@ -600,19 +610,24 @@ static bool chunk_plan(const fa_decode_args& a, ChunkPlan& c) {
   if (units > (1 << 28) || cap > (1 << 30)) return false;
   c.units = (int)units;
   c.capacity = (int)cap;
+  if (a.tree_mask) {
+    c.parts = tree_sm100_ranges(a, c.pack_log2);
+    c.q_bytes = ((size_t)a.batch * (a.seqlen_q + 1) * ((a.seqlen_q + 31) / 32) * sizeof(uint32_t) + 15) / 16 * 16;
+    c.piece_bytes = tree_sm100_piece_bytes(a, c.pack_log2);
+    return true;
+  }
   // pieces of at least four key tiles, only while the units leave SMs idle
   const int64_t fill = sm_count(a.device) / units, most = (cap + 511) / 512;
   c.parts = (int)(fill < most ? fill : most);
   if (c.parts < 1) c.parts = 1;
   c.q_bytes = a.rotary_cos ? (size_t)a.batch * a.seqlen_q * a.heads_q * a.head_dim * 2 : 0;
-  if (a.tree_mask) c.q_bytes = ((size_t)a.batch * (a.seqlen_q + 1) * ((a.seqlen_q + 31) / 32) * sizeof(uint32_t) + 15) / 16 * 16;
   c.piece_bytes = c.parts > 1 ? (size_t)c.units * c.parts * 128 * (a.head_dim + 1) * sizeof(float) : 0;
   return true;
 }
 
 int decode_num_counters(const fa_decode_args& a) {
   ChunkPlan c;
-  if (chunk_plan(a, c)) return c.parts > 1 ? c.units : 0;
+  if (chunk_plan(a, c)) return c.parts > 1 && !a.tree_mask ? c.units : 0;
   return a.batch * a.heads_kv * decode_row_groups(a);
 }
 
@@ -630,7 +645,7 @@ size_t decode_workspace_bytes(const fa_decode_args& a) {
   ChunkPlan c;
   if (chunk_plan(a, c)) {
     if (c.q_bytes + c.piece_bytes == 0) return 0;
-    return c.q_bytes + c.piece_bytes + (c.parts > 1 && !a.counters ? (size_t)c.units * sizeof(uint32_t) : 0);
+    return c.q_bytes + c.piece_bytes + (c.parts > 1 && !a.counters && !a.tree_mask ? (size_t)c.units * sizeof(uint32_t) : 0);
   }
   const size_t pieces = decode_piece_bytes(a, decode_geometry(a));
   return pieces == 0 ? 0 : pieces + (a.counters ? 0 : (size_t)decode_num_counters(a) * sizeof(uint32_t));
@@ -747,7 +762,7 @@ static int chunk_run(const fa_decode_args& args, const ChunkPlan& c, uint32_t* h
   geo.capacity = c.capacity;
   geo.ws = reinterpret_cast<float*>(ws + c.q_bytes);
   geo.bad = dev;
-  if (c.parts > 1) {
+  if (c.parts > 1 && !a.tree_mask) {
     geo.counters = a.counters;
     if (geo.counters == nullptr) {
       geo.counters = reinterpret_cast<uint32_t*>(ws + c.q_bytes + c.piece_bytes);
@@ -784,6 +799,7 @@ static int chunk_run(const fa_decode_args& args, const ChunkPlan& c, uint32_t* h
   }
   const int64_t qs[3] = {(int64_t)a.seqlen_q * a.heads_q * a.head_dim, (int64_t)a.heads_q * a.head_dim, a.head_dim};
   const ScoreCfg cfg = make_score_cfg(a.softmax_scale, 0.f, a.causal, a.window_left, a.window_right, a.alibi_slopes != nullptr);
+  if (tree_bits) return tree_sm100(a, geo, cfg, st);
   return cache_attention_sm100(a, q_out ? q_out : a.q, q_out ? qs : a.q_stride, geo, cfg, st);
 }
 

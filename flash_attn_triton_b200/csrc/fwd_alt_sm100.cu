@@ -143,8 +143,7 @@ struct Tile {
 // kGrid: the CTA's tile is its grid index (dense calls whose order does not matter, packed ones without a list); as one of
 // several ways in one kernel it took a CTA 0.2 us longer to start: 4096 packed sequences of 16 to 128, 8 heads of 256,
 // 2063 -> 2001 us.
-// kTree: a tree of drafted tokens against a cache: of the last geo.tokens keys, a row sees those of its bits (geo.tree_bits).
-template <typename T, int D, bool kExtras, bool kCache, int kPoly, bool kGrid = false, bool kTree = false>
+template <typename T, int D, bool kExtras, bool kCache, int kPoly, bool kGrid = false>
 __global__ void __launch_bounds__(kThreads, 1)
 fwd_alt_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -406,30 +405,6 @@ fwd_alt_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           advance();
         }
         if (!ok) break;
-        if constexpr (kTree) {
-          // Nodes that no row sees (of a request that uses fewer than others) may hold anything, and 0 times a NaN is one:
-          // their values become 0.  Here, because this warp alone knows that the ring entry is loaded.
-          const int k0 = (w.n_hi - 1 - j) * kBN;
-          if (k0 + kBN > w.pos0) {
-            const uint32_t* any = geo.tree_bits + ((int64_t)w.b * (geo.tokens + 1) + geo.tokens) * geo.tree_words;
-            bool zeroed = false;
-            for (int c0 = 0; c0 < kBN; c0 += 32) {
-              const int node = k0 + c0 + lane - w.pos0;
-              const bool dead = node >= 0 && node < geo.tokens && (any[node >> 5] >> (node & 31) & 1u) == 0u;
-              for (unsigned rest = __ballot_sync(0xffffffffu, dead); rest; rest &= rest - 1) {
-                const int r = c0 + __ffs(rest) - 1;
-                zeroed = true;
-                for (int c = lane; c < NU * C::kBoxes * 8; c += 32)
-                  *reinterpret_cast<uint4*>(tiles + C::kQBytes + st[c / (C::kBoxes * 8)] * C::kUnitBytes + (c / 8 % C::kBoxes) * (kBN * 128) +
-                                            r * 128 + c % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-              }
-            }
-            if (zeroed) {
-              fence_proxy_async();
-              __syncwarp();
-            }
-          }
-        }
         if (kPvSplit) {
           wwait(&sh->p_half[buf], par, 25);
           if (!ok) break;
@@ -490,21 +465,6 @@ fwd_alt_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       if (cfg.causal) masked |= (k0 + kBN - 1 > tq_min);
       if (cfg.wl >= 0) masked |= (k0 < tq_end - cfg.wl);
       if (cfg.wr >= 0) masked |= (k0 + kBN - 1 > tq_min + cfg.wr);
-      // the nodes that this row sees, of the 128 keys of the tile: asked for ahead of the scores
-      uint32_t nodes[4];
-      if constexpr (kTree) {
-        masked |= k0 + kBN > w.pos0;
-        if (masked) {
-          const uint32_t* bits = geo.tree_bits + ((int64_t)w.b * (geo.tokens + 1) + min(row >> w.pack_log2, geo.tokens - 1)) * geo.tree_words;
-          const int shift = k0 - w.pos0;             // node of the tile's first key; below 0: context, which all see
-          auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < geo.tree_words ? bits[i] : 0u; };
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = (shift >> 5) + i;
-            nodes[i] = __funnelshift_r(word(at), word(at + 1), shift & 31);
-          }
-        }
-      }
 
       ok = wait_bar(&sh->s_full[buf], par, sh, 31 + x);
       if (!ok) break;
@@ -556,7 +516,7 @@ fwd_alt_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 float v = __uint_as_float(r[cc][i]) * cfg.scale_log2;
-                if (kMask) v = col_visible(cm, cc * 32 + i) && (!kTree || (nodes[cc] >> i & 1u)) ? v : -INFINITY;
+                if (kMask) v = col_visible(cm, cc * 32 + i) ? v : -INFINITY;
                 r[cc][i] = __float_as_uint(v);
               }
             }
@@ -991,8 +951,6 @@ static int launch_cache(const fa_decode_args& d, const void* q, const int64_t* q
   }
   const int mtiles = (d.seqlen_q * pack + kBM - 1) / kBM;
   const dim3 grid((unsigned)d.batch * (d.heads_q / pack) * mtiles * geo.parts);
-  if (geo.tree_bits)
-    return launch_alt(fwd_alt_sm100_kernel<T, D, false, true, 0, false, true>, ACfg<D>::kSmemBytes, grid, st, tm, a, cfg, geo);
   if (cfg.has_alibi)
     return launch_alt(fwd_alt_sm100_kernel<T, D, true, true, 0>, ACfg<D>::kSmemBytes, grid, st, tm, a, cfg, geo);
   return launch_alt(fwd_alt_sm100_kernel<T, D, false, true, 0>, ACfg<D>::kSmemBytes, grid, st, tm, a, cfg, geo);
