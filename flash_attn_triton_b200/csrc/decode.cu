@@ -588,14 +588,20 @@ struct ChunkPlan {
   int pack_log2, units, parts, capacity;
   size_t q_bytes, piece_bytes;   // workspace: rotated queries or the bits of a tree's mask, pieces, then the counters if the caller brings none
 };
-#ifndef FA_TREE_ROWS
-#define FA_TREE_ROWS 16
-#endif
-constexpr int kTreeRows = FA_TREE_ROWS;   // query rows per KV head up to which a tree stays with decode_kernel
+// Whether a tree takes the kernel for it (tree_sm100.cu): more than 8 query rows per KV head, and more than two tiles of 64 keys and 16 rows for
+// each CTA of decode_kernel that runs at a time.  Measured, decode_kernel against it (us, 8 KV heads of 128): 48 x 6250 tokens, 16 rows 256, 225;
+// 8 rows 233, 220; 1 x 8000, 16 rows 29, 24; 1 x 1900, 32 rows 18, 20; 64 rows 22, 21; 1 x 500, 32 rows 15, 16; 2 x 300, 2 heads of 64,
+// 20 rows 10, 18: few tiles are bounded by launches, of which decode_kernel is one and a tree's are three.
+static bool tree_kernel_is_faster(const fa_decode_args& a, int64_t capacity) {
+  const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
+  return rows > 8 && a.batch * a.heads_kv * ((rows + 15) / 16) * ((capacity + kTile - 1) / kTile) > 4ll * sm_count(a.device);
+}
 // Whether a call is a chunk, and how it is cut.
 static bool chunk_plan(const fa_decode_args& a, ChunkPlan& c) {
   const int G = a.heads_q / a.heads_kv;
-  if (a.num_splits != 0 || a.seqlen_q * G <= (a.tree_mask ? kTreeRows : 16) || a.softmax_scale < 0.f) return false;
+  const int64_t cap = a.block_table ? (int64_t)a.block_table_stride * a.page_size : a.page_size;
+  if (a.num_splits != 0 || a.softmax_scale < 0.f) return false;
+  if (a.tree_mask ? !tree_kernel_is_faster(a, cap) : a.seqlen_q * G <= 16) return false;
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
   if (a.block_table) {       // a tile of 128 keys is whole pages, or lies inside one
     const bool pow2 = (a.page_size & (a.page_size - 1)) == 0;
@@ -604,7 +610,6 @@ static bool chunk_plan(const fa_decode_args& a, ChunkPlan& c) {
   c.pack_log2 = 0;
   if ((G & (G - 1)) == 0 && G <= 64)
     while ((1 << c.pack_log2) < G) ++c.pack_log2;
-  const int64_t cap = a.block_table ? (int64_t)a.block_table_stride * a.page_size : a.page_size;
   const int mtiles = (int)((((int64_t)a.seqlen_q << c.pack_log2) + 127) / 128);
   const int64_t units = (int64_t)a.batch * (a.heads_q >> c.pack_log2) * mtiles;
   if (units > (1 << 28) || cap > (1 << 30)) return false;
