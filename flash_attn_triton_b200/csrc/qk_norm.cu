@@ -5,9 +5,14 @@
 //   for one another.
 //   Bound.  HBM: forward 2, backward 3 words an element.  D / 8 lanes have a head and 8 elements each, 16 bytes of a 16-bit type, so that a
 //   head is one access, its sums are shuffles, and a pair's other half (rotate-half) comes from another lane of the head.  A group of
-//   lanes takes several heads of a token, one after another, with the token's angles in registers.
+//   lanes has an even share of all heads of all tokens, one after another, with a token's angles in registers, first of q and then of k, so
+//   that a thread has one set of weights and sums at a time and divides only where its share begins.  Every thread has a ring of its own in shared memory that its loads go to
+//   (cp.async, 128 bytes in flight), so that no barrier is needed and registers do not bound the loads in flight: 16380 tokens of 40 heads
+//   of 128, bf16, forward 69 us with four loads in registers, backward 110.
 //   Weight gradients: a thread's sums over its heads, those of a CTA through shared memory, those of the CTAs by a second kernel in
 //   order.  The grid depends on the sizes and the GPU alone, so the result does not change from call to call.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace fa {
@@ -23,11 +28,16 @@ template <typename T> __device__ __forceinline__ Raw<T> load8(const T* p) { retu
 template <> __device__ __forceinline__ Raw<float> load8(const float* p) {
   return Raw<float>{reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]};
 }
+// Two numbers of a word.  (bf16: the upper halves of fp32 numbers.  __bfloat1622float2 takes two or three instructions for each.)
+template <typename T> __device__ __forceinline__ float2 pair_of(uint32_t w) { return Elem<T>::unpack(w); }
+template <> __device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <typename T> __device__ __forceinline__ void widen(const Raw<T>& r, float (&x)[8]) {
   const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = Elem<T>::unpack(w[i]);
+    const float2 f = pair_of<T>(w[i]);
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
@@ -48,6 +58,49 @@ template <> __device__ __forceinline__ void store8(float* p, const float (&x)[8]
   reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
+// The same as four pairs.
+template <typename T> __device__ __forceinline__ void pairs_of(const Raw<T>& r, float2 (&x)[4]) {
+  const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = pair_of<T>(w[i]);
+}
+template <> __device__ __forceinline__ void pairs_of(const Raw<float>& r, float2 (&x)[4]) {
+  x[0] = make_float2(r.a.x, r.a.y);
+  x[1] = make_float2(r.a.z, r.a.w);
+  x[2] = make_float2(r.b.x, r.b.y);
+  x[3] = make_float2(r.b.z, r.b.w);
+}
+template <typename T> __device__ __forceinline__ void store_pairs(T* p, const float2 (&x)[4]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::pack(x[0].x, x[0].y), Elem<T>::pack(x[1].x, x[1].y), Elem<T>::pack(x[2].x, x[2].y),
+                                            Elem<T>::pack(x[3].x, x[3].y));
+}
+template <> __device__ __forceinline__ void store_pairs(float* p, const float2 (&x)[4]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
+}
+// The other element of each pair, as it was loaded: next to it (interleaved), or in lane `other` of the L that have the head.
+template <int L, bool kSideBySide, typename T> __device__ __forceinline__ Raw<T> other_of(const Raw<T>& r, int other) {
+  Raw<T> z;
+  if constexpr (kSideBySide) {
+    z.v = make_uint4(__byte_perm(r.v.x, 0u, 0x1032), __byte_perm(r.v.y, 0u, 0x1032), __byte_perm(r.v.z, 0u, 0x1032), __byte_perm(r.v.w, 0u, 0x1032));
+  } else {
+    z.v = make_uint4(__shfl_sync(0xffffffffu, r.v.x, other, L), __shfl_sync(0xffffffffu, r.v.y, other, L), __shfl_sync(0xffffffffu, r.v.z, other, L),
+                     __shfl_sync(0xffffffffu, r.v.w, other, L));
+  }
+  return z;
+}
+template <int L, bool kSideBySide> __device__ __forceinline__ Raw<float> other_of(const Raw<float>& r, int other) {
+  Raw<float> z;
+  if constexpr (kSideBySide) {
+    z.a = make_float4(r.a.y, r.a.x, r.a.w, r.a.z);
+    z.b = make_float4(r.b.y, r.b.x, r.b.w, r.b.z);
+  } else {
+    auto from = [&](float x) { return __shfl_sync(0xffffffffu, x, other, L); };
+    z.a = make_float4(from(r.a.x), from(r.a.y), from(r.a.z), from(r.a.w));
+    z.b = make_float4(from(r.b.x), from(r.b.y), from(r.b.z), from(r.b.w));
+  }
+  return z;
+}
 template <typename T> __device__ __forceinline__ float one(const T* p);
 template <> __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
 template <> __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -62,24 +115,63 @@ template <typename T> __device__ __forceinline__ float at(const void* p, int wid
   return wide ? static_cast<const float*>(p)[i] : one(static_cast<const T*>(p) + i);
 }
 
-// How a call is cut: groups of lanes take `heads` heads of a token each, `chunks` of them a token.
-struct Cut {
-  int heads, chunks;
-  int64_t items;
-};
+// kN (4 or 8) numbers of a table from p on, aligned to their size.
+template <typename T, int kN> __device__ __forceinline__ void entries(const void* p, int wide, int64_t i, float (&x)[8]) {
+  if (wide) {
+    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+    for (int k = 0; k < kN / 4; ++k) {
+      const float4 v = f[k];
+      x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const uint2* f = reinterpret_cast<const uint2*>(static_cast<const T*>(p) + i);
+#pragma unroll
+    for (int k = 0; k < kN / 4; ++k) {
+      const uint2 v = f[k];
+      const float2 a = Elem<T>::unpack(v.x), b = Elem<T>::unpack(v.y);
+      x[4 * k] = a.x; x[4 * k + 1] = a.y; x[4 * k + 2] = b.x; x[4 * k + 3] = b.y;
+    }
+  }
+}
 
 // The rotation of this lane's 8 elements d .. d + 7 of a head, as cos and sin per element; elements behind rotary_dim have cos = 1,
 // sin = 0.  The sign of the sine is that of the forward rotation of the element: out = y cos + (its pair's y) sin.
 template <typename T>
-__device__ __forceinline__ void angles(const fa_qk_norm_args& p, int64_t pos, int d, float (&c)[8], float (&s)[8]) {
+__device__ __forceinline__ void angles(const fa_qk_norm_args& p, bool whole, int64_t pos, int d, float (&c)[8], float (&s)[8]) {
   const int half = p.rotary_dim >> 1;
-  const bool turned = p.cos != nullptr && pos >= 0 && pos < p.rotary_seqlen;
+  if (p.cos == nullptr || pos < 0 || pos >= p.rotary_seqlen || d >= p.rotary_dim) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[e] = 1.f;
+      s[e] = 0.f;
+    }
+    return;
+  }
+  if (whole) {                                   // these 8 have 8 entries in a row, side by side pairs 4
+    if (p.interleaved) {
+      float x[8];
+      entries<T, 4>(p.cos, p.table_wide, pos * half + (d >> 1), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = x[e >> 1];
+      entries<T, 4>(p.sin, p.table_wide, pos * half + (d >> 1), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = e & 1 ? x[e >> 1] : -x[e >> 1];
+    } else {
+      const int64_t i = pos * half + (d < half ? d : d - half);
+      entries<T, 8>(p.cos, p.table_wide, i, c);
+      entries<T, 8>(p.sin, p.table_wide, i, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = d < half ? -s[e] : s[e];
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int j = d + e;
     c[e] = 1.f;
     s[e] = 0.f;
-    if (turned && j < p.rotary_dim) {
+    if (j < p.rotary_dim) {
       const bool first = p.interleaved ? (j & 1) == 0 : j < half;
       const int64_t i = pos * half + (p.interleaved ? j >> 1 : first ? j : j - half);
       c[e] = at<T>(p.cos, p.table_wide, i);
@@ -122,137 +214,248 @@ template <int L> __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-struct Weights {
-  float q[8], k[8];
+// One of q and k.
+struct Side {
+  const void* x;
+  const void* g;                                 // backward: the gradient of the result
+  void* out;                                     // the result; backward: the gradient of x
+  const void* weight;
+  int64_t xs[3], gs[3], os[3];
+  int heads;
 };
-template <typename T> __device__ __forceinline__ Weights weights_of(const fa_qk_norm_args& p, int d) {
-  Weights w;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    w.q[e] = p.q_weight ? at<T>(p.q_weight, p.weight_wide, d + e) : 1.f;
-    w.k[e] = p.k_weight ? at<T>(p.k_weight, p.weight_wide, d + e) : 1.f;
-  }
-  return w;
+struct Sides {
+  Side side[2];
+};
+
+// The lane with the other halves of this lane's pairs.
+__device__ __forceinline__ int other_lane(const fa_qk_norm_args& p, int lane) {
+  const int half = p.rotary_dim >> 1, d = lane * 8;
+  return d < half ? lane + half / 8 : d < p.rotary_dim ? lane - half / 8 : lane;
 }
 
-template <typename T>
-__device__ __forceinline__ const T* row_of(const void* q, const void* k, const int64_t* qs, const int64_t* ks, int heads_q, int b, int t, int h) {
-  return h < heads_q ? static_cast<const T*>(q) + b * qs[0] + t * qs[1] + h * qs[2]
-                     : static_cast<const T*>(k) + b * ks[0] + t * ks[1] + (h - heads_q) * ks[2];
+// The table rows of a position, on their way to L1.
+__device__ __forceinline__ void prefetch_angles(const fa_qk_norm_args& p, int64_t pos, int d, int bytes) {
+  const int half = p.rotary_dim >> 1;
+  if (p.cos == nullptr || pos < 0 || pos >= p.rotary_seqlen || d >= half) return;
+  const int64_t i = (pos * half + d) * bytes;
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.cos) + i));
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(p.sin) + i));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) qk_norm_kernel(const fa_qk_norm_args p, const Cut cut) {
-  constexpr int L = D / 8, G = kThreads / L, kU = 4;
-  __shared__ float rows[G][D];
-  const int group = threadIdx.x / L, lane = threadIdx.x % L, d = lane * 8;
-  const int heads = p.heads_q + p.heads_kv;
-  const Weights w = weights_of<T>(p, d);
-  // (the lanes of a warp stay together: groups without work do what their neighbours do, and store nothing)
-  for (int64_t base = (int64_t)blockIdx.x * G; base < cut.items; base += (int64_t)gridDim.x * G) {
-    const bool mine = base + group < cut.items;
-    const int64_t item = mine ? base + group : cut.items - 1;
-    const int64_t token = item / cut.chunks;
-    const int h0 = (int)(item - token * cut.chunks) * cut.heads, h1 = min(heads, h0 + cut.heads);
-    const int b = (int)(token / p.seqlen), t = (int)(token - (int64_t)b * p.seqlen);
-    float c[8], s[8];
-    angles<T>(p, p.positions ? (int64_t)p.positions[b * p.pos_stride[0] + t * p.pos_stride[1]] : t, d, c, s);
-    for (int j0 = 0; j0 < cut.heads; j0 += kU) {
-      Raw<T> x[kU];
-#pragma unroll
-      for (int j = 0; j < kU; ++j)
-        if (j0 + j < cut.heads) x[j] = load8(row_of<T>(p.q, p.k, p.q_stride, p.k_stride, p.heads_q, b, t, min(h0 + j0 + j, h1 - 1)) + d);
-#pragma unroll
-      for (int j = 0; j < kU; ++j) {
-        if (j0 + j >= cut.heads) break;
-        const int h = min(h0 + j0 + j, h1 - 1);
-        float y[8], z[8];
-        widen<T>(x[j], y);
-        float sq = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sq = fmaf(y[e], y[e], sq);
-        const float r = rsqrtf(group_sum<L>(sq) * (1.f / D) + p.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = y[e] * r * (h < p.heads_q ? w.q[e] : w.k[e]);
-        partners<D>(p, lane, y, z, rows[group]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = y[e] * c[e] + z[e] * s[e];
-        if (mine && h0 + j0 + j < h1)
-          store8(const_cast<T*>(row_of<T>(p.q_out, p.k_out, p.qo_stride, p.ko_stride, p.heads_q, b, t, h)) + d, y);
-      }
-    }
-  }
-}
+constexpr int kSlots = 8;                        // 16-byte slots of a thread's ring
 
-// ws: 2 D sums of every CTA
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) qk_norm_bwd_kernel(const fa_qk_norm_args p, const Cut cut, float* ws) {
-  constexpr int L = D / 8, G = kThreads / L, kU = 2;
-  __shared__ float rows[G][D];
-  const int group = threadIdx.x / L, lane = threadIdx.x % L, d = lane * 8;
-  const int heads = p.heads_q + p.heads_kv;
-  const Weights w = weights_of<T>(p, d);
-  float dwq[8], dwk[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) dwq[e] = dwk[e] = 0.f;
-  for (int64_t base = (int64_t)blockIdx.x * G; base < cut.items; base += (int64_t)gridDim.x * G) {
-    const bool mine = base + group < cut.items;
-    const int64_t item = mine ? base + group : cut.items - 1;
-    const int64_t token = item / cut.chunks;
-    const int h0 = (int)(item - token * cut.chunks) * cut.heads, h1 = min(heads, h0 + cut.heads);
-    const int b = (int)(token / p.seqlen), t = (int)(token - (int64_t)b * p.seqlen);
-    float c[8], s[8];
-    angles<T>(p, p.positions ? (int64_t)p.positions[b * p.pos_stride[0] + t * p.pos_stride[1]] : t, d, c, s);
-    for (int j0 = 0; j0 < cut.heads; j0 += kU) {
-      Raw<T> xr[kU], gr[kU];
-#pragma unroll
-      for (int j = 0; j < kU; ++j) {
-        if (j0 + j >= cut.heads) break;
-        const int h = min(h0 + j0 + j, h1 - 1);
-        xr[j] = load8(row_of<T>(p.q, p.k, p.q_stride, p.k_stride, p.heads_q, b, t, h) + d);
-        gr[j] = load8(row_of<T>(p.d_qo, p.d_ko, p.d_qo_stride, p.d_ko_stride, p.heads_q, b, t, h) + d);
-      }
-#pragma unroll
-      for (int j = 0; j < kU; ++j) {
-        if (j0 + j >= cut.heads) break;
-        const int h = min(h0 + j0 + j, h1 - 1);
-        const bool live = mine && h0 + j0 + j < h1;
-        float x[8], g[8], z[8];
-        widen<T>(xr[j], x);
-        widen<T>(gr[j], g);
-        partners<D>(p, lane, g, z, rows[group]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = g[e] * c[e] - z[e] * s[e];      // rotated back
-        float sq = 0.f, hx = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sq = fmaf(x[e], x[e], sq);
-          hx = fmaf(g[e] * (h < p.heads_q ? w.q[e] : w.k[e]), x[e], hx);
-        }
-        const float r = rsqrtf(group_sum<L>(sq) * (1.f / D) + p.eps);
-        const float mean = group_sum<L>(hx) * (1.f / D) * r;               // of h x r
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float unit = x[e] * r, gu = g[e] * unit;
-          if (live) (h < p.heads_q ? dwq[e] : dwk[e]) += gu;
-          x[e] = r * (g[e] * (h < p.heads_q ? w.q[e] : w.k[e]) - unit * mean);
-        }
-        if (live) store8(const_cast<T*>(row_of<T>(p.d_q, p.d_k, p.d_q_stride, p.d_k_stride, p.heads_q, b, t, h)) + d, x);
-      }
-    }
-  }
-  if (ws == nullptr) return;
-#pragma unroll
+// kTurn: whether a lane's 8 elements are turned as one (whole_lanes()), and where the other elements of their pairs are.  If they are, and with x' the other element of each pair, the forward is
+// r (x (c w) + x' (s w')), the two products in brackets made once for all heads of a token, and all of it in pairs of fp32: element by
+// element, 177 instructions for 8 elements of a lane bound the forward, 253 the backward.  ws: backward, D sums of every CTA for q, then for k.
+enum Turn { kAnyhow, kHalves, kSideBySide };
+template <typename T, int D, bool kBackward, Turn kTurn>
+__global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(const fa_qk_norm_args p, const Sides sides, float* ws) {
+  constexpr bool kWhole = kTurn != kAnyhow;
+  constexpr int L = D / 8, G = kThreads / L;
+  constexpr int W = sizeof(T) / 2, kOf = W * (kBackward ? 2 : 1), S = kSlots / kOf;      // slots of 8 elements, of a head; heads in flight
+  __shared__ uint4 ring[kSlots][kThreads];
+  __shared__ float rows[kWhole ? 1 : G][kWhole ? 1 : D];
+  const int tid = threadIdx.x, group = tid / L, lane = tid % L, d = lane * 8;
+  const int entry = p.table_wide ? 4 : (int)sizeof(T);
+  const int other = other_lane(p, lane);
+  const bool side_by_side = p.interleaved != 0;
+  const int64_t groups = (int64_t)gridDim.x * G, me = (int64_t)blockIdx.x * G + group, tokens = (int64_t)p.batch * p.seqlen;
+#pragma unroll 1
   for (int which = 0; which < 2; ++which) {
-    __syncthreads();
+    const Side& a = sides.side[which];
+    const int heads = a.heads;
+    float2 w[4], wo[4], dw[4];                   // weights, those of the other elements of the pairs
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rows[group][d + e] = which ? dwk[e] : dwq[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < D; i += kThreads) {
-      float sum = 0.f;
-      for (int g = 0; g < G; ++g) sum += rows[g][i];
-      ws[((int64_t)blockIdx.x * 2 + which) * D + i] = sum;
+    for (int e = 0; e < 4; ++e) {
+      w[e] = a.weight ? make_float2(at<T>(a.weight, p.weight_wide, d + 2 * e), at<T>(a.weight, p.weight_wide, d + 2 * e + 1)) : make_float2(1.f, 1.f);
+      wo[e] = side_by_side ? make_float2(w[e].y, w[e].x) : make_float2(__shfl_sync(0xffffffffu, w[e].x, other, L), __shfl_sync(0xffffffffu, w[e].y, other, L));
+      dw[e] = make_float2(0.f, 0.f);
     }
+    // this group's heads: `mine` of them from `begin` on; the groups of a warp stay together for `steps`
+    const int64_t total = tokens * heads, begin = total * me / groups;
+    const int mine = (int)(total * (me + 1) / groups - begin), steps = (int)((total + groups - 1) / groups);
+    const int64_t token = heads ? begin / heads : 0;
+    const int b0 = (int)(token / p.seqlen), t0 = (int)(token - (int64_t)b0 * p.seqlen), h0 = (int)(begin - token * heads);
+
+    // loading: S heads ahead of their use
+    const int64_t xh = a.xs[2], gh = a.gs[2], oh = a.os[2];
+    int lb = b0, lt = t0, lh = h0, left = mine;
+    const T* lx = static_cast<const T*>(a.x) + lb * a.xs[0] + lt * a.xs[1] + lh * xh + d;
+    const T* lg = kBackward ? static_cast<const T*>(a.g) + lb * a.gs[0] + lt * a.gs[1] + lh * gh + d : nullptr;
+    constexpr uint32_t kPitch = kThreads * 16;
+    const uint32_t own = smem_u32(&ring[0][tid]);
+    uint32_t turn = 0;                           // of the ring: bytes from this thread's first slot
+    auto ask = [&](uint32_t to) {
+      if (left > 0) {
+        --left;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          cp_async16(to + k * kPitch, lx + k * (16 / sizeof(T)), 16);
+          if (kBackward) cp_async16(to + (W + k) * kPitch, lg + k * (16 / sizeof(T)), 16);
+        }
+        lx += xh;
+        if (kBackward) lg += gh;
+        if (++lh == heads) {
+          lh = 0;
+          if (++lt == p.seqlen) {
+            lt = 0;
+            ++lb;
+          }
+          lx = static_cast<const T*>(a.x) + lb * a.xs[0] + lt * a.xs[1] + d;
+          if (kBackward) lg = static_cast<const T*>(a.g) + lb * a.gs[0] + lt * a.gs[1] + d;
+        }
+      }
+      cp_async_commit();
+    };
+    auto word = [&](uint32_t from) {
+      uint4 v;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+      return v;
+    };
+    auto read = [&](uint32_t from) {
+      Raw<T> r;
+      if constexpr (sizeof(T) == 2) {
+        r.v = word(from);
+      } else {
+        const uint4 v = word(from), u = word(from + kPitch);
+        r.a = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+        r.b = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+      }
+      return r;
+    };
+#pragma unroll
+    for (int k = 0; k < S; ++k) ask(own + k * kOf * kPitch);
+
+    int b = b0, t = t0, h = h0;
+    auto position_of = [&](int pb, int pt) {
+      return p.positions ? (int64_t)p.positions[pb * p.pos_stride[0] + pt * p.pos_stride[1]] : (int64_t)pt;
+    };
+    float2 c[4], s[4];                           // of the token at hand; forward, whole lanes: times the weights
+    auto turn_to = [&](int64_t pos) {
+      float cs[8], sn[8];
+      angles<T>(p, kWhole, pos, d, cs, sn);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[e] = make_float2(cs[2 * e], cs[2 * e + 1]);
+        s[e] = make_float2(sn[2 * e], sn[2 * e + 1]);
+        if constexpr (kWhole && !kBackward) {
+          c[e] = f2mul(c[e], w[e]);
+          s[e] = f2mul(s[e], wo[e]);
+        }
+      }
+    };
+    int64_t next_pos = 0;
+    T* out = static_cast<T*>(a.out) + b * a.os[0] + t * a.os[1] + h * oh + d;
+    if (mine > 0) turn_to(position_of(b, t));
+    bool fresh = true;                           // the next token's position is not known yet
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      cp_async_wait<S - 1>();
+      const Raw<T> xr = read(own + turn);
+      Raw<T> gr;
+      if (kBackward) gr = read(own + turn + W * kPitch);
+      ask(own + turn);
+      turn = (turn + kOf * kPitch) & (kSlots * kPitch - 1);
+      const bool live = step < mine;
+      if constexpr (kWhole && !kBackward) {
+        float2 y[4], z[4], sq = make_float2(0.f, 0.f);
+        pairs_of<T>(xr, y);
+        pairs_of<T>(other_of<L, kTurn == kSideBySide>(xr, other), z);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sq = f2fma(y[e], y[e], sq);
+        const float r = rsqrtf(group_sum<L>(sq.x + sq.y) * (1.f / D) + p.eps);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = f2mul(f2fma(z[e], s[e], f2mul(y[e], c[e])), make_float2(r, r));
+        if (live) store_pairs(out, y);
+      } else if constexpr (kWhole) {
+        float2 x[4], g[4], z[4], sq = make_float2(0.f, 0.f), hx = make_float2(0.f, 0.f);
+        pairs_of<T>(xr, x);
+        pairs_of<T>(gr, g);
+        pairs_of<T>(other_of<L, kTurn == kSideBySide>(gr, other), z);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          g[e] = f2fma(z[e], make_float2(-s[e].x, -s[e].y), f2mul(g[e], c[e]));     // rotated back
+          z[e] = f2mul(g[e], x[e]);
+          sq = f2fma(x[e], x[e], sq);
+          hx = f2fma(z[e], w[e], hx);
+        }
+        const float r = rsqrtf(group_sum<L>(sq.x + sq.y) * (1.f / D) + p.eps);
+        const float k = group_sum<L>(hx.x + hx.y) * (-1.f / D) * r * r * r;
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            dw[e] = f2fma(z[e], make_float2(r, r), dw[e]);
+            x[e] = f2fma(x[e], make_float2(k, k), f2mul(f2mul(g[e], w[e]), make_float2(r, r)));
+          }
+          store_pairs(out, x);
+        }
+      } else {
+        float x[8], g[8], z[8], sq = 0.f, hx = 0.f;
+        widen<T>(xr, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sq = fmaf(x[e], x[e], sq);
+        const float r = rsqrtf(group_sum<L>(sq) * (1.f / D) + p.eps);
+        auto one_of = [](const float2& v, int e) { return e & 1 ? v.y : v.x; };
+        if constexpr (!kBackward) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * r * one_of(w[e >> 1], e);
+          partners<D>(p, lane, x, z, rows[kWhole ? 0 : group]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * one_of(c[e >> 1], e) + z[e] * one_of(s[e >> 1], e);
+        } else {
+          widen<T>(gr, g);
+          partners<D>(p, lane, g, z, rows[kWhole ? 0 : group]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            g[e] = g[e] * one_of(c[e >> 1], e) - z[e] * one_of(s[e >> 1], e);      // rotated back
+            hx = fmaf(g[e] * one_of(w[e >> 1], e), x[e], hx);
+          }
+          const float mean = group_sum<L>(hx) * (1.f / D) * r;                     // of h x r
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float unit = x[e] * r, gu = live ? g[e] * unit : 0.f;
+            if (e & 1) dw[e >> 1].y = live ? dw[e >> 1].y + gu : dw[e >> 1].y;
+            else dw[e >> 1].x = live ? dw[e >> 1].x + gu : dw[e >> 1].x;
+            x[e] = r * (g[e] * one_of(w[e >> 1], e) - unit * mean);
+          }
+        }
+        if (live) store8(out, x);
+      }
+      // on to the next head
+      if (step + 1 < mine) {
+        out += oh;
+        if (++h == heads) {
+          h = 0;
+          if (++t == p.seqlen) {
+            t = 0;
+            ++b;
+          }
+          out = static_cast<T*>(a.out) + b * a.os[0] + t * a.os[1] + d;
+          turn_to(fresh ? position_of(b, t) : next_pos);
+          fresh = true;
+        } else if (kWhole && fresh && h + 4 >= heads && mine - step - 1 > heads - h) {
+          const bool end = t + 1 == p.seqlen;
+          next_pos = position_of(b + end, end ? 0 : t + 1);
+          fresh = false;
+          prefetch_angles(p, next_pos, d, entry);
+        }
+      }
+      __syncwarp();
+    }
+    cp_async_wait<0>();
+    if (!kBackward || ws == nullptr) continue;
+    // over the ring: every group's sums, 8 KB
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(sums + group * D + d + 2 * e) = dw[e];
+    __syncthreads();
+    for (int i = tid; i < D; i += kThreads) {
+      float sum = 0.f;
+      for (int g = 0; g < G; ++g) sum += sums[g * D + i];
+      ws[((int64_t)which * gridDim.x + blockIdx.x) * D + i] = sum;
+    }
+    __syncthreads();
   }
 }
 
@@ -262,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_dw_kernel(const float* ws, i
   const int i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (i >= 2 * D) return;
   float sum = 0.f;
-  for (int c = lane; c < ctas; c += 32) sum += ws[(int64_t)c * 2 * D + i];
+  for (int c = lane; c < ctas; c += 32) sum += ws[((int64_t)(i / D) * ctas + c) * D + i % D];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   void* out = i < D ? dq : dk;
@@ -271,34 +474,46 @@ __global__ void __launch_bounds__(kThreads) qk_norm_dw_kernel(const float* ws, i
   else static_cast<T*>(out)[i % D] = narrow<T>(sum);
 }
 
-constexpr int kBwdPerSm = 4;
-
-Cut cut_of(const fa_qk_norm_args& a) {
-  const int heads = a.heads_q + a.heads_kv, groups = kThreads / (a.head_dim / 8);
-  const int64_t tokens = (int64_t)a.batch * a.seqlen;
-  // eight heads of a token, fewer while that leaves SMs idle
-  Cut c;
-  c.heads = 8;
-  while (c.heads > 1 && tokens * ((heads + c.heads - 1) / c.heads) < (int64_t)groups * 2 * sm_count(a.device)) c.heads /= 2;
-  c.chunks = (heads + c.heads - 1) / c.heads;
-  c.items = tokens * c.chunks;
-  return c;
-}
-
-int grid_of(const fa_qk_norm_args& a, const Cut& c, int per_sm) {
-  const int64_t groups = kThreads / (a.head_dim / 8), need = (c.items + groups - 1) / groups, fit = (int64_t)per_sm * sm_count(a.device);
+// As many CTAs as run at a time, fewer where there is not a head for every group of lanes.
+int grid_of(const fa_qk_norm_args& a, bool backward) {
+  const int groups = kThreads / (a.head_dim / 8);
+  const int64_t need = ((int64_t)a.batch * a.seqlen * std::max(a.heads_q, a.heads_kv) + groups - 1) / groups, fit = (backward ? 2ll : 3ll) * sm_count(a.device);
   return (int)(need < fit ? need : fit);
+}
+// The 8 elements of a lane are turned as one: see angles().
+bool whole_lanes(const fa_qk_norm_args& a) {
+  const int half = a.rotary_dim / 2;
+  return half % (a.interleaved ? 4 : 8) == 0 && ((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15) == 0 &&
+         (a.dtype != FA_F32 || a.table_wide);
 }
 
 template <typename T, int D> int run(const fa_qk_norm_args& a, bool backward, cudaStream_t st) {
-  const Cut c = cut_of(a);
+  Sides sides = {};
+  for (int i = 0; i < 2; ++i) {
+    Side& s = sides.side[i];
+    s.heads = i ? a.heads_kv : a.heads_q;
+    s.x = i ? a.k : a.q;
+    s.g = i ? a.d_ko : a.d_qo;
+    s.out = backward ? (i ? a.d_k : a.d_q) : (i ? a.k_out : a.q_out);
+    s.weight = i ? a.k_weight : a.q_weight;
+    for (int d = 0; d < 3; ++d) {
+      s.xs[d] = (i ? a.k_stride : a.q_stride)[d];
+      s.gs[d] = (i ? a.d_ko_stride : a.d_qo_stride)[d];
+      s.os[d] = backward ? (i ? a.d_k_stride : a.d_q_stride)[d] : (i ? a.ko_stride : a.qo_stride)[d];
+    }
+  }
+  const bool whole = whole_lanes(a);
+  const int grid = grid_of(a, backward);
   if (!backward) {
-    qk_norm_kernel<T, D><<<grid_of(a, c, 64), kThreads, 0, st>>>(a, c);
+    if (!whole) qk_norm_kernel<T, D, false, kAnyhow><<<grid, kThreads, 0, st>>>(a, sides, nullptr);
+    else if (a.interleaved) qk_norm_kernel<T, D, false, kSideBySide><<<grid, kThreads, 0, st>>>(a, sides, nullptr);
+    else qk_norm_kernel<T, D, false, kHalves><<<grid, kThreads, 0, st>>>(a, sides, nullptr);
     return check_launch("qk_norm");
   }
-  const int grid = grid_of(a, c, kBwdPerSm);
   float* ws = a.d_q_weight || a.d_k_weight ? static_cast<float*>(a.workspace) : nullptr;
-  qk_norm_bwd_kernel<T, D><<<grid, kThreads, 0, st>>>(a, c, ws);
+  if (!whole) qk_norm_kernel<T, D, true, kAnyhow><<<grid, kThreads, 0, st>>>(a, sides, ws);
+  else if (a.interleaved) qk_norm_kernel<T, D, true, kSideBySide><<<grid, kThreads, 0, st>>>(a, sides, ws);
+  else qk_norm_kernel<T, D, true, kHalves><<<grid, kThreads, 0, st>>>(a, sides, ws);
   if (int r = check_launch("qk_norm_bwd")) return r;
   if (ws == nullptr) return FA_OK;
   qk_norm_dw_kernel<T><<<2 * D / (kThreads / 32), kThreads, 0, st>>>(ws, grid, D, a.d_q_weight, a.d_k_weight, a.weight_wide);
@@ -319,7 +534,7 @@ template <typename T> int run_dim(const fa_qk_norm_args& a, bool backward, cudaS
 
 size_t qk_norm_bwd_workspace_bytes(const fa_qk_norm_args& a) {
   if ((int64_t)a.batch * a.seqlen == 0) return 0;
-  return (size_t)grid_of(a, cut_of(a), kBwdPerSm) * 2 * a.head_dim * sizeof(float);
+  return (size_t)grid_of(a, true) * 2 * a.head_dim * sizeof(float);
 }
 
 int qk_norm(const fa_qk_norm_args& a, bool backward, cudaStream_t st) {

@@ -7,9 +7,10 @@
 //   Sums and products are in 64 bits: a decision next to a border then depends on the order of a sum only within 1e-16 of it.
 //   Bound.  Latency for small batches, else 2 vocab words a request out of HBM and the conversions to 64 bits.
 //   A cluster of CTAs has a request.  Each loads all nodes' numbers at once and walks the tree on its own (ballots over 32 nodes), so
-//   that the walk takes no round trip to memory; a warp has an even, contiguous share of the vocabulary, its sums go to all CTAs of the cluster
-//   through distributed shared memory, and every warp adds them up in the same order.  The warp whose share the random number falls
-//   into reads that share again.
+//   that the walk takes no round trip to memory.  The node at hand stays in shared memory where it fits (kCached), for the passes after the
+//   first: those of a request come one behind the other, and the request with the most of them sets the time.  A warp has an even, contiguous share of the vocabulary, its sums go to all CTAs of the cluster
+//   through distributed shared memory, and every warp adds them up in the same order.  The share that the random number falls into is
+//   cut among the warps of its CTA in the same way, and one of them finds the token.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -22,7 +23,6 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kNodes = 1024;
 constexpr int kMaxCluster = 8;
 
 template <typename T> __device__ __forceinline__ float wide(T x);
@@ -32,11 +32,48 @@ template <> __device__ __forceinline__ float wide(float x) { return x; }
 
 __device__ __forceinline__ double left_of(double p, double q, double c) { return fmax(fma(-c, q, p), 0.0); }
 
-struct Shared {
-  float p[kNodes], q[kNodes], u[kNodes];   // of a node: target and draft at its parent, its random number
-  int parent[kNodes];
-  double part[2][kMaxCluster * kWarps];    // sums of all warps of the cluster, of one pass and the next
+// Of a node: target and draft at its parent, its random number, its parent or -1.  In dynamic shared memory, ahead of the share of p and q.
+struct Node {
+  float p, q, u;
+  int parent;
 };
+struct Shared {
+  double part[2][kMaxCluster * kWarps];    // sums of all warps of the cluster, of one pass and the next
+  double cut[kWarps];                      // of the warps' parts of one share
+};
+
+// Where `bound` falls among n sums in a row, the first of them preceded by `run`: the first one that reaches beyond it, else the last that
+// holds anything (-1: none does); *before: what comes ahead of it.  By a warp, the same for each lane.
+__device__ __forceinline__ int place_of(const double* part, int n, double bound, double run, int lane, double* before) {
+  const int per = (n + 31) / 32, i0 = min(n, lane * per), i1 = min(n, i0 + per);
+  double mine = 0.0;
+  for (int i = i0; i < i1; ++i) mine += part[i];
+  double inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  run += inc - mine;
+  int at = -1, last = -1;
+  double at_before = 0.0, last_before = 0.0;
+  for (int i = i0; i < i1; ++i) {
+    if (part[i] > 0.0) {
+      last = i;
+      last_before = run;
+      if (at < 0 && run + part[i] > bound) {
+        at = i;
+        at_before = run;
+      }
+    }
+    run += part[i];
+  }
+  const unsigned found = __ballot_sync(0xffffffffu, at >= 0), some = __ballot_sync(0xffffffffu, last >= 0);
+  if (some == 0u) return -1;
+  const int src = found ? __ffs(found) - 1 : 31 - __clz(some);
+  *before = __shfl_sync(0xffffffffu, found ? at_before : last_before, src);
+  return __shfl_sync(0xffffffffu, found ? at : last, src);
+}
 
 // NaN where an argument of max() is: fmax() would drop it.
 __device__ __forceinline__ double rest_of(float p, float q, double c) {
@@ -44,8 +81,30 @@ __device__ __forceinline__ double rest_of(float p, float q, double c) {
   return r > 0.0 ? r : (r == r ? 0.0 : r);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const fa_verify_args a) {
+// Sum of what is left over [v0, v1), by a warp; kAtOnce numbers of a lane are in flight together.
+constexpr int kAtOnce = 8;
+template <typename F>
+__device__ __forceinline__ double share_sum(F at, int64_t v0, int64_t v1, double c, int lane) {
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int64_t v = v0 + lane; v < v1; v += 32 * kAtOnce) {
+    float2 x[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) x[k] = v + 32 * k < v1 ? at(v + 32 * k) : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) s[k & 3] += rest_of(x[k].x, x[k].y, c);
+  }
+  double sum = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// kCached: the CTA's share of p and q at one node lies in dynamic shared memory.
+template <typename T, bool kCached>
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_args a) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  Node* nodes = reinterpret_cast<Node*>(dynamic);
+  float2* held = reinterpret_cast<float2*>(nodes + a.nodes);
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -61,30 +120,28 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const fa_verify_args a
       p = wide(target[parent * a.target_stride[1] + token]);
       q = wide(draft[parent * a.draft_stride[1] + token]);
     }
-    sh.parent[i] = used ? parent : -1;
-    sh.p[i] = p;
-    sh.q[i] = q;
-    sh.u[i] = a.accept[(int64_t)b * a.nodes + i];
+    nodes[i] = Node{p, q, a.accept[(int64_t)b * a.nodes + i], used ? parent : -1};
   }
   cluster.sync();                          // all of its CTAs run: their shared memory may be written
 
   // this warp's share of the vocabulary
   const int slots = C * kWarps, slot = rank * kWarps + warp;
   const int64_t v0 = a.vocab * slot / slots, v1 = a.vocab * (slot + 1) / slots;
-  int pass = 0;
-  // Sums of max(p - c q, 0) over the shares at `node`: in part[.] of every CTA.
-  auto sums = [&](int node, double c) -> const double* {
+  const int64_t c0 = a.vocab * (rank * kWarps) / slots;          // of the CTA
+  int pass = 0, holds = -1;                                    // holds: the node that is in shared memory
+  // p and q at `node` (q is not read where nothing of it is taken off: it is 0 then)
+  auto with_node = [&](int node, double c, auto use) {
     const T* pr = target + node * a.target_stride[1];
     const T* qr = draft + node * a.draft_stride[1];
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int64_t v = v0 + lane; v < v1; v += 128) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (v + 32 * k < v1) s[k] += rest_of(wide(pr[v + 32 * k]), c != 0.0 ? wide(qr[v + 32 * k]) : 0.f, c);
-    }
-    double sum = (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (kCached && holds == node && c != 0.0) return use([&](int64_t v) { return held[v - c0]; });
+    if (c == 0.0) return use([&](int64_t v) { return make_float2(wide(pr[v]), 0.f); });
+    if (!kCached) return use([&](int64_t v) { return make_float2(wide(pr[v]), wide(qr[v])); });
+    holds = node;
+    return use([&](int64_t v) { return held[v - c0] = make_float2(wide(pr[v]), wide(qr[v])); });
+  };
+  // Sums of max(p - c q, 0) over the shares at `node`: in part[.] of every CTA.
+  auto sums = [&](int node, double c) -> const double* {
+    const double sum = with_node(node, c, [&](auto at) { return share_sum(at, v0, v1, c, lane); });
     double* mine = sh.part[pass & 1];
     ++pass;
     if (lane < C) *cluster.map_shared_rank(mine + slot, lane) = sum;
@@ -109,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const fa_verify_args a
   for (int i0 = 0; i0 < a.nodes; i0 += 32) {
     int from = 0;                                // of these 32, those still to be looked at
     for (;;) {
-      const bool child = i0 + lane < a.nodes && lane >= from && sh.parent[i0 + lane] == node;
+      const bool child = i0 + lane < a.nodes && lane >= from && nodes[i0 + lane].parent == node;
       const unsigned any = __ballot_sync(0xffffffffu, child);
       if (any == 0u) break;
       const int i = i0 + __ffs(any) - 1;
@@ -118,8 +175,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const fa_verify_args a
         mass = total_of(sums(node, c));
         fresh = true;
       }
-      const double p = sh.p[i], q = sh.q[i];
-      if ((double)sh.u[i] * q * mass < left_of(p, q, c)) {
+      const double p = nodes[i].p, q = nodes[i].q;
+      if ((double)nodes[i].u * q * mass < left_of(p, q, c)) {
         node = i;
         c = 0.0;
         mass = 1.0;
@@ -148,55 +205,50 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const fa_verify_args a
     if (rank == 0 && tid == 0) a.next_token[b] = -1;
     return;
   }
-  // the first share whose running sum exceeds the bound, else the last one that holds anything
   const double bound = (double)a.sample[b] * sum;
-  double run = 0.0, before = 0.0, last_before = 0.0;
-  int at = -1, last = -1;
-  for (int i = 0; i < slots && at < 0; ++i) {
-    const double x = part[i];
-    if (x > 0.0) {
-      last = i;
-      last_before = run;
-    }
-    if (x > 0.0 && run + x > bound) {
-      at = i;
-      before = run;
-    }
-    run += x;
-  }
-  if (at < 0) {
-    at = last;
-    before = last_before;
-  }
-  if (at != slot) return;
-  const T* pr = target + node * a.target_stride[1];
-  const T* qr = draft + node * a.draft_stride[1];
-  int64_t token = -1, positive = -1;
-  run = before;
-  for (int64_t v = v0; v < v1; v += 32) {
-    const double r = v + lane < v1 ? rest_of(wide(pr[v + lane]), c != 0.0 ? wide(qr[v + lane]) : 0.f, c) : 0.0;
-    double s = r;
+  double run = 0.0;
+  const int at = place_of(part, slots, bound, 0.0, lane, &run);
+  if (at / kWarps != rank) return;
+  // that share, [w0, w1), in the CTA that has it: a part of it for each warp
+  const int64_t w0 = a.vocab * at / slots, w1 = a.vocab * (at + 1) / slots, n = w1 - w0;
+  const int64_t u0 = w0 + n * warp / kWarps, u1 = w0 + n * (warp + 1) / kWarps;
+  __syncthreads();                               // (one warp's share in shared memory, read by all)
+  const double mine = with_node(node, c, [&](auto at) { return share_sum(at, u0, u1, c, lane); });
+  if (lane == 0) sh.cut[warp] = mine;
+  __syncthreads();
+  if (place_of(sh.cut, kWarps, bound, run, lane, &run) != warp) return;
+  const int64_t token = with_node(node, c, [&](auto at) {
+    int64_t positive = -1;
+    double before = run;
+    for (int64_t v = u0; v < u1; v += 32) {
+      const float2 x = v + lane < u1 ? at(v + lane) : make_float2(0.f, 0.f);
+      const double r = rest_of(x.x, x.y, c);
+      double s = r;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += x;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && before + s > bound), some = __ballot_sync(0xffffffffu, r > 0.0);
+      if (some) positive = v + 31 - __clz(some);
+      if (over) return v + __ffs(over) - 1;
+      before += __shfl_sync(0xffffffffu, s, 31);
     }
-    const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && run + s > bound), some = __ballot_sync(0xffffffffu, r > 0.0);
-    if (some) positive = v + 31 - __clz(some);
-    if (over) {
-      token = v + __ffs(over) - 1;
-      break;
-    }
-    run += __shfl_sync(0xffffffffu, s, 31);
-  }
-  if (lane == 0) a.next_token[b] = token >= 0 ? token : positive;
+    return positive;
+  });
+  if (lane == 0) a.next_token[b] = token;
 }
 
-template <typename T>
-int launch_verify(const fa_verify_args& a, cudaStream_t st) {
-  // shares of a few hundred tokens at least
-  int cluster = 1;
-  while (cluster < kMaxCluster && a.vocab > (int64_t)cluster * kThreads * 4) cluster *= 2;
+template <typename T, bool kCached>
+int launch(const fa_verify_args& a, int cluster, size_t smem, cudaStream_t st) {
+  auto kern = verify_kernel<T, kCached>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+      set_error("verify_draft_tree: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      return FA_ERR_LAUNCH;
+    }
+  }
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -204,11 +256,23 @@ int launch_verify(const fa_verify_args& a, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   lc.gridDim = dim3((unsigned)a.batch * cluster);
   lc.blockDim = dim3(kThreads);
+  lc.dynamicSmemBytes = smem;
   lc.stream = st;
   lc.attrs = &attr;
   lc.numAttrs = 1;
-  cudaLaunchKernelEx(&lc, verify_kernel<T>, a);
+  cudaLaunchKernelEx(&lc, kern, a);
   return check_launch("verify_draft_tree");
+}
+
+template <typename T>
+int launch_verify(const fa_verify_args& a, cudaStream_t st) {
+  // shares of a few hundred tokens at least
+  int cluster = 1;
+  while (cluster < kMaxCluster && a.vocab > (int64_t)cluster * kThreads * 4) cluster *= 2;
+  // a CTA's share in shared memory, beside another CTA's, or alone on its SM where there are no more CTAs than SMs
+  const size_t nodes = a.nodes * sizeof(Node), all = nodes + ((size_t)a.vocab / cluster + kWarps) * sizeof(float2);
+  const size_t room = ((int64_t)a.batch * cluster <= sm_count(a.device) ? 224 : 110) * 1024;
+  return all <= room ? launch<T, true>(a, cluster, all, st) : launch<T, false>(a, cluster, nodes, st);
 }
 
 }  // namespace
