@@ -73,10 +73,49 @@ __device__ __forceinline__ void answer(uint32_t* host, uint32_t bad) {
   __threadfence_system();
 }
 
+// Of all requests, ahead of the kernel that moves: a step of a path per thread, the reads of kAtOnce of them in flight together.
 __global__ void __launch_bounds__(1024) compact_check_kernel(const fa_compact_args p, int shift, uint32_t* host, uint32_t* dev) {
-  // a warp has a request
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int kAtOnce = 4;
+  const int64_t cap = capacity_of(p), all = (int64_t)p.batch * p.path_len;
   uint32_t bad = 0;
-  for (int b = threadIdx.x >> 5; b < p.batch; b += 32) bad |= request_checks(p, shift, b, threadIdx.x & 31, 32);
+  for (int b = threadIdx.x; b < p.batch; b += 1024) {
+    const int n = p.num_accepted[b], row = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
+    if (n < 0 || n > p.path_len) bad |= FA_COMPACT_COUNT;
+    if (p.cache_seqlens[b] < 0 || (p.cache_leftpad && p.cache_leftpad[b] < 0)) bad |= FA_COMPACT_LENGTHS;
+    if (p.block_table == nullptr && (unsigned)row >= (unsigned)p.num_pages) bad |= FA_COMPACT_PAGES;
+  }
+  for (int64_t i0 = threadIdx.x; i0 < all; i0 += 1024 * kAtOnce) {
+    int x[kAtOnce], before[kAtOnce], page[2 * kAtOnce];
+    int64_t len[kAtOnce];
+    bool in[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t at = min(i0 + k * 1024, all - 1);
+      const int b = (int)(at / p.path_len), i = (int)(at - (int64_t)b * p.path_len);
+      const int32_t* path = p.path + (int64_t)b * p.path_stride;
+      in[k] = i0 + k * 1024 < all && i < min(p.num_accepted[b], p.path_len);
+      len[k] = max((int64_t)p.cache_seqlens[b] + (p.cache_leftpad ? p.cache_leftpad[b] : 0), (int64_t)0);
+      x[k] = path[i];
+      before[k] = i > 0 ? path[i - 1] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t at = min(i0 + k * 1024, all - 1);
+      const int b = (int)(at / p.path_len), i = (int)(at - (int64_t)b * p.path_len);
+      const int64_t from = len[k] + x[k], to = len[k] + i;
+      if (in[k] && (x[k] <= before[k] || x[k] < 0)) bad |= FA_COMPACT_PATH;
+      in[k] = in[k] && x[k] > before[k] && x[k] >= 0;
+      if (in[k] && (from >= cap || to >= cap)) bad |= FA_COMPACT_LENGTHS;
+      in[k] = in[k] && from < cap && to < cap;
+      const int32_t* table = p.block_table ? p.block_table + (int64_t)b * p.block_table_stride : nullptr;
+      page[2 * k] = table && in[k] ? table[page_index(p, shift, from)] : 0;
+      page[2 * k + 1] = table && in[k] ? table[page_index(p, shift, to)] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 2 * kAtOnce; ++k)
+      if (p.block_table && in[k / 2] && (unsigned)page[k] >= (unsigned)p.num_pages) bad |= FA_COMPACT_PAGES;
+  }
   bad = all_of(bad);
   if (threadIdx.x == 0) {
     *dev = bad;
@@ -95,8 +134,9 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const fa_compact_args
     bad = all_of(bad);
     if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) answer(host, bad);
     if (bad) return;
-  } else if (dev && *dev) {
-    return;
+  } else if (dev) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");         // the kernel with the checks may still run
+    if (*dev) return;
   }
   const int tensor = blockIdx.x / stripes, stripe = blockIdx.x - tensor * stripes;
   const int which = tensor & 1, layer = tensor >> 1;
@@ -162,7 +202,18 @@ int launch_compact(const fa_compact_args& a, uint32_t* host, const uint32_t* dev
   }
   const int stripes = (a.heads * (a.head_dim / 8) + kThreads - 1) / kThreads;
   const dim3 grid((unsigned)(2 * a.layers * stripes), (unsigned)(a.batch < 65535 ? a.batch : 65535));
-  compact_kernel<<<grid, kThreads, 0, st>>>(a, l, shift_of(a.page_size), stripes, host, dev);
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute attr;
+  lc.gridDim = grid;
+  lc.blockDim = dim3(kThreads);
+  lc.stream = st;
+  if (dev) {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = &attr;
+    lc.numAttrs = 1;
+  }
+  cudaLaunchKernelEx(&lc, compact_kernel, a, l, shift_of(a.page_size), stripes, host, dev);
   return check_launch("compact");
 }
 
@@ -210,10 +261,12 @@ int compact_checked(const fa_compact_args& a, uint32_t* failed, cudaStream_t st)
 namespace {
 
 constexpr int kPageThreads = 256;
+constexpr int kFirsts = 4096;          // requests whose first pages are held in shared memory, and found by one bisection
+constexpr int kPagesOfThread = 4;      // one behind the other
 
 __global__ void __launch_bounds__(kPageThreads) release_kernel(const fa_release_args p, int shift, uint32_t* host) {
   __shared__ int64_t warps[kPageThreads / 32];
-  __shared__ int first[kPageThreads];
+  __shared__ int first[kPageThreads], begins[kFirsts];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto pages_of = [&](int64_t n) { return shift >= 0 ? (n + p.page_size - 1) >> shift : (n + p.page_size - 1) / p.page_size; };
   const int per = (p.batch + kPageThreads - 1) / kPageThreads;
@@ -261,29 +314,59 @@ __global__ void __launch_bounds__(kPageThreads) release_kernel(const fa_release_
   }
   first[tid] = (int)before;            // (a sum that passed the checks is below 2^31)
   __syncthreads();
-  for (int64_t i = from; i < p.num_pages; i += step) {
-    int page = -1;
-    if (i < all) {
-      int s = 0;                       // last stretch of requests with first[s] <= i
+  const bool held = p.batch <= kFirsts;
+  if (held) {
+    int at = (int)before;
+    for (int b = b0; b < b1; ++b) {
+      begins[b] = at;
+      at += (int)(pages_of(p.held_lens[b]) - pages_of(p.kept_lens[b]));
+    }
+    __syncthreads();
+  }
+  int log2 = 1;
+  while (held && log2 < p.batch) log2 <<= 1;
+  for (int64_t i0 = from * kPagesOfThread; i0 < p.num_pages; i0 += step * kPagesOfThread) {
+    int page[kPagesOfThread], b = 0, left = 0;
+    if (i0 < all) {
+      if (held) {                      // last request that begins at i0 or before
+        for (int k = log2 >> 1; k > 0; k >>= 1)
+          if (b + k < p.batch && begins[b + k] <= (int)i0) b += k;
+        left = (int)i0 - begins[b];
+      } else {
+        int s = 0;                     // last stretch of requests that does
 #pragma unroll
-      for (int k = kPageThreads / 2; k > 0; k >>= 1)
-        if (first[s + k] <= (int)i) s += k;
-      int left = (int)i - first[s];
-      for (int b = s * per;; ++b) {
-        const int keep = (int)pages_of(p.kept_lens[b]), gone = (int)pages_of(p.held_lens[b]) - keep;
-        if (left < gone) {
-          page = p.block_table[(int64_t)b * p.table_stride + keep + left];
-          break;
-        }
-        left -= gone;
+        for (int k = kPageThreads / 2; k > 0; k >>= 1)
+          if (first[s + k] <= (int)i0) s += k;
+        b = s * per;
+        left = (int)i0 - first[s];
       }
     }
-    p.pages[i] = page;
+#pragma unroll
+    for (int e = 0; e < kPagesOfThread; ++e) {
+      page[e] = -1;
+      if (i0 + e < all) {
+        int keep, gone;
+        for (;; ++b, left -= gone) {
+          keep = (int)pages_of(p.kept_lens[b]);
+          gone = (int)pages_of(p.held_lens[b]) - keep;
+          if (left < gone) break;
+        }
+        page[e] = p.block_table[(int64_t)b * p.table_stride + keep + left];
+        ++left;
+      }
+    }
+    if ((reinterpret_cast<uintptr_t>(p.pages) & 15) == 0 && i0 + kPagesOfThread <= p.num_pages) {
+      *reinterpret_cast<int4*>(p.pages + i0) = make_int4(page[0], page[1], page[2], page[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPagesOfThread; ++e)
+        if (i0 + e < p.num_pages) p.pages[i0 + e] = page[e];
+    }
   }
 }
 
 int launch_release(const fa_release_args& a, uint32_t* host, cudaStream_t st) {
-  const int64_t need = ((int64_t)a.num_pages + kPageThreads - 1) / kPageThreads, fit = 4ll * sm_count(a.device);
+  const int64_t need = ((int64_t)a.num_pages + kPageThreads * kPagesOfThread - 1) / (kPageThreads * kPagesOfThread), fit = 4ll * sm_count(a.device);
   const unsigned grid = (unsigned)(need < 1 ? 1 : need < fit ? need : fit);
   release_kernel<<<grid, kPageThreads, 0, st>>>(a, shift_of(a.page_size), host);
   return check_launch("release_pages");

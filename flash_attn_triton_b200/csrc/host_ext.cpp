@@ -990,6 +990,37 @@ PyObject* py_verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// caches_match([k_cache], [v_cache]) -> 0, or what differs among the caches: 1 shapes, 2 types, 3 strides (of keys, of values), 4 an address
+// that the kernels cannot read at, 5 devices, 6 the same cache twice.  (In Python this took a call over 48 caches 60 us.)
+PyObject* py_caches_match(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a{args, n};
+  std::vector<const void*> seen;
+  const Tensor* first = nullptr;
+  for (int w = 0; w < 2; ++w) {
+    PyObject* list = a.next();
+    TORCH_CHECK_TYPE(PyList_Check(list), "expected a list of tensors");
+    const Tensor* of_list = nullptr;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+      PyObject* o = PyList_GET_ITEM(list, i);
+      TORCH_CHECK_TYPE(THPVariable_Check(o), "expected a tensor");
+      const Tensor& t = THPVariable_Unpack(o);
+      if (first == nullptr) first = &t;
+      if (of_list == nullptr) of_list = &t;
+      if (t.sizes() != first->sizes()) return PyLong_FromLong(1);
+      if (t.scalar_type() != first->scalar_type()) return PyLong_FromLong(2);
+      if (t.strides() != of_list->strides()) return PyLong_FromLong(3);
+      if (!kernel_ready(t)) return PyLong_FromLong(4);
+      if (t.device() != first->device()) return PyLong_FromLong(5);
+      seen.push_back(t.data_ptr());
+    }
+  }
+  std::sort(seen.begin(), seen.end());
+  const bool twice = first != nullptr && first->numel() > 0 && std::adjacent_find(seen.begin(), seen.end()) != seen.end();
+  return PyLong_FromLong(twice ? 6 : 0);
+  END_HANDLE_TH_ERRORS
+}
+
 // compact([k_cache], [v_cache], seqlens, path, num_accepted, block_table, batch_idx, leftpad, checks) -> the mask of the value checks that failed
 PyObject* py_compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1199,6 +1230,48 @@ struct QkNormBackward : public Node {
   }
 };
 
+// What a call is refused for: here and not in Python, where it took as long as the rest of a decoding step's call (6 us).
+void check_norm(const NormCall& c) {
+  const auto q = c.q.sizes(), k = c.k.sizes();
+  const size_t dims = q.size();
+  TORCH_CHECK_VALUE((dims == 3 || dims == 4) && k.size() == dims && q[0] == k[0] && (dims == 3 || q[1] == k[1]) && q[dims - 1] == k[dims - 1],
+                    "q and k must have shape (batch, seqlen, heads, headdim) or (tokens, heads, headdim)");
+  const auto type = c.q.scalar_type();
+  TORCH_CHECK_VALUE((type == at::kHalf || type == at::kBFloat16 || type == at::kFloat) && c.k.scalar_type() == type,
+                    "qk_norm_rotary supports matching FP16, BF16 or FP32 tensors");
+  const int64_t dim = q[dims - 1];
+  TORCH_CHECK_VALUE(dim == 16 || dim == 32 || dim == 64 || dim == 128 || dim == 256, "head dimension must be one of 16, 32, 64, 128, or 256");
+  TORCH_CHECK_VALUE(q[dims - 2] > 0 && k[dims - 2] > 0, "q and k need at least one head");
+  const Tensor* first = nullptr;
+  for (const Tensor* w : {&c.q_weight, &c.k_weight}) {
+    if (!w->defined()) continue;
+    if (first == nullptr) first = w;
+    TORCH_CHECK_VALUE(w->dim() == 1 && w->size(0) == dim && (w->scalar_type() == type || w->scalar_type() == at::kFloat) &&
+                          w->scalar_type() == first->scalar_type(),
+                      "the weights must have shape (headdim,) and both the dtype of q and k, or both FP32");
+  }
+  TORCH_CHECK_VALUE(c.cos.defined() == c.sin.defined(), "rotary_cos and rotary_sin must be supplied together");
+  if (c.cos.defined()) {
+    TORCH_CHECK_VALUE(c.cos.dim() == 2 && c.cos.sizes() == c.sin.sizes(), "rotary_cos and rotary_sin must be (seqlen_ro, rotary_dim / 2)");
+    TORCH_CHECK_VALUE(c.cos.size(1) * 2 <= dim, "rotary tables exceed the head dimension");
+    TORCH_CHECK_VALUE((c.cos.scalar_type() == type || c.cos.scalar_type() == at::kFloat) && c.sin.scalar_type() == c.cos.scalar_type(),
+                      "the rotary tables must both have the dtype of q and k, or both FP32");
+    TORCH_CHECK_VALUE(!c.cos.requires_grad() && !c.sin.requires_grad(),
+                      "gradients of the rotary tables are not produced; pass tensors that do not require grad");
+  }
+  if (c.positions.defined()) {
+    const auto p = c.positions.sizes();
+    TORCH_CHECK_VALUE(c.positions.scalar_type() == at::kInt || c.positions.scalar_type() == at::kLong, "positions must use int32 or int64");
+    const int64_t tokens = dims == 3 ? q[0] : q[1];
+    TORCH_CHECK_VALUE((p.size() == 1 && p[0] == tokens) || (dims == 4 && p.size() == 2 && (p[0] == q[0] || p[0] == 1) && p[1] == tokens),
+                      "positions must have one value per token: (batch, seqlen), (seqlen,) or, packed, (tokens,)");
+  }
+  TORCH_CHECK_VALUE(c.eps >= 0.0, "eps must be non-negative");
+  TORCH_CHECK_VALUE(c.q.is_cuda(), "All tensors must be CUDA tensors");
+  for (const Tensor* t : {&c.k, &c.q_weight, &c.k_weight, &c.cos, &c.sin, &c.positions})
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == c.q.device(), "All tensors must be on the same CUDA device");
+}
+
 // qk_norm(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved) -> (q_out, k_out)
 PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1213,6 +1286,7 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   c.positions = a.tensor_or_none();
   c.eps = a.real();
   c.interleaved = a.truth();
+  check_norm(c);
   c10::cuda::CUDAGuard guard(c.q.device());
   variable_list in = {c.q, c.k, c.q_weight, c.k_weight};
   for (const auto& t : in)
@@ -1227,6 +1301,10 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::AutoDispatchBelowADInplaceOrView below;
     c.q = readable(c.q);
     c.k = readable(c.k);
+    for (Tensor* t : {&c.q_weight, &c.k_weight, &c.cos, &c.sin})
+      if (t->defined()) *t = t->contiguous();
+    // (positions that do not fit 32 bits stay outside any table)
+    if (c.positions.defined() && c.positions.scalar_type() == at::kLong) c.positions = c.positions.clamp(INT32_MIN, INT32_MAX).to(at::kInt);
     const auto dev = c.q.device();
     qo = empty_cuda(c.q.sizes(), c.q.scalar_type(), dev);
     ko = empty_cuda(c.k.sizes(), c.k.scalar_type(), dev);
@@ -1321,6 +1399,7 @@ PyMethodDef g_methods[] = {
     {"append8", FAST(py_append8), "packed tokens into an 8-bit KV cache"},
     {"block_table", FAST(py_block_table), "pages, slots and cu_seqlens of a step"},
     {"verify", FAST(py_verify), "verification of drafted tokens"},
+    {"caches_match", FAST(py_caches_match), "whether caches can go into one call"},
     {"compact", FAST(py_compact), "accepted tokens moved together in a KV cache"},
     {"release", FAST(py_release), "pages that are no longer needed"},
     {"qk_norm", FAST(py_qk_norm), "norms of queries and keys with the rotation"},

@@ -16,7 +16,7 @@ import torch
 from . import _native as N
 from . import flash_attn_interface as _api
 
-_NORM_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_PROB_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def _i32(x):
@@ -40,44 +40,8 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, rotary_cos=None, rotary_s
     of q's dtype or both fp32, None for ones; tables (seqlen_ro, rotary_dim / 2) of q's dtype or fp32, None for no rotation.  positions:
     integers, (batch, seqlen) or (seqlen,), packed (tokens,); None for the rows' own numbers.  The tokens of a drafted tree sit at the
     length of the context plus their depth.  A position outside the tables rotates nothing."""
-    if q.ndim not in (3, 4) or k.ndim != q.ndim or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
-        raise ValueError("q and k must have shape (batch, seqlen, heads, headdim) or (tokens, heads, headdim)")
-    if q.dtype not in _NORM_DTYPES or k.dtype != q.dtype:
-        raise ValueError("qk_norm_rotary supports matching FP16, BF16 or FP32 tensors")
-    head_dim = q.shape[-1]
-    _api._check_head_dim(head_dim)
-    if q.shape[-2] == 0 or k.shape[-2] == 0:
-        raise ValueError("q and k need at least one head")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    if any(w.shape != (head_dim,) or w.dtype not in (q.dtype, torch.float32) or w.dtype != weights[0].dtype for w in weights):
-        raise ValueError("the weights must have shape (headdim,) and both the dtype of q and k, or both FP32")
-    if (rotary_cos is None) != (rotary_sin is None):
-        raise ValueError("rotary_cos and rotary_sin must be supplied together")
-    if rotary_cos is not None:
-        if rotary_cos.shape != rotary_sin.shape or rotary_cos.ndim != 2:
-            raise ValueError("rotary_cos and rotary_sin must be (seqlen_ro, rotary_dim / 2)")
-        if rotary_cos.shape[1] * 2 > head_dim:
-            raise ValueError("rotary tables exceed the head dimension")
-        if rotary_cos.dtype not in (q.dtype, torch.float32) or rotary_sin.dtype != rotary_cos.dtype:
-            raise ValueError("the rotary tables must both have the dtype of q and k, or both FP32")
-        if rotary_cos.requires_grad or rotary_sin.requires_grad:
-            raise ValueError("gradients of the rotary tables are not produced; pass tensors that do not require grad")
-    if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64):
-            raise ValueError("positions must use int32 or int64")
-        if not (positions.shape == q.shape[:-2] or (q.ndim == 4 and positions.shape in (q.shape[1:2], (1, q.shape[1])))):
-            raise ValueError("positions must have one value per token: (batch, seqlen), (seqlen,) or, packed, (tokens,)")
-    if not eps >= 0.0:
-        raise ValueError("eps must be non-negative")
     if torch._C._get_tracing_state() is not None:
         raise ValueError("qk_norm_rotary cannot be recorded by torch.jit.trace")
-    _on(q.device, k, q_weight, k_weight, rotary_cos, rotary_sin, positions)
-    if weights:
-        q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    if rotary_cos is not None:
-        rotary_cos, rotary_sin = rotary_cos.contiguous(), rotary_sin.contiguous()
-    if positions is not None:
-        positions = _i32(positions)
     return N.host().qk_norm(q, k, q_weight, k_weight, rotary_cos, rotary_sin, positions, eps, rotary_interleaved)
 
 
@@ -99,7 +63,7 @@ def verify_draft_tree(draft_tokens, parents, target_probs, draft_probs, accept_u
     A chain of drafts is parents = (-1, 0, 1, ...).  The distributions are taken to sum to 1."""
     if target_probs.ndim != 3 or draft_probs.shape != target_probs.shape:
         raise ValueError("target_probs and draft_probs must have the same shape (batch, nodes, vocab)")
-    if target_probs.dtype not in _NORM_DTYPES or draft_probs.dtype != target_probs.dtype:
+    if target_probs.dtype not in _PROB_DTYPES or draft_probs.dtype != target_probs.dtype:
         raise ValueError("target_probs and draft_probs must be matching FP32, FP16 or BF16 tensors")
     batch, nodes, vocab = target_probs.shape
     if not 1 <= nodes <= 1024:
@@ -130,6 +94,14 @@ _COMPACT_ERRORS = ("num_accepted must be between 0 and the length of a path",
                    "block_table or cache_batch_idx contains an index that does not exist")
 
 
+_CACHES_DIFFER = ("the KV caches must have the same shape (num_pages, page_size, nheads_k, headdim)",
+                  "kvcache_compact supports matching FP16 or BF16 caches",
+                  "the caches of all layers must have the same strides",
+                  "KV caches must have a unit head-dim stride and 16-byte aligned rows",
+                  "All tensors must be on the same CUDA device",
+                  "the KV caches must not overlap")
+
+
 def kvcache_compact(k_cache, v_cache, cache_seqlens, path, num_accepted, block_table=None, cache_batch_idx=None, cache_leftpad=None):
     """Move the rows of accepted tokens together, in place: for i < num_accepted[b], the row at position cache_seqlens[b] + i takes
     what the one at cache_seqlens[b] + path[b, i] holds.  With the path of `verify_draft_tree` and the lengths from before the drafted tokens
@@ -145,18 +117,16 @@ def kvcache_compact(k_cache, v_cache, cache_seqlens, path, num_accepted, block_t
     if not k_caches or len(k_caches) != len(v_caches):
         raise ValueError("k_cache and v_cache must be tensors, or lists of as many tensors")
     first = k_caches[0]
-    if first.ndim != 4 or any(c.shape != first.shape for c in k_caches + v_caches):
+    if first.ndim != 4:
         raise ValueError("the KV caches must have the same shape (num_pages, page_size, nheads_k, headdim)")
-    if first.dtype not in _api._KERNEL_DTYPES or any(c.dtype != first.dtype for c in k_caches + v_caches):
+    if first.dtype not in _api._KERNEL_DTYPES:
         raise ValueError("kvcache_compact supports matching FP16 or BF16 caches")
     _api._check_head_dim(first.shape[3])
     if first.shape[2] == 0:
         raise ValueError("the KV caches need at least one head")
-    for caches in (k_caches, v_caches):
-        if any(c.stride() != caches[0].stride() for c in caches):
-            raise ValueError("the caches of all layers must have the same strides")
-    if not all(N.kernel_ready(c) for c in k_caches + v_caches):
-        raise ValueError("KV caches must have a unit head-dim stride and 16-byte aligned rows")
+    differs = N.host().caches_match(k_caches, v_caches)
+    if differs:
+        raise ValueError(_CACHES_DIFFER[differs - 1])
     if path.ndim != 2 or path.dtype not in (torch.int32, torch.int64):
         raise ValueError("path must have shape (batch, n) and use int32 or int64")
     batch, device = path.shape[0], first.device
@@ -171,15 +141,13 @@ def kvcache_compact(k_cache, v_cache, cache_seqlens, path, num_accepted, block_t
             raise ValueError("cache_batch_idx cannot be combined with paged KV caches")
     elif cache_batch_idx is None and first.shape[0] < batch:
         raise ValueError("cache_batch_idx must contain valid cache-row indices")
-    _on(device, path, *k_caches, *v_caches)
+    _on(device, path)
     lens, accepted, rows, pads = (None if x is None else _api._as_i32(x, device) for x in (cache_seqlens, num_accepted, cache_batch_idx, cache_leftpad))
     for x, name in ((lens, "cache_seqlens"), (accepted, "num_accepted"), (rows, "cache_batch_idx"), (pads, "cache_leftpad")):
         if x is not None and x.numel() != batch:
             raise ValueError(f"{name} must contain one value per request")
     if batch == 0:
         return
-    if len({c.data_ptr() for c in k_caches + v_caches}) != 2 * len(k_caches):
-        raise ValueError("the KV caches must not overlap")
     if block_table is not None:
         block_table = _i32(block_table).to(device).contiguous()
         if block_table.shape[1] == 0:                    # no pages: only paths of nothing are allowed
