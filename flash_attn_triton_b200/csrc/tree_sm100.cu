@@ -18,9 +18,11 @@
 //   warp  17    MMA issuer      : S[j] = Q K_j^T (SS);  O += P_j V_j (A = P_j from tensor memory)
 //   warps 18-19 idle (they complete the warpgroup that gives its registers to the softmax warps)
 //
-// Tensor memory, the reference of the exponents and P in two 16-bit parts: as in fwd_alt_sm100.cu.  Here the tiles of all segments are
-// counted through (J), and barrier parities follow that count.  With two groups of four warps, a tile each, the softmax set the pace, not
-// the memory: 18 x 16384 tokens, 8 KV heads, 254 us also out of L2.  So there are four warps per scheduler.
+// Tensor memory and the reference of the exponents: as in fwd_alt_sm100.cu.  Here the tiles of all segments are counted through (J), and
+// barrier parities follow that count.  What a tile costs beside its bytes counts twice, for the memory and the SMs together reach the limit of
+// the GPU's power, and the clock falls.  18 x 16384 tokens, 64 rows over each of 8 KV heads of 128 (floor 185 us): two groups of four
+// softmax warps, a tile each, 254 us, also out of L2; four warps per scheduler 228; P rounded to 16 bits once and not in two parts, as chunks of
+// a cache have it, and no work on rows that do not exist 185.  (Errors against float64, fp16, 4 to 16 nodes: 2.1e-4 of two parts, 2.6e-4.)
 #include "cache_geo.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
@@ -76,26 +78,21 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, TShared
   return bounded_wait(bar, parity, &sh->abort_flag, &g_tree_status, code);
 }
 // Barrier 1 of the softmax threads: is the predicate set in any of them?
-__device__ __forceinline__ bool any_of_all(bool x) {
+template <int kCount> __device__ __forceinline__ bool any_of_all(bool x) {
   int r;
   asm volatile(
       "{\n"
       ".reg .pred p, q;\n"
       "setp.ne.s32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, 512, p;\n"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n"
       "selp.s32 %0, 1, 0, q;\n"
       "}\n"
-      : "=r"(r) : "r"((int)x) : "memory");
+      : "=r"(r) : "r"((int)x), "n"(kCount) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void sync_all() { asm volatile("bar.sync 1, 512;\n" ::: "memory"); }
+template <int kCount> __device__ __forceinline__ void sync_all() { asm volatile("bar.sync 1, %0;\n" ::"n"(kCount) : "memory"); }
 // The two warps that have the halves of the same rows.
 __device__ __forceinline__ void sync_halves(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
-
-// First of two 16-bit parts of a probability: rounded from a little less, so that the rest is never negative.
-template <typename T> __device__ __forceinline__ float2 first_part(float2 p);
-template <> __device__ __forceinline__ float2 first_part<__half>(float2 p) { return f2mul(p, make_float2(1.f - 0x1p-11f, 1.f - 0x1p-11f)); }
-template <> __device__ __forceinline__ float2 first_part<__nv_bfloat16>(float2 p) { return f2mul(p, make_float2(1.f - 0x1p-8f, 1.f - 0x1p-8f)); }
 
 template <typename T> struct TFmt;
 template <> struct TFmt<__half> { static constexpr int code = 0; };
@@ -150,10 +147,7 @@ __device__ __forceinline__ int ranges_of(int64_t total, int batch, int parts) {
 }  // namespace
 
 // geo.parts: ranges that the grid has room for.
-// kSplit = 2: no more than 64 query rows.  They are in the tile twice, and P has the first 16-bit parts of the probabilities in the first
-// copy and what they leave in the second: one product per 16 keys does for both, where a full tile of rows needs two (1024 cycles of the tensor
-// pipe a tile of keys, not 1536).  The softmax of the second copy is that of the first once more, and at the end of a segment the
-// accumulators are added up.
+// kSplit = 2: no more than 64 query rows.
 template <typename T, int D, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -211,22 +205,27 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int i = 0; i < NB; ++i) {
       mbar_init(smem_u32(&sh->s_full[i]), 1);
       mbar_init(smem_u32(&sh->o_done[i]), 1);
-      mbar_init(smem_u32(&sh->p_ready[0][i]), 128);
-      mbar_init(smem_u32(&sh->p_ready[1][i]), 128);
+      mbar_init(smem_u32(&sh->p_ready[0][i]), 128 / kSplit);
+      mbar_init(smem_u32(&sh->p_ready[1][i]), 128 / kSplit);
     }
     for (int i = 0; i < S; ++i) {
       mbar_init(smem_u32(&sh->kv_full[i]), 1);
       mbar_init(smem_u32(&sh->kv_empty[i]), 1);
     }
-    mbar_init(smem_u32(&sh->decided[0]), 256);
-    mbar_init(smem_u32(&sh->decided[1]), 256);
-    mbar_init(smem_u32(&sh->o_free), kSoftmax);
+    mbar_init(smem_u32(&sh->decided[0]), 256 / kSplit);
+    mbar_init(smem_u32(&sh->decided[1]), 256 / kSplit);
+    mbar_init(smem_u32(&sh->o_free), kSoftmax / kSplit);
     sh->abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 16) {
     tmem_alloc(smem_u32(&sh->tmem_base), 512);
     tmem_relinquish();
+  }
+  if (kSplit > 1) {                                            // rows that do not exist: 0, and so are their scores and probabilities
+    for (int i = tid; i < NQ * (D / 64) * (kBM / 2) * 8; i += kThreads)
+      st_shared_v4(sQ + i / ((kBM / 2) * 8) * (kBM * 128) + (kBM / 2) * 128 + i % ((kBM / 2) * 8) * 16, make_uint4(0u, 0u, 0u, 0u));
+    fence_proxy_async();
   }
   // the append kernel before this one may still run: it writes the cache, the bits of the mask and the result of the checks
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -319,13 +318,9 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               if (segs >= NQ) ok = ok && wait_bar(&sh->q_empty[qb], (segs / NQ - 1) & 1, sh, 15);
               if (ok) {
                 const uint32_t bar = smem_u32(&sh->q_full[qb]);
-                mbar_expect_tx(bar, C::kQBytes);
-                for (int bx = 0; bx < D / 64; ++bx) {
-#pragma unroll
-                  for (int v = 0; v < kSplit; ++v)
-                    tma_load_4d(sQ + qb * C::kQBytes + bx * (kBM * 128) + v * (kBM / kSplit) * 128, &tmQ, bar, bx * 64, h, m0 >> geo.pack_log2,
-                                now.fresh);
-                }
+                mbar_expect_tx(bar, C::kQBytes / kSplit);
+                for (int bx = 0; bx < D / 64; ++bx)
+                  tma_load_4d(sQ + qb * C::kQBytes + bx * (kBM * 128), &tmQ, bar, bx * 64, h, m0 >> geo.pack_log2, now.fresh);
               }
             }
             if (many) ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -414,8 +409,6 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int kk = 0; kk < kBN / 32; ++kk) {
               mma_f16_ts_lp(tmem + C::kOCol + un * C::kUnitCols, a + (kk / 2) * 32 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, kk > 0 ? 1u : fresh, leader);
-              if (kSplit == 1)
-                mma_f16_ts_lp(tmem + C::kOCol + un * C::kUnitCols, a + (kk / 2) * 32 + 16 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, 1u, leader);
             }
           }
           wwait(&sh->p_ready[1][vbuf], par, 26);
@@ -426,8 +419,6 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
             for (int kk = kBN / 32; kk < kBN / 16; ++kk) {
               mma_f16_ts_lp(tmem + C::kOCol + un * C::kUnitCols, a + (kk / 2) * 32 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, 1u, leader);
-              if (kSplit == 1)
-                mma_f16_ts_lp(tmem + C::kOCol + un * C::kUnitCols, a + (kk / 2) * 32 + 16 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, 1u, leader);
             }
             mma_commit_lp(smem_u32(&sh->kv_empty[st[un]]), leader);
           }
@@ -464,13 +455,14 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
+  } else if (kSplit > 1 && (warp & 2)) {
+    reg_alloc<104>();                                // (rows that do not exist)
   } else {
     // ------------------------------- softmax groups -------------------------------------
     reg_alloc<104>();
     const int x = warp >> 3, half = (warp >> 2) & 1;
     const int row_in_tile = (warp & 3) * 32 + lane;  // TMEM lane
-    const int copy = kSplit > 1 ? (warp >> 1) & 1 : 0;
-    const int row = m0 + row_in_tile - copy * (kBM / kSplit), node_of = min(row >> geo.pack_log2, geo.tokens - 1);
+    const int row = m0 + row_in_tile, node_of = min(row >> geo.pack_log2, geo.tokens - 1);
     const int together = 2 + x * 4 + (warp & 3);     // barrier with the warp of the other half
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + lane_addr + C::kOCol;
@@ -559,7 +551,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           m_own = m_use;
         }
 
-        // ---- P = exp2(s - m) in two parts, row sum, P -> TMEM: both parts of 32 keys over their scores ---------------
+        // ---- P = exp2(s - m), row sum, P -> TMEM over the scores: those of 32 keys over the first 16 columns of theirs ---------------
         const float2 mul2 = make_float2(mul, mul), nm2 = make_float2(-m_safe, -m_safe);
         float2 acc2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
@@ -568,21 +560,15 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           tmem_ld32(tS + cc * 32, r);
           tmem_wait_ld();
           if (masked) mask_chunk(r, cc);
-          uint32_t pk[32 / kSplit];
+          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const float2 a = f2fma(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), mul2, nm2);
             const float2 pe = make_float2(ex2(a.x), ex2(a.y));
             acc2[(i >> 1) & 1] = f2add(acc2[(i >> 1) & 1], pe);
-            const float2 first = first_part<T>(pe);
-            pk[i >> 1] = Elem<T>::pack(first.x, first.y);
-            if (kSplit == 1 || copy) {
-              const float2 left = f2fma(Elem<T>::unpack(pk[i >> 1]), make_float2(-1.f, -1.f), pe);
-              pk[(kSplit == 1 ? 16 : 0) + (i >> 1)] = Elem<T>::pack(left.x, left.y);
-            }
+            pk[i >> 1] = Elem<T>::pack(pe.x, pe.y);
           }
-          if constexpr (kSplit == 1) tmem_st32(tS + cc * 32, pk);
-          else tmem_st16(tS + cc * 32, pk);
+          tmem_st16(tS + cc * 32, pk);
         }
         sum += (acc2[0].x + acc2[0].y) + (acc2[1].x + acc2[1].y);
         tmem_wait_st();
@@ -591,14 +577,14 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
 
       // ---- end of the segment: a quarter of the columns each -------------------------------
-      sync_all();                                          // every decision is made
+      sync_all<kSoftmax / kSplit>();                                          // every decision is made
       const int last = J0 + nt - 1;
       const float m_fin = sh->mref[row_in_tile];
       sh->part[2 * x + half][row_in_tile] = m_own == m_fin ? sum : sum * exp2f(m_own - m_fin);
-      sync_all();
+      sync_all<kSoftmax / kSplit>();
       const float l_all = (sh->part[0][row_in_tile] + sh->part[1][row_in_tile]) + (sh->part[2][row_in_tile] + sh->part[3][row_in_tile]);
       if (ok) ok = wait_bar(&sh->o_done[last % NB], (last / NB) & 1, sh, 37 + x);
-      if (any_of_all(!ok || sh->abort_flag != 0)) break;
+      if (any_of_all<kSoftmax / kSplit>(!ok || sh->abort_flag != 0)) break;
       tc_fence_after();
       const bool piece = nt < seg.all;
       const float inv = l_all > 0.f ? 1.f / l_all : 0.f;
@@ -606,24 +592,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int64_t slot = (int64_t)blockIdx.x * 2 + (seg.first == 0);
       T* og = reinterpret_cast<T*>(p.o) + (int64_t)seg.b * p.o_stride[0] + (int64_t)(row >> geo.pack_log2) * p.o_stride[1] +
               (int64_t)(h + (row & ((1 << geo.pack_log2) - 1))) * p.o_stride[2];
-      // (the second copy goes by way of L2: 64 rows of D numbers in this CTA's own place, columns of four together)
-      float4* laid = reinterpret_cast<float4*>(ws_l + (int64_t)gridDim.x * 2 * kBM) + (int64_t)blockIdx.x * (kBM / 2) * (D / 4) + (row_in_tile & 63);
       const int c_first = (2 * x + half) * (D / 4);
-      if (kSplit > 1) {
-        if (copy) {
-#pragma unroll 1
-          for (int c0 = c_first; c0 < c_first + D / 4; c0 += 16) {
-            uint32_t ra[16];
-            tmem_ld16(tO + c0, ra);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              laid[(c0 + i) / 4 * (kBM / 2)] = make_float4(__uint_as_float(ra[i]), __uint_as_float(ra[i + 1]), __uint_as_float(ra[i + 2]), __uint_as_float(ra[i + 3]));
-          }
-        }
-        sync_all();
-      }
-      if (copy == 0) {
+      {
 #pragma unroll 1
         for (int c0 = c_first; c0 < c_first + D / 4; c0 += 16) {
           uint32_t ra[16];
@@ -632,16 +602,6 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(ra[i]);
-          if (kSplit > 1) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 b = __ldcg(laid + (c0 + i) / 4 * (kBM / 2));
-              o[i] += b.x;
-              o[i + 1] += b.y;
-              o[i + 2] += b.z;
-              o[i + 3] += b.w;
-            }
-          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] *= inv;
           if (row_ok && piece) {
@@ -659,7 +619,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&sh->o_free));
-      if (piece && x == 0 && half == 0 && copy == 0 && row_ok) ws_l[slot * kBM + row_in_tile] = l_all > 0.f ? m_fin + log2f(l_all) : -INFINITY;
+      if (piece && x == 0 && half == 0 && row_ok) ws_l[slot * kBM + row_in_tile] = l_all > 0.f ? m_fin + log2f(l_all) : -INFINITY;
     }
   }
 
@@ -761,12 +721,10 @@ int tree_sm100_ranges(const fa_decode_args& d, int pack_log2) {
   return best;
 }
 static bool few_rows(const fa_decode_args& d, int pack_log2) { return ((int64_t)d.seqlen_q << pack_log2) <= kBM / 2; }
-// Two pieces of every CTA, with their LSEs, and a place for the second copy of its rows.
+// Two pieces of every CTA, with their LSEs.
 size_t tree_sm100_piece_bytes(const fa_decode_args& d, int pack_log2) {
   const int ranges = tree_sm100_ranges(d, pack_log2);
-  const bool few = few_rows(d, pack_log2);
-  if (ranges == 1 && !few) return 0;
-  return (size_t)units_of(d, pack_log2) * ranges * (2 * kBM * (d.head_dim + 1) + (few ? kBM / 2 * d.head_dim : 0)) * sizeof(float);
+  return ranges == 1 ? 0 : (size_t)units_of(d, pack_log2) * ranges * 2 * kBM * (d.head_dim + 1) * sizeof(float);
 }
 
 static bool encode_rows(CUtensorMap* m, const void* base, int D, int heads, int64_t rows, int64_t batch, const int64_t* stride, int box_heads,
