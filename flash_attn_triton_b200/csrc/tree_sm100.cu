@@ -629,7 +629,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (tid == 0) report_abort(sh->abort_flag, host_status);
 }
 
-// Adds up the pieces of the sequences that are cut, 256 / (D / 4) rows of a unit per CTA: grid (row groups x units, sequences).
+// Adds up the pieces of the sequences that are cut, 256 / (D / 4) rows of a unit per CTA: grid (row groups x units, sequences or, where there are
+// fewer of them, ends of ranges: one that is the first inside a sequence stands for it).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const fa_attn_args p, const CacheGeo geo) {
   constexpr int kRows = 256 / (D / 4);
@@ -640,61 +641,66 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const fa_attn_args p, c
   walk.seqlens = geo.seqlens;
   walk.n_new = geo.n_new;
   walk.capacity = geo.capacity;
-  for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
-    int64_t before = 0, total = 0;
-    for (int i = lane; i < p.batch; i += 32) {
-      const int nt = walk.tiles_of(i);
-      total += nt;
-      if (i < b) before += nt;
-    }
+  const int per = (p.batch + 31) / 32, b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
+  int64_t mine = 0;
+  for (int i = b0; i < b1; ++i) mine += walk.tiles_of(i);
+  int64_t inc = mine;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-    }
-    const int64_t ranges = ranges_of(total, p.batch, geo.parts);
-    // the range of a tile: the last one that begins at it or before
-    const int first = (int)(((before + 1) * ranges - 1) / total), last = (int)(((before + walk.tiles_of(b)) * ranges - 1) / total);
-    if (b == blockIdx.y) asm volatile("griddepcontrol.wait;" ::: "memory");      // (what has been read so far is no other kernel's work)
-    if (first == last || m0 + r >= rows || (geo.bad != nullptr && *geo.bad != 0u)) continue;
-    const float* ws_l = geo.ws + (int64_t)geo.parts * U * 2 * kBM * D;
-    const int parts = last - first + 1;
-    // the piece that begins the sequence is in its CTA's second slot
-    auto slot_of = [&](int i) { return ((int64_t)(first + i) * U + u) * 2 + (i == 0); };
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float wsum = 0.f, m = -INFINITY;
-    for (int i0 = 0; i0 < parts; i0 += kMergeAtOnce) {
-      float l[kMergeAtOnce];
-      float4 v[kMergeAtOnce];
-#pragma unroll
-      for (int k = 0; k < kMergeAtOnce; ++k) {
-        const int64_t at = slot_of(min(i0 + k, parts - 1)) * kBM + r;
-        l[k] = i0 + k < parts ? ws_l[at] : -INFINITY;
-        v[k] = *reinterpret_cast<const float4*>(geo.ws + at * D + d);
-      }
-      float mn = m;
-#pragma unroll
-      for (int k = 0; k < kMergeAtOnce; ++k) mn = fmaxf(mn, l[k]);
-      const float mf = mn == -INFINITY ? 0.f : mn, sc = exp2f(m - mf);
-      acc.x *= sc; acc.y *= sc; acc.z *= sc; acc.w *= sc;
-      wsum *= sc;
-      m = mn;
-#pragma unroll
-      for (int k = 0; k < kMergeAtOnce; ++k) {
-        if (i0 + k >= parts) break;
-        const float w = exp2f(l[k] - mf);              // pieces without a finite score weigh 0, which a NaN in them survives
-        wsum += w;
-        acc.x += w * v[k].x; acc.y += w * v[k].y; acc.z += w * v[k].z; acc.w += w * v[k].w;
-      }
-    }
-    const float f = wsum > 0.f ? 1.f / wsum : 0.f;
-    const int gr = m0 + r;
-    uint2 pk;
-    pk.x = Elem<T>::pack(acc.x * f, acc.y * f);
-    pk.y = Elem<T>::pack(acc.z * f, acc.w * f);
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + (int64_t)b * p.o_stride[0] + (int64_t)(gr >> geo.pack_log2) * p.o_stride[1] +
-                              (int64_t)(h + (gr & ((1 << geo.pack_log2) - 1))) * p.o_stride[2] + d) = pk;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
   }
+  const int64_t total = __shfl_sync(0xffffffffu, inc, 31), ranges = ranges_of(total, p.batch, geo.parts);
+  // the sequence and its first tile, `before`
+  const bool by_sequence = p.batch < geo.parts;
+  const int64_t cut = total * (blockIdx.y + 1) / ranges;       // end of range blockIdx.y
+  const bool owner = by_sequence ? (int)blockIdx.y >= b0 && (int)blockIdx.y < b1 : cut >= inc - mine && cut < inc;
+  const unsigned who = __ballot_sync(0xffffffffu, owner);
+  asm volatile("griddepcontrol.wait;" ::: "memory");           // (what has been read so far is no other kernel's work)
+  if (who == 0u || (!by_sequence && (int64_t)blockIdx.y + 1 >= ranges)) return;
+  int b = __shfl_sync(0xffffffffu, b0, __ffs(who) - 1), nt = 0;
+  int64_t before = __shfl_sync(0xffffffffu, inc - mine, __ffs(who) - 1);
+  for (; nt = walk.tiles_of(b), by_sequence ? b < (int)blockIdx.y : before + nt <= cut; ++b) before += nt;
+  // the range of a tile: the last one that begins at it or before
+  const int first = (int)(((before + 1) * ranges - 1) / total), last = (int)(((before + nt) * ranges - 1) / total);
+  if (first == last || (!by_sequence && first != (int)blockIdx.y) || m0 + r >= rows || (geo.bad != nullptr && *geo.bad != 0u)) return;
+  const float* ws_l = geo.ws + (int64_t)geo.parts * U * 2 * kBM * D;
+  const int parts = last - first + 1;
+  // the piece that begins the sequence is in its CTA's second slot
+  auto slot_of = [&](int i) { return ((int64_t)(first + i) * U + u) * 2 + (i == 0); };
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float wsum = 0.f, m = -INFINITY;
+  for (int i0 = 0; i0 < parts; i0 += kMergeAtOnce) {
+    float l[kMergeAtOnce];
+    float4 v[kMergeAtOnce];
+#pragma unroll
+    for (int k = 0; k < kMergeAtOnce; ++k) {
+      const int64_t at = slot_of(min(i0 + k, parts - 1)) * kBM + r;
+      l[k] = i0 + k < parts ? ws_l[at] : -INFINITY;
+      v[k] = *reinterpret_cast<const float4*>(geo.ws + at * D + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < kMergeAtOnce; ++k) mn = fmaxf(mn, l[k]);
+    const float mf = mn == -INFINITY ? 0.f : mn, sc = exp2f(m - mf);
+    acc.x *= sc; acc.y *= sc; acc.z *= sc; acc.w *= sc;
+    wsum *= sc;
+    m = mn;
+#pragma unroll
+    for (int k = 0; k < kMergeAtOnce; ++k) {
+      if (i0 + k >= parts) break;
+      const float w = exp2f(l[k] - mf);              // pieces without a finite score weigh 0, which a NaN in them survives
+      wsum += w;
+      acc.x += w * v[k].x; acc.y += w * v[k].y; acc.z += w * v[k].z; acc.w += w * v[k].w;
+    }
+  }
+  const float f = wsum > 0.f ? 1.f / wsum : 0.f;
+  const int gr = m0 + r;
+  uint2 pk;
+  pk.x = Elem<T>::pack(acc.x * f, acc.y * f);
+  pk.y = Elem<T>::pack(acc.z * f, acc.w * f);
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.o) + (int64_t)b * p.o_stride[0] + (int64_t)(gr >> geo.pack_log2) * p.o_stride[1] +
+                            (int64_t)(h + (gr & ((1 << geo.pack_log2) - 1))) * p.o_stride[2] + d) = pk;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -777,7 +783,7 @@ static int launch_tree(const fa_decode_args& d, const CacheGeo& geo, float scale
   cudaLaunchKernelEx(&lc, kern, tm[0], tm[1], tm[2], a, scale_log2, rescale_at, geo, host_wait_word(d.device));
   if (int r = check_launch("tree_sm100")) return r;
   if (geo.parts == 1) return FA_OK;
-  lc.gridDim = dim3((unsigned)units_of(d, geo.pack_log2) * (kBM * D / 4 / 256), (unsigned)(d.batch < 65535 ? d.batch : 65535));
+  lc.gridDim = dim3((unsigned)units_of(d, geo.pack_log2) * (kBM * D / 4 / 256), (unsigned)(d.batch < geo.parts ? d.batch : geo.parts - 1));
   lc.blockDim = dim3(256);
   lc.dynamicSmemBytes = 0;
   cudaLaunchKernelEx(&lc, tree_merge_kernel<T, D>, a, geo);

@@ -164,16 +164,17 @@ def test_norm_of_zeros_and_of_rows_that_are_no_numbers():
 
 
 # ---- attention under the mask of a tree -------------------------------------------------------------------------------------------
-def make_cache(gen, dtype, lens, room, heads_kv, dim, page, pads=None):
-    """Caches, paged from a shuffled pool or contiguous (page 0), and where position p of sequence b lies: (first index, row)."""
+def make_cache(gen, dtype, lens, room, heads_kv, dim, page, pads=None, capacity=0):
+    """Caches, paged from a shuffled pool or contiguous (page 0), and where position p of sequence b lies: (first index, row).  capacity: of a
+    sequence, at least; with a large one a call takes the kernel for long caches."""
     if page == 0:
-        rows = max(lens) + room + (max(pads) if pads else 0)
+        rows = max(max(lens) + room + (max(pads) if pads else 0), capacity)
         kc, vc = (rand(gen, len(lens) + 1, rows, heads_kv, dim).to(dtype) for _ in range(2))
         order = torch.randperm(len(lens) + 1, generator=gen)[:len(lens)].to(torch.int32)
         return kc, vc, None, order, lambda b, p: (int(order[b]), p + (pads[b] if pads else 0))
     need = [-(-(n + room) // page) for n in lens]
     pool = torch.randperm(sum(need) + 2, generator=gen).to(torch.int32)
-    table, at = torch.zeros(len(lens), max(need), dtype=torch.int32), 0
+    table, at = torch.zeros(len(lens), max(max(need), -(-capacity // page)), dtype=torch.int32), 0
     for b, n in enumerate(need):
         table[b, :n] = pool[at:at + n]
         table[b, n:] = pool[at]
@@ -183,7 +184,7 @@ def make_cache(gen, dtype, lens, room, heads_kv, dim, page, pads=None):
 
 
 TREES = [
-    # dtype, lens, nodes, heads, heads_kv, dim, page, causal: the decode kernel, with 8 and 16 rows a unit and several groups of rows; chunks
+    # dtype, lens, nodes, heads, heads_kv, dim, page, causal
     (F16, [0, 1, 130], 1, 8, 8, 128, 16, False),
     (BF16, [70, 0, 5], 4, 8, 4, 128, 16, False),
     (F16, [513, 64, 63], 7, 4, 2, 64, 48, False),
@@ -200,10 +201,16 @@ TREES = [
 ]
 
 
-def run_tree(seed, case, new=True, used=None, spoil=None, mask=None, **kw):
+def wide_enough(case):
+    """A capacity with which a call of more than 8 query rows per head takes the kernel for long caches (more tiles than a few per SM)."""
+    _, lens, nodes, heads, heads_kv, _, _, _ = case
+    return 64 * 4 * 148 // (len(lens) * heads_kv * -(-nodes * heads // heads_kv // 16)) + 64
+
+
+def run_tree(seed, case, new=True, used=None, spoil=None, mask=None, wide=False, **kw):
     dtype, lens, nodes, heads, heads_kv, dim, page, causal = case
     gen = torch.Generator().manual_seed(seed)
-    kc, vc, table, rows, where = make_cache(gen, dtype, lens, nodes, heads_kv, dim, page)
+    kc, vc, table, rows, where = make_cache(gen, dtype, lens, nodes, heads_kv, dim, page, capacity=wide_enough(case) if wide else 0)
     q, k, v = (rand(gen, len(lens), nodes, h, dim).to(dtype) for h in (heads, heads_kv, heads_kv))
     _, seen = ref.tree(gen, len(lens), nodes, used or [max(1, nodes - 3 * b) for b in range(len(lens))])
     if mask is not None:
@@ -239,43 +246,82 @@ def run_tree(seed, case, new=True, used=None, spoil=None, mask=None, **kw):
     return out, seen
 
 
+WIDE = pytest.mark.parametrize("wide", [False, True], ids=["few_tiles", "long_cache"])
+
+
+@WIDE
 @pytest.mark.parametrize("i", range(len(TREES)))
-def test_tree(i):
-    run_tree(i, TREES[i])
+def test_tree(i, wide):
+    run_tree(i, TREES[i], wide=wide)
 
 
+@WIDE
 @pytest.mark.parametrize("i", [1, 3, 6, 7, 10])
-def test_tree_of_tokens_that_are_in_the_cache(i):
-    run_tree(100 + i, TREES[i], new=False)
+def test_tree_of_tokens_that_are_in_the_cache(i, wide):
+    run_tree(100 + i, TREES[i], new=False, wide=wide)
 
 
+@WIDE
 @pytest.mark.parametrize("spoil", [math.nan, math.inf])
 @pytest.mark.parametrize("new", [False, True])
 @pytest.mark.parametrize("i", [1, 2, 3, 6, 7, 8, 9, 10, 12])
-def test_nodes_that_nobody_sees_may_hold_anything(i, new, spoil):
+def test_nodes_that_nobody_sees_may_hold_anything(i, new, spoil, wide):
     lens, nodes = TREES[i][1], TREES[i][2]
-    run_tree(200 + i, TREES[i], new=new, used=[max(1, nodes // 2)] + [1] * (len(lens) - 1), spoil=spoil)
+    run_tree(200 + i, TREES[i], new=new, used=[max(1, nodes // 2)] + [1] * (len(lens) - 1), spoil=spoil, wide=wide)
 
 
+@WIDE
 @pytest.mark.parametrize("i", [1, 2, 3, 6, 7, 10])
-def test_rows_that_see_nothing_and_any_mask(i):
+def test_rows_that_see_nothing_and_any_mask(i, wide):
     """Without a context such rows are zeros; a mask need be no tree."""
     lens = [0] * len(TREES[i][1])
     case = (TREES[i][0], lens, *TREES[i][2:])
     gen = torch.Generator().manual_seed(i)
-    _, seen = run_tree(300 + i, case, mask=lambda m: torch.rand(m.shape, generator=gen) < 0.3)
-    out, seen = run_tree(310 + i, case, mask=lambda m: torch.zeros_like(m))
+    _, seen = run_tree(300 + i, case, mask=lambda m: torch.rand(m.shape, generator=gen) < 0.3, wide=wide)
+    out, seen = run_tree(310 + i, case, mask=lambda m: torch.zeros_like(m), wide=wide)
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("batch,longest,nodes,heads,heads_kv,dim,page", [
+    (40, 700, 12, 4, 4, 64, 16),        # several sequences to a range, and the other way round
+    (33, 300, 5, 8, 2, 128, 32),
+    (200, 150, 20, 2, 2, 256, 64),      # more sequences than ranges
+    (160, 400, 9, 2, 1, 128, 128),
+    (300, 140, 40, 4, 1, 64, 0),        # two tiles of rows
+    (3, 2000, 70, 32, 16, 64, 64),      # more units than SMs have room for at a time
+    (2, 9000, 3, 8, 1, 128, 256),       # one unit, many ranges
+])
+def test_ranges_of_many_sequences(batch, longest, nodes, heads, heads_kv, dim, page):
+    """How the sequences' tiles are cut into ranges: every place where a range may end.  Against the call for one sequence at a time, whose
+    results are within the same bounds of the definition (test_tree)."""
+    gen = torch.Generator().manual_seed(batch + nodes)
+    lens = torch.randint(longest + 1, (batch,), generator=gen).tolist()
+    lens[0], lens[-1] = 0, longest
+    kc, vc, table, rows, _ = make_cache(gen, F16, lens, nodes, heads_kv, dim, page)
+    kc, vc = kc.to(DEV), vc.to(DEV)
+    q, k, v = (rand(gen, batch, nodes, h, dim).to(F16).to(DEV) for h in (heads, heads_kv, heads_kv))
+    _, seen = ref.tree(gen, batch, nodes)
+    seen, lengths = seen.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def call(at):
+        return fa.flash_attn_with_kvcache(q[at], kc, vc, k[at], v[at], cache_seqlens=lengths[at], tree_mask=seen[at],
+                                          block_table=None if table is None else table.to(DEV)[at], cache_batch_idx=None if rows is None else rows.to(DEV)[at])
+    out = call(slice(None))
+    assert torch.equal(out, call(slice(None)))
+    largest = v.abs().max().item() + vc.abs().max().item()
+    for b in range(batch):
+        want = call(slice(b, b + 1))[0].cpu().double()
+        within(out[b], want, 2 * (half(F16) * want.abs() + (half(F16) + 2.0 ** -12) * largest), b)
 
 
 def test_tree_masks_of_other_shapes():
     """One mask for all requests; rows of other strides.  A chain is the causal mask: bit for bit where the kernel is the same, few rows; else both
-    results are within half a step of their own and 2^-12 sum p |v| <= 2^-12 max |v| of the same number (see the top), so within twice that of one
-    another."""
+    results are within half a step of their own and (half + 2^-12) sum p |v| <= (half + 2^-12) max |v| of the same number (see the top), so
+    within twice that of one another."""
     gen = torch.Generator().manual_seed(7)
     for nodes, heads, heads_kv, page in ((4, 8, 4, 16), (40, 8, 2, 64)):
         lens = torch.tensor([60, 200], dtype=torch.int32, device=DEV)
-        kc, vc, table, _, _ = make_cache(gen, F16, [60, 200], nodes, heads_kv, 128, page)
+        kc, vc, table, _, _ = make_cache(gen, F16, [60, 200], nodes, heads_kv, 128, page, capacity=6000 if nodes > 4 else 0)
         q, k, v = (rand(gen, 2, nodes, h, 128).to(F16).to(DEV) for h in (heads, heads_kv, heads_kv))
 
         def call(**kw):
@@ -294,7 +340,7 @@ def test_tree_masks_of_other_shapes():
                 assert torch.equal(got, want)
             else:
                 largest = max(x.abs().max().item() for x in (vc.float(), v.float()))
-                within(got, want.cpu().double(), 2 * half(F16) * (want.cpu().double().abs() + 2.0 ** -11) + 2.0 ** -11 * largest, "chain")
+                within(got, want.cpu().double(), 2 * half(F16) * (want.cpu().double().abs() + 2.0 ** -11) + 2 * (half(F16) + 2.0 ** -12) * largest, "chain")
         same(call(tree_mask=chain), call(causal=True))
         same(call(tree_mask=torch.ones_like(chain), causal=True), call(causal=True))
         same(call(tree_mask=torch.ones_like(chain)), call())
@@ -640,7 +686,7 @@ def test_streams_and_graphs():
     """All calls captured into a graph on a stream of its own and replayed beside the same calls on another stream."""
     gen = torch.Generator().manual_seed(2)
     B, N = 3, 20
-    kc, vc, table, _, _ = make_cache(gen, F16, [500, 40, 3000], N, 2, 128, 64)
+    kc, vc, table, _, _ = make_cache(gen, F16, [500, 40, 3000], N, 2, 128, 64, capacity=5000)
     lens = torch.tensor([500, 40, 3000], dtype=torch.int32, device=DEV)
     q, k, v = (rand(gen, B, N, h, 128).to(F16).to(DEV) for h in (8, 2, 2))
     _, seen = ref.tree(gen, B, N)
