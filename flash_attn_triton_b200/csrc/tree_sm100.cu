@@ -40,21 +40,25 @@ constexpr int kBN = 128;          // keys per tile
 constexpr int kSoftmax = 512;     // threads of the softmax warps
 constexpr int kThreads = kSoftmax + 128;
 constexpr int kMaxStages = 8;
+constexpr int kSharedBytes = 3 * 1024;   // reserve for TShared
 constexpr int kMergeAtOnce = 8;   // pieces whose rows are in flight together
 
-template <int D> struct TCfg {
+// kApart: few rows and head_dim up to 128.  Two warps of their own write the results, from one of two accumulators, so that a segment's end
+// lies under the next segment's tiles.
+template <int D, bool kApart> struct TCfg {
   static constexpr int kUnitCols = D < 128 ? D : 128;
   static constexpr int kUnits = D / kUnitCols;                      // ring entries of a K (or V) tile
   static constexpr int kUnitBytes = kBN * kUnitCols * 2;
   static constexpr int kBoxes = kUnitCols / 64;                     // TMA boxes of an entry
   static constexpr int kStages = D == 64 ? 8 : 5;
   static constexpr int kQBuf = D == 256 ? 1 : 2;
-  static constexpr int kSBuf = D == 256 ? 2 : 3;                    // score buffers
+  static constexpr int kSBuf = D == 256 || (kApart && D == 128) ? 2 : 3;      // score buffers
+  static constexpr int kOBuf = kApart ? 2 : 1;                      // accumulators
   static constexpr int kOCol = kSBuf * 128;                         // first column of the accumulator
   static constexpr int kQBytes = kBM * D * 2;
   static constexpr int kRing = kQBuf * kQBytes;                     // where the ring begins
   static constexpr int kSmemTiles = kRing + kStages * kUnitBytes;
-  static constexpr int kSmemBytes = kSmemTiles + 3072 /*TShared*/;
+  static constexpr int kSmemBytes = kSmemTiles + kSharedBytes;
 };
 
 struct TShared {
@@ -66,28 +70,30 @@ struct TShared {
   uint64_t p_ready[2][3];  // [half][buffer]: P of these warps written back (128 arrivals)
   uint64_t o_done[3];      // [buffer]: its P V finished
   uint64_t decided[2];     // [pair]: mref settled for the pair's tile (256 arrivals)
-  uint64_t o_free;         // the accumulator has been read (512 arrivals)
+  uint64_t o_free[2];      // [accumulator]: it has been read, and the sums of its segment (all that read it)
+  uint64_t o_last[2];      // [accumulator]: its segment's last P V finished
+  uint64_t ended[2];       // [accumulator]: its segment's sums are written (all softmax threads that have rows)
   uint32_t tmem_base;
   volatile int abort_flag;
   alignas(16) float mref[kBM];
   float part[4][kBM];      // [2 pair + half]: row maxima of the two halves of a tile; at the end of a segment row sums
 };
-static_assert(sizeof(TShared) <= 3072, "TShared must fit its reserve");
+static_assert(sizeof(TShared) <= kSharedBytes, "TShared must fit its reserve");
 
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, TShared* sh, int code) {
   return bounded_wait(bar, parity, &sh->abort_flag, &g_tree_status, code);
 }
-// Barrier 1 of the softmax threads: is the predicate set in any of them?
-template <int kCount> __device__ __forceinline__ bool any_of_all(bool x) {
+// The predicate, set in any of the kCount threads that meet at barrier `id`?
+template <int kCount> __device__ __forceinline__ bool any_of(bool x, int id) {
   int r;
   asm volatile(
       "{\n"
       ".reg .pred p, q;\n"
       "setp.ne.s32 p, %1, 0;\n"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n"
+      "barrier.cta.red.or.pred q, %3, %2, p;\n"
       "selp.s32 %0, 1, 0, q;\n"
       "}\n"
-      : "=r"(r) : "r"((int)x), "n"(kCount) : "memory");
+      : "=r"(r) : "r"((int)x), "n"(kCount), "r"(id) : "memory");
   return r != 0;
 }
 template <int kCount> __device__ __forceinline__ void sync_all() { asm volatile("bar.sync 1, %0;\n" ::"n"(kCount) : "memory"); }
@@ -152,8 +158,10 @@ template <typename T, int D, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const fa_attn_args p, const float scale_log2, const float rescale_at, const CacheGeo geo, int* const host_status) {
-  using C = TCfg<D>;
-  constexpr int S = C::kStages, NB = C::kSBuf, NU = C::kUnits, NQ = C::kQBuf;
+  constexpr bool kApart = kSplit > 1 && D <= 128;
+  using C = TCfg<D, kApart>;
+  constexpr int S = C::kStages, NB = C::kSBuf, NU = C::kUnits, NQ = C::kQBuf, NO = C::kOBuf;
+  constexpr int kTmaWarp = kApart ? 18 : 16, kMmaWarp = kTmaWarp + 1;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* tiles = smem_raw;                             // (a kernel's dynamic shared memory alone begins at 1024 bytes; checked below)
   TShared* sh = reinterpret_cast<TShared*>(tiles + C::kSmemTiles);
@@ -214,11 +222,15 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     mbar_init(smem_u32(&sh->decided[0]), 256 / kSplit);
     mbar_init(smem_u32(&sh->decided[1]), 256 / kSplit);
-    mbar_init(smem_u32(&sh->o_free), kSoftmax / kSplit);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh->o_free[i]), kApart ? kBM / 2 : kSoftmax / kSplit);
+      mbar_init(smem_u32(&sh->o_last[i]), 1);
+      mbar_init(smem_u32(&sh->ended[i]), kSoftmax / kSplit);
+    }
     sh->abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 16) {
+  if (warp == kTmaWarp) {
     tmem_alloc(smem_u32(&sh->tmem_base), 512);
     tmem_relinquish();
   }
@@ -237,9 +249,44 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const bool nothing = (geo.bad != nullptr && *geo.bad != 0u) || (sQ & 1023u) != 0u;
   if ((sQ & 1023u) != 0u && tid == 0) sh->abort_flag = 97;
 
-  if (warp >= 18) {
+  // The sums of the segments' rows, (reference, sum) of the four parts of a row: over rows of the first queries' tile that do not exist.
+  float2* ends = reinterpret_cast<float2*>(tiles + (kBM / 2) * 128);
+  static_assert(!kApart || 2 * 4 * (kBM / 2) * 8 <= (kBM / 2) * 128, "room for the sums");
+  // Columns [c0, c1) of a row from the accumulator at tO: to the output, or to a piece of it.
+  auto write_rows = [&](const Segment& seg, int row, bool row_ok, float l_all, float m_fin, uint32_t tO, int c0, int c1, float* ws_l) {
+    const bool piece = seg.nt < seg.all;
+    const float inv = l_all > 0.f ? 1.f / l_all : 0.f;
+    // a piece that begins its sequence goes to the CTA's second slot, any other (it then begins the range) to the first
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (seg.first == 0);
+    const int64_t at = slot * kBM + row - m0;
+    T* og = reinterpret_cast<T*>(p.o) + (int64_t)seg.b * p.o_stride[0] + (int64_t)(row >> geo.pack_log2) * p.o_stride[1] +
+            (int64_t)(h + (row & ((1 << geo.pack_log2) - 1))) * p.o_stride[2];
+#pragma unroll 1
+    for (int c = c0; c < c1; c += 16) {
+      uint32_t ra[16];
+      float o[16];
+      tmem_ld16(tO + c, ra);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(ra[i]) * inv;
+      if (row_ok && piece) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(geo.ws + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      } else if (row_ok) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 8)
+          *reinterpret_cast<uint4*>(og + c + i) = make_uint4(Elem<T>::pack(o[i], o[i + 1]), Elem<T>::pack(o[i + 2], o[i + 3]),
+                                                             Elem<T>::pack(o[i + 4], o[i + 5]), Elem<T>::pack(o[i + 6], o[i + 7]));
+      }
+      __syncwarp();
+    }
+    if (piece && c0 == 0 && row_ok) ws_l[at] = l_all > 0.f ? m_fin + log2f(l_all) : -INFINITY;
+  };
+
+  if (!kApart && warp >= 18) {
     reg_dealloc<64>();
-  } else if (warp == 16) {
+  } else if (warp == kTmaWarp) {
     // ------------------------------- TMA producer ---------------------------------------
     reg_dealloc<64>();
     const bool many = geo.box_rows < kBN;                      // a tile of keys is several pages
@@ -331,7 +378,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
-  } else if (warp == 17) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------- MMA issuer -----------------------------------------
     // The whole warp runs the control flow in lock step and every lane polls the barriers;
     // the lane chosen once by elect_one issues the MMAs and commits.
@@ -400,7 +447,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
           }
           const uint32_t fresh = vj > 0 ? 1u : 0u;             // (accumulate)
-          if (vj == 0 && vsegs > 1) wwait(&sh->o_free, vsegs & 1, 27);
+          const int ob = (vsegs - 1) % NO;                     // accumulator
+          if (vj == 0 && vsegs > NO) wwait(&sh->o_free[ob], ((vsegs - 1) / NO - 1) & 1, 27);
           wwait(&sh->p_ready[0][vbuf], par, 25);
           if (!ok) break;
 #pragma unroll
@@ -408,7 +456,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint64_t dv = make_smem_desc(v[un], kBN * 128, 1024);
 #pragma unroll
             for (int kk = 0; kk < kBN / 32; ++kk) {
-              mma_f16_ts_lp(tmem + C::kOCol + un * C::kUnitCols, a + (kk / 2) * 32 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, kk > 0 ? 1u : fresh, leader);
+              mma_f16_ts_lp(tmem + C::kOCol + ob * D + un * C::kUnitCols, a + (kk / 2) * 32 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, kk > 0 ? 1u : fresh, leader);
             }
           }
           wwait(&sh->p_ready[1][vbuf], par, 26);
@@ -418,12 +466,12 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const uint64_t dv = make_smem_desc(v[un], kBN * 128, 1024);
 #pragma unroll
             for (int kk = kBN / 32; kk < kBN / 16; ++kk) {
-              mma_f16_ts_lp(tmem + C::kOCol + un * C::kUnitCols, a + (kk / 2) * 32 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, 1u, leader);
+              mma_f16_ts_lp(tmem + C::kOCol + ob * D + un * C::kUnitCols, a + (kk / 2) * 32 + (kk % 2) * 8, dv + ((kk * 2048) >> 4), idesc_pv, 1u, leader);
             }
             mma_commit_lp(smem_u32(&sh->kv_empty[st[un]]), leader);
           }
           mma_commit_lp(smem_u32(&sh->o_done[vbuf]), leader);
-          ++vj;
+          if (++vj == vs.nt && kApart) mma_commit_lp(smem_u32(&sh->o_last[ob]), leader);
           if (++vbuf == NB) { vbuf = 0; par ^= 1; }
         }
         if (i < count) {                                       // S[qbuf] = Q K^T of tile i
@@ -455,6 +503,32 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
+  } else if (kApart && warp >= 16) {
+    // ------------------------------- results --------------------------------------------
+    reg_dealloc<64>();
+    const int row = (warp & 1) * 32 + lane;          // also the TMEM lane
+    const bool row_ok = row < rows;
+    const uint32_t lane_addr = (uint32_t)((warp & 1) * 32) << 16;
+    float* ws_l = geo.ws + (int64_t)gridDim.x * 2 * kBM * D;
+    Segment seg;
+    for (int segs = 0; !nothing && walk.next(seg); ++segs) {
+      const int ob = segs & 1;
+      const uint32_t par = (segs >> 1) & 1;
+      if (!__all_sync(0xffffffffu, wait_bar(&sh->ended[ob], par, sh, 36) && wait_bar(&sh->o_last[ob], par, sh, 37))) break;
+      tc_fence_after();
+      float2 e[4];
+      float m_fin = -INFINITY, l_all = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = ends[(ob * 4 + i) * (kBM / 2) + row];
+        m_fin = fmaxf(m_fin, e[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l_all += e[i].x == m_fin ? e[i].y : e[i].y * exp2f(e[i].x - m_fin);
+      write_rows(seg, row, row_ok, l_all, m_fin, tmem + lane_addr + C::kOCol + ob * D, 0, D, ws_l);
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh->o_free[ob]));
+    }
   } else if (kSplit > 1 && (warp & 2)) {
     reg_alloc<104>();                                // (rows that do not exist)
   } else {
@@ -465,7 +539,6 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int row = m0 + row_in_tile, node_of = min(row >> geo.pack_log2, geo.tokens - 1);
     const int together = 2 + x * 4 + (warp & 3);     // barrier with the warp of the other half
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tO = tmem + lane_addr + C::kOCol;
     const bool row_ok = row < rows;
     float* ws_l = geo.ws + (int64_t)gridDim.x * 2 * kBM * D;
     bool ok = true;
@@ -473,6 +546,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     Segment seg;
     for (int segs = 0; !nothing && ok && walk.next(seg); ++segs, J0 += seg.nt) {
       const int nt = seg.nt;
+      const uint32_t tO = tmem + lane_addr + C::kOCol + segs % NO * D;
       float m_own = -INFINITY, sum = 0.f;            // of this thread's keys: their sum relative to m_own
       for (int j = (J0 & 1) ^ x; j < nt; j += 2) {
         const int J = J0 + j, buf = J % NB;
@@ -518,7 +592,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
         // ---- the maximum the exponents are relative to, settled in tile order -------------
         // (the halves of a tile come to the same: the reference before it and the larger of their maxima)
-        if (j > 0 && ok) ok = __all_sync(0xffffffffu, wait_bar(&sh->decided[x ^ 1], ((J - 1) >> 1) & 1, sh, 33 + x));
+        // (also for the first tile of a segment: its reference takes the place of the last segment's)
+        if (J > 0 && ok) ok = __all_sync(0xffffffffu, wait_bar(&sh->decided[x ^ 1], ((J - 1) >> 1) & 1, sh, 33 + x));
         const float m_old = j > 0 ? sh->mref[row_in_tile] : -INFINITY;
         sync_halves(together);
         mx = fmaxf(mx, sh->part[2 * x + (half ^ 1)][row_in_tile]);
@@ -576,56 +651,34 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         mbar_arrive(smem_u32(&sh->p_ready[half][buf]));
       }
 
-      // ---- end of the segment: a quarter of the columns each -------------------------------
-      sync_all<kSoftmax / kSplit>();                                          // every decision is made
+      // ---- end of the segment --------------------------------------------------------------
+      if constexpr (kApart) {
+        if (ok && segs >= 2) ok = wait_bar(&sh->o_free[segs & 1], ((segs >> 1) - 1) & 1, sh, 38);      // (the sums there have been read)
+        ends[((segs & 1) * 4 + 2 * x + half) * (kBM / 2) + row_in_tile] = make_float2(m_own, sum);
+        mbar_arrive(smem_u32(&sh->ended[segs & 1]));
+        ok = !any_of<64>(!ok, together);                   // (the warps of both halves leave together)
+        continue;
+      }
+      // a quarter of the columns each
+      sync_all<kSoftmax / kSplit>();                       // every decision is made
       const int last = J0 + nt - 1;
       const float m_fin = sh->mref[row_in_tile];
       sh->part[2 * x + half][row_in_tile] = m_own == m_fin ? sum : sum * exp2f(m_own - m_fin);
       sync_all<kSoftmax / kSplit>();
       const float l_all = (sh->part[0][row_in_tile] + sh->part[1][row_in_tile]) + (sh->part[2][row_in_tile] + sh->part[3][row_in_tile]);
       if (ok) ok = wait_bar(&sh->o_done[last % NB], (last / NB) & 1, sh, 37 + x);
-      if (any_of_all<kSoftmax / kSplit>(!ok || sh->abort_flag != 0)) break;
+      if (any_of<kSoftmax / kSplit>(!ok || sh->abort_flag != 0, 1)) break;
       tc_fence_after();
-      const bool piece = nt < seg.all;
-      const float inv = l_all > 0.f ? 1.f / l_all : 0.f;
-      // a piece that begins its sequence goes to the CTA's second slot, any other (it then begins the range) to the first
-      const int64_t slot = (int64_t)blockIdx.x * 2 + (seg.first == 0);
-      T* og = reinterpret_cast<T*>(p.o) + (int64_t)seg.b * p.o_stride[0] + (int64_t)(row >> geo.pack_log2) * p.o_stride[1] +
-              (int64_t)(h + (row & ((1 << geo.pack_log2) - 1))) * p.o_stride[2];
-      const int c_first = (2 * x + half) * (D / 4);
-      {
-#pragma unroll 1
-        for (int c0 = c_first; c0 < c_first + D / 4; c0 += 16) {
-          uint32_t ra[16];
-          float o[16];
-          tmem_ld16(tO + c0, ra);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(ra[i]);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] *= inv;
-          if (row_ok && piece) {
-            float* dst = geo.ws + (slot * kBM + row_in_tile) * D + c0;
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          } else if (row_ok) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 8)
-              *reinterpret_cast<uint4*>(og + c0 + i) = make_uint4(Elem<T>::pack(o[i], o[i + 1]), Elem<T>::pack(o[i + 2], o[i + 3]),
-                                                                  Elem<T>::pack(o[i + 4], o[i + 5]), Elem<T>::pack(o[i + 6], o[i + 7]));
-          }
-          __syncwarp();
-        }
-      }
+      const int c0 = (2 * x + half) * (D / 4);
+      write_rows(seg, row, row_ok, l_all, m_fin, tO, c0, c0 + D / 4, ws_l);
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh->o_free));
-      if (piece && x == 0 && half == 0 && row_ok) ws_l[slot * kBM + row_in_tile] = l_all > 0.f ? m_fin + log2f(l_all) : -INFINITY;
+      mbar_arrive(smem_u32(&sh->o_free[0]));
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) tmem_dealloc(tmem, 512);
+  if (warp == kTmaWarp) tmem_dealloc(tmem, 512);
   if (tid == 0) report_abort(sh->abort_flag, host_status);
 }
 
@@ -762,7 +815,7 @@ static int launch_tree(const fa_decode_args& d, const CacheGeo& geo, float scale
     set_error("tree_sm100: cuTensorMapEncodeTiled failed");
     return FA_ERR_LAUNCH;
   }
-  using C = TCfg<D>;
+  using C = TCfg<D, (kSplit > 1 && D <= 128)>;
   static_assert(C::kSmemBytes <= 227 * 1024, "shared memory budget");
   auto kern = tree_sm100_kernel<T, D, kSplit>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
