@@ -55,6 +55,7 @@ size_t tree_sm100_piece_bytes(const fa_decode_args& d, int pack_log2);
 int tree_sm100(const fa_decode_args& d, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st);
 
 __global__ void __launch_bounds__(1024) decode_check_kernel(const fa_decode_args p, uint32_t* host, uint32_t* dev) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");        // the kernel behind it gets ready meanwhile
   const uint32_t bad = decode_checks(p, threadIdx.x, blockDim.x);
   if (threadIdx.x == 0) {
     if (dev) *dev = bad;
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
       __threadfence_system();
     }
     if (bad) return;
-  } else if (dev && *dev) {
+  } else if (!kTree && dev && *dev) {
     return;
   }
   if (kTree) {
@@ -545,6 +546,11 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
       }
       const uint32_t bits = __ballot_sync(0xffffffffu, seen);
       if (lane == 0) tree_bits[i] = bits;
+    }
+    if (dev && !check_here) {
+      // launched while the check kernel may still run (programmatic dependent launch): neither the mask nor where its bits go is its
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (*dev) return;
     }
   }
   const int D = p.head_dim, cpr_log2 = 31 - __clz(D / 8);      // (a power of two)
@@ -795,7 +801,18 @@ static int chunk_run(const fa_decode_args& args, const ChunkPlan& c, uint32_t* h
       using T = std::remove_pointer_t<decltype(q)>;
       auto kern = tree_bits ? cache_append_kernel<T, int64_t, true>
                   : small   ? cache_append_kernel<T, uint32_t, false> : cache_append_kernel<T, int64_t, false>;
-      kern<<<grid, 256, 0, st>>>(a, q, shift, host, dev, inside, tree_bits);
+      cudaLaunchConfig_t lc = {};
+      cudaLaunchAttribute attr;
+      lc.gridDim = dim3(grid);
+      lc.blockDim = dim3(256);
+      lc.stream = st;
+      if (tree_bits && dev && !inside) {
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        lc.attrs = &attr;
+        lc.numAttrs = 1;
+      }
+      cudaLaunchKernelEx(&lc, kern, a, q, shift, host, dev, inside, tree_bits);
     };
     if (a.dtype == FA_BF16) append(static_cast<__nv_bfloat16*>(q_out));
     else append(static_cast<__half*>(q_out));

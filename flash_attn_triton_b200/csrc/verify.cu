@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
   const double bound = (double)a.sample[b] * sum;
   double run = 0.0;
   const int at = place_of(part, slots, bound, 0.0, lane, &run);
-  if (at / kWarps != rank) return;
+  if (at < 0 || at / kWarps != rank) return;         // (at >= 0: the sum is positive)
   // that share, [w0, w1), in the CTA that has it: a part of it for each warp
   const int64_t w0 = a.vocab * at / slots, w1 = a.vocab * (at + 1) / slots, n = w1 - w0;
   const int64_t u0 = w0 + n * warp / kWarps, u1 = w0 + n * (warp + 1) / kWarps;
