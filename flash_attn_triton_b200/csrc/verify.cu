@@ -81,11 +81,10 @@ __device__ __forceinline__ double rest_of(float p, float q, double c) {
   return r > 0.0 ? r : (r == r ? 0.0 : r);
 }
 
-// Sum of what is left over [v0, v1), by a warp; kAtOnce numbers of a lane are in flight together.
+// Adds up what is left over [v0, v1), by a warp; kAtOnce numbers of a lane are in flight together.
 constexpr int kAtOnce = 8;
 template <typename F>
-__device__ __forceinline__ double share_sum(F at, int64_t v0, int64_t v1, double c, int lane) {
-  double s[4] = {0.0, 0.0, 0.0, 0.0};
+__device__ __forceinline__ void add_left(double (&s)[4], F at, int64_t v0, int64_t v1, double c, int lane) {
   for (int64_t v = v0 + lane; v < v1; v += 32 * kAtOnce) {
     float2 x[kAtOnce];
 #pragma unroll
@@ -93,15 +92,11 @@ __device__ __forceinline__ double share_sum(F at, int64_t v0, int64_t v1, double
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) s[k & 3] += rest_of(x[k].x, x[k].y, c);
   }
-  double sum = (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
 }
 
-// kCached: the CTA's share of p and q at one node lies in dynamic shared memory.
-template <typename T, bool kCached>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_args a) {
+// hold: numbers at the start of a warp's share that stay in dynamic shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_args a, const int hold) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   Node* nodes = reinterpret_cast<Node*>(dynamic);
   float2* held = reinterpret_cast<float2*>(nodes + a.nodes);
@@ -126,22 +121,32 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
 
   // this warp's share of the vocabulary
   const int slots = C * kWarps, slot = rank * kWarps + warp;
-  const int64_t v0 = a.vocab * slot / slots, v1 = a.vocab * (slot + 1) / slots;
-  const int64_t c0 = a.vocab * (rank * kWarps) / slots;          // of the CTA
   int pass = 0, holds = -1;                                    // holds: the node that is in shared memory
-  // p and q at `node` (q is not read where nothing of it is taken off: it is 0 then)
-  auto with_node = [&](int node, double c, auto use) {
+  // What is left at `node` over [u0, u1) of the share that begins at w0 and has its place in shared memory at `own`.  (q is not read where
+  // nothing of it is taken off.)
+  auto sum_of = [&](int node, double c, int64_t w0, float2* own, int64_t u0, int64_t u1) {
     const T* pr = target + node * a.target_stride[1];
     const T* qr = draft + node * a.draft_stride[1];
-    if (kCached && holds == node && c != 0.0) return use([&](int64_t v) { return held[v - c0]; });
-    if (c == 0.0) return use([&](int64_t v) { return make_float2(wide(pr[v]), 0.f); });
-    if (!kCached) return use([&](int64_t v) { return make_float2(wide(pr[v]), wide(qr[v])); });
-    holds = node;
-    return use([&](int64_t v) { return held[v - c0] = make_float2(wide(pr[v]), wide(qr[v])); });
+    auto load = [&](int64_t v) { return make_float2(wide(pr[v]), wide(qr[v])); };
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    if (c == 0.0) {
+      add_left(s, [&](int64_t v) { return make_float2(wide(pr[v]), 0.f); }, u0, u1, c, lane);
+    } else {
+      const int64_t vh = max(u0, min(u1, w0 + hold));
+      if (holds == node) add_left(s, [&](int64_t v) { return own[v - w0]; }, u0, vh, c, lane);
+      else add_left(s, [&](int64_t v) { return own[v - w0] = load(v); }, u0, vh, c, lane);
+      add_left(s, load, vh, u1, c, lane);
+    }
+    double sum = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
   };
   // Sums of max(p - c q, 0) over the shares at `node`: in part[.] of every CTA.
   auto sums = [&](int node, double c) -> const double* {
-    const double sum = with_node(node, c, [&](auto at) { return share_sum(at, v0, v1, c, lane); });
+    const int64_t v0 = a.vocab * slot / slots, v1 = a.vocab * (slot + 1) / slots;
+    const double sum = sum_of(node, c, v0, held + warp * hold, v0, v1);
+    if (c != 0.0) holds = node;
     double* mine = sh.part[pass & 1];
     ++pass;
     if (lane < C) *cluster.map_shared_rank(mine + slot, lane) = sum;
@@ -212,36 +217,47 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
   // that share, [w0, w1), in the CTA that has it: a part of it for each warp
   const int64_t w0 = a.vocab * at / slots, w1 = a.vocab * (at + 1) / slots, n = w1 - w0;
   const int64_t u0 = w0 + n * warp / kWarps, u1 = w0 + n * (warp + 1) / kWarps;
-  __syncthreads();                               // (one warp's share in shared memory, read by all)
-  const double mine = with_node(node, c, [&](auto at) { return share_sum(at, u0, u1, c, lane); });
+  float2* own = held + (at - rank * kWarps) * hold;
+  __syncthreads();                               // (one warp's share in shared memory, read by all: where c is not 0, it holds the node)
+  const double mine = sum_of(node, c, w0, own, u0, u1);
   if (lane == 0) sh.cut[warp] = mine;
   __syncthreads();
   if (place_of(sh.cut, kWarps, bound, run, lane, &run) != warp) return;
-  const int64_t token = with_node(node, c, [&](auto at) {
-    int64_t positive = -1;
-    double before = run;
-    for (int64_t v = u0; v < u1; v += 32) {
-      const float2 x = v + lane < u1 ? at(v + lane) : make_float2(0.f, 0.f);
-      const double r = rest_of(x.x, x.y, c);
-      double s = r;
+  const T* pr = target + node * a.target_stride[1];
+  const T* qr = draft + node * a.draft_stride[1];
+  int64_t token = -1;
+  for (int64_t v = u0; v < u1; v += 32) {
+    const int64_t i = v + lane;
+    const double r = i < u1 ? rest_of(wide(pr[i]), c != 0.0 ? wide(qr[i]) : 0.f, c) : 0.0;
+    double s = r;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && before + s > bound), some = __ballot_sync(0xffffffffu, r > 0.0);
-      if (some) positive = v + 31 - __clz(some);
-      if (over) return v + __ffs(over) - 1;
-      before += __shfl_sync(0xffffffffu, s, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
     }
-    return positive;
-  });
+    const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && run + s > bound), some = __ballot_sync(0xffffffffu, r > 0.0);
+    if (some) token = v + 31 - __clz(some);
+    if (over) {
+      token = v + __ffs(over) - 1;
+      break;
+    }
+    run += __shfl_sync(0xffffffffu, s, 31);
+  }
   if (lane == 0) a.next_token[b] = token;
 }
 
-template <typename T, bool kCached>
-int launch(const fa_verify_args& a, int cluster, size_t smem, cudaStream_t st) {
-  auto kern = verify_kernel<T, kCached>;
+template <typename T>
+int launch_verify(const fa_verify_args& a, cudaStream_t st) {
+  // shares of a few hundred tokens at least, and no more CTAs than run at a time
+  const int sms = sm_count(a.device);
+  int cluster = 1;
+  while (cluster < kMaxCluster && a.vocab > (int64_t)cluster * kThreads * 4 && (int64_t)a.batch * cluster * 2 <= 2 * sms) cluster *= 2;
+  // what fits of a share in shared memory, beside another CTA's, or alone on its SM where there are no more CTAs than SMs
+  const size_t nodes = a.nodes * sizeof(Node), room = ((int64_t)a.batch * cluster <= sms ? 224 : 110) * 1024 - nodes;
+  const int64_t share = a.vocab / (cluster * kWarps) + 1, fit = (int64_t)(room / sizeof(float2) / kWarps);
+  const int hold = (int)(share < fit ? share : fit);
+  const size_t smem = nodes + (size_t)hold * kWarps * sizeof(float2);
+  auto kern = verify_kernel<T>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) {
@@ -260,19 +276,8 @@ int launch(const fa_verify_args& a, int cluster, size_t smem, cudaStream_t st) {
   lc.stream = st;
   lc.attrs = &attr;
   lc.numAttrs = 1;
-  cudaLaunchKernelEx(&lc, kern, a);
+  cudaLaunchKernelEx(&lc, kern, a, hold);
   return check_launch("verify_draft_tree");
-}
-
-template <typename T>
-int launch_verify(const fa_verify_args& a, cudaStream_t st) {
-  // shares of a few hundred tokens at least
-  int cluster = 1;
-  while (cluster < kMaxCluster && a.vocab > (int64_t)cluster * kThreads * 4) cluster *= 2;
-  // a CTA's share in shared memory, beside another CTA's, or alone on its SM where there are no more CTAs than SMs
-  const size_t nodes = a.nodes * sizeof(Node), all = nodes + ((size_t)a.vocab / cluster + kWarps) * sizeof(float2);
-  const size_t room = ((int64_t)a.batch * cluster <= sm_count(a.device) ? 224 : 110) * 1024;
-  return all <= room ? launch<T, true>(a, cluster, all, st) : launch<T, false>(a, cluster, nodes, st);
 }
 
 }  // namespace
