@@ -11,6 +11,8 @@
 //   first: those of a request come one behind the other, and the request with the most of them sets the time.  A warp has an even, contiguous share of the vocabulary, its sums go to all CTAs of the cluster
 //   through distributed shared memory, and every warp adds them up in the same order.  The share that the random number falls into is
 //   cut among the warps of its CTA in the same way, and one of them finds the token.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -81,17 +83,43 @@ __device__ __forceinline__ double rest_of(float p, float q, double c) {
   return r > 0.0 ? r : (r == r ? 0.0 : r);
 }
 
-// Adds up what is left over [v0, v1), by a warp; kAtOnce numbers of a lane are in flight together.
+// The bits of a positive finite x, moved up, are the double x 2^-896 exactly, the smallest and 0 too: an integer product in place of a conversion.
+__device__ __forceinline__ double scaled(float x) { return __longlong_as_double((long long)(__float_as_uint(x) * (1ull << 29))); }
+constexpr double kScale = 0x1p896;
+
+// Adds up what is left over [v0, v1), by a warp, times 1 / kScale; kAtOnce numbers of a lane are in flight together.  top: at least the bits of
+// all numbers; from those of infinity on, the sum is not one (NaN, infinity, negative).  kAll: c is 0.
 constexpr int kAtOnce = 8;
-template <typename F>
-__device__ __forceinline__ void add_left(double (&s)[4], F at, int64_t v0, int64_t v1, double c, int lane) {
-  for (int64_t v = v0 + lane; v < v1; v += 32 * kAtOnce) {
+// from(v): gives the numbers at v + 32 k.
+template <bool kAll, typename F>
+__device__ __forceinline__ void add_left(double (&s)[2], uint32_t& top, F from, uint32_t v0, uint32_t v1, double c, int lane) {
+  auto add = [&](double& to, float2 x) {
+    if (kAll) {
+      top = max(top, __float_as_uint(x.x));
+      to += scaled(x.x);
+      return;
+    }
+    top = max(max(top, __float_as_uint(x.x)), __float_as_uint(x.y));
+    const double r = fma(-c, scaled(x.y), scaled(x.x));
+    if (__double2hiint(r) >= 0) to += r;
+  };
+  uint32_t v = v0 + lane;
+#pragma unroll 1
+  for (; v + 32 * (kAtOnce - 1) < v1; v += 32 * kAtOnce) {
+    auto at = from(v);
     float2 x[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) x[k] = v + 32 * k < v1 ? at(v + 32 * k) : make_float2(0.f, 0.f);
+    for (int k = 0; k < kAtOnce; ++k) x[k] = at(k);
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) s[k & 3] += rest_of(x[k].x, x[k].y, c);
+    for (int k = 0; k < kAtOnce; ++k) add(s[k & 1], x[k]);
   }
+  if (v >= v1) return;
+  auto at = from(v);
+  float2 x[kAtOnce];
+#pragma unroll
+  for (int k = 0; k < kAtOnce - 1; ++k) x[k] = v + 32 * k < v1 ? at(k) : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kAtOnce - 1; ++k) add(s[k & 1], x[k]);
 }
 
 // hold: numbers at the start of a warp's share that stay in dynamic shared memory.
@@ -120,31 +148,45 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
   cluster.sync();                          // all of its CTAs run: their shared memory may be written
 
   // this warp's share of the vocabulary
-  const int slots = C * kWarps, slot = rank * kWarps + warp;
+  const int slots = C * kWarps, slots_log2 = 31 - __clz(slots), slot = rank * kWarps + warp;       // (a power of two)
+  auto share_at = [&](int i) { return (uint32_t)((a.vocab * i) >> slots_log2); };
+  const uint32_t v0 = share_at(slot), v1 = share_at(slot + 1);
   int pass = 0, holds = -1;                                    // holds: the node that is in shared memory
   // What is left at `node` over [u0, u1) of the share that begins at w0 and has its place in shared memory at `own`.  (q is not read where
   // nothing of it is taken off.)
-  auto sum_of = [&](int node, double c, int64_t w0, float2* own, int64_t u0, int64_t u1) {
+  auto sum_of = [&](int node, double c, uint32_t w0, float2* own, uint32_t u0, uint32_t u1) {
     const T* pr = target + node * a.target_stride[1];
     const T* qr = draft + node * a.draft_stride[1];
-    auto load = [&](int64_t v) { return make_float2(wide(pr[v]), wide(qr[v])); };
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    double s[2] = {0.0, 0.0};
+    uint32_t top = 0;
     if (c == 0.0) {
-      add_left(s, [&](int64_t v) { return make_float2(wide(pr[v]), 0.f); }, u0, u1, c, lane);
+      add_left<true>(s, top, [&](uint32_t v) {
+        return [p = pr + v](int k) { return make_float2(wide(p[32 * k]), 0.f); };
+      }, u0, u1, c, lane);
     } else {
-      const int64_t vh = max(u0, min(u1, w0 + hold));
-      if (holds == node) add_left(s, [&](int64_t v) { return own[v - w0]; }, u0, vh, c, lane);
-      else add_left(s, [&](int64_t v) { return own[v - w0] = load(v); }, u0, vh, c, lane);
-      add_left(s, load, vh, u1, c, lane);
+      const uint32_t vh = max(u0, min(u1, w0 + hold));
+      if (holds == node) {
+        add_left<false>(s, top, [&](uint32_t v) { return [o = own + (v - w0)](int k) { return o[32 * k]; }; }, u0, vh, c, lane);
+      } else {
+        add_left<false>(s, top, [&](uint32_t v) {
+          return [p = pr + v, q = qr + v, o = own + (v - w0)](int k) { return o[32 * k] = make_float2(wide(p[32 * k]), wide(q[32 * k])); };
+        }, u0, vh, c, lane);
+      }
+      add_left<false>(s, top, [&](uint32_t v) {
+        return [p = pr + v, q = qr + v](int k) { return make_float2(wide(p[32 * k]), wide(q[32 * k])); };
+      }, vh, u1, c, lane);
     }
-    double sum = (s[0] + s[1]) + (s[2] + s[3]);
+    double sum = (s[0] + s[1]) * kScale;
+    if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {
+      sum = 0.0;
+      for (uint32_t v = u0 + lane; v < u1; v += 32) sum += rest_of(wide(pr[v]), c != 0.0 ? wide(qr[v]) : 0.f, c);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
   };
   // Sums of max(p - c q, 0) over the shares at `node`: in part[.] of every CTA.
   auto sums = [&](int node, double c) -> const double* {
-    const int64_t v0 = a.vocab * slot / slots, v1 = a.vocab * (slot + 1) / slots;
     const double sum = sum_of(node, c, v0, held + warp * hold, v0, v1);
     if (c != 0.0) holds = node;
     double* mine = sh.part[pass & 1];
@@ -215,8 +257,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
   const int at = place_of(part, slots, bound, 0.0, lane, &run);
   if (at < 0 || at / kWarps != rank) return;         // (at >= 0: the sum is positive)
   // that share, [w0, w1), in the CTA that has it: a part of it for each warp
-  const int64_t w0 = a.vocab * at / slots, w1 = a.vocab * (at + 1) / slots, n = w1 - w0;
-  const int64_t u0 = w0 + n * warp / kWarps, u1 = w0 + n * (warp + 1) / kWarps;
+  const uint32_t w0 = share_at(at), n = share_at(at + 1) - w0;
+  const uint32_t u0 = w0 + (uint32_t)((uint64_t)n * warp / kWarps), u1 = w0 + (uint32_t)((uint64_t)n * (warp + 1) / kWarps);
   float2* own = held + (at - rank * kWarps) * hold;
   __syncthreads();                               // (one warp's share in shared memory, read by all: where c is not 0, it holds the node)
   const double mine = sum_of(node, c, w0, own, u0, u1);
@@ -226,8 +268,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
   const T* pr = target + node * a.target_stride[1];
   const T* qr = draft + node * a.draft_stride[1];
   int64_t token = -1;
-  for (int64_t v = u0; v < u1; v += 32) {
-    const int64_t i = v + lane;
+  for (uint32_t v = u0; v < u1; v += 32) {
+    const uint32_t i = v + lane;
     const double r = i < u1 ? rest_of(wide(pr[i]), c != 0.0 ? wide(qr[i]) : 0.f, c) : 0.0;
     double s = r;
 #pragma unroll
@@ -236,9 +278,9 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const fa_verify_arg
       if (lane >= o) s += y;
     }
     const unsigned over = __ballot_sync(0xffffffffu, r > 0.0 && run + s > bound), some = __ballot_sync(0xffffffffu, r > 0.0);
-    if (some) token = v + 31 - __clz(some);
+    if (some) token = (int64_t)v + 31 - __clz(some);
     if (over) {
-      token = v + __ffs(over) - 1;
+      token = (int64_t)v + __ffs(over) - 1;
       break;
     }
     run += __shfl_sync(0xffffffffu, s, 31);
@@ -252,11 +294,14 @@ int launch_verify(const fa_verify_args& a, cudaStream_t st) {
   const int sms = sm_count(a.device);
   int cluster = 1;
   while (cluster < kMaxCluster && a.vocab > (int64_t)cluster * kThreads * 4 && (int64_t)a.batch * cluster * 2 <= 2 * sms) cluster *= 2;
-  // what fits of a share in shared memory, beside another CTA's, or alone on its SM where there are no more CTAs than SMs
-  const size_t nodes = a.nodes * sizeof(Node), room = ((int64_t)a.batch * cluster <= sms ? 224 : 110) * 1024 - nodes;
+  // what fits of a share in shared memory, beside another CTA's, or alone on its SM where there are SMs enough: with all of them asked
+  // for (16 clusters of 8) one cluster waits for another's end, for a cluster lies within one part of the GPU
+  const bool alone = (int64_t)a.batch * cluster <= sms * 3 / 4;
+  const size_t nodes = a.nodes * sizeof(Node), room = (alone ? 224 : 110) * 1024 - nodes;
   const int64_t share = a.vocab / (cluster * kWarps) + 1, fit = (int64_t)(room / sizeof(float2) / kWarps);
   const int hold = (int)(share < fit ? share : fit);
-  const size_t smem = nodes + (size_t)hold * kWarps * sizeof(float2);
+  // (more than half of an SM's, so that CTAs do not share an SM while others have none)
+  const size_t smem = std::max(nodes + (size_t)hold * kWarps * sizeof(float2), (size_t)(alone ? 116 * 1024 : 0));
   auto kern = verify_kernel<T>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
