@@ -12,6 +12,7 @@ import torch
 
 import drafting_reference as ref
 import flash_attn_triton_b200 as fa
+from flash_attn_triton_b200 import _native as native
 from util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -207,10 +208,10 @@ def wide_enough(case):
     return 64 * 4 * 148 // (len(lens) * heads_kv * -(-nodes * heads // heads_kv // 16)) + 64
 
 
-def run_tree(seed, case, new=True, used=None, spoil=None, mask=None, wide=False, **kw):
+def run_tree(seed, case, new=True, used=None, spoil=None, mask=None, wide=False, pads=None, view=lambda x: x, **kw):
     dtype, lens, nodes, heads, heads_kv, dim, page, causal = case
     gen = torch.Generator().manual_seed(seed)
-    kc, vc, table, rows, where = make_cache(gen, dtype, lens, nodes, heads_kv, dim, page, capacity=wide_enough(case) if wide else 0)
+    kc, vc, table, rows, where = make_cache(gen, dtype, lens, nodes, heads_kv, dim, page, pads, wide_enough(case) if wide else 0)
     q, k, v = (rand(gen, len(lens), nodes, h, dim).to(dtype) for h in (heads, heads_kv, heads_kv))
     _, seen = ref.tree(gen, len(lens), nodes, used or [max(1, nodes - 3 * b) for b in range(len(lens))])
     if mask is not None:
@@ -219,13 +220,14 @@ def run_tree(seed, case, new=True, used=None, spoil=None, mask=None, wide=False,
         dead = ~seen.any(1)
         k[dead], v[dead] = spoil, spoil
     scale = kw.pop("softmax_scale", dim ** -0.5)
-    kd, vd = kc.to(DEV), vc.to(DEV)
+    kd, vd = view(kc.to(DEV)), view(vc.to(DEV))
     if not new:
         for b, n in enumerate(lens):
             for i in range(nodes):
                 kd[where(b, n + i)], vd[where(b, n + i)] = k[b, i].to(DEV), v[b, i].to(DEV)
     common = dict(block_table=None if table is None else table.to(DEV), cache_batch_idx=None if rows is None else rows.to(DEV),
-                  softmax_scale=scale, causal=causal, tree_mask=seen.to(DEV), **kw)
+                  softmax_scale=scale, causal=causal, tree_mask=seen.to(DEV),
+                  cache_leftpad=torch.tensor(pads, dtype=torch.int32, device=DEV) if pads else None, **kw)
     if new:
         out = fa.flash_attn_with_kvcache(q.to(DEV), kd, vd, k.to(DEV), v.to(DEV), cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=DEV), **common)
     else:
@@ -280,6 +282,62 @@ def test_rows_that_see_nothing_and_any_mask(i, wide):
     _, seen = run_tree(300 + i, case, mask=lambda m: torch.rand(m.shape, generator=gen) < 0.3, wide=wide)
     out, seen = run_tree(310 + i, case, mask=lambda m: torch.zeros_like(m), wide=wide)
     assert (out == 0).all()
+
+
+@WIDE
+@pytest.mark.parametrize("i", [3, 4, 6, 10, 11])
+def test_tree_in_caches_of_other_layouts(i, wide):
+    """Contiguous ones with padding on the left, head-major ones, views of a larger tensor."""
+    dtype, lens, nodes, heads, heads_kv, dim, page, causal = TREES[i]
+    flat = (dtype, lens, nodes, heads, heads_kv, dim, 0, causal)
+    for new in (True, False):
+        run_tree(400 + i, flat, new=new, wide=wide, pads=[7 * b + 3 for b in range(len(lens))])
+        run_tree(410 + i, TREES[i], new=new, wide=wide, view=lambda x: x.transpose(1, 2).contiguous().transpose(1, 2))
+        run_tree(420 + i, TREES[i], new=new, wide=wide, view=lambda x: torch.cat((x, x, x), 2)[:, :, heads_kv:2 * heads_kv])
+
+
+@WIDE
+@pytest.mark.parametrize("kw", [dict(softmax_scale=-0.1), dict(softmax_scale=0.0), dict(num_splits=1), dict(num_splits=3)])
+@pytest.mark.parametrize("i", [3, 6, 7])
+def test_tree_with_other_scales_and_splits(i, kw, wide):
+    run_tree(430 + i, TREES[i], wide=wide, **kw)
+
+
+@pytest.mark.parametrize("dim,heads,nodes", [(64, 8, 16), (128, 8, 16), (256, 4, 12), (64, 8, 40), (128, 8, 40)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_what_one_sequence_holds_reaches_no_other(dim, heads, nodes, value):
+    """Contexts that are no numbers, in sequences that share a range with others: those come out bit for bit as without them."""
+    gen = torch.Generator().manual_seed(dim + nodes)
+    lens = [500, 130, 700, 90, 260, 40] * 6
+    kc, vc, table, _, _ = make_cache(gen, BF16, lens, nodes, 2, dim, 16, capacity=6000)
+    q, k, v = (rand(gen, len(lens), nodes, h, dim).to(BF16).to(DEV) for h in (heads, 2, 2))
+    seen = ref.tree(gen, 1, nodes)[1][0].to(DEV)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def call(kc, vc):
+        return fa.flash_attn_with_kvcache(q, kc.to(DEV), vc.to(DEV), k, v, cache_seqlens=lengths, block_table=table.to(DEV), tree_mask=seen)
+    want = call(kc, vc)
+    odd = [b for b in range(len(lens)) if b % 3 == 1]
+    for what in range(2):
+        cache = [kc.clone(), vc.clone()]
+        for b in odd:
+            cache[what][table[b, 1].item(), 3] = value
+        got = call(*cache)
+        rest = [b for b in range(len(lens)) if b not in odd]
+        assert torch.equal(got[rest], want[rest]) and not torch.equal(got[odd], want[odd])
+
+
+def test_tree_after_a_wait_that_ran_out():
+    """The kernel for long caches is refused then, before anything is appended; the other one needs no waits."""
+    dev = torch.cuda.current_device()
+    assert native.lib().fa_debug_set_wait_status(dev, 31) == 0
+    try:
+        with pytest.raises(native.DeviceWaitError):
+            run_tree(1, TREES[6], wide=True)
+        run_tree(1, TREES[6], num_splits=1)
+    finally:
+        assert native.lib().fa_device_wait_clear(dev) == 0
+    run_tree(1, TREES[6], wide=True)
 
 
 @pytest.mark.parametrize("batch,longest,nodes,heads,heads_kv,dim,page", [
@@ -457,6 +515,30 @@ def test_verify_borders():
     none = [x[:0] for x in verify_case(1, 1, 3, 9, F32)]
     path, count, token = fa.verify_draft_tree(*(x.to(DEV) for x in none))
     assert path.shape == (0, 3) and count.shape == token.shape == (0,)
+
+
+@pytest.mark.parametrize("batch,vocab", [(1, 300007), (160, 20011), (13, 40009), (16, 40009), (300, 9000)])
+def test_verify_shares_that_shared_memory_has_no_room_for(batch, vocab):
+    """A node is read again for every rejection, partly from shared memory; clusters of 1 to 8."""
+    gen = torch.Generator().manual_seed(batch)
+    base = torch.rand(4, 3, vocab, generator=gen)
+    base[0] *= torch.rand(3, vocab, generator=gen) < 0.5      # zeros, as top-p leaves them
+    base[1] *= 2.0 ** -140                                    # numbers below the smallest normal one
+    p = base.clone()
+    p[[0, 2]] /= base[[0, 2]].double().sum(-1, keepdim=True).float()
+    q = torch.rand(3, vocab, generator=gen).double()
+    q = (q / q.sum(-1, keepdim=True)).float()
+    tokens, parents = torch.randint(vocab, (batch, 3), generator=gen), torch.tensor([-1, 0, 0], dtype=torch.int32)
+    pick = torch.arange(batch) % 4
+    check_verify([tokens, parents, p[pick], q.expand(batch, 3, vocab), 0.8 + 0.2 * torch.rand(batch, 3, generator=gen), torch.rand(batch, generator=gen)])
+    # one number that is none, wherever it lies: no token follows
+    spoilt = p[:2].clone()
+    spoilt[0, 0, vocab - 1], spoilt[1, 0, 5] = math.nan, math.inf
+    for up in (torch.full((3,), -1, dtype=torch.int32), parents):
+        args = [torch.full((2, 3), 7), up, spoilt, q.expand(2, 3, vocab), torch.ones(2, 3), torch.rand(2, generator=gen)]
+        args[2][:, 0, 7] = 0
+        check_verify(args)
+        assert (fa.verify_draft_tree(*(x.to(DEV) for x in args))[2] == -1).all()
 
 
 def test_verified_tokens_are_distributed_as_the_target():
