@@ -542,6 +542,7 @@ __global__ void __launch_bounds__(256, kAppendPerSm) cache_append_kernel(const f
         // (causal: a row sees no node behind its own)
         if (row < n) seen = m[row * p.tree_stride[1]] != 0 && !(p.causal && j > row);
         else
+#pragma unroll 16
           for (int r = p.causal ? j : 0; r < n; ++r) seen |= m[r * p.tree_stride[1]] != 0;
       }
       const uint32_t bits = __ballot_sync(0xffffffffu, seen);

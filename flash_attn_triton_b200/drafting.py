@@ -109,7 +109,8 @@ def kvcache_compact(k_cache, v_cache, cache_seqlens, path, num_accepted, block_t
 
     k_cache, v_cache: fp16 or bf16 caches as in flash_attn_with_kvcache, or lists of them, one per layer, of the same shape, dtype and strides,
     none of which overlaps another; all layers are moved by one launch.  path (batch, n) integers, ascending in its first num_accepted[b]
-    entries; cache_seqlens, num_accepted (batch,).
+    entries; cache_seqlens, num_accepted (batch,).  The rows of drafted tokens belong to one request: requests that name the same cache row
+    (cache_batch_idx), or share a page behind their contexts, may come out with either one's tokens.
 
     With value checks on, values that do not fit raise ValueError and nothing is moved; off (see set_validation), such requests are passed
     over."""
