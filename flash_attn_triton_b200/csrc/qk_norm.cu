@@ -12,6 +12,7 @@
 //   Weight gradients: a thread's sums over its heads, those of a CTA through shared memory, those of the CTAs by a second kernel in
 //   order.  The grid depends on the sizes and the GPU alone, so the result does not change from call to call.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -66,36 +67,31 @@ template <> __device__ __forceinline__ void pairs_of(const Raw<float>& r, float2
   x[2] = make_float2(r.b.x, r.b.y);
   x[3] = make_float2(r.b.z, r.b.w);
 }
-template <typename T> __device__ __forceinline__ void store_pairs(T* p, const float2 (&x)[4]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::pack(x[0].x, x[0].y), Elem<T>::pack(x[1].x, x[1].y), Elem<T>::pack(x[2].x, x[2].y),
-                                            Elem<T>::pack(x[3].x, x[3].y));
-}
-template <> __device__ __forceinline__ void store_pairs(float* p, const float2 (&x)[4]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
-}
-// The other element of each pair, as it was loaded: next to it (interleaved), or in lane `other` of the L that have the head.
-template <int L, bool kSideBySide, typename T> __device__ __forceinline__ Raw<T> other_of(const Raw<T>& r, int other) {
-  Raw<T> z;
-  if constexpr (kSideBySide) {
-    z.v = make_uint4(__byte_perm(r.v.x, 0u, 0x1032), __byte_perm(r.v.y, 0u, 0x1032), __byte_perm(r.v.z, 0u, 0x1032), __byte_perm(r.v.w, 0u, 0x1032));
+// To p and, the second four, to p + off.
+template <bool kApart, typename T> __device__ __forceinline__ void store_pairs(T* p, int off, const float2 (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+    *reinterpret_cast<float4*>(p + off) = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
   } else {
-    z.v = make_uint4(__shfl_sync(0xffffffffu, r.v.x, other, L), __shfl_sync(0xffffffffu, r.v.y, other, L), __shfl_sync(0xffffffffu, r.v.z, other, L),
-                     __shfl_sync(0xffffffffu, r.v.w, other, L));
+    const uint2 a = make_uint2(Elem<T>::pack(x[0].x, x[0].y), Elem<T>::pack(x[1].x, x[1].y));
+    const uint2 b = make_uint2(Elem<T>::pack(x[2].x, x[2].y), Elem<T>::pack(x[3].x, x[3].y));
+    if constexpr (kApart) {
+      *reinterpret_cast<uint2*>(p) = a;
+      *reinterpret_cast<uint2*>(p + off) = b;
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(a.x, a.y, b.x, b.y);
+    }
   }
-  return z;
 }
-template <int L, bool kSideBySide> __device__ __forceinline__ Raw<float> other_of(const Raw<float>& r, int other) {
-  Raw<float> z;
-  if constexpr (kSideBySide) {
-    z.a = make_float4(r.a.y, r.a.x, r.a.w, r.a.z);
-    z.b = make_float4(r.b.y, r.b.x, r.b.w, r.b.z);
-  } else {
-    auto from = [&](float x) { return __shfl_sync(0xffffffffu, x, other, L); };
-    z.a = make_float4(from(r.a.x), from(r.a.y), from(r.a.z), from(r.a.w));
-    z.b = make_float4(from(r.b.x), from(r.b.y), from(r.b.z), from(r.b.w));
+// The other element of each pair of a lane's 8: next to it, or four further on.  unpaired: elements that are not rotated (0 times their neighbour, an
+// infinity, would be no number).
+template <bool kSideBySide> __device__ __forceinline__ void others_of(const float2 (&x)[4], float2 (&z)[4], bool unpaired) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = kSideBySide ? make_float2(x[e].y, x[e].x) : x[e ^ 2];
+  if (unpaired) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = make_float2(0.f, 0.f);
   }
-  return z;
 }
 template <typename T> __device__ __forceinline__ float one(const T* p);
 template <> __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
@@ -111,27 +107,19 @@ template <typename T> __device__ __forceinline__ float at(const void* p, int wid
   return wide ? static_cast<const float*>(p)[i] : one(static_cast<const T*>(p) + i);
 }
 
-// kN (4 or 8) numbers of a table from p on, aligned to their size.
-template <typename T, int kN> __device__ __forceinline__ void entries(const void* p, int wide, int64_t i, float (&x)[8]) {
+// Four numbers of a table, aligned to their size.
+template <typename T> __device__ __forceinline__ void entries(const void* p, int wide, int64_t i, float (&x)[8]) {
   if (wide) {
-    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-#pragma unroll
-    for (int k = 0; k < kN / 4; ++k) {
-      const float4 v = f[k];
-      x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
-    }
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
   } else if constexpr (sizeof(T) == 2) {
-    const uint2* f = reinterpret_cast<const uint2*>(static_cast<const T*>(p) + i);
-#pragma unroll
-    for (int k = 0; k < kN / 4; ++k) {
-      const uint2 v = f[k];
-      const float2 a = Elem<T>::unpack(v.x), b = Elem<T>::unpack(v.y);
-      x[4 * k] = a.x; x[4 * k + 1] = a.y; x[4 * k + 2] = b.x; x[4 * k + 3] = b.y;
-    }
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const T*>(p) + i);
+    const float2 a = Elem<T>::unpack(v.x), b = Elem<T>::unpack(v.y);
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
   }
 }
 
-// The rotation of this lane's 8 elements d .. d + 7 of a head, as cos and sin per element; elements behind rotary_dim have cos = 1,
+// The rotation of this lane's 8 elements of a head -- from d on, or whole halves: four from d on and their partners --, as cos and sin per element; those behind rotary_dim have cos = 1,
 // sin = 0.  The sign of the sine is that of the forward rotation of the element: out = y cos + (its pair's y) sin.
 template <typename T>
 __device__ __forceinline__ void angles(const fa_qk_norm_args& p, bool whole, int64_t pos, int d, float (&c)[8], float (&s)[8]) {
@@ -144,22 +132,15 @@ __device__ __forceinline__ void angles(const fa_qk_norm_args& p, bool whole, int
     }
     return;
   }
-  if (whole) {                                   // these 8 have 8 entries in a row, side by side pairs 4
-    if (p.interleaved) {
-      float x[8];
-      entries<T, 4>(p.cos, p.table_wide, pos * half + (d >> 1), x);
+  if (whole) {                                   // 4 pairs with 4 entries in a row
+    const int64_t i = pos * half + (p.interleaved ? d >> 1 : d);
+    float x[8];
+    entries<T>(p.cos, p.table_wide, i, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] = x[e >> 1];
-      entries<T, 4>(p.sin, p.table_wide, pos * half + (d >> 1), x);
+    for (int e = 0; e < 8; ++e) c[e] = p.interleaved ? x[e >> 1] : x[e & 3];
+    entries<T>(p.sin, p.table_wide, i, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = e & 1 ? x[e >> 1] : -x[e >> 1];
-    } else {
-      const int64_t i = pos * half + (d < half ? d : d - half);
-      entries<T, 8>(p.cos, p.table_wide, i, c);
-      entries<T, 8>(p.sin, p.table_wide, i, s);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = d < half ? -s[e] : s[e];
-    }
+    for (int e = 0; e < 8; ++e) s[e] = p.interleaved ? (e & 1 ? x[e >> 1] : -x[e >> 1]) : (e & 4 ? x[e & 3] : -x[e & 3]);
     return;
   }
 #pragma unroll
@@ -223,12 +204,6 @@ struct Sides {
   Side side[2];
 };
 
-// The lane with the other halves of this lane's pairs.
-__device__ __forceinline__ int other_lane(const fa_qk_norm_args& p, int lane) {
-  const int half = p.rotary_dim >> 1, d = lane * 8;
-  return d < half ? lane + half / 8 : d < p.rotary_dim ? lane - half / 8 : lane;
-}
-
 // The table rows of a position, on their way to L1.
 __device__ __forceinline__ void prefetch_angles(const fa_qk_norm_args& p, int64_t pos, int d, int bytes) {
   const int half = p.rotary_dim >> 1;
@@ -240,21 +215,26 @@ __device__ __forceinline__ void prefetch_angles(const fa_qk_norm_args& p, int64_
 
 constexpr int kSlots = 8;                        // 16-byte slots of a thread's ring
 
-// kTurn: whether a lane's 8 elements are turned as one (whole_lanes()), and where the other elements of their pairs are.  If they are, and with x' the other element of each pair, the forward is
-// r (x (c w) + x' (s w')), the two products in brackets made once for all heads of a token, and all of it in pairs of fp32: element by
-// element, 177 instructions for 8 elements of a lane bound the forward, 253 the backward.  ws: backward, D sums of every CTA for q, then for k.
+// kTurn: whether a lane has four whole pairs (whole_lanes()): 8 elements in a row where a pair lies side by side, else four of the first half and
+// the four that belong to them.  If it has, and with x' the other element of each pair, the forward is r (x (c w) + x' (s w')), the two products in brackets made
+// once for all heads of a token, and all of it in pairs of fp32: element by element, 177 instructions for 8 elements of a lane bound the forward, 253 the
+// backward.  Partners from another lane's 8 in a row took a shuffle and an unpacking more for each pair.
+// kAll: the whole head is rotated.  ws: backward, D sums of every CTA for q, then for k.
 enum Turn { kAnyhow, kHalves, kSideBySide };
-template <typename T, int D, bool kBackward, Turn kTurn>
+template <typename T, int D, bool kBackward, Turn kTurn, bool kAll>
 __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(const fa_qk_norm_args p, const Sides sides, float* ws) {
   constexpr bool kWhole = kTurn != kAnyhow;
   constexpr int L = D / 8, G = kThreads / L;
   constexpr int W = sizeof(T) / 2, kOf = W * (kBackward ? 2 : 1), S = kSlots / kOf;      // slots of 8 elements, of a head; heads in flight
   __shared__ uint4 ring[kSlots][kThreads];
   __shared__ float rows[kWhole ? 1 : G][kWhole ? 1 : D];
-  const int tid = threadIdx.x, group = tid / L, lane = tid % L, d = lane * 8;
+  const int tid = threadIdx.x, group = tid / L, lane = tid % L;
   const int entry = p.table_wide ? 4 : (int)sizeof(T);
-  const int other = other_lane(p, lane);
-  const bool side_by_side = p.interleaved != 0;
+  // the lane's elements: d .. d + 3 and d + off .. d + off + 3
+  constexpr bool kApart = kTurn == kHalves;
+  const int half = p.rotary_dim >> 1;
+  const int d = kApart && lane < half / 4 ? lane * 4 : kApart ? 2 * half + (lane - half / 4) * 8 : lane * 8;
+  const int off = kApart && lane < half / 4 ? half : 4;
   const int64_t groups = (int64_t)gridDim.x * G, me = (int64_t)blockIdx.x * G + group, tokens = (int64_t)p.batch * p.seqlen;
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
@@ -263,10 +243,11 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
     float2 w[4], wo[4], dw[4];                   // weights, those of the other elements of the pairs
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      w[e] = a.weight ? make_float2(at<T>(a.weight, p.weight_wide, d + 2 * e), at<T>(a.weight, p.weight_wide, d + 2 * e + 1)) : make_float2(1.f, 1.f);
-      wo[e] = side_by_side ? make_float2(w[e].y, w[e].x) : make_float2(__shfl_sync(0xffffffffu, w[e].x, other, L), __shfl_sync(0xffffffffu, w[e].y, other, L));
+      const int i = d + (e & 1) * 2 + (e >> 1) * off;
+      w[e] = a.weight ? make_float2(at<T>(a.weight, p.weight_wide, i), at<T>(a.weight, p.weight_wide, i + 1)) : make_float2(1.f, 1.f);
       dw[e] = make_float2(0.f, 0.f);
     }
+    others_of<kTurn == kSideBySide>(w, wo, false);
     // this group's heads: `mine` of them from `begin` on; the groups of a warp stay together for `steps`
     const int64_t total = tokens * heads, begin = total * me / groups;
     const int mine = (int)(total * (me + 1) / groups - begin), steps = (int)((total + groups - 1) / groups);
@@ -281,14 +262,22 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
     constexpr uint32_t kPitch = kThreads * 16;
     const uint32_t own = smem_u32(&ring[0][tid]);
     uint32_t turn = 0;                           // of the ring: bytes from this thread's first slot
+    auto fetch = [&](uint32_t to, const T* from) {
+      if constexpr (W == 2) {
+        cp_async16(to, from, 16);
+        cp_async16(to + kPitch, from + off, 16);
+      } else if constexpr (kApart) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to), "l"(from) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8), "l"(from + off) : "memory");
+      } else {
+        cp_async16(to, from, 16);
+      }
+    };
     auto ask = [&](uint32_t to) {
       if (left > 0) {
         --left;
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-          cp_async16(to + k * kPitch, lx + k * (16 / sizeof(T)), 16);
-          if (kBackward) cp_async16(to + (W + k) * kPitch, lg + k * (16 / sizeof(T)), 16);
-        }
+        fetch(to, lx);
+        if (kBackward) fetch(to + W * kPitch, lg);
         lx += xh;
         if (kBackward) lg += gh;
         if (++lh == heads) {
@@ -356,18 +345,18 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
       if constexpr (kWhole && !kBackward) {
         float2 y[4], z[4], sq = make_float2(0.f, 0.f);
         pairs_of<T>(xr, y);
-        pairs_of<T>(other_of<L, kTurn == kSideBySide>(xr, other), z);
+        others_of<kTurn == kSideBySide>(y, z, !kAll && d >= p.rotary_dim);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sq = f2fma(y[e], y[e], sq);
         const float r = rsqrtf(group_sum<L>(sq.x + sq.y) * (1.f / D) + p.eps);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = f2mul(f2fma(z[e], s[e], f2mul(y[e], c[e])), make_float2(r, r));
-        if (live) store_pairs(out, y);
+        if (live) store_pairs<kApart>(out, off, y);
       } else if constexpr (kWhole) {
         float2 x[4], g[4], z[4], sq = make_float2(0.f, 0.f), hx = make_float2(0.f, 0.f);
         pairs_of<T>(xr, x);
         pairs_of<T>(gr, g);
-        pairs_of<T>(other_of<L, kTurn == kSideBySide>(gr, other), z);
+        others_of<kTurn == kSideBySide>(g, z, !kAll && d >= p.rotary_dim);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           g[e] = f2fma(z[e], make_float2(-s[e].x, -s[e].y), f2mul(g[e], c[e]));     // rotated back
@@ -383,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
             dw[e] = f2fma(z[e], make_float2(r, r), dw[e]);
             x[e] = f2fma(x[e], make_float2(k, k), f2mul(f2mul(g[e], w[e]), make_float2(r, r)));
           }
-          store_pairs(out, x);
+          store_pairs<kApart>(out, off, x);
         }
       } else {
         float x[8], g[8], z[8], sq = 0.f, hx = 0.f;
@@ -444,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
     __syncthreads();
     float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(sums + group * D + d + 2 * e) = dw[e];
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(sums + group * D + d + (e & 1) * 2 + (e >> 1) * off) = dw[e];
     __syncthreads();
     for (int i = tid; i < D; i += kThreads) {
       float sum = 0.f;
@@ -476,10 +465,10 @@ int grid_of(const fa_qk_norm_args& a, bool backward) {
   const int64_t need = ((int64_t)a.batch * a.seqlen * std::max(a.heads_q, a.heads_kv) + groups - 1) / groups, fit = (backward ? 2ll : 3ll) * sm_count(a.device);
   return (int)(need < fit ? need : fit);
 }
-// The 8 elements of a lane are turned as one: see angles().
+// The 8 elements of a lane are four pairs: see angles().
 bool whole_lanes(const fa_qk_norm_args& a) {
   const int half = a.rotary_dim / 2;
-  return half % (a.interleaved ? 4 : 8) == 0 && ((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15) == 0 &&
+  return half % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15) == 0 &&
          (a.dtype != FA_F32 || a.table_wide);
 }
 
@@ -500,17 +489,18 @@ template <typename T, int D> int run(const fa_qk_norm_args& a, bool backward, cu
   }
   const bool whole = whole_lanes(a);
   const int grid = grid_of(a, backward);
-  if (!backward) {
-    if (!whole) qk_norm_kernel<T, D, false, kAnyhow><<<grid, kThreads, 0, st>>>(a, sides, nullptr);
-    else if (a.interleaved) qk_norm_kernel<T, D, false, kSideBySide><<<grid, kThreads, 0, st>>>(a, sides, nullptr);
-    else qk_norm_kernel<T, D, false, kHalves><<<grid, kThreads, 0, st>>>(a, sides, nullptr);
-    return check_launch("qk_norm");
-  }
-  float* ws = a.d_q_weight || a.d_k_weight ? static_cast<float*>(a.workspace) : nullptr;
-  if (!whole) qk_norm_kernel<T, D, true, kAnyhow><<<grid, kThreads, 0, st>>>(a, sides, ws);
-  else if (a.interleaved) qk_norm_kernel<T, D, true, kSideBySide><<<grid, kThreads, 0, st>>>(a, sides, ws);
-  else qk_norm_kernel<T, D, true, kHalves><<<grid, kThreads, 0, st>>>(a, sides, ws);
-  if (int r = check_launch("qk_norm_bwd")) return r;
+  float* ws = backward && (a.d_q_weight || a.d_k_weight) ? static_cast<float*>(a.workspace) : nullptr;
+  auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, st>>>(a, sides, ws); };
+  auto turned = [&](auto direction) {
+    constexpr bool kBackward = decltype(direction)::value;
+    const bool all = a.rotary_dim == D;
+    if (!whole) launch(qk_norm_kernel<T, D, kBackward, kAnyhow, true>);
+    else if (a.interleaved) all ? launch(qk_norm_kernel<T, D, kBackward, kSideBySide, true>) : launch(qk_norm_kernel<T, D, kBackward, kSideBySide, false>);
+    else all ? launch(qk_norm_kernel<T, D, kBackward, kHalves, true>) : launch(qk_norm_kernel<T, D, kBackward, kHalves, false>);
+  };
+  if (backward) turned(std::true_type{});
+  else turned(std::false_type{});
+  if (int r = check_launch(backward ? "qk_norm_bwd" : "qk_norm")) return r;
   if (ws == nullptr) return FA_OK;
   qk_norm_dw_kernel<T><<<2 * D / (kThreads / 32), kThreads, 0, st>>>(ws, grid, D, a.d_q_weight, a.d_k_weight, a.weight_wide);
   return check_launch("qk_norm_dw");

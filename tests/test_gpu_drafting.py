@@ -152,6 +152,7 @@ def test_norm_is_the_same_every_time_and_over_strides():
 
 
 def test_norm_of_zeros_and_of_rows_that_are_no_numbers():
+    """A row with an infinity has the norm of one: its numbers become 0, the infinity none."""
     q = torch.ones(1, 4, 2, 64, dtype=F16)
     q[0, 0] = 0
     q[0, 1, 0, 3], q[0, 2, 1, 7] = math.nan, math.inf
@@ -162,6 +163,10 @@ def test_norm_of_zeros_and_of_rows_that_are_no_numbers():
     assert (a[0, 0] == 0).all() and torch.isfinite(g[0, 0]).all()
     for out in (a, b):
         assert out[0, 1, 0].isnan().all() and torch.isfinite(out[0, 1, 1]).all() and torch.isfinite(out[0, 2, 0]).all() and (out[0, 3] == 1).all()
+        assert out[0, 2, 1, 7].isnan() and (out[0, 2, 1, :7] == 0).all() and (out[0, 2, 1, 8:] == 0).all()
+    angle = torch.zeros(4, 16, dtype=F16, device=DEV)
+    out = fa.qk_norm_rotary(x, x, w, w, angle + 1, angle)[0]                                # the 32 that are not rotated, and the rest but the pair
+    assert out[0, 2, 1, 7].isnan() and (out[0, 2, 1, 32:] == 0).all() and (out[0, 2, 1, 8:23] == 0).all()
 
 
 # ---- attention under the mask of a tree -------------------------------------------------------------------------------------------
