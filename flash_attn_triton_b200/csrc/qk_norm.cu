@@ -256,9 +256,9 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
 
     // loading: S heads ahead of their use
     const int64_t xh = a.xs[2], gh = a.gs[2], oh = a.os[2];
-    int lb = b0, lt = t0, lh = h0, left = mine;
-    const T* lx = static_cast<const T*>(a.x) + lb * a.xs[0] + lt * a.xs[1] + lh * xh + d;
-    const T* lg = kBackward ? static_cast<const T*>(a.g) + lb * a.gs[0] + lt * a.gs[1] + lh * gh + d : nullptr;
+    int lb = b0, lt = t0, asked = 0, ask_end = heads - h0;       // steps, the one with which the token ends
+    const T* lx = static_cast<const T*>(a.x) + lb * a.xs[0] + lt * a.xs[1] + h0 * xh + d;
+    const T* lg = kBackward ? static_cast<const T*>(a.g) + lb * a.gs[0] + lt * a.gs[1] + h0 * gh + d : nullptr;
     constexpr uint32_t kPitch = kThreads * 16;
     const uint32_t own = smem_u32(&ring[0][tid]);
     uint32_t turn = 0;                           // of the ring: bytes from this thread's first slot
@@ -274,14 +274,13 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
       }
     };
     auto ask = [&](uint32_t to) {
-      if (left > 0) {
-        --left;
+      if (asked < mine) {
         fetch(to, lx);
         if (kBackward) fetch(to + W * kPitch, lg);
         lx += xh;
         if (kBackward) lg += gh;
-        if (++lh == heads) {
-          lh = 0;
+        if (++asked == ask_end) {
+          ask_end += heads;
           if (++lt == p.seqlen) {
             lt = 0;
             ++lb;
@@ -311,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
 #pragma unroll
     for (int k = 0; k < S; ++k) ask(own + k * kOf * kPitch);
 
-    int b = b0, t = t0, h = h0;
+    int b = b0, t = t0;
     auto position_of = [&](int pb, int pt) {
       return p.positions ? (int64_t)p.positions[pb * p.pos_stride[0] + pt * p.pos_stride[1]] : (int64_t)pt;
     };
@@ -330,9 +329,11 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
       }
     };
     int64_t next_pos = 0;
-    T* out = static_cast<T*>(a.out) + b * a.os[0] + t * a.os[1] + h * oh + d;
+    T* out = static_cast<T*>(a.out) + b * a.os[0] + t * a.os[1] + h0 * oh + d;
     if (mine > 0) turn_to(position_of(b, t));
-    bool fresh = true;                           // the next token's position is not known yet
+    // steps with which this token ends, and with which something is to be done: the next token's angles are asked for four heads ahead
+    int end = heads - h0, event = kWhole ? max(end - 4, 1) : end;
+    bool known = false;                          // the next token's position
 #pragma unroll 1
     for (int step = 0; step < steps; ++step) {
       cp_async_wait<S - 1>();
@@ -407,22 +408,24 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
         if (live) store8(out, x);
       }
       // on to the next head
-      if (step + 1 < mine) {
-        out += oh;
-        if (++h == heads) {
-          h = 0;
-          if (++t == p.seqlen) {
-            t = 0;
-            ++b;
+      out += oh;
+      if (step + 1 == event && event < mine) {
+        const bool wraps = t + 1 == p.seqlen;
+        if (event < end) {
+          if (end < mine) {
+            next_pos = position_of(b + wraps, wraps ? 0 : t + 1);
+            known = true;
+            prefetch_angles(p, next_pos, d, entry);
           }
+          event = end;
+        } else {
+          t = wraps ? 0 : t + 1;
+          b += wraps;
           out = static_cast<T*>(a.out) + b * a.os[0] + t * a.os[1] + d;
-          turn_to(fresh ? position_of(b, t) : next_pos);
-          fresh = true;
-        } else if (kWhole && fresh && h + 4 >= heads && mine - step - 1 > heads - h) {
-          const bool end = t + 1 == p.seqlen;
-          next_pos = position_of(b + end, end ? 0 : t + 1);
-          fresh = false;
-          prefetch_angles(p, next_pos, d, entry);
+          turn_to(known ? next_pos : position_of(b, t));
+          known = false;
+          event = kWhole ? max(end + heads - 4, end + 1) : end + heads;
+          end += heads;
         }
       }
       __syncwarp();
