@@ -3,12 +3,12 @@
 //   Mathematics.  r = rsqrt(mean(x^2) + eps), y = x r w, out = R y with R the rotation of the pairs.  R is orthogonal, so g = R^T dout; then
 //   dw = sum g x r, and with h = g w:  dx = r (h - x r^2 mean(h x)).  Both means of the backward pass are sums over the head that do not wait
 //   for one another.
-//   Bound.  HBM: forward 2, backward 3 words an element.  D / 8 lanes have a head and 8 elements each, 16 bytes of a 16-bit type, so that a
-//   head is one access, its sums are shuffles, and a pair's other half (rotate-half) comes from another lane of the head.  A group of
-//   lanes has an even share of all heads of all tokens, one after another, with a token's angles in registers, first of q and then of k, so
-//   that a thread has one set of weights and sums at a time and divides only where its share begins.  Every thread has a ring of its own in shared memory that its loads go to
-//   (cp.async, 128 bytes in flight), so that no barrier is needed and registers do not bound the loads in flight: 16380 tokens of 40 heads
-//   of 128, bf16, forward 62 us (69 with four loads in registers), 0.83 of the copy rate, backward 91 (110), 0.85.
+//   Bound.  HBM: forward 2, backward 3 words an element.  D / 8 lanes have a head and 8 elements each: the two halves of four pairs (rotate-half), 8
+//   in a row otherwise.  Its sums are shuffles.  A group of lanes has an even share of all heads of all tokens, one after another, with a token's
+//   angles in registers, first of q and then of k, so that a thread has one set of weights and sums at a time and divides only where its
+//   share begins.  Every thread has a ring of its own in shared memory that its loads go to (cp.async, 128 bytes in flight), so that no
+//   barrier is needed and registers do not bound the loads in flight.  16380 tokens of 40 heads of 128, bf16, forward 58 to 60 us, 0.86 of the copy rate,
+//   backward 89, 0.86, what is left being instructions (two thirds of the issue slots): with four loads in registers and partners from another lane 69 and 110.
 //   Weight gradients: a thread's sums over its heads, those of a CTA through shared memory, those of the CTAs by a second kernel in
 //   order.  The grid depends on the sizes and the GPU alone, so the result does not change from call to call.
 #include <algorithm>
@@ -199,6 +199,8 @@ struct Side {
   const void* weight;
   int64_t xs[3], gs[3], os[3];
   int heads;
+  bool few;                                      // heads of all tokens: 32 bits count them
+  int64_t share, more;                           // of a group, and how many groups have one more
 };
 struct Sides {
   Side side[2];
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
   const int half = p.rotary_dim >> 1;
   const int d = kApart && lane < half / 4 ? lane * 4 : kApart ? 2 * half + (lane - half / 4) * 8 : lane * 8;
   const int off = kApart && lane < half / 4 ? half : 4;
-  const int64_t groups = (int64_t)gridDim.x * G, me = (int64_t)blockIdx.x * G + group, tokens = (int64_t)p.batch * p.seqlen;
+  const int64_t me = (int64_t)blockIdx.x * G + group;
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     const Side& a = sides.side[which];
@@ -249,10 +251,20 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 2 : 3) qk_norm_kernel(co
     }
     others_of<kTurn == kSideBySide>(w, wo, false);
     // this group's heads: `mine` of them from `begin` on; the groups of a warp stay together for `steps`
-    const int64_t total = tokens * heads, begin = total * me / groups;
-    const int mine = (int)(total * (me + 1) / groups - begin), steps = (int)((total + groups - 1) / groups);
-    const int64_t token = heads ? begin / heads : 0;
-    const int b0 = (int)(token / p.seqlen), t0 = (int)(token - (int64_t)b0 * p.seqlen), h0 = (int)(begin - token * heads);
+    const int64_t begin = a.share * me + (me < a.more ? me : a.more);
+    const int mine = (int)a.share + (me < a.more), steps = (int)a.share + (a.more > 0);
+    int b0 = 0, t0 = 0, h0 = 0;
+    if (a.few) {                                 // (64-bit divisions take a hundred instructions each)
+      const uint32_t token = (uint32_t)begin / (uint32_t)max(heads, 1);
+      h0 = (int)((uint32_t)begin - token * heads);
+      b0 = (int)(token / (uint32_t)p.seqlen);
+      t0 = (int)(token - (uint32_t)b0 * p.seqlen);
+    } else {
+      const int64_t token = begin / heads;
+      h0 = (int)(begin - token * heads);
+      b0 = (int)(token / p.seqlen);
+      t0 = (int)(token - (int64_t)b0 * p.seqlen);
+    }
 
     // loading: S heads ahead of their use
     const int64_t xh = a.xs[2], gh = a.gs[2], oh = a.os[2];
@@ -492,6 +504,12 @@ template <typename T, int D> int run(const fa_qk_norm_args& a, bool backward, cu
   }
   const bool whole = whole_lanes(a);
   const int grid = grid_of(a, backward);
+  for (Side& s : sides.side) {
+    const int64_t all = (int64_t)a.batch * a.seqlen * s.heads, groups = (int64_t)grid * (kThreads / (D / 8));
+    s.few = all <= UINT32_MAX;
+    s.share = all / groups;
+    s.more = all % groups;
+  }
   float* ws = backward && (a.d_q_weight || a.d_k_weight) ? static_cast<float*>(a.workspace) : nullptr;
   auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, st>>>(a, sides, ws); };
   auto turned = [&](auto direction) {

@@ -14,12 +14,15 @@
 //
 //   warps 0-7   softmax pair 0  : every other tile of keys, warps 0-3 its first 64 keys, warps 4-7 the other 64
 //   warps 8-15  softmax pair 1  : the other tiles
-//   warp  16    TMA producer    : Q of a segment, K/V through a ring of 128-key x 128-column entries
-//   warp  17    MMA issuer      : S[j] = Q K_j^T (SS);  O += P_j V_j (A = P_j from tensor memory)
-//   warps 18-19 idle (they complete the warpgroup that gives its registers to the softmax warps)
+//   two warps   TMA producer    : Q of a segment, K/V through a ring of 128-key x 128-column entries
+//               MMA issuer      : S[j] = Q K_j^T (SS);  O += P_j V_j (A = P_j from tensor memory)
+//   two warps   results of a segment, up to 64 rows and head_dim up to 128 (kApart); else idle (they complete the warpgroup that gives its
+//               registers to the softmax warps), and the softmax warps write the results
 //
 // Tensor memory and the reference of the exponents: as in fwd_alt_sm100.cu.  Here the tiles of all segments are counted through (J), and
-// barrier parities follow that count.  What a tile costs beside its bytes counts twice, for the memory and the SMs together reach the limit of
+// barrier parities follow that count.  kApart has two accumulators (and at head_dim 128 a score buffer less), so that the end of a segment lies under the
+// next one's tiles: 16-node trees of 144 sequences of 512 tokens, 32 heads over 8, 82 -> 75 us, at head_dim 64 61 -> 51; 18 of 4096 60 -> 61, 46 -> 41.
+// What a tile costs beside its bytes counts twice, for the memory and the SMs together reach the limit of
 // the GPU's power, and the clock falls.  18 x 16384 tokens, 64 rows over each of 8 KV heads of 128 (floor 185 us): two groups of four
 // softmax warps, a tile each, 254 us, also out of L2; four warps per scheduler 228; P rounded to 16 bits once and not in two parts, as chunks of
 // a cache have it, and no work on rows that do not exist 185.  (Errors against float64, fp16, 4 to 16 nodes: 2.1e-4 of two parts, 2.6e-4.)
@@ -65,8 +68,8 @@ struct TShared {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kMaxStages], kv_empty[kMaxStages];
   uint64_t s_full[3];      // [buffer]: scores computed
-  // (Barriers that count threads: none may arrive for a phase before the one ahead of it is complete, see fwd_alt_sm100.cu; between
-  // segments all softmax threads meet.)
+  // (Barriers that count threads: none may arrive for a phase before the one ahead of it is complete, see fwd_alt_sm100.cu: every tile waits
+  // for the decision about the one before, the first of a segment too.)
   uint64_t p_ready[2][3];  // [half][buffer]: P of these warps written back (128 arrivals)
   uint64_t o_done[3];      // [buffer]: its P V finished
   uint64_t decided[2];     // [pair]: mref settled for the pair's tile (256 arrivals)

@@ -5,12 +5,15 @@
 //   is the number c, which grows by Z, and Z, the mass that is then left.  The first child of a node has c = 0, Z = 1 and reads two numbers; only
 //   a node with a rejected child and another one behind it, and the node where the path ends, is read over its whole vocabulary.
 //   Sums and products are in 64 bits: a decision next to a border then depends on the order of a sum only within 1e-16 of it.
-//   Bound.  Latency for small batches, else 2 vocab words a request out of HBM and the conversions to 64 bits.
-//   A cluster of CTAs has a request.  Each loads all nodes' numbers at once and walks the tree on its own (ballots over 32 nodes), so
-//   that the walk takes no round trip to memory.  The node at hand stays in shared memory where it fits (kCached), for the passes after the
-//   first: those of a request come one behind the other, and the request with the most of them sets the time.  A warp has an even, contiguous share of the vocabulary, its sums go to all CTAs of the cluster
-//   through distributed shared memory, and every warp adds them up in the same order.  The share that the random number falls into is
-//   cut among the warps of its CTA in the same way, and one of them finds the token.
+//   Bound.  Latency for small batches, else 2 vocab words a request out of HBM; after that the passes of one request, which come one behind the
+//   other: a pass of 100003 tokens takes a request 2.4 us where its CTAs have an SM each, 3.7 where two share one, most of it instructions and the
+//   cluster's barrier.  A number becomes a double by an integer product and not by a conversion, of which an SM makes 16 a clock.
+//   A cluster of CTAs has a request, as large as all requests leave room for: a second wave starts from the beginning (64 requests of 100003 tokens,
+//   one pass each: clusters of 8 in two waves 20.2 us, of 4 in one 12.3, now 9.7).  Each CTA loads all nodes' numbers at once and walks the tree on its own (ballots
+//   over 32 nodes), so that the walk takes no round trip to memory.  What fits of the node at hand stays in shared memory for the passes after the first.
+//   A warp has an even, contiguous share of the vocabulary, its sums go to all CTAs of the cluster through distributed shared memory, and every
+//   warp adds them up in the same order.  The share that the random number falls into is cut among the warps of its CTA in the same way, and one of
+//   them finds the token.
 #include <algorithm>
 
 #include <cooperative_groups.h>
