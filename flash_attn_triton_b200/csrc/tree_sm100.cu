@@ -25,7 +25,9 @@
 // What a tile costs beside its bytes counts twice, for the memory and the SMs together reach the limit of
 // the GPU's power, and the clock falls.  18 x 16384 tokens, 64 rows over each of 8 KV heads of 128 (floor 185 us): two groups of four
 // softmax warps, a tile each, 254 us, also out of L2; four warps per scheduler 228; P rounded to 16 bits once and not in two parts, as chunks of
-// a cache have it, and no work on rows that do not exist 185.  (Errors against float64, fp16, 4 to 16 nodes: 2.1e-4 of two parts, 2.6e-4.)
+// a cache have it, and no work on rows that do not exist 185; 16 rows, softmax for 32 in place of 64, 48 x 500 to 12000 tokens 245 -> 238.  (Errors against float64, fp16, 4 to 16 nodes: 2.1e-4 of two parts, 2.6e-4.)
+#include <type_traits>
+
 #include "cache_geo.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
@@ -156,12 +158,13 @@ __device__ __forceinline__ int ranges_of(int64_t total, int batch, int parts) {
 }  // namespace
 
 // geo.parts: ranges that the grid has room for.
-// kSplit = 2: no more than 64 query rows.
+// kSplit: 128 / kSplit query rows at most (1, 2 or 4); warps and results of the others are left out.
 template <typename T, int D, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const fa_attn_args p, const float scale_log2, const float rescale_at, const CacheGeo geo, int* const host_status) {
   constexpr bool kApart = kSplit > 1 && D <= 128;
+  constexpr int kRows = kBM / kSplit;
   using C = TCfg<D, kApart>;
   constexpr int S = C::kStages, NB = C::kSBuf, NU = C::kUnits, NQ = C::kQBuf, NO = C::kOBuf;
   constexpr int kTmaWarp = kApart ? 18 : 16, kMmaWarp = kTmaWarp + 1;
@@ -226,7 +229,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     mbar_init(smem_u32(&sh->decided[0]), 256 / kSplit);
     mbar_init(smem_u32(&sh->decided[1]), 256 / kSplit);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sh->o_free[i]), kApart ? kBM / 2 : kSoftmax / kSplit);
+      mbar_init(smem_u32(&sh->o_free[i]), kApart ? kRows : kSoftmax / kSplit);
       mbar_init(smem_u32(&sh->o_last[i]), 1);
       mbar_init(smem_u32(&sh->ended[i]), kSoftmax / kSplit);
     }
@@ -237,9 +240,10 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tmem_alloc(smem_u32(&sh->tmem_base), 512);
     tmem_relinquish();
   }
-  if (kSplit > 1) {                                            // rows that do not exist: 0, and so are their scores and probabilities
-    for (int i = tid; i < NQ * (D / 64) * (kBM / 2) * 8; i += kThreads)
-      st_shared_v4(sQ + i / ((kBM / 2) * 8) * (kBM * 128) + (kBM / 2) * 128 + i % ((kBM / 2) * 8) * 16, make_uint4(0u, 0u, 0u, 0u));
+  if constexpr (kSplit > 1) {                                  // rows that do not exist: 0, and so are their scores and probabilities
+    constexpr int kEmpty = (kBM - kRows) * 8;
+    for (int i = tid; i < NQ * (D / 64) * kEmpty; i += kThreads)
+      st_shared_v4(sQ + i / kEmpty * (kBM * 128) + kRows * 128 + i % kEmpty * 16, make_uint4(0u, 0u, 0u, 0u));
     fence_proxy_async();
   }
   // the append kernel before this one may still run: it writes the cache, the bits of the mask and the result of the checks
@@ -253,8 +257,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if ((sQ & 1023u) != 0u && tid == 0) sh->abort_flag = 97;
 
   // The sums of the segments' rows, (reference, sum) of the four parts of a row: over rows of the first queries' tile that do not exist.
-  float2* ends = reinterpret_cast<float2*>(tiles + (kBM / 2) * 128);
-  static_assert(!kApart || 2 * 4 * (kBM / 2) * 8 <= (kBM / 2) * 128, "room for the sums");
+  float2* ends = reinterpret_cast<float2*>(tiles + kRows * 128);
+  static_assert(!kApart || 2 * 4 * kRows * 8 <= (kBM - kRows) * 128, "room for the sums");
   // Columns [c0, c1) of a row from the accumulator at tO: to the output, or to a piece of it.
   auto write_rows = [&](const Segment& seg, int row, bool row_ok, float l_all, float m_fin, uint32_t tO, int c0, int c1, float* ws_l) {
     const bool piece = seg.nt < seg.all;
@@ -506,6 +510,8 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
+  } else if (kApart && warp >= 16 + kRows / 32) {
+    reg_dealloc<64>();
   } else if (kApart && warp >= 16) {
     // ------------------------------- results --------------------------------------------
     reg_dealloc<64>();
@@ -523,7 +529,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       float m_fin = -INFINITY, l_all = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        e[i] = ends[(ob * 4 + i) * (kBM / 2) + row];
+        e[i] = ends[(ob * 4 + i) * kRows + row];
         m_fin = fmaxf(m_fin, e[i].x);
       }
 #pragma unroll
@@ -532,7 +538,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_before();
       mbar_arrive(smem_u32(&sh->o_free[ob]));
     }
-  } else if (kSplit > 1 && (warp & 2)) {
+  } else if ((warp & 3) >= kRows / 32) {
     reg_alloc<104>();                                // (rows that do not exist)
   } else {
     // ------------------------------- softmax groups -------------------------------------
@@ -657,7 +663,7 @@ tree_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // ---- end of the segment --------------------------------------------------------------
       if constexpr (kApart) {
         if (ok && segs >= 2) ok = wait_bar(&sh->o_free[segs & 1], ((segs >> 1) - 1) & 1, sh, 38);      // (the sums there have been read)
-        ends[((segs & 1) * 4 + 2 * x + half) * (kBM / 2) + row_in_tile] = make_float2(m_own, sum);
+        ends[((segs & 1) * 4 + 2 * x + half) * kRows + row_in_tile] = make_float2(m_own, sum);
         mbar_arrive(smem_u32(&sh->ended[segs & 1]));
         ok = !any_of<64>(!ok, together);                   // (the warps of both halves leave together)
         continue;
@@ -782,7 +788,6 @@ int tree_sm100_ranges(const fa_decode_args& d, int pack_log2) {
   }
   return best;
 }
-static bool few_rows(const fa_decode_args& d, int pack_log2) { return ((int64_t)d.seqlen_q << pack_log2) <= kBM / 2; }
 // Two pieces of every CTA, with their LSEs.
 size_t tree_sm100_piece_bytes(const fa_decode_args& d, int pack_log2) {
   const int ranges = tree_sm100_ranges(d, pack_log2);
@@ -848,12 +853,16 @@ static int launch_tree(const fa_decode_args& d, const CacheGeo& geo, float scale
 
 template <typename T>
 static int launch_rows(const fa_decode_args& d, const CacheGeo& geo, const ScoreCfg& cfg, cudaStream_t st) {
-  const bool few = few_rows(d, geo.pack_log2);
-  const float s = cfg.scale_log2, r = cfg.rescale_at;
+  const int64_t rows = (int64_t)d.seqlen_q << geo.pack_log2;
+  auto launch = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    const float s = cfg.scale_log2, r = cfg.rescale_at;
+    return rows <= 32 ? launch_tree<T, D, 4>(d, geo, s, r, st) : rows <= 64 ? launch_tree<T, D, 2>(d, geo, s, r, st) : launch_tree<T, D, 1>(d, geo, s, r, st);
+  };
   switch (d.head_dim) {
-    case 64: return few ? launch_tree<T, 64, 2>(d, geo, s, r, st) : launch_tree<T, 64, 1>(d, geo, s, r, st);
-    case 128: return few ? launch_tree<T, 128, 2>(d, geo, s, r, st) : launch_tree<T, 128, 1>(d, geo, s, r, st);
-    case 256: return few ? launch_tree<T, 256, 2>(d, geo, s, r, st) : launch_tree<T, 256, 1>(d, geo, s, r, st);
+    case 64: return launch(std::integral_constant<int, 64>{});
+    case 128: return launch(std::integral_constant<int, 128>{});
+    case 256: return launch(std::integral_constant<int, 256>{});
   }
   set_error("tree_sm100: head_dim %d", d.head_dim);
   return FA_ERR_UNSUPPORTED;
