@@ -29,6 +29,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kMostShared = 224 * 1024;  // dynamic shared memory of a CTA
 
 template <typename T> __device__ __forceinline__ float wide(T x);
 template <> __device__ __forceinline__ float wide(__half x) { return __half2float(x); }
@@ -300,14 +301,15 @@ int launch_verify(const fa_verify_args& a, cudaStream_t st) {
   // what fits of a share in shared memory, beside another CTA's, or alone on its SM where there are SMs enough: with all of them asked
   // for (16 clusters of 8) one cluster waits for another's end, for a cluster lies within one part of the GPU
   const bool alone = (int64_t)a.batch * cluster <= sms * 3 / 4;
-  const size_t nodes = a.nodes * sizeof(Node), room = (alone ? 224 : 110) * 1024 - nodes;
+  const size_t nodes = a.nodes * sizeof(Node), room = (alone ? kMostShared : kMostShared / 2 - 2048) - nodes;
   const int64_t share = a.vocab / (cluster * kWarps) + 1, fit = (int64_t)(room / sizeof(float2) / kWarps);
   const int hold = (int)(share < fit ? share : fit);
   // (more than half of an SM's, so that CTAs do not share an SM while others have none)
   const size_t smem = std::max(nodes + (size_t)hold * kWarps * sizeof(float2), (size_t)(alone ? 116 * 1024 : 0));
   auto kern = verify_kernel<T>;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (the most that any call takes: another thread's call may come between this and the launch)
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) {
       set_error("verify_draft_tree: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return FA_ERR_LAUNCH;

@@ -6,6 +6,7 @@ roundings, its root and the reciprocal 3, the products and the rotation 4, each 
 and the gradients' second mean.  Weight gradients: chains of up to 200 additions, 2^-16.  Attention: probabilities rounded to the type once, half a step
 of sum p |v| beside that of the output; scores in fp32 (128 products of size 1 in units of the scale): 2^-12."""
 import math
+import threading
 
 import pytest
 import torch
@@ -544,6 +545,30 @@ def test_verify_shares_that_shared_memory_has_no_room_for(batch, vocab):
         args[2][:, 0, 7] = 0
         check_verify(args)
         assert (fa.verify_draft_tree(*(x.to(DEV) for x in args))[2] == -1).all()
+
+
+def test_verify_from_two_threads():
+    """Calls that need different amounts of shared memory, at the same time on streams of their own."""
+    given = [[x.to(DEV) for x in verify_case(40 + i, batch, nodes, vocab, F32)] for i, (batch, nodes, vocab) in enumerate([(2, 6, 200003), (40, 3, 9001)])]
+    want = [fa.verify_draft_tree(*x) for x in given]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    got = fa.verify_draft_tree(*given[i])
+                torch.cuda.current_stream().synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want[i]))
+        except BaseException as e:
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
 
 
 def test_verified_tokens_are_distributed_as_the_target():
