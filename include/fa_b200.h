@@ -41,7 +41,7 @@ typedef enum fa_status {
   FA_ERR_DEVICE_WAIT = -5  /* a bounded device-side wait ran out (kernel set its flag) */
 } fa_status;
 
-typedef enum fa_dtype { FA_F16 = 0, FA_BF16 = 1, FA_F32 = 2 /* rotary / row movers only */ } fa_dtype;
+typedef enum fa_dtype { FA_F16 = 0, FA_BF16 = 1, FA_F32 = 2 /* rotary, row movers, norms and verification only */ } fa_dtype;
 
 /* Kernel family selector (fa_attn_args.impl). */
 typedef enum fa_impl {
