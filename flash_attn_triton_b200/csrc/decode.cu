@@ -301,12 +301,13 @@ __global__ void __launch_bounds__(128, D <= 128 ? 2 : 1)
       }
       __syncwarp();
     }
-    // Nodes that no row sees (of a request that uses fewer than others) may hold anything: 0 times a NaN would be one.
+    // Nodes that no row sees (of a request that uses fewer than others) may hold anything: 0 times a NaN would be one.  (causal: the rows
+    // before a node do not see it, whatever the mask has there)
     if (kTree && keyw + 16 > tree0) {
       const int node = keyw + (lane & 15) - tree0;
       bool dead = node >= 0 && node < p.seqlen_q;
       if (dead)
-        for (int i = 0; i < p.seqlen_q; ++i) dead = dead && seen[i * p.tree_stride[1] + node] == 0;
+        for (int i = p.causal ? node : 0; i < p.seqlen_q; ++i) dead = dead && seen[i * p.tree_stride[1] + node] == 0;
       for (unsigned rest = __ballot_sync(0xffffffffu, dead) & 0xffffu; rest; rest &= rest - 1)
         if (lane < CPR) *reinterpret_cast<uint4*>(tV + (__ffs(rest) - 1) * P + lane * 8) = make_uint4(0u, 0u, 0u, 0u);
       __syncwarp();
