@@ -15,6 +15,7 @@
 //   warp adds them up in the same order.  The share that the random number falls into is cut among the warps of its CTA in the same way, and one of
 //   them finds the token.
 #include <algorithm>
+#include <atomic>
 
 #include <cooperative_groups.h>
 
@@ -307,13 +308,18 @@ int launch_verify(const fa_verify_args& a, cudaStream_t st) {
   // (more than half of an SM's, so that CTAs do not share an SM while others have none)
   const size_t smem = std::max(nodes + (size_t)hold * kWarps * sizeof(float2), (size_t)(alone ? 116 * 1024 : 0));
   auto kern = verify_kernel<T>;
-  if (smem > 48 * 1024) {
-    // (the most that any call takes: another thread's call may come between this and the launch)
+  // Once per kernel and device, the most that any call takes (another thread's call may come between this and the launch).  By every first
+  // call: without it 48 KB are the limit of dynamic and static shared memory together.
+  static_assert(kMostShared + sizeof(Shared) <= 227 * 1024, "shared memory budget");
+  static std::atomic<uint64_t> prepared{0};
+  const uint64_t bit = a.device < 64 ? 1ull << a.device : 0;
+  if ((prepared.load(std::memory_order_relaxed) & bit) == 0) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) {
       set_error("verify_draft_tree: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return FA_ERR_LAUNCH;
     }
+    prepared.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr;

@@ -1,5 +1,9 @@
 """More of decoding with trees of drafted tokens; definitions and tolerances as in test_gpu_drafting.py."""
 import math
+import os
+import subprocess
+import sys
+import textwrap
 
 import pytest
 import torch
@@ -47,3 +51,24 @@ def test_nodes_that_causal_hides_may_hold_anything(i, splits, new, spoil, wide):
         every = torch.cat((torch.ones(nodes, n, dtype=torch.bool), sees[b]), 1)
         want, size = ref.attend(q[b], torch.cat((kc[x, y], k[b])), torch.cat((vc[x, y], v[b])), every, dim ** -0.5)
         base.within(out[b], want, base.half(dtype) * want.abs() + (base.half(dtype) + 2.0 ** -12) * size + 1e-6, ("out", b))
+
+
+# ---- the first verification of a process -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("batch,nodes,vocab", [(160, 3, 6000), (64, 8, 24000), (30, 16, 47000)])
+def test_first_verification_of_a_process(batch, nodes, vocab):
+    """Shares of the vocabulary for which the kernel needs a little more than 48 KB of shared memory in all, its static part counted: nothing
+    that an earlier call has asked for may be missing."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = f"""
+        import torch
+        import test_gpu_drafting as base
+        for dtype in (torch.float32, torch.float16, torch.bfloat16):
+            given = base.verify_case(1, 2, {nodes}, {vocab}, dtype, 0.7)
+            pick = torch.arange({batch}) % 2
+            parents = given[1][pick]
+            given = [x[pick] for x in given]
+            base.check_verify([x[:2] for x in given], **{{"_%d" % i: (lambda y: lambda x: y.to(base.DEV))(y) for i, y in enumerate(given)}})
+    """
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)]))
+    done = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], env=env, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
