@@ -1,13 +1,17 @@
 """Decoding with trees of drafted tokens: a small model drafts a tree of tokens for each request, the large one verifies all of
 them in one step over its KV cache.  No counterpart in the reference.  A step, with `flash_attn_with_kvcache(tree_mask=)` between:
 
-    slots, cu, used = build_block_table(cache_seqlens, nodes_of, free_pages, block_table, page_size, num_tokens)
+    slots, cu, used = build_block_table(cache_seqlens, torch.full_like(cache_seqlens, nodes), free_pages, block_table, page_size, batch * nodes)
     q, k = qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=cache_seqlens[:, None] + depth)          # each layer
     out = flash_attn_with_kvcache(q, k_cache, v_cache, k, v, cache_seqlens=cache_seqlens, block_table=block_table, tree_mask=mask)
     path, accepted, token = verify_draft_tree(draft_tokens, parents, target_probs, draft_probs, accept_uniforms, sample_uniforms)
     kvcache_compact(k_caches, v_caches, cache_seqlens, path, accepted, block_table=block_table)                    # all layers
-    pages, n = release_pages(cache_seqlens + nodes_of, cache_seqlens + accepted, block_table, page_size, num_pages)
+    pages, n = release_pages(cache_seqlens + nodes, cache_seqlens + accepted, block_table, page_size, num_pages)
     cache_seqlens += accepted                                     # `token` is the root of the next tree
+
+`nodes` is the seqlen_q of the call, the nodes of the largest tree.  The call appends that many rows for every request, those of nodes that a
+request does not use too, so that every request needs pages for all of them: an entry of the table that this step did not fill may name a
+page that is another request's by now.
 """
 from __future__ import annotations
 

@@ -385,8 +385,9 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     tree_mask: the query rows are the nodes of a tree of drafted tokens, the last seqlen_q tokens of the sequence after the append.  Bool,
     (batch, seqlen_q, seqlen_q) or (seqlen_q, seqlen_q): row i sees node j where [.., i, j] is true -- itself and its ancestors, as a
     rule -- and all tokens before the tree; with `causal`, only j <= i.  Rows of nodes that a request does not use may be all false
-    (they see the context alone; zeros without one), and what nodes hold that no row sees does not matter.  For 16-bit caches, without window, ALiBi
-    and rotary tables: a node's position is not its slot, see `qk_norm_rotary`.
+    (they see the context alone; zeros without one), and what nodes hold that no row sees does not matter.  They are appended all the same: block_table
+    must have pages for seqlen_q tokens of every request, used or not.  For 16-bit caches, without window, ALiBi and rotary tables: a node's
+    position is not its slot, see `qk_norm_rotary`.
 
     With value checks on (the default) the kernel makes them first (page indices in range, lengths
     fit the cache and the rotary tables) and the call waits for that one flag, not for the attention;

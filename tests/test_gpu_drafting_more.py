@@ -11,9 +11,11 @@ import torch
 import drafting_reference as ref
 import flash_attn_triton_b200 as fa
 import test_gpu_drafting as base
+from flash_attn_triton_b200 import drafting
 from util import DEV
 
 pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 
 
 # ---- nodes that only rows before them have in the mask -----------------------------------------------------------------------------
@@ -72,3 +74,53 @@ def test_first_verification_of_a_process(batch, nodes, vocab):
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)]))
     done = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], env=env, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ---- the step as it is written in drafting.py --------------------------------------------------------------------------------------
+def test_the_documented_step_leaves_other_requests_alone():
+    """Trees of different sizes in one call, and tables whose unused entries still name pages that other requests own (no call clears them):
+    contexts stay as they were, accepted rows follow them, and every page has one owner."""
+    gen = torch.Generator().manual_seed(9)
+    batch, nodes, heads, heads_kv, dim, page, pool, vocab = 3, 40, 4, 2, 64, 16, 32, 61
+    lens, nodes_of = [30, 16, 5], [nodes, 2, 1]
+    order = torch.randperm(pool, generator=gen).to(torch.int32)
+    table, at = torch.zeros(batch, 8, dtype=torch.int32), 0
+    for b, n in enumerate(lens):
+        held = -(-n // page)
+        table[b, :held] = order[at:at + held]
+        at += held
+    for b in range(batch):                                    # behind each request's pages: those of the next one
+        table[b, -(-lens[b] // page):] = table[(b + 1) % batch, 0]
+    parents, seen = ref.tree(gen, batch, nodes, nodes_of)
+    kc, vc = (base.rand(gen, pool, page, heads_kv, dim).to(F16) for _ in range(2))
+    q, k, v = (base.rand(gen, batch, nodes, h, dim).to(F16) for h in (heads, heads_kv, heads_kv))
+    draft = torch.softmax(base.rand(gen, batch, nodes, vocab), -1)
+    angle = torch.outer(torch.arange(128.0), 100.0 ** (-torch.arange(0, dim, 2) / dim))
+    at_gpu = dict(cache_seqlens=torch.tensor(lens, dtype=torch.int32), nodes_of=torch.tensor(nodes_of, dtype=torch.int32), free_pages=order[at:],
+                  block_table=table, q=q, k=k, v=v, k_cache=kc, v_cache=vc, mask=seen, cos=angle.cos(), sin=angle.sin(),
+                  depth=(seen.sum(-1) - 1).clamp_min(0).int(), draft_tokens=torch.randint(vocab, (batch, nodes), generator=gen), parents=parents,
+                  target_probs=draft.clone(), draft_probs=draft, accept_uniforms=torch.zeros(batch, nodes),
+                  sample_uniforms=torch.rand(batch, generator=gen))
+    names = {n: x.clone().to(DEV) for n, x in at_gpu.items()}
+    names.update(batch=batch, nodes=nodes, page_size=page, num_pages=pool, num_tokens=batch * nodes, q_weight=None, k_weight=None, torch=torch)
+    names.update({n: getattr(fa, n) for n in ("build_block_table", "qk_norm_rotary", "flash_attn_with_kvcache", "verify_draft_tree",
+                                              "kvcache_compact", "release_pages")})
+    names["k_caches"], names["v_caches"] = [names["k_cache"]], [names["v_cache"]]
+    step = [line for line in drafting.__doc__.splitlines() if line.startswith("    ")]
+    assert len(step) == 7
+    exec(textwrap.dedent("\n".join(step)), names)
+    _, keys = fa.qk_norm_rotary(*(at_gpu[n].to(DEV) for n in ("q", "k")), None, None, names["cos"], names["sin"],
+                                positions=torch.tensor(lens, device=DEV)[:, None] + names["depth"])
+    keys, got_k, got_v, rows = keys.cpu(), names["k_cache"].cpu(), names["v_cache"].cpu(), names["block_table"].cpu()
+    path, accepted = names["path"].cpu(), names["accepted"].tolist()
+    assert max(accepted) > 2 and names["cache_seqlens"].tolist() == [n + m for n, m in zip(lens, accepted)]
+    for b, n in enumerate(lens):
+        for p in range(n):
+            was, now = (int(table[b, p // page]), p % page), (int(rows[b, p // page]), p % page)
+            assert torch.equal(got_k[now], kc[was]) and torch.equal(got_v[now], vc[was]), ("context", b, p)
+        for i in range(accepted[b]):
+            now = int(rows[b, (n + i) // page]), (n + i) % page
+            assert torch.equal(got_k[now], keys[b, path[b, i]]) and torch.equal(got_v[now], v[b, path[b, i]]), ("accepted", b, i)
+    owned = [x for b in range(batch) for x in rows[b, :-(-(lens[b] + accepted[b]) // page)].tolist()]
+    free = names["free_pages"].tolist()[names["used"].item():] + names["pages"].tolist()[:names["n"].item()]
+    assert sorted(owned + free) == list(range(pool))
