@@ -7,6 +7,7 @@
 // through the addresses of libfa_b200.so's C functions, handed over once by init(), so that any build
 // of that library can be driven.
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -1175,6 +1176,17 @@ void fill_norm(fa_qk_norm_args& p, const NormCall& c) {
   }
 }
 
+// Gradients that a backward of `node` has made from `grads`, under create_graph: the kernels' gradients have no derivative, so whoever
+// differentiates through these is told.  Without a history they would be constants, and a part of the second gradient missing without a word.
+void refuse_second_gradient(Node& node, const variable_list& grads, const variable_list& made, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list edges = node.next_edges();           // (what was saved may be a copy, which has no history)
+  for (auto& e : torch::autograd::collect_next_edges(grads)) edges.push_back(std::move(e));
+  const std::shared_ptr<Node> error(new torch::autograd::Error(std::string(what) + " cannot be differentiated twice", std::move(edges)),
+                                    torch::autograd::deleteNode);
+  torch::autograd::set_history(made, error);
+}
+
 struct QkNormBackward : public Node {
   SavedVariable saved[7];
   double eps;
@@ -1221,6 +1233,7 @@ struct QkNormBackward : public Node {
       p.workspace = ws.mutable_data_ptr();
     }
     check(g_abi.qk_norm_bwd(&p, stream_of(c.q)), "fa_qk_norm_bwd");
+    refuse_second_gradient(*this, grads, out, "qk_norm_rotary");
     return out;
   }
   std::string name() const override { return "QkNormRotaryBackward"; }

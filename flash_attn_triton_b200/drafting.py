@@ -38,7 +38,7 @@ def _on(device, *tensors):
 def qk_norm_rotary(q, k, q_weight=None, k_weight=None, rotary_cos=None, rotary_sin=None, positions=None, eps=1e-6,
                    rotary_interleaved=False):
     """RMS norm of every head of q and k, then the rotary embedding, in one pass: y = x * rsqrt(mean(x^2) + eps) * weight over
-    head_dim, rotated at the token's position.  In fp32, rounded once.  Returns (q, k) as new tensors; differentiable in q, k and the weights.
+    head_dim, rotated at the token's position.  In fp32, rounded once.  Returns (q, k) as new tensors; differentiable in q, k and the weights, once.
 
     q (batch, seqlen, nheads, d) or packed (tokens, nheads, d), fp16, bf16 or fp32; k the same with its own number of heads; weights (d,)
     of q's dtype or both fp32, None for ones; tables (seqlen_ro, rotary_dim / 2) of q's dtype or fp32, None for no rotation.  positions:

@@ -124,3 +124,50 @@ def test_the_documented_step_leaves_other_requests_alone():
     owned = [x for b in range(batch) for x in rows[b, :-(-(lens[b] + accepted[b]) // page)].tolist()]
     free = names["free_pages"].tolist()[names["used"].item():] + names["pages"].tolist()[:names["n"].item()]
     assert sorted(owned + free) == list(range(pool))
+
+
+# ---- gradients of gradients --------------------------------------------------------------------------------------------------------
+def norm_call(leaf):
+    return fa.qk_norm_rotary(leaf, leaf[..., :1, :])[0]
+
+
+def refuses_second_gradients(call, leaf):
+    """The first gradient is what it is without create_graph; a loss that reaches through it, whatever else is in it, is refused."""
+    def first(**kw):
+        return torch.autograd.grad(call(leaf).float().square().sum(), leaf, **kw)[0]
+    want, got = first(), first(create_graph=True)
+    assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
+    for loss in (got.float().square().sum(), got.float().sum() + leaf.float().square().sum()):
+        with pytest.raises(RuntimeError, match="differentiated twice"):
+            torch.autograd.grad(loss, leaf, retain_graph=True)
+    # what does not reach through it has its gradient
+    (g,) = torch.autograd.grad(got.detach().float().sum() + leaf.float().sum(), leaf)
+    assert (g == 1).all()
+    call(leaf).float().square().sum().backward(create_graph=True)
+    assert torch.equal(leaf.grad, want)
+    leaf.grad = None
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("behind", [0, 1])                     # 1: not on a 16-byte boundary, so that the call works on a copy
+def test_gradients_of_gradients_of_the_norm_are_refused(dtype, behind):
+    leaf = base.rand(torch.Generator().manual_seed(1), 2 * 5 * 3 * 64 + behind).to(dtype).to(DEV)[behind:].view(2, 5, 3, 64).requires_grad_()
+    refuses_second_gradients(norm_call, leaf)
+
+
+def test_gradients_of_gradients_of_the_norms_weights_are_refused():
+    """dq depends on the weight also where q itself takes no gradient of its own, and the weight's gradient on the result's."""
+    gen = torch.Generator().manual_seed(2)
+    q, w, scale = base.rand(gen, 2, 5, 3, 64).to(DEV), torch.ones(64, device=DEV, requires_grad=True), torch.ones((), device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad((fa.qk_norm_rotary(q, q, w, w)[0] * scale).sum(), w, create_graph=True)
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        g.sum().backward()
+
+
+def test_norm_under_function_transforms_is_refused():
+    q = base.rand(torch.Generator().manual_seed(3), 4, 2, 5, 3, 64).to(DEV)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda x: fa.qk_norm_rotary(x, x)[0])(q)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: fa.qk_norm_rotary(x, x)[0].sum())(q[0])
