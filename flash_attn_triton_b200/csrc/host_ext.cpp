@@ -390,6 +390,17 @@ variable_list run_backward(const Params& c, const variable_list& in, const Tenso
   return g;
 }
 
+// Gradients that a backward of `node` has made from `grads`, under create_graph: the kernels' gradients have no derivative, so whoever
+// differentiates through these is told.  Without a history they would be constants, and a part of the second gradient missing without a word.
+void refuse_second_gradient(Node& node, const variable_list& grads, const variable_list& made, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list edges = node.next_edges();           // (what was saved may be a copy, which has no history)
+  for (auto& e : torch::autograd::collect_next_edges(grads)) edges.push_back(std::move(e));
+  const std::shared_ptr<Node> error(new torch::autograd::Error(std::string(what) + " cannot be differentiated twice", std::move(edges)),
+                                    torch::autograd::deleteNode);
+  torch::autograd::set_history(made, error);
+}
+
 // Every tensor that the backward reads is a saved variable: one that was changed in place since the forward is
 // refused, and the saved-tensor hooks (offloading, checkpointing) see all of them.  Params::bias alone is held as it
 // is: expanded over broadcast dimensions, it would be written out in full by a hook that copies.
@@ -422,7 +433,9 @@ struct AttnBackward : public Node {
       dq = task_should_compute_output(0);
       dkdv = task_should_compute_output(1) || (p.packing == kSeparate && task_should_compute_output(2));
     }
-    return run_backward(p, x, o, l, grad, dq, dkdv);
+    variable_list made = run_backward(p, x, o, l, grad, dq, dkdv);
+    refuse_second_gradient(*this, grads, made, "attention");
+    return made;
   }
   std::string name() const override { return "FlashAttnBackward"; }
   void release_variables() override {
@@ -1174,17 +1187,6 @@ void fill_norm(fa_qk_norm_args& p, const NormCall& c) {
     p.pos_stride[0] = rows && c.positions.size(0) > 1 ? c.positions.stride(0) : 0;
     p.pos_stride[1] = c.positions.stride(rows ? 1 : 0);
   }
-}
-
-// Gradients that a backward of `node` has made from `grads`, under create_graph: the kernels' gradients have no derivative, so whoever
-// differentiates through these is told.  Without a history they would be constants, and a part of the second gradient missing without a word.
-void refuse_second_gradient(Node& node, const variable_list& grads, const variable_list& made, const char* what) {
-  if (!at::GradMode::is_enabled()) return;
-  torch::autograd::edge_list edges = node.next_edges();           // (what was saved may be a copy, which has no history)
-  for (auto& e : torch::autograd::collect_next_edges(grads)) edges.push_back(std::move(e));
-  const std::shared_ptr<Node> error(new torch::autograd::Error(std::string(what) + " cannot be differentiated twice", std::move(edges)),
-                                    torch::autograd::deleteNode);
-  torch::autograd::set_history(made, error);
 }
 
 struct QkNormBackward : public Node {
