@@ -598,8 +598,13 @@ struct ChunkPlan {
 };
 // Whether a tree takes the kernel for it (tree_sm100.cu): more than 8 query rows per KV head, and more than two tiles of 64 keys and 16 rows for
 // each CTA of decode_kernel that runs at a time.  Measured, decode_kernel against it (us, 8 KV heads of 128): 48 x 6250 tokens, 16 rows 256, 225;
-// 8 rows 233, 220; 1 x 8000, 16 rows 29, 24; 1 x 1900, 32 rows 18, 20; 64 rows 22, 21; 1 x 500, 32 rows 15, 16; 2 x 300, 2 heads of 64,
-// 20 rows 10, 18: few tiles are bounded by launches, of which decode_kernel is one and a tree's are three.
+// 1 x 8000, 16 rows 29, 24; 1 x 1900, 32 rows 18, 20; 64 rows 22, 21.
+// Up to 8 rows, which are one row group of decode_kernel, there is no border by tiles alone: 8 rows of 16 x 2000 tokens 36, 41; 4 x 2000 18.5, 21;
+// 1 x 8000 23, 24.5; 64 x 2000 99, 99.5; 32 x 1024 to 16384 229, 193; 48 x 500 to 12000 235, 203, 4 rows 215, 193.  They stay with decode_kernel,
+// one launch without a workspace for bits; what that costs is the tenth to seventh of the large batches.
+// The capacity stands for the lengths, which are on the device: short trees in tables for 32768 tokens take this kernel too.  Tables for their own
+// length and such ones: 2 x 300, 2 heads of 64, 20 rows, calls from the host 14.5, 20.5, for three launches are not one, in a graph 12, 12.5; 8 heads
+// of 128, 8 x 200, 16 rows 18, 20, in a graph 17, 14; 1 x 200, 128 rows per head and more 21 to 23, 20.5, in a graph the same.
 static bool tree_kernel_is_faster(const fa_decode_args& a, int64_t capacity) {
   const int64_t rows = (int64_t)a.seqlen_q * (a.heads_q / a.heads_kv);
   return rows > 8 && a.batch * a.heads_kv * ((rows + 15) / 16) * ((capacity + kTile - 1) / kTile) > 4ll * sm_count(a.device);

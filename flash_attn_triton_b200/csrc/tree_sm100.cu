@@ -25,7 +25,7 @@
 // What a tile costs beside its bytes counts twice, for the memory and the SMs together reach the limit of
 // the GPU's power, and the clock falls.  18 x 16384 tokens, 64 rows over each of 8 KV heads of 128 (floor 185 us): two groups of four
 // softmax warps, a tile each, 254 us, also out of L2; four warps per scheduler 228; P rounded to 16 bits once and not in two parts, as chunks of
-// a cache have it, and no work on rows that do not exist 185; 16 rows, softmax for 32 in place of 64, 48 x 500 to 12000 tokens 245 -> 238.  (Errors against float64, fp16, 4 to 16 nodes: 2.1e-4 of two parts, 2.6e-4.)
+// a cache have it, and no work on rows that do not exist 185; 16 rows, softmax for 32 in place of 64, 48 x 500 to 12000 tokens 245 -> 238.  (Errors against float64, relative: fp16 2.1e-4 of two parts, 2.9e-4 of one; bf16 1.6e-3, 2.3e-3.)
 #include <type_traits>
 
 #include "cache_geo.cuh"
@@ -772,7 +772,9 @@ static int units_of(const fa_decode_args& d, int pack_log2) {
   return (d.heads_q >> pack_log2) * (int)((((int64_t)d.seqlen_q << pack_log2) + kBM - 1) / kBM);
 }
 
-// Ranges for U units: as many as there are SMs for, and beyond that the number of waves (up to 8) whose last one is the fullest.
+// Ranges for U units: as many as there are SMs for, and beyond that the number of ranges (up to 8) whose last wave is the fullest, less a fiftieth
+// for each wave.  Measured with 0, 0.02, 0.1 in its place (us, head_dim 64): 100 units, 4 x 1000 tokens 69, 52, 51; 16 x 4000 376, 368, 368;
+// 128 units, 8 x 4000 383, 385, 391 to 403; head_dim 128, 90 units, 16 x 4000 492, 466, 465; 110 units 576, 584, 575.
 int tree_sm100_ranges(const fa_decode_args& d, int pack_log2) {
   const int U = units_of(d, pack_log2), sms = sm_count(d.device);
   if (2 * U <= sms) return sms / U;

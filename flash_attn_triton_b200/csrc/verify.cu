@@ -299,8 +299,9 @@ int launch_verify(const fa_verify_args& a, cudaStream_t st) {
   const int sms = sm_count(a.device);
   int cluster = 1;
   while (cluster < kMaxCluster && a.vocab > (int64_t)cluster * kThreads * 4 && (int64_t)a.batch * cluster * 2 <= 2 * sms) cluster *= 2;
-  // what fits of a share in shared memory, beside another CTA's, or alone on its SM where there are SMs enough: with all of them asked
-  // for (16 clusters of 8) one cluster waits for another's end, for a cluster lies within one part of the GPU
+  // what fits of a share in shared memory, beside another CTA's, or alone on its SM where there are SMs enough: the nearer the CTAs come to
+  // the SMs' number, the more clusters wait for another's end, for a cluster lies within one part of the GPU.  Alone and not, us, 24 children of one
+  // node, 40009 tokens: 10 and 14 clusters of 8 the same, 16 53, 61; 18 56, 53; 100003 tokens: 16 63.5, 64; 18 69, 68.
   const bool alone = (int64_t)a.batch * cluster <= sms * 3 / 4;
   const size_t nodes = a.nodes * sizeof(Node), room = (alone ? kMostShared : kMostShared / 2 - 2048) - nodes;
   const int64_t share = a.vocab / (cluster * kWarps) + 1, fit = (int64_t)(room / sizeof(float2) / kWarps);

@@ -387,7 +387,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     rule -- and all tokens before the tree; with `causal`, only j <= i.  Rows of nodes that a request does not use may be all false
     (they see the context alone; zeros without one), and what nodes hold that no row sees does not matter.  They are appended all the same: block_table
     must have pages for seqlen_q tokens of every request, used or not.  For 16-bit caches, without window, ALiBi and rotary tables: a node's
-    position is not its slot, see `qk_norm_rotary`.
+    position is not its slot, see `qk_norm_rotary`.  Probabilities are rounded to the dtype of the cache once before their product with the values, as for
+    few query rows without a mask; larger chunks without one keep them in two parts, so that the same chain as `causal` is 1.4 times as exact there.
 
     With value checks on (the default) the kernel makes them first (page indices in range, lengths
     fit the cache and the rotary tables) and the call waits for that one flag, not for the attention;

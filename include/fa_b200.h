@@ -222,8 +222,8 @@ typedef struct fa_decode_args {
 
   /* A tree of drafted tokens, or NULL: the last seqlen_q positions after the append are its nodes, and query row i sees, of
    * the keys there, those j with tree_mask[b * tree_stride[0] + i * tree_stride[1] + j] != 0 (bytes), besides all keys before them;
-   * with `causal`, only j <= i.  Values of nodes that no row sees are not read as numbers (they may be NaN).  16-bit caches;
-   * no window, ALiBi or rotary tables (the position of a node is not its slot). */
+   * with `causal`, only j <= i.  Values of nodes that no row sees are not read as numbers (they may be NaN), but are appended like the others:
+   * the block table needs pages for all of them.  16-bit caches; no window, ALiBi or rotary tables (the position of a node is not its slot). */
   const uint8_t* tree_mask;
   int64_t tree_stride[2];
 } fa_decode_args;
